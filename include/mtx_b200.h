@@ -696,6 +696,65 @@ int mtx_layered_step_graph(mtx_layered* e, const mtx_ragged_batch* b, mtx_stream
 int mtx_sample_rows(const float* logits, int rows, long long ld, int vocab, int strategy, int top_k, float nucleus_p, float temperature,
                     uint32_t* rng_state, int row_offset, void* scratch, int32_t* token_out, float* log_prob_out, mtx_stream stream);
 
+/* ---- 8-bit products ------------------------------------------------------------------------- */
+
+/* Types of values. */
+#define MTX_BF16 0
+#define MTX_F32 1
+#define MTX_E4M3 2 /* 8-bit floating point (float8_e4m3fn) with a scale per block of 128 */
+
+/* x [rows, k] (pitch ldx values) of type MTX_BF16 or MTX_F32 as 8-bit values with scales.  block_rows = 1: a scale per 128 values of a row
+ * (activations); block_rows = 128: a scale per 128 x 128 block (weights); the last blocks may be smaller.  With A = max(max |x|, 2^-96) over
+ * a block: scale = A / 448, q = e4m3(x * (448 / A)), both fractions and the product rounded to fp32.  A NaN makes its block's scale
+ * and values NaN, an infinity the scale infinite and itself NaN, so that products of its row are NaN.
+ * q: pitch ldq, both base and pitch whole 16 bytes (bytes from k to ldq of a row are left as they are); scale: fp32
+ * [ceil(rows / block_rows), ceil(k / 128)]. */
+int mtx_quantize_fp8(const void* x, int x_type, long long ldx, int rows, int k, int block_rows, void* q, long long ldq, float* scale, mtx_stream stream);
+
+/* out[m, n] = sum over the blocks b of 128 columns of x_scale[m, b] * w_scale[n / 128, b] * sum_{k in b} x[m, k] * wq[n, k], sums in fp32:
+ * beside mtx_linear, with weights of mtx_quantize_fp8(block_rows = 128) and any number of rows.  x: MTX_E4M3 values with their x_scale
+ * [rows, ceil(k / 128)] (block_rows = 1), or MTX_BF16 / MTX_F32 values, which the call quantises in the same way (x_scale is not read) in `scratch`:
+ * mtx_linear_fp8_scratch_bytes(rows, k) bytes, 16-byte aligned, written by every call and so not for two calls at once.  8-bit
+ * operands: base and pitch whole 16 bytes.  out: MTX_BF16 or MTX_F32, pitch ldo values; it may not overlap an input. */
+size_t mtx_linear_fp8_scratch_bytes(int rows, int k);
+int mtx_linear_fp8(const void* x, int x_type, long long ldx, const float* x_scale, const void* wq, long long ldw, const float* w_scale, void* out, int out_type, long long ldo,
+                   int rows, int n, int k, void* scratch, size_t scratch_bytes, mtx_stream stream);
+
+/* ---- controls of logits ---------------------------------------------------------------------- */
+
+/* What a batch's logits pass between the projection and the sampler; every part may be left out (NULL).  The record of seen tokens has a row
+ * per slot: `seen` a 16-bit word per token (bit 15: the prompt held it; bits 0..14: how often it was generated, at most 32767), `touched` a
+ * bit per eight tokens (token t: bit t / 8 % 32 of word t / 256), set where any of their words is not zero.  Zeroing both makes a slot forget. */
+typedef struct {
+  int32_t slots;              /* rows of the record and of the penalties */
+  const int32_t* slot;        /* [rows]; NULL: row r is slot r.  A row whose slot is not in [0, slots) has no penalties */
+  const uint16_t* seen;       /* [slots, ld_seen]: 16-byte aligned, ld_seen a multiple of 8 */
+  long long ld_seen;
+  const uint32_t* touched;    /* [slots, ld_touched] or NULL: the words are then all read */
+  long long ld_touched;
+  const float* repetition;    /* [slots] or NULL: the logit of a seen token is divided by it where it is positive, else multiplied */
+  const float* presence;      /* [slots] or NULL: taken off the logits of generated tokens */
+  const float* frequency;     /* [slots] or NULL: times a token's count taken off its logit */
+  const int32_t* bias_off;    /* [rows + 1]: row r's biases are the entries [bias_off[r], bias_off[r + 1]) of the two arrays below, their */
+  const int32_t* bias_token;  /* tokens ascending; of entries with one token the first counts, tokens outside the vocabulary are skipped */
+  const float* bias_value;
+  int32_t allowed_rows;
+  const int32_t* allowed_row; /* [rows]; NULL: row r has mask r.  A row whose mask is not in [0, allowed_rows) is not masked */
+  const uint32_t* allowed;    /* [allowed_rows, ld_allowed]: token t is allowed by bit t % 32 of word t / 32 */
+  long long ld_allowed;
+} mtx_logit_controls;
+
+/* out = controlled logits, rows x vocab each: repetition, then frequency, then presence penalty, then the bias; the logits of tokens that are not
+ * allowed are -infinity whatever they were (a row whose mask allows nothing is -infinity throughout).  Every operation is rounded to fp32.
+ * out == logits (with ldo == ld): in place, and then only what changes is read and written; otherwise the two may not overlap. */
+int mtx_control_logits(const float* logits, long long ld, float* out, long long ldo, int rows, int vocab, const mtx_logit_controls* c, mtx_stream stream);
+
+/* Notes n tokens in the record: token[i] in slot slot[i] (NULL: slot i, n <= slots), as the prompt's (prompt != 0) or as generated once more.  The
+ * same token may come several times; tokens outside [0, vocab) and slots outside [0, slots) are skipped.  touched may be NULL (and is
+ * then NULL in the controls too). */
+int mtx_note_tokens(uint16_t* seen, long long ld_seen, uint32_t* touched, long long ld_touched, int slots, int vocab, const int32_t* token, const int32_t* slot, int n, int prompt,
+                    mtx_stream stream);
+
 /* ---- misc ---------------------------------------------------------------------------------- */
 
 /* Measurement aid: grid-barrier timeline of the persistent step kernel.  While a device buffer of

@@ -213,6 +213,18 @@ class RaggedBatch(ctypes.Structure):
               ("n_tiles", ctypes.c_int32), ("tile_row0", ctypes.c_void_p), ("n_runs", ctypes.c_int32), ("run_row0", ctypes.c_void_p)]
 
 
+BF16, F32, E4M3 = 0, 1, 2  # types of values (MTX_BF16, MTX_F32, MTX_E4M3)
+
+
+class LogitControls(ctypes.Structure):
+  """mtx_logit_controls."""
+
+  _fields_ = [("slots", ctypes.c_int32), ("slot", ctypes.c_void_p), ("seen", ctypes.c_void_p), ("ld_seen", ctypes.c_longlong), ("touched", ctypes.c_void_p),
+              ("ld_touched", ctypes.c_longlong), ("repetition", ctypes.c_void_p), ("presence", ctypes.c_void_p), ("frequency", ctypes.c_void_p),
+              ("bias_off", ctypes.c_void_p), ("bias_token", ctypes.c_void_p), ("bias_value", ctypes.c_void_p), ("allowed_rows", ctypes.c_int32),
+              ("allowed_row", ctypes.c_void_p), ("allowed", ctypes.c_void_p), ("ld_allowed", ctypes.c_longlong)]
+
+
 def sources() -> list[str]:
   return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".cc"))) + [HEADER]
 
@@ -231,7 +243,7 @@ def _jaxlib_include() -> list[str]:
     return []
 
 
-UNITS = ("engine.cu", "layered.cu", "mtx_jax_ffi.cc")  # translation units of the library, compiled separately and linked
+UNITS = ("engine.cu", "layered.cu", "fp8_linear.cu", "logit_controls.cu", "mtx_jax_ffi.cc")  # translation units of the library, compiled separately and linked
 
 
 def _unit_deps(path: str, seen=None) -> set:
@@ -396,6 +408,17 @@ def _declare(lib) -> None:
   lib.mtx_layered_step_graph.argtypes = [vp, c.POINTER(RaggedBatch), vp]
   lib.mtx_sample_rows.restype = i32
   lib.mtx_sample_rows.argtypes = [vp, i32, c.c_longlong, i32, i32, i32, f32, f32, vp, i32, vp, vp, vp, vp]
+  i64 = c.c_longlong
+  lib.mtx_quantize_fp8.restype = i32
+  lib.mtx_quantize_fp8.argtypes = [vp, i32, i64, i32, i32, i32, vp, i64, vp, vp]
+  lib.mtx_linear_fp8_scratch_bytes.restype = sz
+  lib.mtx_linear_fp8_scratch_bytes.argtypes = [i32, i32]
+  lib.mtx_linear_fp8.restype = i32
+  lib.mtx_linear_fp8.argtypes = [vp, i32, i64, vp, vp, i64, vp, vp, i32, i64, i32, i32, i32, vp, sz, vp]
+  lib.mtx_control_logits.restype = i32
+  lib.mtx_control_logits.argtypes = [vp, i64, vp, i64, i32, i32, c.POINTER(LogitControls), vp]
+  lib.mtx_note_tokens.restype = i32
+  lib.mtx_note_tokens.argtypes = [vp, i64, vp, i64, i32, i32, vp, vp, i32, i32, vp]
   lib.mtx_engine_rebind_state.restype = i32
   lib.mtx_engine_rebind_state.argtypes = [vp, c.POINTER(DecodeState)]
 
