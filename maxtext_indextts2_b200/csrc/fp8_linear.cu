@@ -38,9 +38,123 @@ int quantize(const void* x, int x_type, long long ldx, int rows, int k, int bloc
   return x_type == MTX_BF16 ? launch_quantize<bf16>(p, block_rows, st) : launch_quantize<float>(p, block_rows, st);
 }
 
-// what a linear keeps of its quantised activations in the caller's scratch: the values at a pitch of whole 16 bytes, then a row's scales side by side
+// what a linear keeps of its quantised activations in the caller's scratch: the values at a pitch of whole 16 bytes, then a block's scales side by side
 size_t scratch_pitch(int k) { return align_up(size_t(k), 16); }
 size_t scratch_scales_at(int rows, int k) { return align_up(size_t(rows) * scratch_pitch(k), 256); }
+
+// 8-bit rows [rows, k] in boxes of `box_rows` rows x 128 columns with the 128-byte swizzle; columns behind k and rows behind the last read as zeros
+int make_map_e4m3(CUtensorMap* m, const void* base, long long k, long long rows, long long ld, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return fail(MTX_ERR_CUDA, "cuTensorMapEncodeTiled is not available (no CUDA driver?)");
+  const cuuint64_t dims[2] = {cuuint64_t(k), cuuint64_t(rows)}, strides[1] = {cuuint64_t(ld)};
+  const cuuint32_t box[2] = {kScaleBlock, box_rows}, estr[2] = {1, 1};
+  CUresult rc = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(MTX_ERR_CUDA, "cuTensorMapEncodeTiled (e4m3) failed with CUresult %d", int(rc));
+  return MTX_OK;
+}
+
+// a result [rows, n] in boxes of 32 rows x 128 bytes
+int make_map_result(CUtensorMap* m, void* base, bool f32, long long n, long long rows, long long ld) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return fail(MTX_ERR_CUDA, "cuTensorMapEncodeTiled is not available (no CUDA driver?)");
+  const cuuint64_t dims[2] = {cuuint64_t(n), cuuint64_t(rows)}, strides[1] = {cuuint64_t(ld) * (f32 ? 4 : 2)};
+  const cuuint32_t box[2] = {f32 ? 32u : 64u, 32}, estr[2] = {1, 1};
+  CUresult rc = fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(MTX_ERR_CUDA, "cuTensorMapEncodeTiled (result) failed with CUresult %d", int(rc));
+  return MTX_OK;
+}
+
+constexpr int kSms = 148;
+
+// a kernel's opt-in to more shared memory, once per device
+template <class Kernel>
+int allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int device;
+  MTX_CUDA(cudaGetDevice(&device));
+  const uint64_t bit = 1ull << (device & 63);
+  if ((done.load(std::memory_order_relaxed) & bit) == 0) {
+    MTX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return MTX_OK;
+}
+
+struct Fp8Call {
+  Fp8LinearParams p;
+  const void* x;
+  long long ldx;
+  const void* w;
+  long long ldw;
+  int k;
+};
+
+template <int BN>
+int launch_stream(const Fp8Call& c, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int kPerSm = BN <= 32 ? 3 : BN == 64 ? 2 : 1;  // CTAs that share an SM (registers: BN sums per thread)
+  constexpr int kStages = BN == 16 ? 4 : BN == 32 ? 3 : BN == 64 ? 4 : 6;
+  Fp8LinearParams p = c.p;
+  const long long tiles = (long long)((p.n + 127) / 128) * ((p.rows + BN - 1) / BN);
+  if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
+  // blocks that the busiest SM takes in, and a cluster's exchange
+  int splits = 1;
+  long long best = 1ll << 62;
+  for (int s = 1; s <= 8 && s <= p.blocks; ++s) {
+    const long long cost = (tiles * s + kSms - 1) / kSms * ((p.blocks + s - 1) / s) + (s > 1 ? 2 : 0);
+    if (cost < best) best = cost, splits = s;
+    if (tiles > 4 * kSms) break;
+  }
+  if (env_int("MTX_FP8_SPLITS", 0) > 0) splits = env_int("MTX_FP8_SPLITS", 0) < p.blocks ? env_int("MTX_FP8_SPLITS", 0) : p.blocks;
+  p.splits = splits;
+  p.stages = kStages;
+  const size_t smem = fp8_stream_smem_bytes<BN>(p.stages);
+  MTX_TRY(allow_smem(fp8_stream_kernel<BN>, smem, done));
+  CUtensorMap tw, tx;
+  MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, 128));
+  MTX_TRY(make_map_e4m3(&tx, c.x, c.k, p.rows, c.ldx, BN));
+  const dim3 grid(unsigned(splits > 1 || tiles < kSms * kPerSm ? tiles : kSms * kPerSm), unsigned(splits));
+  g_cluster_y = splits;
+  const int rc = launch(fp8_stream_kernel<BN>, grid, dim3(64 + 32 * fp8_stream_warps<BN>()), smem, st, tw, tx, p);
+  g_cluster_y = 1;
+  return rc;
+}
+
+template <int BN, class OUT>
+int launch_pair(const Fp8Call& c, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  Fp8LinearParams p = c.p;
+  const long long tiles = (long long)((p.rows + kFp8PairRows - 1) / kFp8PairRows) * ((p.n + BN - 1) / BN);
+  if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
+  p.stages = fp8_pair_stages<BN>();
+  p.tma_store = fits16(p.out, p.ldo * (long long)sizeof(OUT));
+  const size_t smem = fp8_pair_smem_bytes<BN>(p.stages);
+  MTX_TRY(allow_smem(fp8_pair_kernel<BN, OUT>, smem, done));
+  CUtensorMap tw, tx, to;
+  MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, BN / 2));
+  MTX_TRY(make_map_e4m3(&tx, c.x, c.k, p.rows, c.ldx, 128));
+  if (p.tma_store) MTX_TRY(make_map_result(&to, p.out, p.out_f32, p.n, p.rows, p.ldo));
+  else to = tx;  // (not read)
+  const unsigned pairs = unsigned(tiles < kSms / 2 ? tiles : kSms / 2);
+  g_cluster_x = 2;
+  const int rc = launch(fp8_pair_kernel<BN, OUT>, dim3(2 * pairs), dim3(fp8_pair_threads<BN>()), smem, st, tw, tx, to, p);
+  g_cluster_x = 1;
+  return rc;
+}
+
+int launch_linear(const Fp8Call& c, cudaStream_t st) {
+  const int rows = c.p.rows;
+  const int form = env_int("MTX_FP8_FORM", 0);
+  if (form == 1 || (form == 0 && rows <= 128)) {
+    if (rows <= 16) return launch_stream<16>(c, st);
+    if (rows <= 32) return launch_stream<32>(c, st);
+    if (rows <= 64) return launch_stream<64>(c, st);
+    return launch_stream<128>(c, st);
+  }
+  if (form == 128) return c.p.out_f32 ? launch_pair<128, float>(c, st) : launch_pair<128, bf16>(c, st);
+  return c.p.out_f32 ? launch_pair<256, float>(c, st) : launch_pair<256, bf16>(c, st);
+}
 
 }  // namespace
 
@@ -77,31 +191,35 @@ int mtx_linear_fp8(const void* x, int x_type, long long ldx, const float* x_scal
     return fail(MTX_ERR_ARG, "values that are quantised here need a 16-byte aligned scratch of mtx_linear_fp8_scratch_bytes(rows, k) bytes");
   MTX_TRY(on_this_device({x, quantised ? x_scale : static_cast<const void*>(scratch), wq, w_scale, out}));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  Fp8LinearParams p;
-  p.x = static_cast<const uint8_t*>(x);
-  p.ldx = ldx;
-  p.x_scale = x_scale;
-  p.blocks = blocks_of(k);
-  p.x_scale_row = p.blocks;
-  p.x_scale_block = 1;
+  Fp8Call c;
+  memset(&c, 0, sizeof(c));
+  c.x = x;
+  c.ldx = ldx;
+  c.w = wq;
+  c.ldw = ldw;
+  c.k = k;
+  c.p.x_scale = x_scale;
+  c.p.blocks = blocks_of(k);
+  c.p.x_scale_row = c.p.blocks;
+  c.p.x_scale_block = 1;
   if (!quantised) {
     uint8_t* q = static_cast<uint8_t*>(scratch);
     float* scales = reinterpret_cast<float*>(q + scratch_scales_at(rows, k));
-    MTX_TRY(quantize(x, x_type, ldx, rows, k, 1, q, (long long)scratch_pitch(k), scales, p.x_scale_row, p.x_scale_block, st));
-    p.x = q;
-    p.ldx = (long long)scratch_pitch(k);
-    p.x_scale = scales;
+    c.p.x_scale_row = 1;  // (a block's scales side by side: neighbouring threads have neighbouring rows)
+    c.p.x_scale_block = rows;
+    MTX_TRY(quantize(x, x_type, ldx, rows, k, 1, q, (long long)scratch_pitch(k), scales, c.p.x_scale_row, c.p.x_scale_block, st));
+    c.x = q;
+    c.ldx = (long long)scratch_pitch(k);
+    c.p.x_scale = scales;
+    c.p.early = 1;
   }
-  p.w = static_cast<const uint8_t*>(wq);
-  p.ldw = ldw;
-  p.w_scale = w_scale;
-  p.out = out;
-  p.ldo = ldo;
-  p.out_f32 = out_type == MTX_F32;
-  p.rows = rows;
-  p.n = n;
-  p.k = k;
-  return launch(fp8_linear_kernel, dim3((n + 15) / 16, (rows + 15) / 16), dim3(256), 0, st, p);
+  c.p.w_scale = w_scale;
+  c.p.out = out;
+  c.p.ldo = ldo;
+  c.p.out_f32 = out_type == MTX_F32;
+  c.p.rows = rows;
+  c.p.n = n;
+  return launch_linear(c, st);
 }
 
 }  // extern "C"

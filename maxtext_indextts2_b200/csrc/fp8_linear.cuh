@@ -4,7 +4,7 @@
 //   product    y[m, n] = sum_b xs[m, b] ws[n / 128, b] sum_{k in block b} xq[m, k] wq[n, k]
 #pragma once
 
-#include "common.cuh"
+#include "gemm_wide.cuh"
 
 namespace mtx {
 
@@ -75,8 +75,8 @@ struct QuantParams {
 // 1 x 128: half a warp per block, eight values per thread.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const QuantParams p) {
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();  // (behind the wait: a product that starts now may read weights that an earlier kernel wrote)
   const int lane = threadIdx.x & 15;
   const uint32_t block = blockIdx.x * (kQuantThreads / 16) + (threadIdx.x >> 4), all = uint32_t(p.rows) * uint32_t(p.blocks);
   const uint32_t row = block / uint32_t(p.blocks), b = block - row * uint32_t(p.blocks);
@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const Quan
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const QuantParams p) {
   __shared__ uint32_t part[kQuantThreads / 32];
-  griddep_launch_dependents();
   griddep_wait();
+  griddep_launch_dependents();
   const int up = blockIdx.x / p.blocks, b = blockIdx.x - up * p.blocks;
   const int row0 = up * kScaleBlock + (threadIdx.x >> 4), c = b * kScaleBlock + (threadIdx.x & 15) * 8;
   float v[8][8];
@@ -127,53 +127,575 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const Qu
 }
 
 // ---- products ----------------------------------------------------------------------------------------------------------------------
+//
+// Both kernels multiply one block of 128 columns at a time on the tensor cores (kind::f8f6f4, four instructions of 32), each into an accumulator of its
+// own in TMEM, and add acc += d * (xs ws) in registers, so that the scales are applied once per block and sums are fp32 throughout.
 
 struct Fp8LinearParams {
-  const uint8_t* x;
-  long long ldx;
   const float* x_scale;
-  long long x_scale_row, x_scale_block;
-  const uint8_t* w;
-  long long ldw;
+  long long x_scale_row, x_scale_block;  // strides of a row and of a block of columns
   const float* w_scale;  // [ceil(n / 128), blocks]
   void* out;
   long long ldo;
   int out_f32;
-  int rows, n, k, blocks;
+  int rows, n, blocks;
+  int splits;       // stream: CTAs of a cluster that share a tile's blocks
+  int stages;
+  int early;        // stream: the weights may be read before the kernel in front is done (it waited for everything before itself)
+  int tma_store;    // pair: the result's base and pitch are whole 16 bytes
 };
 
-__device__ __forceinline__ float e4m3_value(uint8_t b) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)b));
-  float f;
-  asm("cvt.f32.f16 %0, %1;" : "=f"(f) : "h"((unsigned short)(h & 0xffff)));
-  return f;
+// Waits that run out (some 2 s: a protocol error) end the kernel instead of the GPU: the CTA's roles go through their loops without waiting and without
+// issuing anything, its copies get time to land, TMEM is freed, and this counter says that results are wrong.  (Everything inline and no way out of
+// the loops: a call or a break behind a wait makes the compiler guard every tcgen05 instruction against divergence.)
+__device__ unsigned int d_fp8_waits_failed = 0;
+
+__device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  do {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (clock64() - t0 > 4000000000LL) {
+      atomicAdd(&d_fp8_waits_failed, 1u);
+      *failed = 1;
+    }
+  } while (*failed == 0);
+  return false;
+}
+// after a wait that ran out: copies and MMAs in flight have a millisecond to end before the CTA's shared memory and TMEM go
+__device__ __forceinline__ void fp8_let_copies_land() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 2000000) __nanosleep(1000);
 }
 
-// a CTA per 16 x 16 outputs
-__global__ void __launch_bounds__(256) fp8_linear_kernel(const Fp8LinearParams p) {
-  __shared__ float xs[16][kScaleBlock + 1], ws[16][kScaleBlock + 1];
-  griddep_launch_dependents();
-  griddep_wait();
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
-  const int m = m0 + ty, n = n0 + tx;
-  float acc = 0.0f;
-  for (int b = 0; b < p.blocks; ++b) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * kScaleBlock; i += 256) {
-      const int r = i / kScaleBlock, c = i % kScaleBlock, k = b * kScaleBlock + c;
-      xs[r][c] = m0 + r < p.rows && k < p.k ? e4m3_value(p.x[(m0 + r) * p.ldx + k]) : 0.0f;
-      ws[r][c] = n0 + r < p.n && k < p.k ? e4m3_value(p.w[(n0 + r) * p.ldw + k]) : 0.0f;
+// Instruction descriptor, kind::f8f6f4: A = B = e4m3 (format 0), D = fp32, both operands K-major.
+__host__ __device__ inline uint32_t umma_idesc_e4m3(int M, int N) { return 1u << 4 | uint32_t(N >> 3) << 17 | uint32_t(M >> 4) << 24; }
+
+__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void fma_pair(unsigned long long& acc, unsigned long long d, unsigned long long s) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(d), "l"(s));
+}
+__device__ __forceinline__ unsigned long long pair_of(uint32_t lo, uint32_t hi) { return (unsigned long long)hi << 32 | lo; }
+__device__ __forceinline__ unsigned long long pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float pair_lo(unsigned long long v) { return __uint_as_float(uint32_t(v)); }
+__device__ __forceinline__ float pair_hi(unsigned long long v) { return __uint_as_float(uint32_t(v >> 32)); }
+
+// Hands an accumulator back to the thread that issues MMAs.  The loads from TMEM are complete (wait::ld) and ordered (tcgen05.fence), nothing else is published:
+// a releasing arrive would wait for the next block's scales, which are on their way from L2 at that moment.
+__device__ __forceinline__ void fp8_release(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fp8_release_leader(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(smem_u32(bar) & kPairLeaderMask) : "memory");
+}
+
+// f(c, v) for 16 accumulator columns c .. at a time; the next ones are on their way meanwhile.  done() behind the last load.
+template <int COLS, class F, class D>
+__device__ __forceinline__ void fp8_columns(uint32_t taddr, F&& f, D&& done) {
+  uint32_t v[2][16];
+  tmem_ld_x16_issue(taddr, v[0]);
+#pragma unroll
+  for (int c = 0; c < COLS; c += 16) {
+    tmem_ld_wait();
+    if (c + 16 < COLS) tmem_ld_x16_issue(taddr + uint32_t(c + 16), v[(c / 16 + 1) & 1]);
+    else done();
+    f(c, v[(c / 16) & 1]);
+  }
+}
+
+// A thread's scales of the next blocks, on their way to its own words of shared memory three blocks ahead: loads into registers one block ahead had not arrived
+// when the block's MMAs were done (a round through L2 takes as long as two blocks), and the sums waited for them.
+constexpr int kFp8Ahead = 3;
+__device__ __forceinline__ void fp8_bring(float* to, const float* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void fp8_bring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void fp8_bring_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kFp8Ahead) : "memory"); }
+
+constexpr int kFp8OperandBytes = 128 * kScaleBlock;  // 128 rows of one block
+constexpr int kFp8MaxStages = 16;
+
+struct Fp8SmemTail {
+  uint64_t full[kFp8MaxStages];  // a stage's operands are there
+  uint64_t done[kFp8MaxStages];  // its MMAs are done: the stage may be filled again, and the block's accumulator is complete (one commit for both)
+  uint64_t tmem_empty[4];        // the epilogue has taken an accumulator in
+  uint32_t tmem_base;
+  int failed;
+};
+
+// ---- few rows: the weights as they stream by ------------------------------------------------------------------------------------------
+//
+// The 128 rows of a weight tile are the MMA's M, BN activation rows its N: nothing is padded but the last few rows, and a CTA takes in 16 KB of weights
+// with BN * 128 bytes of activations per block.  An epilogue thread owns a weight row and BN sums.  Bound: the weights' bytes.
+// Few tiles are shared by the CTAs of a cluster, each with a part of the blocks, and the parts are added over distributed shared memory in
+// the order of the blocks (so that a result never depends on timing).
+
+template <int BN>
+__host__ __device__ constexpr int fp8_stream_warps() { return BN <= 32 ? 4 : BN / 8; }  // epilogue warps: 16 or 32 activation rows each
+template <int BN>
+__host__ __device__ constexpr int fp8_stream_buffers() { return BN <= 64 && BN != 32 ? 4 : 2; }  // accumulators in TMEM: two or more CTAs share an SM's 512 columns
+template <int BN>
+__host__ __device__ constexpr int fp8_stream_stage_bytes() { return kFp8OperandBytes + BN * kScaleBlock; }
+template <int BN>
+constexpr size_t fp8_stream_smem_bytes(int stages) {
+  return 1024 + size_t(stages) * fp8_stream_stage_bytes<BN>() + 4 * 2 * BN * sizeof(float) + fp8_stream_warps<BN>() * (kFp8Ahead + 1) * 64 * sizeof(float) + sizeof(Fp8SmemTail) + 16;
+}
+
+template <int BN>
+__global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                                                                                      const Fp8LinearParams p) {
+  constexpr int NB = fp8_stream_buffers<BN>(), kStage = fp8_stream_stage_bytes<BN>(), kTmemCols = NB * BN, kWarps = fp8_stream_warps<BN>(), kCols = BN * 4 / kWarps;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* factors = reinterpret_cast<float*>(smem + size_t(p.stages) * kStage);  // [warps][2][kCols]
+  float* scales = factors + kWarps * 2 * kCols;                                  // [warps][ahead][row's, weights'][lanes]
+  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(scales + kWarps * (kFp8Ahead + 1) * 64);
+  volatile int* failed = &tail->failed;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.y;
+  const int b0 = int((long long)part * p.blocks / p.splits), b1 = int((long long)(part + 1) * p.blocks / p.splits), per = b1 - b0;
+  const int tiles_n = (p.n + 127) / 128, tiles = tiles_n * ((p.rows + BN - 1) / BN);
+  const int mine = int(blockIdx.x) < tiles ? (tiles - 1 - int(blockIdx.x)) / int(gridDim.x) + 1 : 0, F = mine * per;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_x);
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&tail->full[s], 1);
+      mbar_init(&tail->done[s], 1);
     }
-    __syncthreads();
-    float part = 0.0f;
-    for (int c = 0; c < kScaleBlock; ++c) part += xs[ty][c] * ws[tx][c];
-    if (m < p.rows && n < p.n) acc += part * (p.x_scale[m * p.x_scale_row + b * p.x_scale_block] * p.w_scale[(n / kScaleBlock) * (long long)p.blocks + b]);
+    for (int b = 0; b < NB; ++b) mbar_init(&tail->tmem_empty[b], kWarps);
+    tail->failed = 0;
+    fence_barrier_init();
   }
-  if (m < p.rows && n < p.n) {
-    if (p.out_f32) static_cast<float*>(p.out)[m * p.ldo + n] = acc;
-    else static_cast<bf16*>(p.out)[m * p.ldo + n] = __float2bfloat16_rn(acc);
+  if (warp == 1) {
+    tmem_alloc(&tail->tmem_base, kTmemCols);
+    tmem_relinquish();
   }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = tail->tmem_base;
+
+  if (warp == 0) {
+    const bool issuer = elect_one();
+    // (tile t: weight rows 128 (t % tiles_n) .., activation rows BN (t / tiles_n) ..)
+    auto load_w = [&](int s, int n0, int b) {
+      mbar_expect_tx(&tail->full[s], kStage);
+      tma_load_2d(smem + s * kStage, &tm_w, b * kScaleBlock, n0, &tail->full[s], p.rows <= BN ? kEvictFirst : kEvictNormal);
+    };
+    auto load_x = [&](int s, int r0, int b) { tma_load_2d(smem + s * kStage + kFp8OperandBytes, &tm_x, b * kScaleBlock, r0, &tail->full[s], kEvictLast); };
+    const int pre = p.early ? min(F, p.stages) : 0;
+    int s = 0, b = b0, t = blockIdx.x;
+    if (issuer)
+      for (int f = 0; f < pre; ++f) {
+        load_w(f, t % tiles_n * 128, b);
+        if (++b == b1) b = b0, t += gridDim.x;
+      }
+    griddep_wait();
+    b = b0;
+    t = blockIdx.x;
+    int n0 = t % tiles_n * 128, r0 = t / tiles_n * BN;
+    uint32_t phase = 1;
+    bool good = true;
+    for (int f = 0; f < F; ++f) {
+      if (f >= p.stages) good &= fp8_wait(&tail->done[s], phase, failed);
+      if (issuer && good) {
+        if (f >= pre) load_w(s, n0, b);
+        load_x(s, r0, b);
+      }
+      if (++s == p.stages) s = 0, phase ^= 1;
+      if (++b == b1) {
+        b = b0;
+        t += gridDim.x;
+        n0 = t % tiles_n * 128;
+        r0 = t / tiles_n * BN;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    const bool issuer = elect_one();
+    const uint32_t idesc = umma_idesc_e4m3(128, BN);
+    int s = 0, buf = 0;
+    uint32_t phase = 0, acc_phase = 1;
+    bool good = true;
+    for (int f = 0; f < F; ++f) {
+      good &= fp8_wait(&tail->full[s], phase, failed);
+      good &= fp8_wait(&tail->tmem_empty[buf], acc_phase, failed);
+      tcgen05_fence_after();
+      if (issuer && good) {
+        const uint64_t dw = umma_desc_sw128(smem + s * kStage), dx = umma_desc_sw128(smem + s * kStage + kFp8OperandBytes);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) umma_e4m3(tmem_base + uint32_t(buf * BN), dw + 2 * kk, dx + 2 * kk, idesc, kk != 0);
+        umma_commit(&tail->done[s]);
+      }
+      if (++s == p.stages) s = 0, phase ^= 1;
+      if (++buf == NB) buf = 0, acc_phase ^= 1;
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, local = quarter * 32 + lane, c0 = (warp - 2) / 4 * kCols;  // this thread's weight row, and the first of its activation rows
+    float* factor = factors + (warp - 2) * 2 * kCols;
+    const uint32_t lanes = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(c0);
+    static_assert(kCols <= 32, "a lane brings the scale of one activation row");
+    griddep_wait();  // (scales and activations of the kernel in front)
+    int t = blockIdx.x, b = b0, s = 0, buf = 0;
+    uint32_t phase = 0;
+    // the tile's weight rows share a scale; a lane brings that and the one of an activation row (behind the last they are not stored: any scale will do)
+    float* const my_scales = scales + (warp - 2) * (kFp8Ahead + 1) * 64 + lane;
+    const float *next_x = p.x_scale, *next_w = p.w_scale;
+    int ahead_f = 0, ahead_b = b0, ahead_t = blockIdx.x;
+    auto bring = [&]() {
+      if (ahead_f < F) {
+        if (ahead_b == b0) {
+          const int rt = ahead_t / tiles_n;
+          next_x = p.x_scale + min(rt * BN + c0 + (lane & (kCols - 1)), p.rows - 1) * p.x_scale_row + b0 * p.x_scale_block;
+          next_w = p.w_scale + (ahead_t - rt * tiles_n) * (long long)p.blocks + b0;
+        }
+        float* to = my_scales + (ahead_f & kFp8Ahead) * 64;
+        fp8_bring(to, next_x);
+        fp8_bring(to + 32, next_w);
+        next_x += p.x_scale_block;
+        ++next_w;
+        ++ahead_f;
+        if (++ahead_b == b1) ahead_b = b0, ahead_t += gridDim.x;
+      }
+      fp8_bring_commit();
+    };
+    for (int i = 0; i < kFp8Ahead; ++i) bring();
+    unsigned long long acc[kCols / 2];
+    for (int f = 0; f < F; ++f) {
+      if (b == b0) {
+#pragma unroll
+        for (int c = 0; c < kCols / 2; ++c) acc[c] = 0;
+      }
+      float* now = factor + (f & 1) * kCols;
+      const bool last = b + 1 == b1;
+      bring();
+      fp8_bring_wait();
+      const float* mine_s = my_scales + (f & kFp8Ahead) * 64;
+      now[lane & (kCols - 1)] = mine_s[0] * mine_s[32];
+      __syncwarp();
+      fp8_wait(&tail->done[s], phase, failed);
+      tcgen05_fence_after();
+      fp8_columns<kCols>(
+          lanes + uint32_t(buf * BN),
+          [&](int c, const uint32_t(&v)[16]) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const float4 by = *reinterpret_cast<const float4*>(now + c + i);
+              fma_pair(acc[(c + i) / 2], pair_of(v[i], v[i + 1]), pair_of(by.x, by.y));
+              fma_pair(acc[(c + i) / 2 + 1], pair_of(v[i + 2], v[i + 3]), pair_of(by.z, by.w));
+            }
+          },
+          [&]() {
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) fp8_release(&tail->tmem_empty[buf]);
+          });
+      if (++s == p.stages) s = 0, phase ^= 1;
+      if (++buf == NB) buf = 0;
+      ++b;
+      if (last && p.splits == 1) {
+        const int n = t % tiles_n * 128 + local, row0 = t / tiles_n * BN + c0, left = p.rows - row0;
+        if (n < p.n) {
+          if (p.out_f32) {
+            float* o = static_cast<float*>(p.out) + row0 * p.ldo + n;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              if (c < left) __stcs(o, c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]));
+              o += p.ldo;
+            }
+          } else {
+            bf16* o = static_cast<bf16*>(p.out) + row0 * p.ldo + n;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              if (c < left) *o = __float2bfloat16_rn(c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]));
+              o += p.ldo;
+            }
+          }
+        }
+        b = b0;
+        t += gridDim.x;
+      }
+    }
+    if (p.splits > 1 && F > 0) {  // (one tile per CTA) the parts lie where the operands were: the last MMA has read them
+      float* parts = reinterpret_cast<float*>(smem) + c0 * 128 + local;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) parts[c * 128] = c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]);
+    }
+    __syncwarp();
+  }
+  if (*failed) fp8_let_copies_land();
+  if (p.splits > 1) {
+    cluster_sync_all();
+    if (warp >= 2) {
+      const int local = (warp & 3) * 32 + lane, t = blockIdx.x, n = t % tiles_n * 128 + local, row0 = t / tiles_n * BN, left = min(BN, p.rows - row0);
+      const uint32_t own = smem_u32(smem) + local * 4;
+      if (n < p.n) {
+        for (int c = part + (warp - 2) / 4 * p.splits; c < left; c += p.splits * (kWarps / 4)) {
+          float sum = 0.0f;
+          for (int q = 0; q < p.splits; ++q) sum += ld_dsmem_f32(dsmem_addr(own + c * 512, q));
+          if (p.out_f32) static_cast<float*>(p.out)[(row0 + c) * p.ldo + n] = sum;
+          else static_cast<bf16*>(p.out)[(row0 + c) * p.ldo + n] = __float2bfloat16_rn(sum);
+        }
+      }
+      __syncwarp();
+    }
+    cluster_sync_all();  // the parts are read from the other CTAs until here
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, kTmemCols);
+}
+
+// ---- many rows: pairs of CTAs ------------------------------------------------------------------------------------------------------------
+//
+// Two CTAs of a cluster (a TPC's two SMs) work on one tile of 256 rows x BN columns with cta_group::2 MMAs: CTA c of the pair holds rows 128 c .. of the
+// activations and half of the weight tile, so an SM takes in 16 KB + BN * 64 bytes per block for BN * 2^15 multiply-adds.  A thread of the
+// epilogue warps owns one row and 64 of the columns: its scale of a block is ONE number, which the sums take in with packed fused
+// multiply-adds while the next block's MMAs run into another accumulator.
+
+constexpr int kFp8PairRows = 256;
+
+// Epilogue warps: 32 rows x half of the columns each.  (Sixteen with a quarter of the columns take longer, 540 us for 420 at 4096 x 5376 x 21504: every
+// arrival at the leader's barrier is on the way from one block's sums to the next MMAs into their accumulator.  So did registers moved from the
+// first warps to these: 480 us.)
+template <int BN>
+__host__ __device__ constexpr int fp8_pair_warps() { return 8; }
+// warp 0: copies, warp 1: MMAs, then the sums
+template <int BN>
+__host__ __device__ constexpr int fp8_pair_threads() { return 64 + 32 * fp8_pair_warps<BN>(); }
+template <int BN>
+constexpr int fp8_pair_staged() { return fp8_pair_warps<BN>() * 4096; }  // 32 rows x 128 bytes per epilogue warp
+
+template <int BN>
+__host__ __device__ constexpr int fp8_pair_stage_bytes() { return kFp8OperandBytes + BN / 2 * kScaleBlock; }
+template <int BN>
+constexpr size_t fp8_pair_smem_bytes(int stages) {
+  return 1024 + size_t(stages) * fp8_pair_stage_bytes<BN>() + fp8_pair_staged<BN>() + sizeof(Fp8SmemTail) + 16;
+}
+template <int BN>
+constexpr int fp8_pair_stages() {
+  const int n = int((227 * 1024 - fp8_pair_smem_bytes<BN>(0)) / fp8_pair_stage_bytes<BN>());
+  return n < kFp8MaxStages ? n : kFp8MaxStages;
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(src)), "r"(c0), "r"(c1) : "memory");
+}
+
+template <int BN, class OUT>
+__global__ void __launch_bounds__(fp8_pair_threads<BN>(), 1)
+fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out, const Fp8LinearParams p) {
+  constexpr int kStage = fp8_pair_stage_bytes<BN>(), NB = 512 / BN > 4 ? 4 : 512 / BN, kHalf = BN / 2, kWarps = fp8_pair_warps<BN>(), kCols = BN * 4 / kWarps, kBox = 128 / int(sizeof(OUT));
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* staged = smem + size_t(p.stages) * kStage;
+  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(staged + kWarps * 4096);
+  volatile int* failed = &tail->failed;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(blockIdx.x) & 1, pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
+  const int m_tiles = (p.rows + kFp8PairRows - 1) / kFp8PairRows, tiles = m_tiles * ((p.n + BN - 1) / BN);
+  const int mine = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0, F = mine * p.blocks;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_out);
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&tail->full[s], 1);
+      mbar_init(&tail->done[s], 1);
+    }
+    for (int b = 0; b < NB; ++b) mbar_init(&tail->tmem_empty[b], 2 * kWarps);  // the epilogue warps of both CTAs
+    tail->failed = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&tail->tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  tcgen05_fence_before();
+  cluster_sync_all();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = tail->tmem_base;
+  griddep_wait();
+
+  if (warp >= 2) {
+    const int c0 = (warp - 2) / 4 * kCols, quarter = warp & 3;
+    uint8_t* stage = staged + (warp - 2) * 4096;
+    const uint32_t lanes = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(c0);
+    int t = pair, s = 0, buf = 0;
+    uint32_t phase = 0;
+    // This thread's scales, of its row and of its columns, come two blocks ahead (a round through L2 takes as long as the MMAs of two); rows and columns behind
+    // the last are not stored: any scale will do.
+    const float *next_x = p.x_scale, *next_w = p.w_scale;
+    float xs[2], ws[2];
+    auto fetch = [&](int i) {
+      xs[i] = __ldg(next_x);
+      ws[i] = __ldg(next_w);
+      next_x += p.x_scale_block;
+      ++next_w;
+    };
+    auto begin = [&](int tt) {
+      const int nt = tt / m_tiles, r = (tt - nt * m_tiles) * kFp8PairRows + rank * 128 + quarter * 32 + lane, c = nt * BN + c0;
+      next_x = p.x_scale + min(r, p.rows - 1) * p.x_scale_row;
+      next_w = p.w_scale + min(c, p.n - 1) / kScaleBlock * (long long)p.blocks;
+      fetch(0);
+      if (p.blocks > 1) fetch(1);
+    };
+    if (mine > 0) begin(t);
+    unsigned long long acc[kCols / 2];
+    auto step = [&](int b, int i) {
+      fp8_wait(&tail->done[s], phase, failed);
+      tcgen05_fence_after();
+      float scale;  // (volatile: multiplied here, not right behind the loads)
+      asm volatile("mul.rn.f32 %0, %1, %2;" : "=f"(scale) : "f"(xs[i]), "f"(ws[i]));
+      if (b + 2 < p.blocks) fetch(i);
+      const unsigned long long by = pair_of(scale, scale);
+      fp8_columns<kCols>(
+          lanes + uint32_t(buf * BN),
+          [&](int c, const uint32_t(&v)[16]) {
+#pragma unroll
+            for (int x = 0; x < 16; x += 2) fma_pair(acc[(c + x) / 2], pair_of(v[x], v[x + 1]), by);
+          },
+          [&]() {
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) fp8_release_leader(&tail->tmem_empty[buf]);
+          });
+      if (++s == p.stages) s = 0, phase ^= 1;
+      if (++buf == NB) buf = 0;
+    };
+    for (int j = 0; j < mine; ++j, t += pairs) {
+#pragma unroll
+      for (int c = 0; c < kCols / 2; ++c) acc[c] = 0;
+      for (int b = 0; b < p.blocks; b += 2) {
+        step(b, 0);
+        if (b + 1 < p.blocks) step(b + 1, 1);
+      }
+      if (j + 1 < mine) begin(t + pairs);
+      {
+        // 32 rows x 128 bytes at a time through shared memory (chunk j of row r at j ^ (r & 7): the 128-byte swizzle of the tensor map)
+        const int row0 = t % m_tiles * kFp8PairRows + rank * 128 + quarter * 32, col0 = t / m_tiles * BN + c0;
+#pragma unroll
+        for (int c = 0; c < kCols; c += kBox) {
+          if (col0 + c < p.n && row0 < p.rows) {
+            uint8_t* to = stage;
+            if (p.tma_store) {
+              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the buffer's last store has been read
+              __syncwarp();
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint4 u;
+              if (sizeof(OUT) == 2) {
+                const unsigned long long* a = acc + (c + 8 * j) / 2;
+                u = make_uint4(pack_bf16x2(pair_lo(a[0]), pair_hi(a[0])), pack_bf16x2(pair_lo(a[1]), pair_hi(a[1])), pack_bf16x2(pair_lo(a[2]), pair_hi(a[2])),
+                               pack_bf16x2(pair_lo(a[3]), pair_hi(a[3])));
+              } else {
+                const unsigned long long* a = acc + (c + 4 * j) / 2;
+                u = make_uint4(uint32_t(a[0]), uint32_t(a[0] >> 32), uint32_t(a[1]), uint32_t(a[1] >> 32));
+              }
+              *reinterpret_cast<uint4*>(to + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
+            }
+            if (p.tma_store) {
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&tm_out, to, col0 + c, row0);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              }
+            } else {  // results at odd places: a row's values by neighbouring lanes
+              __syncwarp();
+              OUT* o = static_cast<OUT*>(p.out) + row0 * p.ldo + col0 + c;
+              const int rows = min(32, p.rows - row0), cols = min(kBox, p.n - col0 - c);
+              for (int r = 0; r < rows; ++r, o += p.ldo)
+                for (int i = lane; i < cols; i += 32) o[i] = *reinterpret_cast<const OUT*>(to + r * 128 + (((i / (kBox / 8)) ^ (r & 7)) << 4) + i % (kBox / 8) * sizeof(OUT));
+              __syncwarp();
+            }
+          }
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  } else {
+    if (warp == 0) {
+      const bool issuer = elect_one();
+      int s = 0, b = 0, t = pair;
+      uint32_t phase = 1;
+      bool good = true;
+      for (int f = 0; f < F; ++f) {
+        if (f >= p.stages) good &= fp8_wait(&tail->done[s], phase, failed);
+        if (issuer && good) {
+          if (rank == 0) mbar_expect_tx(&tail->full[s], 2 * kStage);
+          tma_load_2d_pair(smem + s * kStage, &tm_x, b * kScaleBlock, t % m_tiles * kFp8PairRows + rank * 128, &tail->full[s], kEvictLast);
+          tma_load_2d_pair(smem + s * kStage + kFp8OperandBytes, &tm_w, b * kScaleBlock, t / m_tiles * BN + rank * kHalf, &tail->full[s], kEvictNormal);
+        }
+        if (++s == p.stages) s = 0, phase ^= 1;
+        if (++b == p.blocks) b = 0, t += pairs;
+      }
+      // the commits of the last stages arrive on this CTA's barriers too: they have to be there before it may leave
+      const int last = min(F, p.stages);
+      for (int f = 0; f < last; ++f) {
+        if (s == 0) s = p.stages, phase ^= 1;
+        --s;
+        fp8_wait(&tail->done[s], phase ^ 1, failed);
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      if (rank == 0) {
+        const bool issuer = elect_one();
+        const uint32_t idesc = umma_idesc_e4m3(kFp8PairRows, BN);
+        const uint64_t d0 = umma_desc_sw128(smem);
+        const uint32_t desc_hi = uint32_t(d0 >> 32), desc_lo = uint32_t(d0);  // (the low words alone count on)
+        int s = 0, buf = 0;
+        uint32_t phase = 0, acc_phase = 1;
+        bool good = true;
+        for (int f = 0; f < F; ++f) {
+          good &= fp8_wait(&tail->full[s], phase, failed);
+          good &= fp8_wait(&tail->tmem_empty[buf], acc_phase, failed);
+          tcgen05_fence_after();
+          if (issuer && good) {
+            const uint32_t at = desc_lo + uint32_t(s) * (kStage >> 4);
+  #pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_e4m3_pair(tmem_base + uint32_t(buf * BN), umma_desc_of(at + kk * 2, desc_hi), umma_desc_of(at + (kFp8OperandBytes >> 4) + kk * 2, desc_hi), idesc, kk != 0);
+            umma_commit_pair(&tail->done[s]);
+          }
+          if (++s == p.stages) s = 0, phase ^= 1;
+          if (++buf == NB) buf = 0, acc_phase ^= 1;
+        }
+      }
+      __syncwarp();
+    }
+  }
+  if (*failed) fp8_let_copies_land();
+  tcgen05_fence_before();
+  cluster_sync_all();  // the pair's shared memory and TMEM are in use until both CTAs are done
+  tcgen05_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
 }
 
 }  // namespace mtx
