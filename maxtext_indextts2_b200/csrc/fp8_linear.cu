@@ -91,31 +91,65 @@ struct Fp8Call {
 };
 
 template <int BN>
+constexpr int fp8_stream_most_stages() {
+  constexpr int n = 200 * 1024 / fp8_stream_stage_bytes<BN>();
+  return n < kFp8MaxStages ? n : kFp8MaxStages;
+}
+
+// Parts of the sum that CTAs of a cluster share: as many as leave every CTA an SM to itself, all clusters at once (a cluster lies in one GPC, so that fewer
+// large ones fit than SMs).  64 rows of 5120 by 1280 columns: 16.9 us in one part, 8.8 in four, 7.8 in eight; 128 rows of 10240 by 2560 columns (20
+// tiles): 14.6 in six, 24.0 in eight, whose clusters take turns.  More tiles than SMs: one part (64 x 2560 by 10240, 80 tiles: 11.3 us, 12.6 in two).
+template <int BN>
+int stream_splits(long long tiles, int blocks) {
+  static std::atomic<int> fit[kFp8MaxSplits + 1];  // clusters of that many CTAs that run at once; 0: not asked yet
+  const size_t smem = fp8_stream_smem_bytes<BN>(fp8_stream_most_stages<BN>());
+  for (int s = kFp8MaxSplits; s > 1; --s) {
+    if (s > blocks || tiles * s > kSms) continue;
+    int n = fit[s].load(std::memory_order_relaxed);
+    if (n == 0) {
+      cudaLaunchConfig_t cfg;
+      memset(&cfg, 0, sizeof(cfg));
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = 1;
+      attr.val.clusterDim.y = unsigned(s);
+      attr.val.clusterDim.z = 1;
+      cfg.gridDim = dim3(kSms / s, s);
+      cfg.blockDim = dim3(64 + 32 * fp8_stream_warps<BN>());
+      cfg.dynamicSmemBytes = smem;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, fp8_stream_kernel<BN>, &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        n = 1;
+      }
+      fit[s].store(n, std::memory_order_relaxed);
+    }
+    if (tiles <= n) return s;
+  }
+  return 1;
+}
+
+template <int BN>
 int launch_stream(const Fp8Call& c, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  constexpr int kPerSm = BN <= 32 ? 3 : BN == 64 ? 2 : 1;  // CTAs that share an SM (registers: BN sums per thread)
-  constexpr int kStages = BN == 16 ? 4 : BN == 32 ? 3 : BN == 64 ? 4 : 6;
+  constexpr int kPerSm = BN <= 32 ? 3 : BN == 64 ? 2 : 1;  // CTAs that may share an SM
+  constexpr int kLeast = BN == 16 ? 4 : BN == 32 ? 3 : BN == 64 ? 4 : 6;
   Fp8LinearParams p = c.p;
   const long long tiles = (long long)((p.n + 127) / 128) * ((p.rows + BN - 1) / BN);
   if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
-  // blocks that the busiest SM takes in, and a cluster's exchange
-  int splits = 1;
-  long long best = 1ll << 62;
-  for (int s = 1; s <= 8 && s <= p.blocks; ++s) {
-    const long long cost = (tiles * s + kSms - 1) / kSms * ((p.blocks + s - 1) / s) + (s > 1 ? 2 : 0);
-    if (cost < best) best = cost, splits = s;
-    if (tiles > 4 * kSms) break;
-  }
-  if (env_int("MTX_FP8_SPLITS", 0) > 0) splits = env_int("MTX_FP8_SPLITS", 0) < p.blocks ? env_int("MTX_FP8_SPLITS", 0) : p.blocks;
-  p.splits = splits;
-  p.stages = kStages;
+  MTX_TRY(allow_smem(fp8_stream_kernel<BN>, fp8_stream_smem_bytes<BN>(fp8_stream_most_stages<BN>()), done));
+  p.splits = stream_splits<BN>(tiles, p.blocks);
+  // an SM's shared memory in stages, whether one CTA has it or several: 64 KB in flight are too few for a CTA alone (16 x 2560 by 10240, 80 CTAs: 11.1 us, 8.8 with all)
+  const long long per_sm = (tiles * p.splits + kSms - 1) / kSms;
+  p.stages = per_sm >= kPerSm ? kLeast : kLeast * kPerSm / int(per_sm);
+  if (p.stages > fp8_stream_most_stages<BN>()) p.stages = fp8_stream_most_stages<BN>();
   const size_t smem = fp8_stream_smem_bytes<BN>(p.stages);
-  MTX_TRY(allow_smem(fp8_stream_kernel<BN>, smem, done));
   CUtensorMap tw, tx;
   MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, 128));
   MTX_TRY(make_map_e4m3(&tx, c.x, c.k, p.rows, c.ldx, BN));
-  const dim3 grid(unsigned(splits > 1 || tiles < kSms * kPerSm ? tiles : kSms * kPerSm), unsigned(splits));
-  g_cluster_y = splits;
+  const dim3 grid(unsigned(p.splits > 1 || tiles < kSms * kPerSm ? tiles : kSms * kPerSm), unsigned(p.splits));
+  g_cluster_y = p.splits;
   const int rc = launch(fp8_stream_kernel<BN>, grid, dim3(64 + 32 * fp8_stream_warps<BN>()), smem, st, tw, tx, p);
   g_cluster_y = 1;
   return rc;
@@ -143,16 +177,24 @@ int launch_pair(const Fp8Call& c, cudaStream_t st) {
   return rc;
 }
 
+// Which kernel: up to 64 rows the streamed weights.  Above, each form's time as it was measured, in ns: what a call takes besides its blocks, and in every wave of
+// tiles the blocks and the tile's end.  (ns at 200 x 10240 x 2560: streamed 23.2 us measured, 25.1 by this; 128 columns 17.9 and 18.3; 256 columns 15.2 and 14.7.  512 x
+// 2560 x 10240: 42.9 and 44.8, 30.2 and 30.4, 40.4 and 39.9.  333 x 1280 x 5120: 11.8 and 12.1, 17.4 and 17.8, 23.2 and 23.1.)
 int launch_linear(const Fp8Call& c, cudaStream_t st) {
   const int rows = c.p.rows;
-  const int form = env_int("MTX_FP8_FORM", 0);
-  if (form == 1 || (form == 0 && rows <= 128)) {
-    if (rows <= 16) return launch_stream<16>(c, st);
-    if (rows <= 32) return launch_stream<32>(c, st);
-    if (rows <= 64) return launch_stream<64>(c, st);
-    return launch_stream<128>(c, st);
-  }
-  if (form == 128) return c.p.out_f32 ? launch_pair<128, float>(c, st) : launch_pair<128, bf16>(c, st);
+  if (rows <= 16) return launch_stream<16>(c, st);
+  if (rows <= 32) return launch_stream<32>(c, st);
+  if (rows <= 64) return launch_stream<64>(c, st);
+  const long long blocks = c.p.blocks, tiles128 = (long long)((rows + 127) / 128) * ((c.p.n + 127) / 128);
+  const int splits = stream_splits<128>(tiles128, c.p.blocks);
+  const long long stream = 4500 + (splits > 1 ? 2300 : 0) + (tiles128 * splits + kSms - 1) / kSms * ((blocks + splits - 1) / splits * 500 + 300);
+  auto pair = [&](int bn, long long base, long long block, long long end) {
+    const long long tiles = (long long)((rows + kFp8PairRows - 1) / kFp8PairRows) * ((c.p.n + bn - 1) / bn);
+    return base + (tiles + kSms / 2 - 1) / (kSms / 2) * (blocks * block + end);
+  };
+  const long long pair128 = pair(128, 4700, 315, 500), pair256 = pair(256, 4300, 420, 2000);
+  if (stream <= pair128 && stream <= pair256) return launch_stream<128>(c, st);
+  if (pair128 <= pair256) return c.p.out_f32 ? launch_pair<128, float>(c, st) : launch_pair<128, bf16>(c, st);
   return c.p.out_f32 ? launch_pair<256, float>(c, st) : launch_pair<256, bf16>(c, st);
 }
 

@@ -223,17 +223,9 @@ __device__ __forceinline__ void fp8_columns(uint32_t taddr, F&& f, D&& done) {
   }
 }
 
-// A thread's scales of the next blocks, on their way to its own words of shared memory three blocks ahead: loads into registers one block ahead had not arrived
-// when the block's MMAs were done (a round through L2 takes as long as two blocks), and the sums waited for them.
-constexpr int kFp8Ahead = 3;
-__device__ __forceinline__ void fp8_bring(float* to, const float* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
-}
-__device__ __forceinline__ void fp8_bring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void fp8_bring_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kFp8Ahead) : "memory"); }
-
 constexpr int kFp8OperandBytes = 128 * kScaleBlock;  // 128 rows of one block
 constexpr int kFp8MaxStages = 16;
+constexpr int kFp8MaxSplits = 8;  // CTAs of a cluster
 
 struct Fp8SmemTail {
   uint64_t full[kFp8MaxStages];  // a stage's operands are there
@@ -258,7 +250,7 @@ template <int BN>
 __host__ __device__ constexpr int fp8_stream_stage_bytes() { return kFp8OperandBytes + BN * kScaleBlock; }
 template <int BN>
 constexpr size_t fp8_stream_smem_bytes(int stages) {
-  return 1024 + size_t(stages) * fp8_stream_stage_bytes<BN>() + 4 * 2 * BN * sizeof(float) + fp8_stream_warps<BN>() * (kFp8Ahead + 1) * 64 * sizeof(float) + sizeof(Fp8SmemTail) + 16;
+  return 1024 + size_t(stages) * fp8_stream_stage_bytes<BN>() + 4 * 2 * BN * sizeof(float) + sizeof(Fp8SmemTail) + 16;
 }
 
 template <int BN>
@@ -268,8 +260,7 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* factors = reinterpret_cast<float*>(smem + size_t(p.stages) * kStage);  // [warps][2][kCols]
-  float* scales = factors + kWarps * 2 * kCols;                                  // [warps][ahead][row's, weights'][lanes]
-  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(scales + kWarps * (kFp8Ahead + 1) * 64);
+  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(factors + kWarps * 2 * kCols);
   volatile int* failed = &tail->failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.y;
   const int b0 = int((long long)part * p.blocks / p.splits), b1 = int((long long)(part + 1) * p.blocks / p.splits), per = b1 - b0;
@@ -358,42 +349,31 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
     const uint32_t lanes = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(c0);
     static_assert(kCols <= 32, "a lane brings the scale of one activation row");
     griddep_wait();  // (scales and activations of the kernel in front)
-    int t = blockIdx.x, b = b0, s = 0, buf = 0;
+    int t = blockIdx.x, s = 0, buf = 0;
     uint32_t phase = 0;
-    // the tile's weight rows share a scale; a lane brings that and the one of an activation row (behind the last they are not stored: any scale will do)
-    float* const my_scales = scales + (warp - 2) * (kFp8Ahead + 1) * 64 + lane;
+    // The tile's weight rows share a scale; a lane brings that and the one of an activation row, two blocks ahead (a round through L2 takes as long as several
+    // blocks); behind the last row they are not stored: any scale will do.
     const float *next_x = p.x_scale, *next_w = p.w_scale;
-    int ahead_f = 0, ahead_b = b0, ahead_t = blockIdx.x;
-    auto bring = [&]() {
-      if (ahead_f < F) {
-        if (ahead_b == b0) {
-          const int rt = ahead_t / tiles_n;
-          next_x = p.x_scale + min(rt * BN + c0 + (lane & (kCols - 1)), p.rows - 1) * p.x_scale_row + b0 * p.x_scale_block;
-          next_w = p.w_scale + (ahead_t - rt * tiles_n) * (long long)p.blocks + b0;
-        }
-        float* to = my_scales + (ahead_f & kFp8Ahead) * 64;
-        fp8_bring(to, next_x);
-        fp8_bring(to + 32, next_w);
-        next_x += p.x_scale_block;
-        ++next_w;
-        ++ahead_f;
-        if (++ahead_b == b1) ahead_b = b0, ahead_t += gridDim.x;
-      }
-      fp8_bring_commit();
+    float xs[2], ws[2];
+    auto fetch = [&](int i) {
+      xs[i] = __ldg(next_x);
+      ws[i] = __ldg(next_w);
+      next_x += p.x_scale_block;
+      ++next_w;
     };
-    for (int i = 0; i < kFp8Ahead; ++i) bring();
+    auto begin = [&](int tt) {
+      const int rt = tt / tiles_n;
+      next_x = p.x_scale + min(rt * BN + c0 + (lane & (kCols - 1)), p.rows - 1) * p.x_scale_row + b0 * p.x_scale_block;
+      next_w = p.w_scale + (tt - rt * tiles_n) * (long long)p.blocks + b0;
+      fetch(0);
+      if (per > 1) fetch(1);
+    };
+    if (mine > 0) begin(t);
     unsigned long long acc[kCols / 2];
-    for (int f = 0; f < F; ++f) {
-      if (b == b0) {
-#pragma unroll
-        for (int c = 0; c < kCols / 2; ++c) acc[c] = 0;
-      }
-      float* now = factor + (f & 1) * kCols;
-      const bool last = b + 1 == b1;
-      bring();
-      fp8_bring_wait();
-      const float* mine_s = my_scales + (f & kFp8Ahead) * 64;
-      now[lane & (kCols - 1)] = mine_s[0] * mine_s[32];
+    auto step = [&](int b, int i) {
+      float* now = factor + i * kCols;
+      now[lane & (kCols - 1)] = xs[i] * ws[i];
+      if (b + 2 < per) fetch(i);
       __syncwarp();
       fp8_wait(&tail->done[s], phase, failed);
       tcgen05_fence_after();
@@ -401,10 +381,10 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
           lanes + uint32_t(buf * BN),
           [&](int c, const uint32_t(&v)[16]) {
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const float4 by = *reinterpret_cast<const float4*>(now + c + i);
-              fma_pair(acc[(c + i) / 2], pair_of(v[i], v[i + 1]), pair_of(by.x, by.y));
-              fma_pair(acc[(c + i) / 2 + 1], pair_of(v[i + 2], v[i + 3]), pair_of(by.z, by.w));
+            for (int x = 0; x < 16; x += 4) {
+              const float4 by = *reinterpret_cast<const float4*>(now + c + x);
+              fma_pair(acc[(c + x) / 2], pair_of(v[x], v[x + 1]), pair_of(by.x, by.y));
+              fma_pair(acc[(c + x) / 2 + 1], pair_of(v[x + 2], v[x + 3]), pair_of(by.z, by.w));
             }
           },
           [&]() {
@@ -414,8 +394,16 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
           });
       if (++s == p.stages) s = 0, phase ^= 1;
       if (++buf == NB) buf = 0;
-      ++b;
-      if (last && p.splits == 1) {
+    };
+    for (int j = 0; j < mine; ++j, t += gridDim.x) {
+#pragma unroll
+      for (int c = 0; c < kCols / 2; ++c) acc[c] = 0;
+      for (int b = 0; b < per; b += 2) {
+        step(b, 0);
+        if (b + 1 < per) step(b + 1, 1);
+      }
+      if (j + 1 < mine) begin(t + int(gridDim.x));
+      if (p.splits == 1) {
         const int n = t % tiles_n * 128 + local, row0 = t / tiles_n * BN + c0, left = p.rows - row0;
         if (n < p.n) {
           if (p.out_f32) {
@@ -434,11 +422,9 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
             }
           }
         }
-        b = b0;
-        t += gridDim.x;
       }
     }
-    if (p.splits > 1 && F > 0) {  // (one tile per CTA) the parts lie where the operands were: the last MMA has read them
+    if (p.splits > 1 && mine > 0) {  // (one tile per CTA) the parts lie where the operands were: the last MMA has read them
       float* parts = reinterpret_cast<float*>(smem) + c0 * 128 + local;
 #pragma unroll
       for (int c = 0; c < kCols; ++c) parts[c * 128] = c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]);
@@ -448,16 +434,26 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
   if (*failed) fp8_let_copies_land();
   if (p.splits > 1) {
     cluster_sync_all();
-    if (warp >= 2) {
-      const int local = (warp & 3) * 32 + lane, t = blockIdx.x, n = t % tiles_n * 128 + local, row0 = t / tiles_n * BN, left = min(BN, p.rows - row0);
-      const uint32_t own = smem_u32(smem) + local * 4;
-      if (n < p.n) {
-        for (int c = part + (warp - 2) / 4 * p.splits; c < left; c += p.splits * (kWarps / 4)) {
-          float sum = 0.0f;
-          for (int q = 0; q < p.splits; ++q) sum += ld_dsmem_f32(dsmem_addr(own + c * 512, q));
-          if (p.out_f32) static_cast<float*>(p.out)[(row0 + c) * p.ldo + n] = sum;
-          else static_cast<bf16*>(p.out)[(row0 + c) * p.ldo + n] = __float2bfloat16_rn(sum);
-        }
+    if (warp >= 2) {  // a thread adds four neighbouring columns of the result, all parts on their way at once
+      const int t = blockIdx.x, n0 = t % tiles_n * 128 + lane * 4, row0 = t / tiles_n * BN, left = min(BN, p.rows - row0), count = min(4, p.n - n0);
+      const uint32_t own = smem_u32(smem) + lane * 16;
+      for (int c = part + (warp - 2) * p.splits; c < left; c += kWarps * p.splits) {
+        float4 v[kFp8MaxSplits];
+#pragma unroll
+        for (int q = 0; q < kFp8MaxSplits; ++q)
+          if (q < p.splits) v[q] = ld_dsmem_f32x4(dsmem_addr(own + c * 512, q));
+        float4 sum = v[0];
+#pragma unroll
+        for (int q = 1; q < kFp8MaxSplits; ++q)
+          if (q < p.splits) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
+        const float o[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < count) {
+            const long long at = (row0 + c) * p.ldo + n0 + i;
+            if (p.out_f32) static_cast<float*>(p.out)[at] = o[i];
+            else static_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(o[i]);
+          }
       }
       __syncwarp();
     }
