@@ -15,7 +15,8 @@ template <class T>
 int launch_quantize(const QuantParams& p, int block_rows, cudaStream_t st) {
   const bool vec = fits16(p.x, p.ldx * (long long)sizeof(T));
   if (block_rows == 1) {
-    const dim3 grid(unsigned(((long long)p.rows * p.blocks + kQuantThreads / 16 - 1) / (kQuantThreads / 16)));
+    const long long units = (long long)p.rows * ((p.blocks + kQuantGroup - 1) / kQuantGroup);
+    const dim3 grid(unsigned((units + kQuantThreads / 16 - 1) / (kQuantThreads / 16)));
     return launch(vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, grid, dim3(kQuantThreads), 0, st, p);
   }
   const dim3 grid(unsigned((p.rows + kScaleBlock - 1) / kScaleBlock) * unsigned(p.blocks));

@@ -11,9 +11,6 @@ namespace mtx {
 constexpr int kScaleBlock = 128;
 constexpr uint32_t kLeastLargest = 0x0F800000u;  // 2^-96: a block of zeros has a scale like any other, and 448 / A stays finite
 
-// |x| of finite values, infinities and NaN in the order of their bits: a maximum over them keeps a NaN, as the definition's does
-__device__ __forceinline__ uint32_t magnitude_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
 // two e4m3 bytes, `lo` in the low one; a product that its rounding put behind 448 becomes 448, NaN stays NaN
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
   unsigned short r;
@@ -21,46 +18,49 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
   return r;
 }
 
-// eight consecutive values of a row, as many as there are (the rest 0)
-template <bool VEC>
-__device__ __forceinline__ void load8(const bf16* p, int n, float (&v)[8]) {
-  if (VEC && n >= 8) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < n ? __bfloat162float(p[i]) : 0.0f;
-}
-template <bool VEC>
-__device__ __forceinline__ void load8(const float* p, int n, float (&v)[8]) {
-  if (VEC && n >= 8) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
-}
+// Eight consecutive values of a row as they lie in memory: the registers of the values that a thread holds until it knows their scale.
+template <class T>
+struct Raw8 {
+  static constexpr int kWords = 2 * sizeof(T);
+  uint32_t w[kWords];
 
-__device__ __forceinline__ void store8_e4m3(uint8_t* p, int n, const float (&v)[8], float by) {
-  uint32_t w[4];
+  // the values from n on become 0
+  __device__ __forceinline__ void cut(int n) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = e4m3_pair(v[2 * i] * by, v[2 * i + 1] * by);
-  if (n >= 8) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-    return;
+    for (int i = 0; i < kWords; ++i) {
+      if (sizeof(T) == 4) w[i] = i < n ? w[i] : 0u;
+      else w[i] &= (2 * i < n ? 0xffffu : 0u) | (2 * i + 1 < n ? 0xffff0000u : 0u);
+    }
   }
+  // the bits of the largest magnitude as fp32: those of finite values, infinities and NaN have the order of their bits, so that a NaN stays (as the definition's does)
+  __device__ __forceinline__ uint32_t largest() const {
+    uint32_t top = 0;
+    if (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) p[i] = uint8_t(w[i / 2] >> (i % 2 * 8));
-}
-
-// ---- quantisation ----------------------------------------------------------------------------------------------------------------
-
-constexpr int kQuantThreads = 256;
+      for (int i = 0; i < kWords; ++i) top = max(top, w[i] & 0x7fffffffu);
+      return top;
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+    return max(top & 0xffff0000u, top << 16);
+  }
+  __device__ __forceinline__ float value(int i) const {
+    if (sizeof(T) == 4) return __uint_as_float(w[i % kWords]);
+    return i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
+  }
+  __device__ __forceinline__ void store_e4m3(uint8_t* p, int n, float by) const {
+    uint32_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = e4m3_pair(value(2 * i) * by, value(2 * i + 1) * by);
+    if (n >= 8) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = uint8_t(e[i / 2] >> (i % 2 * 8));
+  }
+};
 
 struct QuantParams {
   const void* x;
@@ -72,46 +72,158 @@ struct QuantParams {
   long long scale_row, scale_block;  // strides of a row (of a row of blocks) and of a block of columns
 };
 
-// 1 x 128: half a warp per block, eight values per thread.
+// N times eight values per thread, 16 lanes side by side: at(i, row, c, n) says that the i-th are row `row`'s from column c on, of which n are there (eight or more: all;
+// none or less: all are 0).  VEC: rows lie on 16 bytes.  Otherwise a lane loads the aligned 16 bytes in which its values
+// begin, takes the following ones from the next lane and shifts, unless that would reach over the matrix's ends.  (4001 x 10239: 32 us with pieces of
+// their own for every lane and a choice per load, 58 value by value.)
+template <class T, bool VEC, int N, class At>
+__device__ __forceinline__ void load_all(const QuantParams& p, At&& at, Raw8<T> (&v)[N]) {
+  constexpr int W = Raw8<T>::kWords, kPieces = W / 4;
+  const T* x = static_cast<const T*>(p.x);
+  const int lane = threadIdx.x & 15;
+  long long row;
+  int c, n;
+  if (!VEC) {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(x), end = reinterpret_cast<uintptr_t>(x + (p.rows - 1) * p.ldx + p.k);
+    bool inside = true;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      at(i, row, c, n);
+      const uintptr_t first = reinterpret_cast<uintptr_t>(x + row * p.ldx + (c - lane * 8)) & ~uintptr_t(15);  // of lane 0
+      inside = inside && first >= begin && first + 16 * (16 * kPieces + 1) <= end;
+    }
+    if (inside) {
+      const uint32_t half = 0xffffu << (threadIdx.x & 16);
+      auto piece_of = [&](int i) {
+        at(i, row, c, n);
+        return reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x + row * p.ldx + c) & ~uintptr_t(15));
+      };
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint4* piece = piece_of(i);
+        const bool any = n + lane * 8 > 0;  // (the half warp's)
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+          const uint4 u = any ? __ldcs(piece + j) : make_uint4(0, 0, 0, 0);
+          v[i].w[4 * j] = u.x, v[i].w[4 * j + 1] = u.y, v[i].w[4 * j + 2] = u.z, v[i].w[4 * j + 3] = u.w;
+        }
+      }
+      uint4 far = make_uint4(0, 0, 0, 0);  // lane i: what follows lane 15's pieces of the i-th
+      if (lane < N) far = __ldg(piece_of(lane) + (15 - lane) * kPieces + kPieces);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        at(i, row, c, n);
+        const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(x + row * p.ldx + c) & 15), by = (off & 3) * 8;
+        const uint32_t f[4] = {far.x, far.y, far.z, far.w};
+        uint32_t w[W + 4];
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j] = v[i].w[j];
+        auto shift = [&](auto words) {  // by that many words and `by` bits
+          constexpr int O = decltype(words)::value;
+#pragma unroll
+          for (int j = 0; j <= O; ++j) {
+            const uint32_t next = __shfl_down_sync(half, w[j], 1, 16), last = __shfl_sync(half, f[j], i, 16);
+            w[W + j] = lane == 15 ? last : next;
+          }
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[i].w[j] = __funnelshift_r(w[j + O], w[j + O + 1], by);
+        };
+        if (off >> 2 == 0) shift(std::integral_constant<int, 0>());  // (one row per half warp: all its lanes shift alike)
+        else if (off >> 2 == 1) shift(std::integral_constant<int, 1>());
+        else if (off >> 2 == 2) shift(std::integral_constant<int, 2>());
+        else shift(std::integral_constant<int, 3>());
+        if (n < 8) v[i].cut(n);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    at(i, row, c, n);
+    const T* from = x + row * p.ldx + c;
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[i].w[j] = 0;
+    if (VEC && n >= 8) {
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(from) + j);
+        v[i].w[4 * j] = u.x, v[i].w[4 * j + 1] = u.y, v[i].w[4 * j + 2] = u.z, v[i].w[4 * j + 3] = u.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) {
+          if (sizeof(T) == 4) v[i].w[j % W] = reinterpret_cast<const uint32_t*>(from)[j];
+          else v[i].w[j / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(from)[j]) << (j % 2 * 16);
+        }
+    }
+  }
+}
+
+// ---- quantisation ----------------------------------------------------------------------------------------------------------------
+//
+// One pass: a thread keeps its values until the block's maximum is known.  Bound: bytes (2 or 4 in, 1 out per value).
+
+constexpr int kQuantThreads = 256;
+constexpr int kQuantGroup = 4;  // blocks of a row that half a warp works on at a time
+
+// 1 x 128: eight values per thread and block, half a warp per four blocks of a row, whose loads are on their way together; the four maxima are halved over the lanes
+// so that a lane divides for one block alone.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const QuantParams p) {
   griddep_wait();
   griddep_launch_dependents();  // (behind the wait: a product that starts now may read weights that an earlier kernel wrote)
   const int lane = threadIdx.x & 15;
-  const uint32_t block = blockIdx.x * (kQuantThreads / 16) + (threadIdx.x >> 4), all = uint32_t(p.rows) * uint32_t(p.blocks);
-  const uint32_t row = block / uint32_t(p.blocks), b = block - row * uint32_t(p.blocks);
-  const bool there = block < all;
-  const int c = int(b) * kScaleBlock + lane * 8, n = there ? p.k - c : 0;
-  float v[8];
-  load8<VEC>(static_cast<const T*>(p.x) + (n > 0 ? row * p.ldx + c : 0), n, v);
-  uint32_t top = kLeastLargest;
+  const uint32_t groups = uint32_t(p.blocks + kQuantGroup - 1) / kQuantGroup, unit = blockIdx.x * (kQuantThreads / 16) + (threadIdx.x >> 4), row = unit / groups;
+  const bool there = row < uint32_t(p.rows);
+  const int b0 = int(unit - row * groups) * kQuantGroup, c = b0 * kScaleBlock + lane * 8, left = there ? p.k - c : 0;
+  Raw8<T> v[kQuantGroup];
+  uint32_t top[kQuantGroup];
+  load_all<T, VEC>(
+      p,
+      [&](int i, long long& r, int& col, int& n) {
+        r = min(row, uint32_t(p.rows) - 1);
+        col = c + i * kScaleBlock;
+        n = left - i * kScaleBlock;
+      },
+      v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(v[i]));
+  for (int i = 0; i < kQuantGroup; ++i) top[i] = max(v[i].largest(), kLeastLargest);
+  const bool up8 = lane & 8, up4 = lane & 4;
+  uint32_t a = max(up8 ? top[2] : top[0], __shfl_xor_sync(0xffffffffu, up8 ? top[0] : top[2], 8));
+  uint32_t b = max(up8 ? top[3] : top[1], __shfl_xor_sync(0xffffffffu, up8 ? top[1] : top[3], 8));
+  uint32_t mine = max(up4 ? b : a, __shfl_xor_sync(0xffffffffu, up4 ? a : b, 4));  // of block lane / 4
+  mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+  mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+  const float by = __fdiv_rn(448.0f, __uint_as_float(mine));
+  if ((lane & 3) == 0 && there && b0 + (lane >> 2) < p.blocks) p.scale[row * p.scale_row + (b0 + (lane >> 2)) * p.scale_block] = __fdiv_rn(__uint_as_float(mine), 448.0f);
 #pragma unroll
-  for (int i = 8; i > 0; i >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, i));
-  if (n > 0) store8_e4m3(p.q + row * p.ldq + c, n, v, __fdiv_rn(448.0f, __uint_as_float(top)));
-  if (lane == 0 && there) p.scale[row * p.scale_row + b * p.scale_block] = __fdiv_rn(__uint_as_float(top), 448.0f);
+  for (int i = 0; i < kQuantGroup; ++i) {
+    const float f = __shfl_sync(0xffffffffu, by, i * 4, 16);
+    if (left - i * kScaleBlock > 0) v[i].store_e4m3(p.q + row * p.ldq + c + i * kScaleBlock, left - i * kScaleBlock, f);
+  }
 }
 
 // 128 x 128: a CTA per block, eight rows of eight values per thread.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const QuantParams p) {
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : VEC ? 4 : 3) quantize_blocks_kernel(const QuantParams p) {
   __shared__ uint32_t part[kQuantThreads / 32];
   griddep_wait();
   griddep_launch_dependents();
   const int up = blockIdx.x / p.blocks, b = blockIdx.x - up * p.blocks;
   const int row0 = up * kScaleBlock + (threadIdx.x >> 4), c = b * kScaleBlock + (threadIdx.x & 15) * 8;
-  float v[8][8];
+  Raw8<T> v[8];
   uint32_t top = kLeastLargest;
+  load_all<T, VEC>(
+      p,
+      [&](int i, long long& r, int& col, int& n) {
+        r = min(row0 + 16 * i, p.rows - 1);
+        col = c;
+        n = row0 + 16 * i < p.rows ? p.k - c : 0;
+      },
+      v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = row0 + 16 * i, n = row < p.rows ? p.k - c : 0;
-    load8<VEC>(static_cast<const T*>(p.x) + (n > 0 ? row * p.ldx + c : 0), n, v[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, magnitude_bits(v[i][j]));
+  for (int i = 0; i < 8; ++i) top = max(top, v[i].largest());
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
   __syncthreads();
@@ -120,8 +232,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_blocks_kernel(const Qu
   const float by = __fdiv_rn(448.0f, __uint_as_float(top));
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int row = row0 + 16 * i, n = row < p.rows ? p.k - c : 0;
-    if (n > 0) store8_e4m3(p.q + row * p.ldq + c, n, v[i], by);
+    const int row = row0 + 16 * i;
+    if (row < p.rows && c < p.k) v[i].store_e4m3(p.q + row * p.ldq + c, p.k - c, by);
   }
   if (threadIdx.x == 0) p.scale[up * p.scale_row + b * p.scale_block] = __fdiv_rn(__uint_as_float(top), 448.0f);
 }
