@@ -24,6 +24,7 @@ int mtx_control_logits(const float* logits, long long ld, float* out, long long 
   if (!c) return fail(MTX_ERR_ARG, "null controls");
   if (rows == 0) return MTX_OK;
   if (!logits || !out) return fail(MTX_ERR_ARG, "null argument");
+  if (((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 3) != 0) return fail(MTX_ERR_ARG, "logits lie on 4 bytes");
   if (logits == out && ld != ldo) return fail(MTX_ERR_ARG, "logits that are controlled in place have one pitch");
   if ((c->repetition || c->presence || c->frequency) && !c->seen) return fail(MTX_ERR_ARG, "penalties need the record of seen tokens");
   ControlParams p;
@@ -59,12 +60,16 @@ int mtx_control_logits(const float* logits, long long ld, float* out, long long 
   p.ldo = ldo;
   p.rows = rows;
   p.vocab = vocab;
-  p.spans = (vocab - 1) / kControlSpan + 1;
+  const long long runs = (vocab + 2) / kControlRun + 1;  // of a row (three tokens more: rows that begin up to three in front of 16 bytes)
+  p.runs = int((rows * runs + kControlWarps - 1) / kControlWarps);
+  if (p.runs > runs) p.runs = int(runs);
+  p.spans = int((runs - 1) / ((long long)p.runs * (kControlThreads / 32)) + 1);
   if ((long long)rows * p.spans >= 1ll << 31) return fail(MTX_ERR_ARG, "rows * vocab is too large for one call");
   MTX_TRY(on_this_device({logits, out, p.seen, p.slot, p.touched, p.repetition, p.presence, p.frequency, p.bias_off, p.bias_token, p.bias_value, p.allowed, p.allowed_row}));
-  const bool vec = ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 && ld % 4 == 0 && ldo % 4 == 0;
-  return launch(vec ? control_logits_kernel<true> : control_logits_kernel<false>, dim3(unsigned(rows) * unsigned(p.spans)), dim3(kControlThreads), 0,
-                static_cast<cudaStream_t>(stream), p);
+  const uintptr_t a = reinterpret_cast<uintptr_t>(logits), o = reinterpret_cast<uintptr_t>(out);
+  const bool aligned = ((a | o) & 15) == 0 && ld % 4 == 0 && ldo % 4 == 0, alike = ((a ^ o) & 15) == 0 && (ld - ldo) % 4 == 0;
+  return launch(aligned ? control_logits_kernel<kControlAligned> : alike ? control_logits_kernel<kControlShifted> : control_logits_kernel<kControlSingle>,
+                dim3(unsigned(rows) * unsigned(p.spans)), dim3(kControlThreads), 0, static_cast<cudaStream_t>(stream), p);
 }
 
 int mtx_note_tokens(uint16_t* seen, long long ld_seen, uint32_t* touched, long long ld_touched, int slots, int vocab, const int32_t* token, const int32_t* slot, int n, int prompt,

@@ -10,15 +10,16 @@
 namespace mtx {
 
 constexpr int kControlThreads = 256;
-constexpr int kControlWords = 4;  // runs of 256 tokens that a warp takes one after the other
-constexpr int kControlSpan = kControlThreads / 32 * kControlWords * 256;
+constexpr int kControlRun = 256;  // tokens that a warp works on at a time: twice four per lane
+constexpr int kControlWarps = 148 * 192;  // warps of a large call: three times as many as run at once (32 registers per thread), for an even end
 
 struct ControlParams {
   const float* logits;
   long long ld;
   float* out;
   long long ldo;
-  int rows, vocab, spans;
+  int rows, vocab;
+  int runs, spans;  // runs of a warp, CTAs of a row
   int slots;
   const int32_t* slot;
   const uint16_t* seen;
@@ -60,80 +61,110 @@ __device__ __forceinline__ int first_at_least(const int32_t* token, int n, int t
   return lo;
 }
 
-// VEC: rows of logits and results lie on 16 bytes: lane l has the tokens 8 l .. 8 l + 7 of a run; otherwise the tokens l, l + 32, ..
-template <bool VEC>
-__global__ void __launch_bounds__(kControlThreads) control_logits_kernel(const ControlParams p) {
+// How a lane's four tokens of a run lie.  Logits and results of a token t lie on 16 bytes where t is ...
+enum ControlForm {
+  kControlAligned,  // ... a multiple of 4, in every row: a lane's tokens lie in one word of the mask, under one bit of `touched` and in 8 bytes of `seen`
+  kControlShifted,  // ... s + a multiple of 4, s = -3 .. 0 by row (vocabularies of odd sizes): they may share two of each
+  kControlSingle,   // ... something else in the results than in the logits: lane l has the tokens l, l + 32, .., one by one
+};
+
+// Bound: bytes, 4 read and 4 written per logit where all is allowed.  Four tokens of which none is allowed are written without being read, and in place four that nothing changes are
+// neither.  64 x 264192 logits: unmasked 26.5 us (5.1 TB/s), behind masks that leave a few 24; at an odd size of the vocabulary 32 (value by value 53).  A warp
+// takes up to three or so neighbouring runs (one each: 27.8, eight each: 30.2); runs fetched ahead in more registers by fewer warps took 30 to 39.
+template <int FORM>
+__global__ void __launch_bounds__(kControlThreads, 8) control_logits_kernel(const ControlParams p) {
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.x / p.spans, span = blockIdx.x - row * p.spans;
-  const int first = span * kControlSpan + (threadIdx.x >> 5) * (kControlWords * 256), last = min(p.vocab, first + kControlWords * 256);
-  if (first >= p.vocab) return;
   const float* in = p.logits + row * p.ld;
   float* out = p.out + row * p.ldo;
   const bool in_place = in == out;
+  const int shift = FORM == kControlShifted ? -int(reinterpret_cast<uintptr_t>(in) >> 2 & 3) : 0;  // in[shift] lies on 16 bytes
+  const int begin = (span * (kControlThreads / 32) + (threadIdx.x >> 5)) * p.runs * kControlRun + shift;  // the warp's tokens
+  const int first = max(begin, 0), last = min(p.vocab, begin + p.runs * kControlRun);
+  if (first >= last) return;
 
+  const int slot = p.seen == nullptr ? -1 : p.slot != nullptr ? p.slot[row] : row;
+  const int mask_row = p.allowed == nullptr ? -1 : p.allowed_row != nullptr ? p.allowed_row[row] : row;
   const uint16_t* seen = nullptr;
-  const uint32_t* touched = nullptr;
+  const uint32_t *touched = nullptr, *allowed = nullptr;
   float repetition = 1.0f, presence = 0.0f, frequency = 0.0f;
-  if (p.seen != nullptr) {
-    const int slot = p.slot != nullptr ? p.slot[row] : row;
-    if (slot >= 0 && slot < p.slots) {
-      if (p.repetition != nullptr) repetition = p.repetition[slot];
-      if (p.presence != nullptr) presence = p.presence[slot];
-      if (p.frequency != nullptr) frequency = p.frequency[slot];
-      if (repetition != 1.0f || presence != 0.0f || frequency != 0.0f) {
-        seen = p.seen + slot * p.ld_seen;
-        if (p.touched != nullptr) touched = p.touched + slot * p.ld_touched;
-      }
+  if (mask_row >= 0 && mask_row < p.allowed_rows) allowed = p.allowed + mask_row * p.ld_allowed;
+  if (slot >= 0 && slot < p.slots) {
+    if (p.repetition != nullptr) repetition = p.repetition[slot];
+    if (p.presence != nullptr) presence = p.presence[slot];
+    if (p.frequency != nullptr) frequency = p.frequency[slot];
+    if (p.repetition != nullptr || p.presence != nullptr || p.frequency != nullptr) {
+      seen = p.seen + slot * p.ld_seen;
+      if (p.touched != nullptr) touched = p.touched + slot * p.ld_touched;
     }
   }
-  const uint32_t* allowed = nullptr;
-  if (p.allowed != nullptr) {
-    const int a = p.allowed_row != nullptr ? p.allowed_row[row] : row;
-    if (a >= 0 && a < p.allowed_rows) allowed = p.allowed + a * p.ld_allowed;
-  }
+  auto may_one = [&](int t) { return allowed == nullptr || (allowed[t >> 5] >> (t & 31) & 1); };
+  auto touched_one = [&](int t) { return seen != nullptr && (touched == nullptr || (touched[t >> 8] >> (t >> 3 & 31) & 1)); };
 
-  for (int t0 = first; t0 < last; t0 += 256) {
-    const uint32_t hit = seen == nullptr ? 0u : touched != nullptr ? touched[t0 >> 8] : 0xffffffffu;
-    if (VEC) {
-      const int t = t0 + lane * 8, n = min(p.vocab - t, 8);
-      if (n <= 0) continue;
-      uint32_t may = 0xffu;
-      if (allowed != nullptr) may = allowed[t >> 5] >> (t & 31) & 0xffu;
-      const bool marked = hit >> lane & 1;
-      if (in_place && may == 0xffu && !marked) continue;
-      uint4 s = make_uint4(0, 0, 0, 0);
-      if (marked) s = *reinterpret_cast<const uint4*>(seen + t);
-      const uint32_t w[4] = {s.x, s.y, s.z, s.w};
-      float v[8];
-      if (n == 8) {
-        if (may != 0) {
-          const float4 a = *reinterpret_cast<const float4*>(in + t), b = *reinterpret_cast<const float4*>(in + t + 4);
-          v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  auto one = [&](int t) {
+    const bool may = may_one(t), marked = touched_one(t);
+    if (in_place && may && !marked) return;
+    out[t] = may ? penalised(in[t], marked ? seen[t] : 0u, repetition, presence, frequency) : -INFINITY;
+  };
+
+  if (FORM == kControlSingle) {
+    for (int t = first + lane; t < last; t += 32) one(t);
+  } else {
+    for (int t0 = begin; t0 < last; t0 += kControlRun) {
+      if (t0 < 0 || t0 + kControlRun > p.vocab) {  // the row's ends
+        for (int t = max(t0, 0) + lane; t < min(t0 + kControlRun, p.vocab); t += 32) one(t);
+        continue;
+      }
+      // everything of the run on its way, then the arithmetic: a lane's four tokens of either half as bits of the mask, logits and words of `seen`
+      uint32_t may[2] = {0xfu, 0xfu};
+      if (allowed != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int t = t0 + j * 128 + lane * 4;
+          const uint32_t lo = allowed[t >> 5], hi = FORM == kControlShifted && (t & 31) > 28 ? allowed[(t >> 5) + 1] : 0u;
+          may[j] = __funnelshift_r(lo, hi, t & 31) & 0xfu;
         }
-      } else {
+      }
+      uint32_t hit[2] = {0, 0};  // of `touched`: one word where runs begin at multiples of 256, else the end of one and nearly all of the next
+      if (seen != nullptr) {
+        hit[0] = touched != nullptr ? touched[t0 >> 8] : 0xffffffffu;
+        if (FORM == kControlShifted) hit[1] = touched != nullptr ? touched[(t0 + kControlRun - 1) >> 8] : 0xffffffffu;
+      }
+      float4 v[2];
+      uint2 w[2];
+      bool same[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? in[t + i] : 0.0f;
+      for (int j = 0; j < 2; ++j) {
+        const int t = t0 + j * 128 + lane * 4;
+        bool marked = hit[FORM == kControlShifted && t >> 8 != t0 >> 8] >> (t >> 3 & 31) & 1;
+        if (FORM == kControlShifted) marked = marked || (hit[(t + 3) >> 8 != t0 >> 8] >> ((t + 3) >> 3 & 31) & 1);
+        marked = marked && may[j] != 0;
+        same[j] = in_place && may[j] == 0xfu && !marked;
+        v[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        w[j] = make_uint2(0, 0);
+        if (may[j] != 0 && !same[j]) v[j] = *reinterpret_cast<const float4*>(in + t);
+        if (marked) {
+          if (FORM == kControlAligned) w[j] = *reinterpret_cast<const uint2*>(seen + t);
+          else w[j] = make_uint2(seen[t] | uint32_t(seen[t + 1]) << 16, seen[t + 2] | uint32_t(seen[t + 3]) << 16);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = may >> i & 1 ? penalised(v[i], w[i / 2] >> (i % 2 * 16) & 0xffffu, repetition, presence, frequency) : -INFINITY;
-      if (n == 8) {
-        *reinterpret_cast<float4*>(out + t) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(out + t + 4) = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < n) out[t + i] = v[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int t = t0 + i * 32 + lane;
-        if (t >= p.vocab) break;
-        const bool may = allowed == nullptr || (allowed[t >> 5] >> lane & 1), marked = hit >> (t >> 3 & 31) & 1;
-        if (in_place && may && !marked) continue;
-        out[t] = may ? penalised(in[t], marked ? seen[t] : 0u, repetition, presence, frequency) : -INFINITY;
+      for (int j = 0; j < 2; ++j) {
+        if (w[j].x != 0) {
+          v[j].x = penalised(v[j].x, w[j].x & 0xffffu, repetition, presence, frequency);
+          v[j].y = penalised(v[j].y, w[j].x >> 16, repetition, presence, frequency);
+        }
+        if (w[j].y != 0) {
+          v[j].z = penalised(v[j].z, w[j].y & 0xffffu, repetition, presence, frequency);
+          v[j].w = penalised(v[j].w, w[j].y >> 16, repetition, presence, frequency);
+        }
+        if (!(may[j] & 1)) v[j].x = -INFINITY;
+        if (!(may[j] & 2)) v[j].y = -INFINITY;
+        if (!(may[j] & 4)) v[j].z = -INFINITY;
+        if (!(may[j] & 8)) v[j].w = -INFINITY;
+        if (!same[j]) *reinterpret_cast<float4*>(out + t0 + j * 128 + lane * 4) = v[j];
       }
     }
   }
@@ -147,7 +178,7 @@ __global__ void __launch_bounds__(kControlThreads) control_logits_kernel(const C
       if (t >= last) break;
       if (t < first) continue;  // (tokens that are not ascending: none is written twice or outside the warp's)
       if (i > 0 && token[i - 1] == t) continue;
-      if (allowed == nullptr || (allowed[t >> 5] >> (t & 31) & 1)) out[t] = __fadd_rn(out[t], p.bias_value[b0 + i]);
+      if (may_one(t)) out[t] = __fadd_rn(out[t], p.bias_value[b0 + i]);
     }
   }
 }

@@ -54,7 +54,7 @@ CONTROL = dict(logits=A, ld=64, out=A + 65536, ldo=64, rows=2, vocab=64, control
 
 @pytest.mark.parametrize("change,word", [
     (dict(rows=-1), "bad rows"), (dict(vocab=0), "bad rows"), (dict(ld=63), "bad rows"), (dict(ldo=63), "bad rows"), (dict(vocab=(1 << 30) + 1, ld=1 << 31, ldo=1 << 31), "bad rows"),
-    (dict(logits=None), "null"), (dict(out=None), "null"), (dict(out=A, ldo=72), "in place"),
+    (dict(logits=None), "null"), (dict(out=None), "null"), (dict(out=A, ldo=72), "in place"), (dict(out=A + 2), "4 bytes"), (dict(logits=A + 1), "4 bytes"),
 ])
 def test_control(lib, change, word):
   refused(lib.mtx_control_logits(*{**CONTROL, "controls": _lib.LogitControls(), **change}.values()), word)
