@@ -101,9 +101,12 @@ constexpr int fp8_stream_most_stages() {
 // large ones fit than SMs).  64 rows of 5120 by 1280 columns: 16.9 us in one part, 8.8 in four, 7.8 in eight; 128 rows of 10240 by 2560 columns (20
 // tiles): 14.6 in six, 24.0 in eight, whose clusters take turns.  More tiles than SMs: one part (64 x 2560 by 10240, 80 tiles: 11.3 us, 12.6 in two).
 template <int BN>
-int stream_splits(long long tiles, int blocks) {
+int stream_splits(long long tiles, int blocks, int* splits) {
   static std::atomic<int> fit[kFp8MaxSplits + 1];  // clusters of that many CTAs that run at once; 0: not asked yet
+  static std::atomic<uint64_t> done{0};
   const size_t smem = fp8_stream_smem_bytes<BN>(fp8_stream_most_stages<BN>());
+  MTX_TRY(allow_smem(fp8_stream_kernel<BN>, smem, done));
+  *splits = 1;
   for (int s = kFp8MaxSplits; s > 1; --s) {
     if (s > blocks || tiles * s > kSms) continue;
     int n = fit[s].load(std::memory_order_relaxed);
@@ -126,21 +129,22 @@ int stream_splits(long long tiles, int blocks) {
       }
       fit[s].store(n, std::memory_order_relaxed);
     }
-    if (tiles <= n) return s;
+    if (tiles <= n) {
+      *splits = s;
+      break;
+    }
   }
-  return 1;
+  return MTX_OK;
 }
 
 template <int BN>
 int launch_stream(const Fp8Call& c, cudaStream_t st) {
-  static std::atomic<uint64_t> done{0};
   constexpr int kPerSm = BN <= 32 ? 3 : BN == 64 ? 2 : 1;  // CTAs that may share an SM
   constexpr int kLeast = BN == 16 ? 4 : BN == 32 ? 3 : BN == 64 ? 4 : 6;
   Fp8LinearParams p = c.p;
   const long long tiles = (long long)((p.n + 127) / 128) * ((p.rows + BN - 1) / BN);
   if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
-  MTX_TRY(allow_smem(fp8_stream_kernel<BN>, fp8_stream_smem_bytes<BN>(fp8_stream_most_stages<BN>()), done));
-  p.splits = stream_splits<BN>(tiles, p.blocks);
+  MTX_TRY(stream_splits<BN>(tiles, p.blocks, &p.splits));
   // an SM's shared memory in stages, whether one CTA has it or several: 64 KB in flight are too few for a CTA alone (16 x 2560 by 10240, 80 CTAs: 11.1 us, 8.8 with all)
   const long long per_sm = (tiles * p.splits + kSms - 1) / kSms;
   p.stages = per_sm >= kPerSm ? kLeast : kLeast * kPerSm / int(per_sm);
@@ -187,7 +191,8 @@ int launch_linear(const Fp8Call& c, cudaStream_t st) {
   if (rows <= 32) return launch_stream<32>(c, st);
   if (rows <= 64) return launch_stream<64>(c, st);
   const long long blocks = c.p.blocks, tiles128 = (long long)((rows + 127) / 128) * ((c.p.n + 127) / 128);
-  const int splits = stream_splits<128>(tiles128, c.p.blocks);
+  int splits;
+  MTX_TRY(stream_splits<128>(tiles128, c.p.blocks, &splits));
   const long long stream = 4500 + (splits > 1 ? 2300 : 0) + (tiles128 * splits + kSms - 1) / kSms * ((blocks + splits - 1) / splits * 500 + 300);
   auto pair = [&](int bn, long long base, long long block, long long end) {
     const long long tiles = (long long)((rows + kFp8PairRows - 1) / kFp8PairRows) * ((c.p.n + bn - 1) / bn);

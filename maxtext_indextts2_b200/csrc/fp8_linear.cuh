@@ -514,6 +514,7 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
         step(b, 0);
         if (b + 1 < per) step(b + 1, 1);
       }
+      __syncwarp();  // (an odd number of blocks: the next tile's first factors go where the last ones were)
       if (j + 1 < mine) begin(t + int(gridDim.x));
       if (p.splits == 1) {
         const int n = t % tiles_n * 128 + local, row0 = t / tiles_n * BN + c0, left = p.rows - row0;
@@ -595,7 +596,7 @@ __host__ __device__ constexpr int fp8_pair_warps() { return 8; }
 template <int BN>
 __host__ __device__ constexpr int fp8_pair_threads() { return 64 + 32 * fp8_pair_warps<BN>(); }
 template <int BN>
-constexpr int fp8_pair_staged() { return fp8_pair_warps<BN>() * 4096; }  // 32 rows x 128 bytes per epilogue warp
+__host__ __device__ constexpr int fp8_pair_staged() { return fp8_pair_warps<BN>() * (BN == 256 ? 8192 : 4096); }  // two buffers (one) of 32 rows x 128 bytes per epilogue warp
 
 template <int BN>
 __host__ __device__ constexpr int fp8_pair_stage_bytes() { return kFp8OperandBytes + BN / 2 * kScaleBlock; }
@@ -616,11 +617,12 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, const void* 
 template <int BN, class OUT>
 __global__ void __launch_bounds__(fp8_pair_threads<BN>(), 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out, const Fp8LinearParams p) {
-  constexpr int kStage = fp8_pair_stage_bytes<BN>(), NB = 512 / BN > 4 ? 4 : 512 / BN, kHalf = BN / 2, kWarps = fp8_pair_warps<BN>(), kCols = BN * 4 / kWarps, kBox = 128 / int(sizeof(OUT));
+  constexpr int kStage = fp8_pair_stage_bytes<BN>(), NB = 512 / BN, kHalf = BN / 2, kWarps = fp8_pair_warps<BN>(), kCols = BN * 4 / kWarps;
+  constexpr int kBuffers = fp8_pair_staged<BN>() / kWarps / 4096, kBox = 128 / int(sizeof(OUT));
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* staged = smem + size_t(p.stages) * kStage;
-  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(staged + kWarps * 4096);
+  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(staged + fp8_pair_staged<BN>());
   volatile int* failed = &tail->failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(blockIdx.x) & 1, pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
@@ -651,7 +653,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
 
   if (warp >= 2) {
     const int c0 = (warp - 2) / 4 * kCols, quarter = warp & 3;
-    uint8_t* stage = staged + (warp - 2) * 4096;
+    uint8_t* stage = staged + (warp - 2) * kBuffers * 4096;
     const uint32_t lanes = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(c0);
     int t = pair, s = 0, buf = 0;
     uint32_t phase = 0;
@@ -679,7 +681,6 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
       tcgen05_fence_after();
       float scale;  // (volatile: multiplied here, not right behind the loads)
       asm volatile("mul.rn.f32 %0, %1, %2;" : "=f"(scale) : "f"(xs[i]), "f"(ws[i]));
-      if (b + 2 < p.blocks) fetch(i);
       const unsigned long long by = pair_of(scale, scale);
       fp8_columns<kCols>(
           lanes + uint32_t(buf * BN),
@@ -692,6 +693,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
             __syncwarp();
             if (lane == 0) fp8_release_leader(&tail->tmem_empty[buf]);
           });
+      if (b + 2 < p.blocks) fetch(i);
       if (++s == p.stages) s = 0, phase ^= 1;
       if (++buf == NB) buf = 0;
     };
@@ -703,101 +705,98 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
         if (b + 1 < p.blocks) step(b + 1, 1);
       }
       if (j + 1 < mine) begin(t + pairs);
-      {
-        // 32 rows x 128 bytes at a time through shared memory (chunk j of row r at j ^ (r & 7): the 128-byte swizzle of the tensor map)
-        const int row0 = t % m_tiles * kFp8PairRows + rank * 128 + quarter * 32, col0 = t / m_tiles * BN + c0;
+      // 32 rows x 128 bytes at a time through shared memory (chunk j of row r at j ^ (r & 7): the 128-byte swizzle of the tensor map)
+      const int row0 = t % m_tiles * kFp8PairRows + rank * 128 + quarter * 32, col0 = t / m_tiles * BN + c0;
 #pragma unroll
-        for (int c = 0; c < kCols; c += kBox) {
-          if (col0 + c < p.n && row0 < p.rows) {
-            uint8_t* to = stage;
-            if (p.tma_store) {
-              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the buffer's last store has been read
-              __syncwarp();
-            }
+      for (int c = 0; c < kCols; c += kBox) {
+        if (col0 + c < p.n && row0 < p.rows) {
+          uint8_t* to = stage + c / kBox % kBuffers * 4096;
+          if (p.tma_store) {  // the buffer's last store has been read: one of the tile before, or of this one's box but kBuffers
+            if (lane == 0 && c == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            if (lane == 0 && c >= kBuffers * kBox) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBuffers - 1) : "memory");
+            __syncwarp();
+          }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint4 u;
-              if (sizeof(OUT) == 2) {
-                const unsigned long long* a = acc + (c + 8 * j) / 2;
-                u = make_uint4(pack_bf16x2(pair_lo(a[0]), pair_hi(a[0])), pack_bf16x2(pair_lo(a[1]), pair_hi(a[1])), pack_bf16x2(pair_lo(a[2]), pair_hi(a[2])),
-                               pack_bf16x2(pair_lo(a[3]), pair_hi(a[3])));
-              } else {
-                const unsigned long long* a = acc + (c + 4 * j) / 2;
-                u = make_uint4(uint32_t(a[0]), uint32_t(a[0] >> 32), uint32_t(a[1]), uint32_t(a[1] >> 32));
-              }
-              *reinterpret_cast<uint4*>(to + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
+          for (int j = 0; j < 8; ++j) {
+            uint4 u;
+            if (sizeof(OUT) == 2) {
+              const unsigned long long* a = acc + (c + 8 * j) / 2;
+              u = make_uint4(pack_bf16x2(pair_lo(a[0]), pair_hi(a[0])), pack_bf16x2(pair_lo(a[1]), pair_hi(a[1])), pack_bf16x2(pair_lo(a[2]), pair_hi(a[2])),
+                             pack_bf16x2(pair_lo(a[3]), pair_hi(a[3])));
+            } else {
+              const unsigned long long* a = acc + (c + 4 * j) / 2;
+              u = make_uint4(uint32_t(a[0]), uint32_t(a[0] >> 32), uint32_t(a[1]), uint32_t(a[1] >> 32));
             }
-            if (p.tma_store) {
-              fence_proxy_async();
-              __syncwarp();
-              if (lane == 0) {
-                tma_store_2d(&tm_out, to, col0 + c, row0);
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-              }
-            } else {  // results at odd places: a row's values by neighbouring lanes
-              __syncwarp();
-              OUT* o = static_cast<OUT*>(p.out) + row0 * p.ldo + col0 + c;
-              const int rows = min(32, p.rows - row0), cols = min(kBox, p.n - col0 - c);
-              for (int r = 0; r < rows; ++r, o += p.ldo)
-                for (int i = lane; i < cols; i += 32) o[i] = *reinterpret_cast<const OUT*>(to + r * 128 + (((i / (kBox / 8)) ^ (r & 7)) << 4) + i % (kBox / 8) * sizeof(OUT));
-              __syncwarp();
+            *reinterpret_cast<uint4*>(to + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
+          }
+          if (p.tma_store) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tm_out, to, col0 + c, row0);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
+          } else {  // results at odd places: a row's values by neighbouring lanes
+            __syncwarp();
+            OUT* o = static_cast<OUT*>(p.out) + row0 * p.ldo + col0 + c;
+            const int rows = min(32, p.rows - row0), cols = min(kBox, p.n - col0 - c);
+            for (int r = 0; r < rows; ++r, o += p.ldo)
+              for (int i = lane; i < cols; i += 32) o[i] = *reinterpret_cast<const OUT*>(to + r * 128 + (((i / (kBox / 8)) ^ (r & 7)) << 4) + i % (kBox / 8) * sizeof(OUT));
+            __syncwarp();
           }
         }
       }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
-  } else {
-    if (warp == 0) {
+  } else if (warp == 0) {
+    const bool issuer = elect_one();
+    int s = 0, b = 0, t = pair;
+    uint32_t phase = 1;
+    bool good = true;
+    for (int f = 0; f < F; ++f) {
+      if (f >= p.stages) good &= fp8_wait(&tail->done[s], phase, failed);
+      if (issuer && good) {
+        if (rank == 0) mbar_expect_tx(&tail->full[s], 2 * kStage);
+        tma_load_2d_pair(smem + s * kStage, &tm_x, b * kScaleBlock, t % m_tiles * kFp8PairRows + rank * 128, &tail->full[s], kEvictLast);
+        tma_load_2d_pair(smem + s * kStage + kFp8OperandBytes, &tm_w, b * kScaleBlock, t / m_tiles * BN + rank * kHalf, &tail->full[s], kEvictNormal);
+      }
+      if (++s == p.stages) s = 0, phase ^= 1;
+      if (++b == p.blocks) b = 0, t += pairs;
+    }
+    // the commits of the last stages arrive on this CTA's barriers too: they have to be there before it may leave
+    const int last = min(F, p.stages);
+    for (int f = 0; f < last; ++f) {
+      if (s == 0) s = p.stages, phase ^= 1;
+      --s;
+      fp8_wait(&tail->done[s], phase ^ 1, failed);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
       const bool issuer = elect_one();
-      int s = 0, b = 0, t = pair;
-      uint32_t phase = 1;
+      const uint32_t idesc = umma_idesc_e4m3(kFp8PairRows, BN);
+      const uint64_t d0 = umma_desc_sw128(smem);
+      const uint32_t desc_hi = uint32_t(d0 >> 32), desc_lo = uint32_t(d0);  // (the low words alone count on)
+      int s = 0, buf = 0;
+      uint32_t phase = 0, acc_phase = 1;
       bool good = true;
       for (int f = 0; f < F; ++f) {
-        if (f >= p.stages) good &= fp8_wait(&tail->done[s], phase, failed);
+        good &= fp8_wait(&tail->full[s], phase, failed);
+        good &= fp8_wait(&tail->tmem_empty[buf], acc_phase, failed);
+        tcgen05_fence_after();
         if (issuer && good) {
-          if (rank == 0) mbar_expect_tx(&tail->full[s], 2 * kStage);
-          tma_load_2d_pair(smem + s * kStage, &tm_x, b * kScaleBlock, t % m_tiles * kFp8PairRows + rank * 128, &tail->full[s], kEvictLast);
-          tma_load_2d_pair(smem + s * kStage + kFp8OperandBytes, &tm_w, b * kScaleBlock, t / m_tiles * BN + rank * kHalf, &tail->full[s], kEvictNormal);
+          const uint32_t at = desc_lo + uint32_t(s) * (kStage >> 4);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_e4m3_pair(tmem_base + uint32_t(buf * BN), umma_desc_of(at + kk * 2, desc_hi), umma_desc_of(at + (kFp8OperandBytes >> 4) + kk * 2, desc_hi), idesc, kk != 0);
+          umma_commit_pair(&tail->done[s]);
         }
         if (++s == p.stages) s = 0, phase ^= 1;
-        if (++b == p.blocks) b = 0, t += pairs;
+        if (++buf == NB) buf = 0, acc_phase ^= 1;
       }
-      // the commits of the last stages arrive on this CTA's barriers too: they have to be there before it may leave
-      const int last = min(F, p.stages);
-      for (int f = 0; f < last; ++f) {
-        if (s == 0) s = p.stages, phase ^= 1;
-        --s;
-        fp8_wait(&tail->done[s], phase ^ 1, failed);
-      }
-      __syncwarp();
-    } else if (warp == 1) {
-      if (rank == 0) {
-        const bool issuer = elect_one();
-        const uint32_t idesc = umma_idesc_e4m3(kFp8PairRows, BN);
-        const uint64_t d0 = umma_desc_sw128(smem);
-        const uint32_t desc_hi = uint32_t(d0 >> 32), desc_lo = uint32_t(d0);  // (the low words alone count on)
-        int s = 0, buf = 0;
-        uint32_t phase = 0, acc_phase = 1;
-        bool good = true;
-        for (int f = 0; f < F; ++f) {
-          good &= fp8_wait(&tail->full[s], phase, failed);
-          good &= fp8_wait(&tail->tmem_empty[buf], acc_phase, failed);
-          tcgen05_fence_after();
-          if (issuer && good) {
-            const uint32_t at = desc_lo + uint32_t(s) * (kStage >> 4);
-  #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_e4m3_pair(tmem_base + uint32_t(buf * BN), umma_desc_of(at + kk * 2, desc_hi), umma_desc_of(at + (kFp8OperandBytes >> 4) + kk * 2, desc_hi), idesc, kk != 0);
-            umma_commit_pair(&tail->done[s]);
-          }
-          if (++s == p.stages) s = 0, phase ^= 1;
-          if (++buf == NB) buf = 0, acc_phase ^= 1;
-        }
-      }
-      __syncwarp();
     }
+    __syncwarp();
   }
   if (*failed) fp8_let_copies_land();
   tcgen05_fence_before();

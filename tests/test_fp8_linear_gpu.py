@@ -125,7 +125,7 @@ def test_every_magnitude_rounds_as_defined():
 SHAPES = [
     (1, 1, 1), (1, 16, 64), (1, 1792, 1280), (2, 129, 127), (7, 128, 128), (8, 300, 2048), (16, 1280, 5120), (17, 257, 640), (31, 130, 130), (33, 100, 1000),
     (64, 1280, 1281), (65, 512, 256), (100, 4000, 272), (127, 33, 3001), (128, 128, 128), (129, 128, 384), (200, 1000, 2560), (256, 256, 1024), (257, 255, 144),
-    (333, 640, 1288), (500, 2051, 260), (700, 64, 4096), (1024, 384, 512),
+    (333, 640, 1288), (500, 2051, 260), (700, 64, 4096), (1024, 384, 512), (1500, 700, 1100), (16, 60001, 100), (3, 70000, 384), (130, 20000, 300), (2049, 1300, 128),
 ]
 
 
