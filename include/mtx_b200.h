@@ -708,14 +708,15 @@ int mtx_sample_rows(const float* logits, int rows, long long ld, int vocab, int 
  * a block: scale = A / 448, q = e4m3(x * (448 / A)), both fractions and the product rounded to fp32.  A NaN makes its block's scale
  * and values NaN, an infinity the scale infinite and itself NaN, so that products of its row are NaN.
  * q: pitch ldq, both base and pitch whole 16 bytes (bytes from k to ldq of a row are left as they are); scale: fp32
- * [ceil(rows / block_rows), ceil(k / 128)]. */
+ * [ceil(rows / block_rows), ceil(k / 128)].  rows, k <= 2^30; results may not overlap x. */
 int mtx_quantize_fp8(const void* x, int x_type, long long ldx, int rows, int k, int block_rows, void* q, long long ldq, float* scale, mtx_stream stream);
 
 /* out[m, n] = sum over the blocks b of 128 columns of x_scale[m, b] * w_scale[n / 128, b] * sum_{k in b} x[m, k] * wq[n, k], sums in fp32:
  * beside mtx_linear, with weights of mtx_quantize_fp8(block_rows = 128) and any number of rows.  x: MTX_E4M3 values with their x_scale
  * [rows, ceil(k / 128)] (block_rows = 1), or MTX_BF16 / MTX_F32 values, which the call quantises in the same way (x_scale is not read) in `scratch`:
  * mtx_linear_fp8_scratch_bytes(rows, k) bytes, 16-byte aligned, written by every call and so not for two calls at once.  8-bit
- * operands: base and pitch whole 16 bytes.  out: MTX_BF16 or MTX_F32, pitch ldo values; it may not overlap an input. */
+ * operands: base and pitch whole 16 bytes.  out: MTX_BF16 or MTX_F32, pitch ldo values; it may not overlap an input.
+ * rows, n, k <= 2^30.  A row of NaN or infinities leaves the other rows as they are; the same call gives the same bits every time. */
 size_t mtx_linear_fp8_scratch_bytes(int rows, int k);
 int mtx_linear_fp8(const void* x, int x_type, long long ldx, const float* x_scale, const void* wq, long long ldw, const float* w_scale, void* out, int out_type, long long ldo,
                    int rows, int n, int k, void* scratch, size_t scratch_bytes, mtx_stream stream);
@@ -746,7 +747,7 @@ typedef struct {
 
 /* out = controlled logits, rows x vocab each: repetition, then frequency, then presence penalty, then the bias; the logits of tokens that are not
  * allowed are -infinity whatever they were (a row whose mask allows nothing is -infinity throughout).  Every operation is rounded to fp32.
- * out == logits (with ldo == ld): in place, and then only what changes is read and written; otherwise the two may not overlap. */
+ * out == logits (with ldo == ld): in place, and then only what changes is read and written; otherwise the two may not overlap.  vocab <= 2^28. */
 int mtx_control_logits(const float* logits, long long ld, float* out, long long ldo, int rows, int vocab, const mtx_logit_controls* c, mtx_stream stream);
 
 /* Notes n tokens in the record: token[i] in slot slot[i] (NULL: slot i, n <= slots), as the prompt's (prompt != 0) or as generated once more.  The

@@ -5,7 +5,7 @@
 
 namespace {
 
-constexpr int kMaxK = 1 << 30;  // (column numbers, rounded up to a block, stay 32-bit)
+constexpr int kMost = 1 << 30;  // rows and columns: their numbers, rounded up to a tile, stay 32-bit
 
 bool fits16(const void* p, long long pitch_bytes) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch_bytes % 16 == 0; }
 
@@ -211,7 +211,7 @@ extern "C" {
 int mtx_quantize_fp8(const void* x, int x_type, long long ldx, int rows, int k, int block_rows, void* q, long long ldq, float* scale, mtx_stream stream) {
   if (x_type != MTX_BF16 && x_type != MTX_F32) return fail(MTX_ERR_ARG, "x_type %d: values of type MTX_BF16 or MTX_F32 are quantised", x_type);
   if (block_rows != 1 && block_rows != kScaleBlock) return fail(MTX_ERR_ARG, "block_rows is 1 (activations) or 128 (weights), not %d", block_rows);
-  if (rows < 0 || k < 1 || k > kMaxK || ldx < k || ldq < k) return fail(MTX_ERR_ARG, "bad rows / k / ldx / ldq");
+  if (rows < 0 || rows > kMost || k < 1 || k > kMost || ldx < k || ldq < k) return fail(MTX_ERR_ARG, "bad rows / k / ldx / ldq");
   if (rows == 0) return MTX_OK;
   if (!x || !q || !scale) return fail(MTX_ERR_ARG, "null argument");
   if (!fits16(q, ldq)) return fail(MTX_ERR_ARG, "8-bit values lie at a 16-byte aligned base and a pitch of whole 16 bytes");
@@ -229,7 +229,7 @@ int mtx_linear_fp8(const void* x, int x_type, long long ldx, const float* x_scal
                    int rows, int n, int k, void* scratch, size_t scratch_bytes, mtx_stream stream) {
   if (x_type != MTX_BF16 && x_type != MTX_F32 && x_type != MTX_E4M3) return fail(MTX_ERR_ARG, "x_type %d is none of MTX_BF16, MTX_F32 and MTX_E4M3", x_type);
   if (out_type != MTX_BF16 && out_type != MTX_F32) return fail(MTX_ERR_ARG, "out_type %d: a product is stored as MTX_BF16 or MTX_F32", out_type);
-  if (rows < 0 || n < 1 || k < 1 || k > kMaxK || ldx < k || ldw < k || ldo < n) return fail(MTX_ERR_ARG, "bad rows / n / k / ldx / ldw / ldo");
+  if (rows < 0 || rows > kMost || n < 1 || n > kMost || k < 1 || k > kMost || ldx < k || ldw < k || ldo < n) return fail(MTX_ERR_ARG, "bad rows / n / k / ldx / ldw / ldo");
   if (rows == 0) return MTX_OK;
   const bool quantised = x_type == MTX_E4M3;
   if (!x || !wq || !w_scale || !out || (quantised && !x_scale)) return fail(MTX_ERR_ARG, "null argument");

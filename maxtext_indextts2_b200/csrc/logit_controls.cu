@@ -5,7 +5,7 @@
 
 namespace {
 
-constexpr int kMaxVocab = 1 << 30;  // (token numbers, rounded up to a warp's run, stay 32-bit)
+constexpr int kMaxVocab = 1 << 28;  // (token numbers, rounded up to what a warp goes through, stay 32-bit)
 
 int check_record(const void* seen, long long ld_seen, const void* touched, long long ld_touched, int slots, int vocab) {
   if (slots < 1 || ld_seen < vocab || ld_seen % 8 != 0 || (reinterpret_cast<uintptr_t>(seen) & 15) != 0)
