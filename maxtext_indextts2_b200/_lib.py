@@ -415,6 +415,8 @@ def _declare(lib) -> None:
   lib.mtx_linear_fp8_scratch_bytes.argtypes = [i32, i32]
   lib.mtx_linear_fp8.restype = i32
   lib.mtx_linear_fp8.argtypes = [vp, i32, i64, vp, vp, i64, vp, vp, i32, i64, i32, i32, i32, vp, sz, vp]
+  lib.mtx_linear_fp8_stalls.restype = i32
+  lib.mtx_linear_fp8_stalls.argtypes = [c.POINTER(c.c_uint32)]
   lib.mtx_control_logits.restype = i32
   lib.mtx_control_logits.argtypes = [vp, i64, vp, i64, i32, i32, c.POINTER(LogitControls), vp]
   lib.mtx_note_tokens.restype = i32

@@ -270,4 +270,10 @@ int mtx_linear_fp8(const void* x, int x_type, long long ldx, const float* x_scal
   return launch_linear(c, st);
 }
 
+int mtx_linear_fp8_stalls(uint32_t* count) {
+  if (!count) return fail(MTX_ERR_ARG, "null argument");
+  MTX_CUDA(cudaMemcpyFromSymbol(count, d_fp8_waits_failed, sizeof(uint32_t)));
+  return MTX_OK;
+}
+
 }  // extern "C"

@@ -74,8 +74,8 @@ struct QuantParams {
 
 // N times eight values per thread, 16 lanes side by side: at(i, row, c, n) says that the i-th are row `row`'s from column c on, of which n are there (eight or more: all;
 // none or less: all are 0).  VEC: rows lie on 16 bytes.  Otherwise a lane loads the aligned 16 bytes in which its values
-// begin, takes the following ones from the next lane and shifts, unless that would reach over the matrix's ends.  (4001 x 10239: 32 us with pieces of
-// their own for every lane and a choice per load, 58 value by value.)
+// begin, takes the following ones from the next lane and shifts, unless that would reach over the matrix's ends.  (4001 x 10239: 27 us; 32 with two pieces of
+// its own for every lane and a choice per load.)
 template <class T, bool VEC, int N, class At>
 __device__ __forceinline__ void load_all(const QuantParams& p, At&& at, Raw8<T> (&v)[N]) {
   constexpr int W = Raw8<T>::kWords, kPieces = W / 4;
@@ -162,7 +162,9 @@ __device__ __forceinline__ void load_all(const QuantParams& p, At&& at, Raw8<T> 
 
 // ---- quantisation ----------------------------------------------------------------------------------------------------------------
 //
-// One pass: a thread keeps its values until the block's maximum is known.  Bound: bytes (2 or 4 in, 1 out per value).
+// One pass: a thread keeps its values until the block's maximum is known.  Bound: bytes (2 or 4 in, 1 out per value).  4001 x 10240 bfloat16 by rows 19.8 us (6.2 TB/s; 29.3 with one
+// load per thread and two divisions per eight values), 264192 x 1280 by blocks 149 us (6.8 TB/s; 455 with the values held as fp32, two CTAs per SM instead
+// of four).  Rows at odd places: 27 and 221 us, the shifts.
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantGroup = 4;  // blocks of a row that half a warp works on at a time
@@ -241,7 +243,8 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : VEC ? 4 : 
 // ---- products ----------------------------------------------------------------------------------------------------------------------
 //
 // Both kernels multiply one block of 128 columns at a time on the tensor cores (kind::f8f6f4, four instructions of 32), each into an accumulator of its
-// own in TMEM, and add acc += d * (xs ws) in registers, so that the scales are applied once per block and sums are fp32 throughout.
+// own in TMEM, and add acc += d * (xs ws) in registers, so that the scales are applied once per block and sums are fp32 throughout.  (The block-scaled
+// MMAs take powers of two alone as scales.)  The way of an accumulator from the MMAs' barrier through registers and back to the next MMAs is what many rows are bound by.
 
 struct Fp8LinearParams {
   const float* x_scale;
@@ -258,8 +261,8 @@ struct Fp8LinearParams {
 };
 
 // Waits that run out (some 2 s: a protocol error) end the kernel instead of the GPU: the CTA's roles go through their loops without waiting and without
-// issuing anything, its copies get time to land, TMEM is freed, and this counter says that results are wrong.  (Everything inline and no way out of
-// the loops: a call or a break behind a wait makes the compiler guard every tcgen05 instruction against divergence.)
+// issuing anything, its copies get time to land, TMEM is freed, and this counter (mtx_linear_fp8_stalls) says that results are wrong.  (Everything inline and no way
+// out of the loops: with a call and breaks behind the waits 4096 x 5376 by 21504 took 833 us, so 451.)
 __device__ unsigned int d_fp8_waits_failed = 0;
 
 __device__ __forceinline__ bool fp8_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
@@ -313,7 +316,7 @@ __device__ __forceinline__ float pair_lo(unsigned long long v) { return __uint_a
 __device__ __forceinline__ float pair_hi(unsigned long long v) { return __uint_as_float(uint32_t(v >> 32)); }
 
 // Hands an accumulator back to the thread that issues MMAs.  The loads from TMEM are complete (wait::ld) and ordered (tcgen05.fence), nothing else is published:
-// a releasing arrive would wait for the next block's scales, which are on their way from L2 at that moment.
+// a releasing arrive would wait for the next block's scales, which are on their way from L2 at that moment (4096 x 5376 by 21504: 1106 us, 833 without).
 __device__ __forceinline__ void fp8_release(uint64_t* bar) {
   asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -352,7 +355,8 @@ struct Fp8SmemTail {
 // The 128 rows of a weight tile are the MMA's M, BN activation rows its N: nothing is padded but the last few rows, and a CTA takes in 16 KB of weights
 // with BN * 128 bytes of activations per block.  An epilogue thread owns a weight row and BN sums.  Bound: the weights' bytes.
 // Few tiles are shared by the CTAs of a cluster, each with a part of the blocks, and the parts are added over distributed shared memory in
-// the order of the blocks (so that a result never depends on timing).
+// the order of the blocks (so that a result never depends on timing).  1 x 1280 by 264192 columns 52.1 us (the weights at 6.5 TB/s), 64 rows 67.4 (the
+// logits, 68 MB, beside them); 64 x 5120 by 1280, ten tiles in eight parts each, 7.8: launch, fill and exchange, the weights are 1.0 of it.
 
 template <int BN>
 __host__ __device__ constexpr int fp8_stream_warps() { return BN <= 32 ? 4 : BN / 8; }  // epilogue warps: 16 or 32 activation rows each
@@ -581,15 +585,17 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
 // ---- many rows: pairs of CTAs ------------------------------------------------------------------------------------------------------------
 //
 // Two CTAs of a cluster (a TPC's two SMs) work on one tile of 256 rows x BN columns with cta_group::2 MMAs: CTA c of the pair holds rows 128 c .. of the
-// activations and half of the weight tile, so an SM takes in 16 KB + BN * 64 bytes per block for BN * 2^15 multiply-adds.  A thread of the
-// epilogue warps owns one row and 64 of the columns: its scale of a block is ONE number, which the sums take in with packed fused
+// activations and half of the weight tile, so an SM takes in 16 KB + BN * 64 bytes per block for BN * 2^14 multiply-adds.  A thread of the
+// epilogue warps owns one row and half of the columns: its scale of a block is ONE number, which the sums take in with packed fused
 // multiply-adds while the next block's MMAs run into another accumulator.
+// 4096 x 5376 by 21504: 400 us, 2.37 PFLOP/s.  A block of a 256-column tile takes 0.42 us where its MMAs take 0.28: TMEM holds two such accumulators, and one is
+// on its way (MMAs, barrier, 128 columns through registers in some 450 cycles, barriers of both CTAs) for two blocks.  Without the sums it is 0.34.
 
 constexpr int kFp8PairRows = 256;
 
-// Epilogue warps: 32 rows x half of the columns each.  (Sixteen with a quarter of the columns take longer, 540 us for 420 at 4096 x 5376 x 21504: every
-// arrival at the leader's barrier is on the way from one block's sums to the next MMAs into their accumulator.  So did registers moved from the
-// first warps to these: 480 us.)
+// Epilogue warps: 32 rows x half of the columns each.  (Sixteen with a quarter of the columns take longer, 532 us for 421 at 4096 x 5376 by 21504: every
+// arrival at the leader's barrier is on the way from one block's sums to the next MMAs into their accumulator.  So do registers moved from the
+// first warps to these, 482 us.)
 template <int BN>
 __host__ __device__ constexpr int fp8_pair_warps() { return 8; }
 // warp 0: copies, warp 1: MMAs, then the sums

@@ -1,5 +1,7 @@
 """8-bit values with a scale per block of 128 and products of them (csrc/fp8_linear.cuh) against their definition in 64 bits."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -234,3 +236,9 @@ def test_refuses_memory_of_the_host():
   x, q, s = torch.zeros(4, 128), torch.zeros(4, 128, dtype=torch.uint8, device="cuda"), torch.zeros(4, 1, device="cuda")
   assert lib.mtx_quantize_fp8(x.data_ptr(), _lib.F32, 128, 4, 128, 1, q.data_ptr(), 128, s.data_ptr(), stream()) == _lib.MTX_ERR_ARG
   assert "not device memory" in _lib.last_error()
+
+
+def test_no_wait_ran_out():
+  count = ctypes.c_uint32(7)
+  _lib.check(_lib.load().mtx_linear_fp8_stalls(ctypes.byref(count)))
+  assert count.value == 0

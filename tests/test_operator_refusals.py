@@ -49,6 +49,10 @@ def test_scratch_of_a_linear(lib):
   assert need >= 3 * 144 + 3 * 2 * 4
 
 
+def test_stalls(lib):
+  refused(lib.mtx_linear_fp8_stalls(None), "null")
+
+
 CONTROL = dict(logits=A, ld=64, out=A + 65536, ldo=64, rows=2, vocab=64, controls=None, stream=None)
 
 
