@@ -5,13 +5,15 @@
 // all of a vocabulary's groups untouched, so that the penalties read 1/64 byte per logit instead of 2.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mtx {
 
 constexpr int kControlThreads = 256;
 constexpr int kControlRun = 256;  // tokens that a warp works on at a time: twice four per lane
-constexpr int kControlWarps = 148 * 192;  // warps of a large call: three times as many as run at once (32 registers per thread), for an even end
+constexpr int kControlWarps = 148 * 192;  // warps of a large call: four times as many as run at once (40 registers per thread), for an even end
 
 struct ControlParams {
   const float* logits;
@@ -69,10 +71,10 @@ enum ControlForm {
 };
 
 // Bound: bytes, 4 read and 4 written per logit where all is allowed.  Four tokens of which none is allowed are written without being read, and in place four that nothing changes are
-// neither.  64 x 264192 logits: unmasked 26.5 us (5.1 TB/s), behind masks that leave a few 24; at an odd size of the vocabulary 32 (value by value 53).  A warp
-// takes up to three or so neighbouring runs (one each: 27.8, eight each: 30.2); runs fetched ahead in more registers by fewer warps took 30 to 39.
+// neither.  64 x 264192 logits: unmasked 26.2 us (5.2 TB/s), behind masks that leave a few 23.0, where the stores alone take 19.5; at an odd size of the vocabulary 33.
+// A warp takes up to three or so neighbouring runs (one each: 29.1 and 30.1, eight each: 28.5 and 23.7); runs fetched ahead in more registers by fewer warps took 30 to 39.
 template <int FORM>
-__global__ void __launch_bounds__(kControlThreads, 8) control_logits_kernel(const ControlParams p) {
+__global__ void __launch_bounds__(kControlThreads, 6) control_logits_kernel(const ControlParams p) {
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31;
@@ -112,61 +114,88 @@ __global__ void __launch_bounds__(kControlThreads, 8) control_logits_kernel(cons
   if (FORM == kControlSingle) {
     for (int t = first + lane; t < last; t += 32) one(t);
   } else {
-    for (int t0 = begin; t0 < last; t0 += kControlRun) {
-      if (t0 < 0 || t0 + kControlRun > p.vocab) {  // the row's ends
-        for (int t = max(t0, 0) + lane; t < min(t0 + kControlRun, p.vocab); t += 32) one(t);
-        continue;
-      }
-      // everything of the run on its way, then the arithmetic: a lane's four tokens of either half as bits of the mask, logits and words of `seen`
-      uint32_t may[2] = {0xfu, 0xfu};
-      if (allowed != nullptr) {
+    auto runs = [&](auto masked) {
+      constexpr bool MASKED = decltype(masked)::value;
+      for (int t0 = begin; t0 < last; t0 += kControlRun) {
+        if (t0 < 0 || t0 + kControlRun > p.vocab) {  // the row's ends
+          for (int t = max(t0, 0) + lane; t < min(t0 + kControlRun, p.vocab); t += 32) one(t);
+          continue;
+        }
+        const int t = t0 + lane * 4;  // and 128 further on
+        float* to = out + t;
+        uint32_t may[2] = {0xfu, 0xfu};
+        if (MASKED) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t* word = allowed + ((t + j * 128) >> 5);
+            const uint32_t hi = FORM == kControlShifted && (t & 31) > 28 ? word[1] : 0u;
+            may[j] = __funnelshift_r(word[0], hi, t & 31) & 0xfu;
+          }
+          if (!__any_sync(0xffffffffu, (may[0] | may[1]) != 0)) {  // (most runs of a mask that leaves one part of the vocabulary)
+            *reinterpret_cast<float4*>(to) = *reinterpret_cast<float4*>(to + 128) = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            continue;
+          }
+        }
+        // of `touched`: one word where runs begin at multiples of 256, else the end of one and nearly all of the next
+        uint32_t hit = 0;
+        if (seen != nullptr) {
+          hit = 0xffffffffu;
+          if (touched != nullptr) {
+            hit = touched[t0 >> 8];
+            if (FORM == kControlShifted) hit |= touched[(t0 + kControlRun - 1) >> 8];
+          }
+        }
+        bool marked[2] = {false, false};
+        if (hit != 0) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (FORM == kControlAligned) marked[j] = hit >> (t + j * 128 >> 3 & 31) & 1;
+            else marked[j] = touched_one(t + j * 128) || touched_one(t + j * 128 + 3);
+            marked[j] = marked[j] && may[j] != 0;
+          }
+        }
+        float4 v[2];
+        uint2 w[2];  // words of `seen`
+        bool write[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int t = t0 + j * 128 + lane * 4;
-          const uint32_t lo = allowed[t >> 5], hi = FORM == kControlShifted && (t & 31) > 28 ? allowed[(t >> 5) + 1] : 0u;
-          may[j] = __funnelshift_r(lo, hi, t & 31) & 0xfu;
+          write[j] = !in_place || may[j] != 0xfu || marked[j];
+          v[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          w[j] = make_uint2(0, 0);
+          if ((!MASKED || may[j] != 0) && write[j]) v[j] = *reinterpret_cast<const float4*>(in + t + j * 128);
+          if (marked[j]) {
+            const uint16_t* word = seen + t + j * 128;
+            if (FORM == kControlAligned) w[j] = *reinterpret_cast<const uint2*>(word);
+            else w[j] = make_uint2(word[0] | uint32_t(word[1]) << 16, word[2] | uint32_t(word[3]) << 16);
+          }
         }
-      }
-      uint32_t hit[2] = {0, 0};  // of `touched`: one word where runs begin at multiples of 256, else the end of one and nearly all of the next
-      if (seen != nullptr) {
-        hit[0] = touched != nullptr ? touched[t0 >> 8] : 0xffffffffu;
-        if (FORM == kControlShifted) hit[1] = touched != nullptr ? touched[(t0 + kControlRun - 1) >> 8] : 0xffffffffu;
-      }
-      float4 v[2];
-      uint2 w[2];
-      bool same[2];
+        if (hit != 0) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int t = t0 + j * 128 + lane * 4;
-        bool marked = hit[FORM == kControlShifted && t >> 8 != t0 >> 8] >> (t >> 3 & 31) & 1;
-        if (FORM == kControlShifted) marked = marked || (hit[(t + 3) >> 8 != t0 >> 8] >> ((t + 3) >> 3 & 31) & 1);
-        marked = marked && may[j] != 0;
-        same[j] = in_place && may[j] == 0xfu && !marked;
-        v[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        w[j] = make_uint2(0, 0);
-        if (may[j] != 0 && !same[j]) v[j] = *reinterpret_cast<const float4*>(in + t);
-        if (marked) {
-          if (FORM == kControlAligned) w[j] = *reinterpret_cast<const uint2*>(seen + t);
-          else w[j] = make_uint2(seen[t] | uint32_t(seen[t + 1]) << 16, seen[t + 2] | uint32_t(seen[t + 3]) << 16);
+          for (int j = 0; j < 2; ++j) {
+            if (w[j].x != 0) {
+              v[j].x = penalised(v[j].x, w[j].x & 0xffffu, repetition, presence, frequency);
+              v[j].y = penalised(v[j].y, w[j].x >> 16, repetition, presence, frequency);
+            }
+            if (w[j].y != 0) {
+              v[j].z = penalised(v[j].z, w[j].y & 0xffffu, repetition, presence, frequency);
+              v[j].w = penalised(v[j].w, w[j].y >> 16, repetition, presence, frequency);
+            }
+          }
         }
-      }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (w[j].x != 0) {
-          v[j].x = penalised(v[j].x, w[j].x & 0xffffu, repetition, presence, frequency);
-          v[j].y = penalised(v[j].y, w[j].x >> 16, repetition, presence, frequency);
+        for (int j = 0; j < 2; ++j) {
+          if (MASKED) {
+            if (!(may[j] & 1)) v[j].x = -INFINITY;
+            if (!(may[j] & 2)) v[j].y = -INFINITY;
+            if (!(may[j] & 4)) v[j].z = -INFINITY;
+            if (!(may[j] & 8)) v[j].w = -INFINITY;
+          }
+          if (write[j]) *reinterpret_cast<float4*>(to + j * 128) = v[j];
         }
-        if (w[j].y != 0) {
-          v[j].z = penalised(v[j].z, w[j].y & 0xffffu, repetition, presence, frequency);
-          v[j].w = penalised(v[j].w, w[j].y >> 16, repetition, presence, frequency);
-        }
-        if (!(may[j] & 1)) v[j].x = -INFINITY;
-        if (!(may[j] & 2)) v[j].y = -INFINITY;
-        if (!(may[j] & 4)) v[j].z = -INFINITY;
-        if (!(may[j] & 8)) v[j].w = -INFINITY;
-        if (!same[j]) *reinterpret_cast<float4*>(out + t0 + j * 128 + lane * 4) = v[j];
       }
-    }
+    };
+    if (allowed != nullptr) runs(std::true_type());
+    else runs(std::false_type());
   }
 
   if (p.bias_off != nullptr) {
