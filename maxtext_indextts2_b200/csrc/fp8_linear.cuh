@@ -365,9 +365,9 @@ __host__ __device__ constexpr int fp8_stream_buffers() { return BN <= 64 && BN !
 template <int BN>
 __host__ __device__ constexpr int fp8_stream_stage_bytes() { return kFp8OperandBytes + BN * kScaleBlock; }
 template <int BN>
-constexpr size_t fp8_stream_smem_bytes(int stages) {
-  return 1024 + size_t(stages) * fp8_stream_stage_bytes<BN>() + 4 * 2 * BN * sizeof(float) + sizeof(Fp8SmemTail) + 16;
-}
+__host__ __device__ constexpr int fp8_stream_tail_at(int stages) { return stages * fp8_stream_stage_bytes<BN>() + 4 * 2 * BN * int(sizeof(float)); }
+template <int BN>
+constexpr size_t fp8_stream_smem_bytes(int stages) { return 1024 + fp8_stream_tail_at<BN>(stages) + sizeof(Fp8SmemTail); }
 
 template <int BN>
 __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
@@ -376,7 +376,8 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* factors = reinterpret_cast<float*>(smem + size_t(p.stages) * kStage);  // [warps][2][kCols]
-  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(factors + kWarps * 2 * kCols);
+  static_assert(kWarps * 2 * kCols == 4 * 2 * BN, "the factors lie between the stages and the tail");
+  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(smem + fp8_stream_tail_at<BN>(p.stages));
   volatile int* failed = &tail->failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.y;
   const int b0 = int((long long)part * p.blocks / p.splits), b1 = int((long long)(part + 1) * p.blocks / p.splits), per = b1 - b0;
@@ -607,9 +608,9 @@ __host__ __device__ constexpr int fp8_pair_staged() { return fp8_pair_warps<BN>(
 template <int BN>
 __host__ __device__ constexpr int fp8_pair_stage_bytes() { return kFp8OperandBytes + BN / 2 * kScaleBlock; }
 template <int BN>
-constexpr size_t fp8_pair_smem_bytes(int stages) {
-  return 1024 + size_t(stages) * fp8_pair_stage_bytes<BN>() + fp8_pair_staged<BN>() + sizeof(Fp8SmemTail) + 16;
-}
+__host__ __device__ constexpr int fp8_pair_tail_at(int stages) { return stages * fp8_pair_stage_bytes<BN>() + fp8_pair_staged<BN>(); }
+template <int BN>
+constexpr size_t fp8_pair_smem_bytes(int stages) { return 1024 + fp8_pair_tail_at<BN>(stages) + sizeof(Fp8SmemTail); }
 template <int BN>
 constexpr int fp8_pair_stages() {
   const int n = int((227 * 1024 - fp8_pair_smem_bytes<BN>(0)) / fp8_pair_stage_bytes<BN>());
@@ -628,7 +629,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* staged = smem + size_t(p.stages) * kStage;
-  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(staged + fp8_pair_staged<BN>());
+  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(smem + fp8_pair_tail_at<BN>(p.stages));
   volatile int* failed = &tail->failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(blockIdx.x) & 1, pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
@@ -742,12 +743,33 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
               tma_store_2d(&tm_out, to, col0 + c, row0);
               asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
-          } else {  // results at odd places: a row's values by neighbouring lanes
+          } else {  // results at odd places: a row's values by neighbouring lanes, sixteen rows on their way at a time (5310 x 4000 by 13887: 418 us row by row, 284 so, 265 at 13888)
             __syncwarp();
-            OUT* o = static_cast<OUT*>(p.out) + row0 * p.ldo + col0 + c;
             const int rows = min(32, p.rows - row0), cols = min(kBox, p.n - col0 - c);
-            for (int r = 0; r < rows; ++r, o += p.ldo)
-              for (int i = lane; i < cols; i += 32) o[i] = *reinterpret_cast<const OUT*>(to + r * 128 + (((i / (kBox / 8)) ^ (r & 7)) << 4) + i % (kBox / 8) * sizeof(OUT));
+            OUT* o = static_cast<OUT*>(p.out) + row0 * p.ldo + col0 + c + lane;
+            auto value = [&](int r, int k) {
+              const int i = lane + 32 * k;
+              return *reinterpret_cast<const OUT*>(to + r * 128 + (((i / (kBox / 8)) ^ (r & 7)) << 4) + i % (kBox / 8) * sizeof(OUT));
+            };
+            if (rows == 32 && cols == kBox) {
+#pragma unroll 1
+              for (int r0 = 0; r0 < 32; r0 += 16) {
+                OUT x[16][kBox / 32];
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+#pragma unroll
+                  for (int k = 0; k < kBox / 32; ++k) x[r][k] = value(r0 + r, k);
+#pragma unroll
+                for (int r = 0; r < 16; ++r, o += p.ldo)
+#pragma unroll
+                  for (int k = 0; k < kBox / 32; ++k) o[32 * k] = x[r][k];
+              }
+            } else {
+              for (int r = 0; r < rows; ++r, o += p.ldo)
+#pragma unroll
+                for (int k = 0; k < kBox / 32; ++k)
+                  if (lane + 32 * k < cols) o[32 * k] = value(r, k);
+            }
             __syncwarp();
           }
         }
