@@ -183,9 +183,9 @@ int launch_pair(const Fp8Call& c, cudaStream_t st) {
 }
 
 // Which kernel: up to 64 rows the streamed weights.  Above, each form's time as it was measured, in ns: what a call takes besides its blocks, and in every wave of
-// tiles the blocks and the tile's end, which goes by the results' type and place.  (Measured and by this, us: 200 x 2560 by 10240 streamed 23.2 and 26.3, 128 columns 17.9 and
-// 18.5, 256 columns 15.2 and 14.3; 512 x 10240 by 2560 42.9 and 45.4, 30.2 and 30.5, 40.4 and 39.5; 333 x 5120 by 1280 11.8 and 12.7, 17.4 and 17.9, 23.2 and 22.7;
-// 1570 x 132 by 10009 in fp32 24.7 and 24.8, 29.9 and 28.1, 31.0 and 30.9.)
+// tiles the blocks and the tile's end, which goes by the results' type and place.  (Measured and by this, us: 200 x 2560 by 10240 streamed 23.2 and 24.3, 128 columns 17.9 and
+// 18.5, 256 columns 15.2 and 14.7; 512 x 10240 by 2560 42.9 and 41.4, 30.2 and 30.5, 40.4 and 40.5; 333 x 5120 by 1280 11.8 and 12.2, 17.4 and 17.9, 23.2 and 23.3; 333 x 2560
+// by 10240 23.3 and 24.3, 24.3 and 25.4, 25.9 and 25.1; 1570 x 132 by 10009 in fp32 24.7 and 24.8, 29.9 and 28.1, 31.0 and 31.0.)
 int launch_linear(const Fp8Call& c, cudaStream_t st) {
   const int rows = c.p.rows;
   if (rows <= 16) return launch_stream<16>(c, st);
@@ -195,13 +195,13 @@ int launch_linear(const Fp8Call& c, cudaStream_t st) {
   const long long blocks = c.p.blocks, tiles128 = (long long)((rows + 127) / 128) * ((c.p.n + 127) / 128);
   int splits;
   MTX_TRY(stream_splits<128>(tiles128, c.p.blocks, &splits));
-  const long long stream = 4500 + (splits > 1 ? 2300 : 0) + (tiles128 * splits + kSms - 1) / kSms * ((blocks + splits - 1) / splits * 500 + (f32 ? 1900 : 900));
+  const long long stream = 4500 + (splits > 1 ? 2300 : 0) + (tiles128 * splits + kSms - 1) / kSms * ((blocks + splits - 1) / splits * 450 + (f32 ? 2000 : 900));
   auto pair = [&](int bn, long long base, long long block, long long end) {
     const long long tiles = (long long)((rows + kFp8PairRows - 1) / kFp8PairRows) * ((c.p.n + bn - 1) / bn);
     return base + (tiles + kSms / 2 - 1) / (kSms / 2) * (blocks * block + end);
   };
   const long long pair128 = pair(128, 4700, 315, f32 ? (aligned ? 1450 : 2300) : aligned ? 600 : 1500);
-  const long long pair256 = pair(256, 4300, 420, f32 ? (aligned ? 3850 : 5800) : aligned ? 1600 : 3700);
+  const long long pair256 = pair(256, 4300, 430, f32 ? (aligned ? 3850 : 5800) : aligned ? 1800 : 3700);
   if (stream <= pair128 && stream <= pair256) return launch_stream<128>(c, st);
   if (pair128 <= pair256) return c.p.out_f32 ? launch_pair<128, float>(c, st) : launch_pair<128, bf16>(c, st);
   return c.p.out_f32 ? launch_pair<256, float>(c, st) : launch_pair<256, bf16>(c, st);
