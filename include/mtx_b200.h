@@ -708,7 +708,8 @@ int mtx_sample_rows(const float* logits, int rows, long long ld, int vocab, int 
  * a block: scale = A / 448, q = e4m3(x * (448 / A)), both fractions and the product rounded to fp32.  A NaN makes its block's scale
  * and values NaN, an infinity the scale infinite and itself NaN, so that products of its row are NaN.
  * q: pitch ldq, both base and pitch whole 16 bytes (bytes from k to ldq of a row are left as they are); scale: fp32
- * [ceil(rows / block_rows), ceil(k / 128)].  rows, k <= 2^30; results may not overlap x. */
+ * [ceil(rows / block_rows), ceil(k / 128)].  rows, k <= 2^30; results may not overlap x.  x at any multiple of its type's size, with any pitch (16-byte
+ * aligned rows are the fast ones).  Pinned host memory is refused here and by mtx_linear_fp8. */
 int mtx_quantize_fp8(const void* x, int x_type, long long ldx, int rows, int k, int block_rows, void* q, long long ldq, float* scale, mtx_stream stream);
 
 /* out[m, n] = sum over the blocks b of 128 columns of x_scale[m, b] * w_scale[n / 128, b] * sum_{k in b} x[m, k] * wq[n, k], sums in fp32:

@@ -141,6 +141,7 @@ template <int BN>
 int launch_stream(const Fp8Call& c, cudaStream_t st) {
   constexpr int kPerSm = BN <= 32 ? 3 : BN == 64 ? 2 : 1;  // CTAs that may share an SM
   constexpr int kLeast = BN == 16 ? 4 : BN == 32 ? 3 : BN == 64 ? 4 : 6;
+  static_assert(kLeast >= fp8_stream_buffers<BN>(), "a stage's barrier would turn twice before the sums have seen it");
   Fp8LinearParams p = c.p;
   const long long tiles = (long long)((p.n + 127) / 128) * ((p.rows + BN - 1) / BN);
   if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
@@ -166,6 +167,7 @@ int launch_pair(const Fp8Call& c, cudaStream_t st) {
   Fp8LinearParams p = c.p;
   const long long tiles = (long long)((p.rows + kFp8PairRows - 1) / kFp8PairRows) * ((p.n + BN - 1) / BN);
   if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
+  static_assert(fp8_pair_stages<BN>() >= 512 / BN, "a stage's barrier would turn twice before the sums have seen it");
   p.stages = fp8_pair_stages<BN>();
   p.tma_store = fits16(p.out, p.ldo * (long long)sizeof(OUT));
   const size_t smem = fp8_pair_smem_bytes<BN>(p.stages);
@@ -218,6 +220,7 @@ int mtx_quantize_fp8(const void* x, int x_type, long long ldx, int rows, int k, 
   if (rows == 0) return MTX_OK;
   if (!x || !q || !scale) return fail(MTX_ERR_ARG, "null argument");
   if (!fits16(q, ldq)) return fail(MTX_ERR_ARG, "8-bit values lie at a 16-byte aligned base and a pitch of whole 16 bytes");
+  if (!lie_on(x_type == MTX_BF16 ? 2 : 4, {x}) || !lie_on(4, {scale})) return fail(MTX_ERR_ARG, "x and scale lie on multiples of their types' sizes");
   if ((long long)rows * blocks_of(k) >= 1ll << 31) return fail(MTX_ERR_ARG, "more than 2^31 blocks");
   MTX_TRY(on_this_device({x, q, scale}));
   return quantize(x, x_type, ldx, rows, k, block_rows, q, ldq, scale, blocks_of(k), 1, static_cast<cudaStream_t>(stream));
@@ -240,6 +243,8 @@ int mtx_linear_fp8(const void* x, int x_type, long long ldx, const float* x_scal
   if ((long long)rows * blocks_of(k) >= 1ll << 31) return fail(MTX_ERR_ARG, "more than 2^31 blocks");
   if (!quantised && (!scratch || scratch_bytes < mtx_linear_fp8_scratch_bytes(rows, k) || (reinterpret_cast<uintptr_t>(scratch) & 15) != 0))
     return fail(MTX_ERR_ARG, "values that are quantised here need a 16-byte aligned scratch of mtx_linear_fp8_scratch_bytes(rows, k) bytes");
+  if (!lie_on(x_type == MTX_BF16 ? 2 : 4, {x}) || !lie_on(out_type == MTX_BF16 ? 2 : 4, {out}) || !lie_on(4, {w_scale, quantised ? x_scale : nullptr}))
+    return fail(MTX_ERR_ARG, "x, out and the scales lie on multiples of their types' sizes");
   MTX_TRY(on_this_device({x, quantised ? x_scale : static_cast<const void*>(scratch), wq, w_scale, out}));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Fp8Call c;

@@ -24,7 +24,8 @@ int mtx_control_logits(const float* logits, long long ld, float* out, long long 
   if (!c) return fail(MTX_ERR_ARG, "null controls");
   if (rows == 0) return MTX_OK;
   if (!logits || !out) return fail(MTX_ERR_ARG, "null argument");
-  if (((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 3) != 0) return fail(MTX_ERR_ARG, "logits lie on 4 bytes");
+  if (!lie_on(4, {logits, out, c->slot, c->repetition, c->presence, c->frequency, c->bias_off, c->bias_token, c->bias_value, c->allowed, c->allowed_row}))
+    return fail(MTX_ERR_ARG, "logits and their controls lie on 4 bytes");
   if (logits == out && ld != ldo) return fail(MTX_ERR_ARG, "logits that are controlled in place have one pitch");
   if ((c->repetition || c->presence || c->frequency) && !c->seen) return fail(MTX_ERR_ARG, "penalties need the record of seen tokens");
   ControlParams p;
@@ -65,7 +66,7 @@ int mtx_control_logits(const float* logits, long long ld, float* out, long long 
   if (p.runs > runs) p.runs = int(runs);
   p.spans = int((runs - 1) / ((long long)p.runs * (kControlThreads / 32)) + 1);
   if ((long long)rows * p.spans >= 1ll << 31) return fail(MTX_ERR_ARG, "rows * vocab is too large for one call");
-  MTX_TRY(on_this_device({logits, out, p.seen, p.slot, p.touched, p.repetition, p.presence, p.frequency, p.bias_off, p.bias_token, p.bias_value, p.allowed, p.allowed_row}));
+  MTX_TRY(on_this_device({logits, out, p.seen, p.slot, p.touched, p.repetition, p.presence, p.frequency, p.bias_off, p.bias_token, p.bias_value, p.allowed, p.allowed_row}, true));
   const uintptr_t a = reinterpret_cast<uintptr_t>(logits), o = reinterpret_cast<uintptr_t>(out);
   const bool aligned = ((a | o) & 15) == 0 && ld % 4 == 0 && ldo % 4 == 0, alike = ((a ^ o) & 15) == 0 && (ld - ldo) % 4 == 0;
   return launch(aligned ? control_logits_kernel<kControlAligned> : alike ? control_logits_kernel<kControlShifted> : control_logits_kernel<kControlSingle>,
@@ -79,7 +80,8 @@ int mtx_note_tokens(uint16_t* seen, long long ld_seen, uint32_t* touched, long l
   if (!seen || !token) return fail(MTX_ERR_ARG, "null argument");
   if (!slot && n > slots) return fail(MTX_ERR_ARG, "without slot, token i belongs to slot i: %d tokens for %d slots", n, slots);
   MTX_TRY(check_record(seen, ld_seen, touched, ld_touched, slots, vocab));
-  MTX_TRY(on_this_device({seen, touched, token, slot}));
+  if (!lie_on(4, {token, slot})) return fail(MTX_ERR_ARG, "token and slot lie on 4 bytes");
+  MTX_TRY(on_this_device({seen, touched, token, slot}, true));
   NoteParams p;
   p.seen = seen;
   p.ld_seen = ld_seen;

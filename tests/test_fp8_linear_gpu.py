@@ -236,6 +236,8 @@ def test_refuses_memory_of_the_host():
   x, q, s = torch.zeros(4, 128), torch.zeros(4, 128, dtype=torch.uint8, device="cuda"), torch.zeros(4, 1, device="cuda")
   assert lib.mtx_quantize_fp8(x.data_ptr(), _lib.F32, 128, 4, 128, 1, q.data_ptr(), 128, s.data_ptr(), stream()) == _lib.MTX_ERR_ARG
   assert "not device memory" in _lib.last_error()
+  x = x.pin_memory()  # (the tensor copies of a product want device memory)
+  assert lib.mtx_quantize_fp8(x.data_ptr(), _lib.F32, 128, 4, 128, 1, q.data_ptr(), 128, s.data_ptr(), stream()) == _lib.MTX_ERR_ARG
 
 
 def test_no_wait_ran_out():

@@ -239,6 +239,17 @@ def test_counts_stop_at_their_largest():
   assert touched.cpu().tolist() == [[1], [1]]
 
 
+def test_tokens_in_pinned_memory_and_refused_memory():
+  """Lists that a server fills on the host may be pinned memory; memory that the device cannot read is refused."""
+  lib, (seen, touched) = _lib.load(), record(2, 100)
+  token = torch.tensor([3, 99], dtype=torch.int32).pin_memory()
+  call = lambda t: lib.mtx_note_tokens(seen.data_ptr(), seen.stride(0), touched.data_ptr(), touched.stride(0), 2, 100, t.data_ptr(), None, 2, 0, stream())  # noqa: E731
+  assert call(token) == _lib.MTX_OK
+  assert seen.cpu().nonzero().tolist() == [[0, 3], [1, 99]]
+  assert call(torch.tensor([3, 99], dtype=torch.int32)) == _lib.MTX_ERR_ARG and "not device memory" in _lib.last_error()
+  torch.cuda.synchronize()
+
+
 def test_slots_by_order_and_a_record_without_bits():
   seen, _ = record(5, 100)
   note(seen, None, 100, [7, 8, -1, 9], None, False)

@@ -23,7 +23,8 @@ QUANT = dict(x=A, x_type=_lib.BF16, ldx=256, rows=4, k=256, block_rows=1, q=A, l
 @pytest.mark.parametrize("change,word", [
     (dict(x_type=_lib.E4M3), "x_type"), (dict(x_type=9), "x_type"), (dict(block_rows=64), "block_rows"), (dict(rows=-1), "bad rows"), (dict(k=0), "bad rows"),
     (dict(ldx=255), "bad rows"), (dict(ldq=255), "bad rows"), (dict(k=(1 << 30) + 1, ldx=1 << 31, ldq=1 << 31), "bad rows"), (dict(x=None), "null"), (dict(q=None), "null"),
-    (dict(scale=None), "null"), (dict(q=A + 8), "16-byte"), (dict(ldq=264), "16"), (dict(rows=1 << 30, k=1024, ldx=1024, ldq=1024), "2^31"), (dict(rows=(1 << 30) + 1, k=16, ldx=16, ldq=16), "bad rows"),
+    (dict(scale=None), "null"), (dict(q=A + 8), "16-byte"), (dict(x=A + 1), "multiples"), (dict(x=A + 2, x_type=_lib.F32), "multiples"), (dict(scale=A + 2), "multiples"),
+    (dict(ldq=264), "16"), (dict(rows=1 << 30, k=1024, ldx=1024, ldq=1024), "2^31"), (dict(rows=(1 << 30) + 1, k=16, ldx=16, ldq=16), "bad rows"),
 ])
 def test_quantize(lib, change, word):
   refused(lib.mtx_quantize_fp8(*{**QUANT, **change}.values()), word)
@@ -37,7 +38,8 @@ LINEAR = dict(x=A, x_type=_lib.BF16, ldx=256, x_scale=None, wq=A, ldw=256, w_sca
     (dict(x_type=3), "x_type"), (dict(out_type=_lib.E4M3), "out_type"), (dict(rows=-1), "bad rows"), (dict(n=0), "bad rows"), (dict(k=0), "bad rows"), (dict(ldx=255), "bad rows"),
     (dict(ldw=255), "bad rows"), (dict(ldo=127), "bad rows"), (dict(x=None), "null"), (dict(wq=None), "null"), (dict(w_scale=None), "null"), (dict(out=None), "null"),
     (dict(x_type=_lib.E4M3), "null"), (dict(wq=A + 4), "16-byte"), (dict(ldw=260), "16-byte"), (dict(x_type=_lib.E4M3, x_scale=A, x=A + 1), "16-byte"),
-    (dict(scratch=None), "scratch"), (dict(scratch=A + 4), "scratch"), (dict(scratch_bytes=100), "scratch"), (dict(rows=1 << 30, k=1024, ldx=1024, ldw=1024), "2^31"), (dict(rows=(1 << 30) + 1), "bad rows"), (dict(n=(1 << 30) + 1, ldo=1 << 31), "bad rows"),
+    (dict(x=A + 1), "multiples"), (dict(out=A + 1), "multiples"), (dict(out=A + 2, out_type=_lib.F32), "multiples"), (dict(w_scale=A + 2), "multiples"),
+    (dict(x_type=_lib.E4M3, x_scale=A + 1), "multiples"), (dict(scratch=None), "scratch"), (dict(scratch=A + 4), "scratch"), (dict(scratch_bytes=100), "scratch"), (dict(rows=1 << 30, k=1024, ldx=1024, ldw=1024), "2^31"), (dict(rows=(1 << 30) + 1), "bad rows"), (dict(n=(1 << 30) + 1, ldo=1 << 31), "bad rows"),
 ])
 def test_linear(lib, change, word):
   refused(lib.mtx_linear_fp8(*{**LINEAR, **change}.values()), word)
@@ -78,7 +80,8 @@ def test_no_rows_is_no_error(lib):
 @pytest.mark.parametrize("fields,word", [
     (dict(repetition=A), "need the record"), (dict(seen=A, slots=0, ld_seen=64), "record"), (dict(seen=A, slots=1, ld_seen=60), "record"), (dict(seen=A, slots=1, ld_seen=68), "record"),
     (dict(seen=A + 2, slots=1, ld_seen=64), "record"), (dict(seen=A, slots=1, ld_seen=64, touched=A), "touched"), (dict(bias_off=A), "together"), (dict(bias_token=A, bias_value=A), "together"),
-    (dict(allowed=A, ld_allowed=2), "allowed"), (dict(allowed=A, allowed_rows=1, ld_allowed=1), "allowed"),
+    (dict(slot=A + 1), "4 bytes"), (dict(seen=A, slots=1, ld_seen=64, presence=A + 2), "4 bytes"), (dict(bias_off=A, bias_token=A + 2, bias_value=A), "4 bytes"),
+    (dict(allowed=A + 1, allowed_rows=1, ld_allowed=2), "4 bytes"), (dict(allowed=A, ld_allowed=2), "allowed"), (dict(allowed=A, allowed_rows=1, ld_allowed=1), "allowed"),
 ])
 def test_fields_of_the_controls(lib, fields, word):
   refused(lib.mtx_control_logits(*{**CONTROL, "controls": _lib.LogitControls(**fields)}.values()), word)
@@ -89,7 +92,7 @@ NOTE = dict(seen=A, ld_seen=64, touched=A, ld_touched=1, slots=4, vocab=64, toke
 
 @pytest.mark.parametrize("change,word", [
     (dict(n=-1), "bad n"), (dict(vocab=0), "bad n"), (dict(vocab=(1 << 28) + 8, ld_seen=1 << 31, ld_touched=1 << 24), "bad n"), (dict(seen=None), "null"), (dict(token=None), "null"),
-    (dict(slot=None, n=5), "slot i"), (dict(ld_seen=56), "record"), (dict(seen=A + 8), "record"), (dict(slots=0), "record"), (dict(ld_touched=0), "touched"), (dict(touched=A + 2), "touched"),
+    (dict(slot=None, n=5), "slot i"), (dict(ld_seen=56), "record"), (dict(seen=A + 8), "record"), (dict(slots=0), "record"), (dict(ld_touched=0), "touched"), (dict(touched=A + 2), "touched"), (dict(token=A + 2), "4 bytes"), (dict(slot=A + 1), "4 bytes"),
 ])
 def test_note(lib, change, word):
   refused(lib.mtx_note_tokens(*{**NOTE, **change}.values()), word)
