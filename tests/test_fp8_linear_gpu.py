@@ -231,6 +231,26 @@ def test_in_a_graph_and_on_another_stream(rows):
     torch.cuda.synchronize()
 
 
+def test_calls_side_by_side():
+  """Products of every kernel on three streams at once, each with a scratch of its own, give what they give alone."""
+  shapes = [(1, 1792, 1280), (16, 2560, 5120), (30, 40000, 384), (64, 1280, 5120), (100, 640, 2048), (300, 1000, 1280), (700, 3000, 900), (2000, 2560, 640)]
+  cases = []
+  for rows, n, k in shapes:
+    x, w = inputs(rows, n, k)
+    wq, ws = quantize(w.cuda(), 128)
+    cases.append((x.cuda(), wq, ws, n, k, torch.float32))
+  alone = [linear(*c) for c in cases]
+  torch.cuda.synchronize()
+  streams, got = [torch.cuda.Stream() for _ in range(3)], []
+  for i in range(60):
+    which = (i * 5 + i // 7) % len(cases)
+    with torch.cuda.stream(streams[i % 3]):
+      got.append((which, linear(*cases[which])))
+  torch.cuda.synchronize()
+  for which, out in got:
+    assert torch.equal(out, alone[which])
+
+
 def test_refuses_memory_of_the_host():
   lib = _lib.load()
   x, q, s = torch.zeros(4, 128), torch.zeros(4, 128, dtype=torch.uint8, device="cuda"), torch.zeros(4, 1, device="cuda")
