@@ -44,6 +44,17 @@ struct Raw8 {
     for (int i = 0; i < kWords; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
     return max(top & 0xffff0000u, top << 16);
   }
+  // the words, and behind them the first M of the next lane's; for the last of 16 lanes those of `far` in lane i
+  template <int M>
+  __device__ __forceinline__ void with_next(uint32_t (&out)[kWords + 4], const uint32_t (&far)[4], int i, uint32_t lanes) const {
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) out[j] = w[j];
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      const uint32_t next = __shfl_down_sync(lanes, w[j], 1, 16), last = __shfl_sync(lanes, far[j], i, 16);
+      out[kWords + j] = (threadIdx.x & 15) == 15 ? last : next;
+    }
+  }
   __device__ __forceinline__ float value(int i) const {
     if (sizeof(T) == 4) return __uint_as_float(w[i % kWords]);
     return i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
@@ -72,36 +83,31 @@ struct QuantParams {
   long long scale_row, scale_block;  // strides of a row (of a row of blocks) and of a block of columns
 };
 
-// N times eight values per thread, 16 lanes side by side: at(i, row, c, n) says that the i-th are row `row`'s from column c on, of which n are there (eight or more: all;
-// none or less: all are 0).  VEC: rows lie on 16 bytes.  Otherwise a lane loads the aligned 16 bytes in which its values
-// begin, takes the following ones from the next lane and shifts, unless that would reach over the matrix's ends.  (4001 x 10239: 27 us; 32 with two pieces of
-// its own for every lane and a choice per load.)
-template <class T, bool VEC, int N, class At>
-__device__ __forceinline__ void load_all(const QuantParams& p, At&& at, Raw8<T> (&v)[N]) {
+// N times eight values per thread, 16 lanes side by side: the i-th are the values from `from` + i * step on, of which left(i) are there (eight or more: all; none or less: all are 0).
+// left(i) + 8 lane is the same in all 16 lanes, or not above 0 in any: nothing is read for it then.  VEC: they lie on 16 bytes.  Otherwise a lane loads the aligned 16
+// bytes in which its values begin, takes the following ones from the next lane and shifts, unless that would reach over the matrix's ends.  ALIKE: all N lie alike (step is whole
+// 16 bytes), so that they shift by one choice.  (4001 x 10239, at odd places: 24.3 us; 27.2 with an address and a choice for every eight values, 32 with two pieces of its own
+// for every lane.)
+template <class T, bool VEC, bool ALIKE, int N, class Left>
+__device__ __forceinline__ void load_all(const QuantParams& p, const T* from, long long step, Left&& left, Raw8<T> (&v)[N]) {
   constexpr int W = Raw8<T>::kWords, kPieces = W / 4;
-  const T* x = static_cast<const T*>(p.x);
-  const int lane = threadIdx.x & 15;
-  long long row;
-  int c, n;
   if (!VEC) {
+    const int lane = threadIdx.x & 15;
+    const T* x = static_cast<const T*>(p.x);
     const uintptr_t begin = reinterpret_cast<uintptr_t>(x), end = reinterpret_cast<uintptr_t>(x + (p.rows - 1) * p.ldx + p.k);
     bool inside = true;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      at(i, row, c, n);
-      const uintptr_t first = reinterpret_cast<uintptr_t>(x + row * p.ldx + (c - lane * 8)) & ~uintptr_t(15);  // of lane 0
-      inside = inside && first >= begin && first + 16 * (16 * kPieces + 1) <= end;
+      const uintptr_t first = reinterpret_cast<uintptr_t>(from - lane * 8 + i * step) & ~uintptr_t(15);  // of lane 0
+      inside = inside && (left(i) + lane * 8 <= 0 || (first >= begin && first + 16 * (16 * kPieces + 1) <= end));
     }
     if (inside) {
       const uint32_t half = 0xffffu << (threadIdx.x & 16);
-      auto piece_of = [&](int i) {
-        at(i, row, c, n);
-        return reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x + row * p.ldx + c) & ~uintptr_t(15));
-      };
+      auto piece_of = [&](int i) { return reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(from + i * step) & ~uintptr_t(15)); };
 #pragma unroll
       for (int i = 0; i < N; ++i) {
+        const bool any = left(i) + lane * 8 > 0;  // (the half warp's)
         const uint4* piece = piece_of(i);
-        const bool any = n + lane * 8 > 0;  // (the half warp's)
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
           const uint4 u = any ? __ldcs(piece + j) : make_uint4(0, 0, 0, 0);
@@ -109,52 +115,62 @@ __device__ __forceinline__ void load_all(const QuantParams& p, At&& at, Raw8<T> 
         }
       }
       uint4 far = make_uint4(0, 0, 0, 0);  // lane i: what follows lane 15's pieces of the i-th
-      if (lane < N) far = __ldg(piece_of(lane) + (15 - lane) * kPieces + kPieces);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        at(i, row, c, n);
-        const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(x + row * p.ldx + c) & 15), by = (off & 3) * 8;
-        const uint32_t f[4] = {far.x, far.y, far.z, far.w};
-        uint32_t w[W + 4];
-#pragma unroll
-        for (int j = 0; j < W; ++j) w[j] = v[i].w[j];
-        auto shift = [&](auto words) {  // by that many words and `by` bits
+      if (lane < N && left(lane) + lane * 8 > 0) far = __ldg(piece_of(lane) + (15 - lane) * kPieces + kPieces);
+      const uint32_t f[4] = {far.x, far.y, far.z, far.w};
+      if (ALIKE) {
+        const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(from) & 15);
+        auto shift = [&](auto words) {
           constexpr int O = decltype(words)::value;
 #pragma unroll
-          for (int j = 0; j <= O; ++j) {
-            const uint32_t next = __shfl_down_sync(half, w[j], 1, 16), last = __shfl_sync(half, f[j], i, 16);
-            w[W + j] = lane == 15 ? last : next;
-          }
+          for (int i = 0; i < N; ++i) {
+            uint32_t w[W + 4];
+            v[i].template with_next<O + 1>(w, f, i, half);
 #pragma unroll
-          for (int j = 0; j < W; ++j) v[i].w[j] = __funnelshift_r(w[j + O], w[j + O + 1], by);
+            for (int j = 0; j < W; ++j) v[i].w[j] = __funnelshift_r(w[j + O], w[j + O + 1], (off & 3) * 8);
+          }
         };
-        if (off >> 2 == 0) shift(std::integral_constant<int, 0>());  // (one row per half warp: all its lanes shift alike)
+        if (off >> 2 == 0) shift(std::integral_constant<int, 0>());
         else if (off >> 2 == 1) shift(std::integral_constant<int, 1>());
         else if (off >> 2 == 2) shift(std::integral_constant<int, 2>());
         else shift(std::integral_constant<int, 3>());
-        if (n < 8) v[i].cut(n);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(from + i * step) & 15);
+          uint32_t w[W + 4];
+          v[i].template with_next<4>(w, f, i, half);
+#pragma unroll
+          for (int j = 0; j < W + 2; ++j) w[j] = off & 8 ? w[j + 2] : w[j];
+#pragma unroll
+          for (int j = 0; j < W + 1; ++j) w[j] = off & 4 ? w[j + 1] : w[j];
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[i].w[j] = __funnelshift_r(w[j], w[j + 1], (off & 3) * 8);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (left(i) < 8) v[i].cut(left(i));
       return;
     }
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    at(i, row, c, n);
-    const T* from = x + row * p.ldx + c;
+    const T* at = from + i * step;
+    const int n = left(i);
 #pragma unroll
     for (int j = 0; j < W; ++j) v[i].w[j] = 0;
     if (VEC && n >= 8) {
 #pragma unroll
       for (int j = 0; j < kPieces; ++j) {
-        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(from) + j);
+        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(at) + j);
         v[i].w[4 * j] = u.x, v[i].w[4 * j + 1] = u.y, v[i].w[4 * j + 2] = u.z, v[i].w[4 * j + 3] = u.w;
       }
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (j < n) {
-          if (sizeof(T) == 4) v[i].w[j % W] = reinterpret_cast<const uint32_t*>(from)[j];
-          else v[i].w[j / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(from)[j]) << (j % 2 * 16);
+          if (sizeof(T) == 4) v[i].w[j % W] = reinterpret_cast<const uint32_t*>(at)[j];
+          else v[i].w[j / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(at)[j]) << (j % 2 * 16);
         }
     }
   }
@@ -164,7 +180,7 @@ __device__ __forceinline__ void load_all(const QuantParams& p, At&& at, Raw8<T> 
 //
 // One pass: a thread keeps its values until the block's maximum is known.  Bound: bytes (2 or 4 in, 1 out per value).  4001 x 10240 bfloat16 by rows 19.8 us (6.2 TB/s; 29.3 with one
 // load per thread and two divisions per eight values), 264192 x 1280 by blocks 149 us (6.8 TB/s; 455 with the values held as fp32, two CTAs per SM instead
-// of four).  Rows at odd places: 27 and 221 us, the shifts.
+// of four).  Rows at odd places: 24.3 and 219 us, the shifts (issue slots three quarters full).
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantGroup = 4;  // blocks of a row that half a warp works on at a time
@@ -178,17 +194,10 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const Quan
   const int lane = threadIdx.x & 15;
   const uint32_t groups = uint32_t(p.blocks + kQuantGroup - 1) / kQuantGroup, unit = blockIdx.x * (kQuantThreads / 16) + (threadIdx.x >> 4), row = unit / groups;
   const bool there = row < uint32_t(p.rows);
-  const int b0 = int(unit - row * groups) * kQuantGroup, c = b0 * kScaleBlock + lane * 8, left = there ? p.k - c : 0;
+  const int b0 = int(unit - row * groups) * kQuantGroup, c = b0 * kScaleBlock + lane * 8, left = there ? p.k - c : -kScaleBlock;
   Raw8<T> v[kQuantGroup];
   uint32_t top[kQuantGroup];
-  load_all<T, VEC>(
-      p,
-      [&](int i, long long& r, int& col, int& n) {
-        r = min(row, uint32_t(p.rows) - 1);
-        col = c + i * kScaleBlock;
-        n = left - i * kScaleBlock;
-      },
-      v);
+  load_all<T, VEC, true>(p, static_cast<const T*>(p.x) + (there ? row * p.ldx : 0) + c, kScaleBlock, [&](int i) { return left - i * kScaleBlock; }, v);
 #pragma unroll
   for (int i = 0; i < kQuantGroup; ++i) top[i] = max(v[i].largest(), kLeastLargest);
   const bool up8 = lane & 8, up4 = lane & 4;
@@ -208,7 +217,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const Quan
 
 // 128 x 128: a CTA per block, eight rows of eight values per thread.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : VEC ? 4 : 3) quantize_blocks_kernel(const QuantParams p) {
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantize_blocks_kernel(const QuantParams p) {
   __shared__ uint32_t part[kQuantThreads / 32];
   griddep_wait();
   griddep_launch_dependents();
@@ -216,14 +225,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : VEC ? 4 : 
   const int row0 = up * kScaleBlock + (threadIdx.x >> 4), c = b * kScaleBlock + (threadIdx.x & 15) * 8;
   Raw8<T> v[8];
   uint32_t top = kLeastLargest;
-  load_all<T, VEC>(
-      p,
-      [&](int i, long long& r, int& col, int& n) {
-        r = min(row0 + 16 * i, p.rows - 1);
-        col = c;
-        n = row0 + 16 * i < p.rows ? p.k - c : 0;
-      },
-      v);
+  load_all<T, VEC, false>(p, static_cast<const T*>(p.x) + row0 * p.ldx + c, 16 * p.ldx, [&](int i) { return row0 + 16 * i < p.rows ? p.k - c : -kScaleBlock; }, v);
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, v[i].largest());
   top = __reduce_max_sync(0xffffffffu, top);
