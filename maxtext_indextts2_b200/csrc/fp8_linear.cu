@@ -98,15 +98,10 @@ constexpr int fp8_stream_most_stages() {
 }
 
 // Parts of the sum that CTAs of a cluster share: as many as leave every CTA an SM to itself, all clusters at once (a cluster lies in one GPC, so that fewer
-// large ones fit than SMs).  64 rows of 5120 by 1280 columns: 16.9 us in one part, 8.8 in four, 7.8 in eight; 128 rows of 10240 by 2560 columns (20
-// tiles): 14.6 in six, 24.0 in eight, whose clusters take turns.  More tiles than SMs: one part (64 x 2560 by 10240, 80 tiles: 11.3 us, 12.6 in two).
-template <int BN>
-int stream_splits(long long tiles, int blocks, int* splits) {
-  static std::atomic<int> fit[kFp8MaxSplits + 1];  // clusters of that many CTAs that run at once; 0: not asked yet
-  static std::atomic<uint64_t> done{0};
-  const size_t smem = fp8_stream_smem_bytes<BN>(fp8_stream_most_stages<BN>());
-  MTX_TRY(allow_smem(fp8_stream_kernel<BN>, smem, done));
-  *splits = 1;
+// large ones fit than SMs).  64 rows of 5120 by 1280 columns: 16.9 us in one part, 8.8 in four, 7.8 in eight; with a CTA of 128 rows of 10240 by 2560 columns
+// (20 tiles) 14.6 in six, 24.0 in eight, whose clusters take turns.  More tiles than SMs: one part (64 x 2560 by 10240, 80 tiles: 11.3 us, 12.6 in two).
+template <class Kernel>
+int cluster_splits(Kernel kernel, int threads, size_t smem, std::atomic<int>* fit, long long tiles, int blocks) {  // fit[s]: clusters of s CTAs that run at once; 0: not asked yet
   for (int s = kFp8MaxSplits; s > 1; --s) {
     if (s > blocks || tiles * s > kSms) continue;
     int n = fit[s].load(std::memory_order_relaxed);
@@ -119,28 +114,44 @@ int stream_splits(long long tiles, int blocks, int* splits) {
       attr.val.clusterDim.y = unsigned(s);
       attr.val.clusterDim.z = 1;
       cfg.gridDim = dim3(kSms / s, s);
-      cfg.blockDim = dim3(64 + 32 * fp8_stream_warps<BN>());
+      cfg.blockDim = dim3(threads);
       cfg.dynamicSmemBytes = smem;
       cfg.attrs = &attr;
       cfg.numAttrs = 1;
-      if (cudaOccupancyMaxActiveClusters(&n, fp8_stream_kernel<BN>, &cfg) != cudaSuccess || n < 1) {
+      if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
         cudaGetLastError();
         n = 1;
       }
       fit[s].store(n, std::memory_order_relaxed);
     }
-    if (tiles <= n) {
-      *splits = s;
-      break;
-    }
+    if (tiles <= n) return s;
   }
+  return 1;
+}
+
+template <int BN>
+int stream_splits(long long tiles, int blocks, int* splits) {
+  static std::atomic<int> fit[kFp8MaxSplits + 1];
+  static std::atomic<uint64_t> done{0};
+  const size_t smem = fp8_stream_smem_bytes<BN>(fp8_stream_most_stages<BN>());
+  MTX_TRY(allow_smem(fp8_stream_kernel<BN>, smem, done));
+  *splits = cluster_splits(fp8_stream_kernel<BN>, 64 + 32 * fp8_stream_warps<BN>(), smem, fit, tiles, blocks);
+  return MTX_OK;
+}
+
+template <class OUT>
+int tile_splits(long long tiles, int blocks, int* splits) {
+  static std::atomic<int> fit[kFp8MaxSplits + 1];
+  static std::atomic<uint64_t> done{0};
+  MTX_TRY(allow_smem(fp8_tile_kernel<OUT>, kFp8TileSmem, done));
+  *splits = cluster_splits(fp8_tile_kernel<OUT>, kFp8TileThreads, kFp8TileSmem, fit, tiles, blocks);
   return MTX_OK;
 }
 
 template <int BN>
 int launch_stream(const Fp8Call& c, cudaStream_t st) {
-  constexpr int kPerSm = BN <= 32 ? 3 : BN == 64 ? 2 : 1;  // CTAs that may share an SM
-  constexpr int kLeast = BN == 16 ? 4 : BN == 32 ? 3 : BN == 64 ? 4 : 6;
+  constexpr int kPerSm = BN <= 32 ? 3 : 2;  // CTAs that may share an SM
+  constexpr int kLeast = BN == 32 ? 3 : 4;
   static_assert(kLeast >= fp8_stream_buffers<BN>(), "a stage's barrier would turn twice before the sums have seen it");
   Fp8LinearParams p = c.p;
   const long long tiles = (long long)((p.n + 127) / 128) * ((p.rows + BN - 1) / BN);
@@ -161,52 +172,67 @@ int launch_stream(const Fp8Call& c, cudaStream_t st) {
   return rc;
 }
 
-template <int BN, class OUT>
+template <class OUT>
 int launch_pair(const Fp8Call& c, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
+  static_assert(kFp8PairStages >= 512 / kFp8PairCols, "a stage's barrier would turn twice before the sums have seen it");
   Fp8LinearParams p = c.p;
-  const long long tiles = (long long)((p.rows + kFp8PairRows - 1) / kFp8PairRows) * ((p.n + BN - 1) / BN);
+  const long long tiles = (long long)((p.rows + kFp8PairRows - 1) / kFp8PairRows) * ((p.n + kFp8PairCols - 1) / kFp8PairCols);
   if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
-  static_assert(fp8_pair_stages<BN>() >= 512 / BN, "a stage's barrier would turn twice before the sums have seen it");
-  p.stages = fp8_pair_stages<BN>();
+  p.stages = kFp8PairStages;
   p.tma_store = fits16(p.out, p.ldo * (long long)sizeof(OUT));
-  const size_t smem = fp8_pair_smem_bytes<BN>(p.stages);
-  MTX_TRY(allow_smem(fp8_pair_kernel<BN, OUT>, smem, done));
+  MTX_TRY(allow_smem(fp8_pair_kernel<OUT>, kFp8PairSmem, done));
   CUtensorMap tw, tx, to;
-  MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, BN / 2));
+  MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, kFp8PairCols / 2));
   MTX_TRY(make_map_e4m3(&tx, c.x, c.k, p.rows, c.ldx, 128));
   if (p.tma_store) MTX_TRY(make_map_result(&to, p.out, p.out_f32, p.n, p.rows, p.ldo));
   else to = tx;  // (not read)
   const unsigned pairs = unsigned(tiles < kSms / 2 ? tiles : kSms / 2);
   g_cluster_x = 2;
-  const int rc = launch(fp8_pair_kernel<BN, OUT>, dim3(2 * pairs), dim3(fp8_pair_threads<BN>()), smem, st, tw, tx, to, p);
+  const int rc = launch(fp8_pair_kernel<OUT>, dim3(2 * pairs), dim3(kFp8PairThreads), kFp8PairSmem, st, tw, tx, to, p);
   g_cluster_x = 1;
   return rc;
 }
 
+template <class OUT>
+int launch_tile(const Fp8Call& c, cudaStream_t st) {
+  static_assert(kFp8TileStages >= 4, "a stage's barrier would turn twice before the sums have seen it");
+  Fp8LinearParams p = c.p;
+  const long long tiles = (long long)((p.rows + 127) / 128) * ((p.n + 127) / 128);
+  if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
+  MTX_TRY(tile_splits<OUT>(tiles, p.blocks, &p.splits));
+  p.tma_store = fits16(p.out, p.ldo * (long long)sizeof(OUT));
+  CUtensorMap tw, tx, to;
+  MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, 128));
+  MTX_TRY(make_map_e4m3(&tx, c.x, c.k, p.rows, c.ldx, 128));
+  if (p.tma_store) MTX_TRY(make_map_result(&to, p.out, p.out_f32, p.n, p.rows, p.ldo));
+  else to = tx;  // (not read)
+  g_cluster_y = p.splits;
+  const int rc = launch(fp8_tile_kernel<OUT>, dim3(unsigned(tiles < kSms ? tiles : kSms), unsigned(p.splits)), dim3(kFp8TileThreads), kFp8TileSmem, st, tw, tx, to, p);
+  g_cluster_y = 1;
+  return rc;
+}
+
 // Which kernel: up to 64 rows the streamed weights.  Above, each form's time as it was measured, in ns: what a call takes besides its blocks, and in every wave of
-// tiles the blocks and the tile's end, which goes by the results' type and place.  (Measured and by this, us: 200 x 2560 by 10240 streamed 23.2 and 24.3, 128 columns 17.9 and
-// 18.5, 256 columns 15.2 and 14.7; 512 x 10240 by 2560 42.9 and 41.4, 30.2 and 30.5, 40.4 and 40.5; 333 x 5120 by 1280 11.8 and 12.2, 17.4 and 17.9, 23.2 and 23.3; 333 x 2560
-// by 10240 23.3 and 24.3, 24.3 and 25.4, 25.9 and 25.1; 1570 x 132 by 10009 in fp32 24.7 and 24.8, 29.9 and 28.1, 31.0 and 31.0.)
+// tiles the blocks and the tile's end, which goes by the results' type and place.  (Measured and by this, us: 200 x 2560 by 10240 a tile per CTA 17.0 and 17.7, pairs 15.3 and 14.7;
+// 333 x 2560 by 10240 17.5 and 17.7, 25.2 and 25.1; 1000 x 2560 by 10240 37.3 and 37.2, 36.6 and 35.5; 333 x 5120 by 1280 10.7 and 10.8, 22.7 and 23.3; 2048 x 5120 by
+// 1280 28.3 and 29.7, 23.9 and 23.3; 419 x 425 by 15262 in fp32 17.2 and 19.1, 17.6 and 19.3.)
 int launch_linear(const Fp8Call& c, cudaStream_t st) {
   const int rows = c.p.rows;
   if (rows <= 16) return launch_stream<16>(c, st);
   if (rows <= 32) return launch_stream<32>(c, st);
   if (rows <= 64) return launch_stream<64>(c, st);
   const bool f32 = c.p.out_f32, aligned = fits16(c.p.out, c.p.ldo * (f32 ? 4 : 2));
-  const long long blocks = c.p.blocks, tiles128 = (long long)((rows + 127) / 128) * ((c.p.n + 127) / 128);
+  const long long blocks = c.p.blocks, tiles = (long long)((rows + 127) / 128) * ((c.p.n + 127) / 128);
+  const long long pairs = (long long)((rows + kFp8PairRows - 1) / kFp8PairRows) * ((c.p.n + kFp8PairCols - 1) / kFp8PairCols);
   int splits;
-  MTX_TRY(stream_splits<128>(tiles128, c.p.blocks, &splits));
-  const long long stream = 4500 + (splits > 1 ? 2300 : 0) + (tiles128 * splits + kSms - 1) / kSms * ((blocks + splits - 1) / splits * 450 + (f32 ? 2000 : 900));
-  auto pair = [&](int bn, long long base, long long block, long long end) {
-    const long long tiles = (long long)((rows + kFp8PairRows - 1) / kFp8PairRows) * ((c.p.n + bn - 1) / bn);
-    return base + (tiles + kSms / 2 - 1) / (kSms / 2) * (blocks * block + end);
-  };
-  const long long pair128 = pair(128, 4700, 315, f32 ? (aligned ? 1450 : 2300) : aligned ? 600 : 1500);
-  const long long pair256 = pair(256, 4300, 430, f32 ? (aligned ? 3850 : 5800) : aligned ? 1800 : 3700);
-  if (stream <= pair128 && stream <= pair256) return launch_stream<128>(c, st);
-  if (pair128 <= pair256) return c.p.out_f32 ? launch_pair<128, float>(c, st) : launch_pair<128, bf16>(c, st);
-  return c.p.out_f32 ? launch_pair<256, float>(c, st) : launch_pair<256, bf16>(c, st);
+  if (f32) MTX_TRY(tile_splits<float>(tiles, c.p.blocks, &splits));
+  else MTX_TRY(tile_splits<bf16>(tiles, c.p.blocks, &splits));
+  const long long tile_end = f32 ? (aligned ? 1400 : 2400) : aligned ? 500 : 1100, pair_end = f32 ? (aligned ? 3850 : 5800) : aligned ? 1800 : 3700;
+  const long long tile = 4700 + (splits > 1 ? 2600 : 0) + (tiles * splits + kSms - 1) / kSms * ((blocks + splits - 1) / splits * 300 + tile_end);
+  const long long pair = 4300 + (pairs + kSms / 2 - 1) / (kSms / 2) * (blocks * 430 + pair_end);
+  if (tile <= pair) return f32 ? launch_tile<float>(c, st) : launch_tile<bf16>(c, st);
+  return f32 ? launch_pair<float>(c, st) : launch_pair<bf16>(c, st);
 }
 
 }  // namespace

@@ -361,9 +361,9 @@ struct Fp8SmemTail {
 // logits, 68 MB, beside them); 64 x 5120 by 1280, ten tiles in eight parts each, 7.8: launch, fill and exchange, the weights are 1.0 of it.
 
 template <int BN>
-__host__ __device__ constexpr int fp8_stream_warps() { return BN <= 32 ? 4 : BN / 8; }  // epilogue warps: 16 or 32 activation rows each
+__host__ __device__ constexpr int fp8_stream_warps() { return BN <= 32 ? 4 : 8; }  // epilogue warps: 16 or 32 activation rows each
 template <int BN>
-__host__ __device__ constexpr int fp8_stream_buffers() { return BN <= 64 && BN != 32 ? 4 : 2; }  // accumulators in TMEM: two or more CTAs share an SM's 512 columns
+__host__ __device__ constexpr int fp8_stream_buffers() { return BN == 32 ? 2 : 4; }  // accumulators in TMEM (two or three CTAs share an SM's 512 columns), at most as many as stages
 template <int BN>
 __host__ __device__ constexpr int fp8_stream_stage_bytes() { return kFp8OperandBytes + BN * kScaleBlock; }
 template <int BN>
@@ -587,51 +587,108 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
 
 // ---- many rows: pairs of CTAs ------------------------------------------------------------------------------------------------------------
 //
-// Two CTAs of a cluster (a TPC's two SMs) work on one tile of 256 rows x BN columns with cta_group::2 MMAs: CTA c of the pair holds rows 128 c .. of the
-// activations and half of the weight tile, so an SM takes in 16 KB + BN * 64 bytes per block for BN * 2^14 multiply-adds.  A thread of the
+// Two CTAs of a cluster (a TPC's two SMs) work on one tile of 256 rows x 256 columns with cta_group::2 MMAs: CTA c of the pair holds rows 128 c .. of the
+// activations and half of the weight tile, so an SM takes in 32 KB per block for 2^22 multiply-adds.  A thread of the
 // epilogue warps owns one row and half of the columns: its scale of a block is ONE number, which the sums take in with packed fused
 // multiply-adds while the next block's MMAs run into another accumulator.
-// 4096 x 5376 by 21504: 400 us, 2.37 PFLOP/s.  A block of a 256-column tile takes 0.42 us where its MMAs take 0.28: TMEM holds two such accumulators, and one is
+// 4096 x 5376 by 21504: 400 us, 2.37 PFLOP/s.  A block of a tile takes 0.42 us where its MMAs take 0.28: TMEM holds two such accumulators, and one is
 // on its way (MMAs, barrier, 128 columns through registers in some 450 cycles, barriers of both CTAs) for two blocks.  (Without the sums in between: 342 us of 421.)
 
-constexpr int kFp8PairRows = 256;
+constexpr int kFp8PairRows = 256, kFp8PairCols = 256;
 
 // Epilogue warps: 32 rows x half of the columns each.  (Sixteen with a quarter of the columns take longer, 532 us for 421 at 4096 x 5376 by 21504: every
 // arrival at the leader's barrier is on the way from one block's sums to the next MMAs into their accumulator.  So do registers moved from the
 // first warps to these, 482 us.)
-template <int BN>
-__host__ __device__ constexpr int fp8_pair_warps() { return 8; }
-// warp 0: copies, warp 1: MMAs, then the sums
-template <int BN>
-__host__ __device__ constexpr int fp8_pair_threads() { return 64 + 32 * fp8_pair_warps<BN>(); }
-template <int BN>
-__host__ __device__ constexpr int fp8_pair_staged() { return fp8_pair_warps<BN>() * (BN == 256 ? 8192 : 4096); }  // two buffers (one) of 32 rows x 128 bytes per epilogue warp
-
-template <int BN>
-__host__ __device__ constexpr int fp8_pair_stage_bytes() { return kFp8OperandBytes + BN / 2 * kScaleBlock; }
-template <int BN>
-__host__ __device__ constexpr int fp8_pair_tail_at(int stages) { return stages * fp8_pair_stage_bytes<BN>() + fp8_pair_staged<BN>(); }
-template <int BN>
-constexpr size_t fp8_pair_smem_bytes(int stages) { return 1024 + fp8_pair_tail_at<BN>(stages) + sizeof(Fp8SmemTail); }
-template <int BN>
-constexpr int fp8_pair_stages() {
-  const int n = int((227 * 1024 - fp8_pair_smem_bytes<BN>(0)) / fp8_pair_stage_bytes<BN>());
-  return n < kFp8MaxStages ? n : kFp8MaxStages;
-}
+constexpr int kFp8PairWarps = 8;
+constexpr int kFp8PairThreads = 64 + 32 * kFp8PairWarps;  // warp 0: copies, warp 1: MMAs, then the sums
+constexpr int kFp8PairStage = kFp8OperandBytes + kFp8PairCols / 2 * kScaleBlock;
+constexpr int kFp8PairStages = 5;
+constexpr int kFp8PairBuffers = 2;  // of 32 rows x 128 bytes per epilogue warp, for results on their way
+__host__ __device__ constexpr int fp8_pair_tail_at(int stages) { return stages * kFp8PairStage + kFp8PairWarps * kFp8PairBuffers * 4096; }
+constexpr size_t kFp8PairSmem = 1024 + fp8_pair_tail_at(kFp8PairStages) + sizeof(Fp8SmemTail);
+static_assert(kFp8PairSmem <= 227 * 1024, "what an SM has");
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, const void* src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(src)), "r"(c0), "r"(c1) : "memory");
 }
 
-template <int BN, class OUT>
-__global__ void __launch_bounds__(fp8_pair_threads<BN>(), 1)
+// A warp's 32 rows from row0 on, COLS columns from col0 on, from registers (a thread has a row) to memory: 32 rows x 128 bytes at a time through shared memory (chunk j of row r at j ^ (r & 7): the 128-byte swizzle of the tensor map).  stage: BUFFERS
+// times 4096 bytes.
+template <int COLS, int BUFFERS, class OUT>
+__device__ __forceinline__ void fp8_store(const unsigned long long (&acc)[COLS / 2], uint8_t* stage, const CUtensorMap& tm_out, const Fp8LinearParams& p, int row0, int col0) {
+  constexpr int kBox = 128 / int(sizeof(OUT));
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < COLS; c += kBox) {
+    if (col0 + c < p.n && row0 < p.rows) {
+      uint8_t* to = stage + c / kBox % BUFFERS * 4096;
+      if (p.tma_store) {  // the buffer's last store has been read: one of the tile before, or of this one's box but BUFFERS
+        if (lane == 0 && c == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        if (lane == 0 && c >= BUFFERS * kBox) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BUFFERS - 1) : "memory");
+        __syncwarp();
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint4 u;
+        if (sizeof(OUT) == 2) {
+          const unsigned long long* a = acc + (c + 8 * j) / 2;
+          u = make_uint4(pack_bf16x2(pair_lo(a[0]), pair_hi(a[0])), pack_bf16x2(pair_lo(a[1]), pair_hi(a[1])), pack_bf16x2(pair_lo(a[2]), pair_hi(a[2])),
+                         pack_bf16x2(pair_lo(a[3]), pair_hi(a[3])));
+        } else {
+          const unsigned long long* a = acc + (c + 4 * j) / 2;
+          u = make_uint4(uint32_t(a[0]), uint32_t(a[0] >> 32), uint32_t(a[1]), uint32_t(a[1] >> 32));
+        }
+        *reinterpret_cast<uint4*>(to + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
+      }
+      if (p.tma_store) {
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&tm_out, to, col0 + c, row0);
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      } else {  // results at odd places: a row's values by neighbouring lanes, sixteen rows on their way at a time (5310 x 4000 by 13887: 418 us row by row, 284 so, 265 at 13888)
+        __syncwarp();
+        const int rows = min(32, p.rows - row0), cols = min(kBox, p.n - col0 - c);
+        OUT* o = static_cast<OUT*>(p.out) + row0 * p.ldo + col0 + c + lane;
+        auto value = [&](int r, int k) {
+          const int i = lane + 32 * k;
+          return *reinterpret_cast<const OUT*>(to + r * 128 + (((i / (kBox / 8)) ^ (r & 7)) << 4) + i % (kBox / 8) * sizeof(OUT));
+        };
+        if (rows == 32 && cols == kBox) {
+#pragma unroll 1
+          for (int r0 = 0; r0 < 32; r0 += 16) {
+            OUT x[16][kBox / 32];
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+#pragma unroll
+              for (int k = 0; k < kBox / 32; ++k) x[r][k] = value(r0 + r, k);
+#pragma unroll
+            for (int r = 0; r < 16; ++r, o += p.ldo)
+#pragma unroll
+              for (int k = 0; k < kBox / 32; ++k) o[32 * k] = x[r][k];
+          }
+        } else {
+          for (int r = 0; r < rows; ++r, o += p.ldo)
+#pragma unroll
+            for (int k = 0; k < kBox / 32; ++k)
+              if (lane + 32 * k < cols) o[32 * k] = value(r, k);
+        }
+        __syncwarp();
+      }
+    }
+  }
+}
+
+template <class OUT>
+__global__ void __launch_bounds__(kFp8PairThreads, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out, const Fp8LinearParams p) {
-  constexpr int kStage = fp8_pair_stage_bytes<BN>(), NB = 512 / BN, kHalf = BN / 2, kWarps = fp8_pair_warps<BN>(), kCols = BN * 4 / kWarps;
-  constexpr int kBuffers = fp8_pair_staged<BN>() / kWarps / 4096, kBox = 128 / int(sizeof(OUT));
+  constexpr int BN = kFp8PairCols, kStage = kFp8PairStage, NB = 512 / BN, kHalf = BN / 2, kWarps = kFp8PairWarps, kCols = BN * 4 / kWarps;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* staged = smem + size_t(p.stages) * kStage;
-  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(smem + fp8_pair_tail_at<BN>(p.stages));
+  // (the number of stages comes with the call: as a constant it leaves the sums' threads too few registers, 408 us for 400 at 4096 x 5376 by 21504)
+  uint8_t* staged = smem + p.stages * kStage;
+  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(smem + fp8_pair_tail_at(p.stages));
   volatile int* failed = &tail->failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(blockIdx.x) & 1, pair = int(blockIdx.x) >> 1, pairs = int(gridDim.x) >> 1;
@@ -662,7 +719,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
 
   if (warp >= 2) {
     const int c0 = (warp - 2) / 4 * kCols, quarter = warp & 3;
-    uint8_t* stage = staged + (warp - 2) * kBuffers * 4096;
+    uint8_t* stage = staged + (warp - 2) * kFp8PairBuffers * 4096;
     const uint32_t lanes = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(c0);
     int t = pair, s = 0, buf = 0;
     uint32_t phase = 0;
@@ -714,68 +771,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
         if (b + 1 < p.blocks) step(b + 1, 1);
       }
       if (j + 1 < mine) begin(t + pairs);
-      // 32 rows x 128 bytes at a time through shared memory (chunk j of row r at j ^ (r & 7): the 128-byte swizzle of the tensor map)
-      const int row0 = t % m_tiles * kFp8PairRows + rank * 128 + quarter * 32, col0 = t / m_tiles * BN + c0;
-#pragma unroll
-      for (int c = 0; c < kCols; c += kBox) {
-        if (col0 + c < p.n && row0 < p.rows) {
-          uint8_t* to = stage + c / kBox % kBuffers * 4096;
-          if (p.tma_store) {  // the buffer's last store has been read: one of the tile before, or of this one's box but kBuffers
-            if (lane == 0 && c == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            if (lane == 0 && c >= kBuffers * kBox) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBuffers - 1) : "memory");
-            __syncwarp();
-          }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            uint4 u;
-            if (sizeof(OUT) == 2) {
-              const unsigned long long* a = acc + (c + 8 * j) / 2;
-              u = make_uint4(pack_bf16x2(pair_lo(a[0]), pair_hi(a[0])), pack_bf16x2(pair_lo(a[1]), pair_hi(a[1])), pack_bf16x2(pair_lo(a[2]), pair_hi(a[2])),
-                             pack_bf16x2(pair_lo(a[3]), pair_hi(a[3])));
-            } else {
-              const unsigned long long* a = acc + (c + 4 * j) / 2;
-              u = make_uint4(uint32_t(a[0]), uint32_t(a[0] >> 32), uint32_t(a[1]), uint32_t(a[1] >> 32));
-            }
-            *reinterpret_cast<uint4*>(to + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
-          }
-          if (p.tma_store) {
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&tm_out, to, col0 + c, row0);
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
-          } else {  // results at odd places: a row's values by neighbouring lanes, sixteen rows on their way at a time (5310 x 4000 by 13887: 418 us row by row, 284 so, 265 at 13888)
-            __syncwarp();
-            const int rows = min(32, p.rows - row0), cols = min(kBox, p.n - col0 - c);
-            OUT* o = static_cast<OUT*>(p.out) + row0 * p.ldo + col0 + c + lane;
-            auto value = [&](int r, int k) {
-              const int i = lane + 32 * k;
-              return *reinterpret_cast<const OUT*>(to + r * 128 + (((i / (kBox / 8)) ^ (r & 7)) << 4) + i % (kBox / 8) * sizeof(OUT));
-            };
-            if (rows == 32 && cols == kBox) {
-#pragma unroll 1
-              for (int r0 = 0; r0 < 32; r0 += 16) {
-                OUT x[16][kBox / 32];
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-#pragma unroll
-                  for (int k = 0; k < kBox / 32; ++k) x[r][k] = value(r0 + r, k);
-#pragma unroll
-                for (int r = 0; r < 16; ++r, o += p.ldo)
-#pragma unroll
-                  for (int k = 0; k < kBox / 32; ++k) o[32 * k] = x[r][k];
-              }
-            } else {
-              for (int r = 0; r < rows; ++r, o += p.ldo)
-#pragma unroll
-                for (int k = 0; k < kBox / 32; ++k)
-                  if (lane + 32 * k < cols) o[32 * k] = value(r, k);
-            }
-            __syncwarp();
-          }
-        }
-      }
+      fp8_store<kCols, kFp8PairBuffers, OUT>(acc, stage, tm_out, p, t % m_tiles * kFp8PairRows + rank * 128 + quarter * 32, t / m_tiles * BN + c0);
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
@@ -833,6 +829,214 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   cluster_sync_all();  // the pair's shared memory and TMEM are in use until both CTAs are done
   tcgen05_fence_after();
   if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
+// ---- some rows: a tile per CTA -------------------------------------------------------------------------------------------------------------
+//
+// 128 rows x 128 columns of a CTA's own, rows as the MMA's M like the pairs' (one scale per thread and block), the sum shared by a cluster's CTAs like the streamed
+// weights'.  TMEM holds four accumulators, and no barrier of another CTA is on an accumulator's way: a block takes 0.30 us.  333 x 2560 by 10240, 240 tiles, 17.5 us; 128 x 2560
+// by 10240 11.0; 333 x 5120 by 1280, 30 tiles in four parts each, 10.7.  (Pairs of CTAs with tiles of 128 columns, 26.1, 18.9 and 17.8, and 128 activation rows
+// as the N of streamed weights, 23.9, 13.7 and 12.1, which this replaces: the pairs for their barriers, the others for a scale per column.)
+
+constexpr int kFp8TileWarps = 8;  // epilogue warps: 32 rows x 64 columns each
+constexpr int kFp8TileThreads = 64 + 32 * kFp8TileWarps;
+constexpr int kFp8TileStage = 2 * kFp8OperandBytes;
+constexpr int kFp8TileStages = 6;
+constexpr int kFp8TileTailAt = kFp8TileStages * kFp8TileStage + kFp8TileWarps * 4096;
+constexpr size_t kFp8TileSmem = 1024 + kFp8TileTailAt + sizeof(Fp8SmemTail);
+static_assert(kFp8TileSmem <= 227 * 1024 && 128 * 128 * sizeof(float) <= kFp8TileStages * kFp8TileStage, "a CTA's part of a tile lies where the operands were");
+
+template <class OUT>
+__global__ void __launch_bounds__(kFp8TileThreads, 1)
+fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out, const Fp8LinearParams p) {
+  constexpr int NB = 4, kCols = 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* staged = smem + kFp8TileStages * kFp8TileStage;
+  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(smem + kFp8TileTailAt);
+  volatile int* failed = &tail->failed;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.y;
+  const int b0 = int((long long)part * p.blocks / p.splits), b1 = int((long long)(part + 1) * p.blocks / p.splits), per = b1 - b0;
+  const int m_tiles = (p.rows + 127) / 128, tiles = m_tiles * ((p.n + 127) / 128);
+  const int mine = int(blockIdx.x) < tiles ? (tiles - 1 - int(blockIdx.x)) / int(gridDim.x) + 1 : 0, F = mine * per;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_out);
+    for (int s = 0; s < kFp8TileStages; ++s) {
+      mbar_init(&tail->full[s], 1);
+      mbar_init(&tail->done[s], 1);
+    }
+    for (int b = 0; b < NB; ++b) mbar_init(&tail->tmem_empty[b], kFp8TileWarps);
+    tail->failed = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tail->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = tail->tmem_base;
+
+  if (warp >= 2) {
+    const int c0 = (warp - 2) / 4 * kCols, quarter = warp & 3;
+    const uint32_t lanes = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(c0);
+    griddep_wait();  // (scales and activations of the kernel in front)
+    int t = blockIdx.x, s = 0, buf = 0;
+    uint32_t phase = 0;
+    // this thread's scales, of its row and of its columns, two blocks ahead; behind the last row any scale will do
+    const float *next_x = p.x_scale, *next_w = p.w_scale;
+    float xs[2], ws[2];
+    auto fetch = [&](int i) {
+      xs[i] = __ldg(next_x);
+      ws[i] = __ldg(next_w);
+      next_x += p.x_scale_block;
+      ++next_w;
+    };
+    auto begin = [&](int tt) {
+      const int nt = tt / m_tiles, r = (tt - nt * m_tiles) * 128 + quarter * 32 + lane;
+      next_x = p.x_scale + min(r, p.rows - 1) * p.x_scale_row + b0 * p.x_scale_block;
+      next_w = p.w_scale + nt * (long long)p.blocks + b0;
+      fetch(0);
+      if (per > 1) fetch(1);
+    };
+    if (mine > 0) begin(t);
+    unsigned long long acc[kCols / 2];
+    auto step = [&](int b, int i) {
+      fp8_wait(&tail->done[s], phase, failed);
+      tcgen05_fence_after();
+      float scale;  // (volatile: multiplied here, not right behind the loads)
+      asm volatile("mul.rn.f32 %0, %1, %2;" : "=f"(scale) : "f"(xs[i]), "f"(ws[i]));
+      const unsigned long long by = pair_of(scale, scale);
+      fp8_columns<kCols>(
+          lanes + uint32_t(buf * 128),
+          [&](int c, const uint32_t(&v)[16]) {
+#pragma unroll
+            for (int x = 0; x < 16; x += 2) fma_pair(acc[(c + x) / 2], pair_of(v[x], v[x + 1]), by);
+          },
+          [&]() {
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) fp8_release(&tail->tmem_empty[buf]);
+          });
+      if (b + 2 < per) fetch(i);
+      if (++s == kFp8TileStages) s = 0, phase ^= 1;
+      if (++buf == NB) buf = 0;
+    };
+    for (int j = 0; j < mine; ++j, t += gridDim.x) {
+#pragma unroll
+      for (int c = 0; c < kCols / 2; ++c) acc[c] = 0;
+      for (int b = 0; b < per; b += 2) {
+        step(b, 0);
+        if (b + 1 < per) step(b + 1, 1);
+      }
+      const int nt = t / m_tiles, row0 = (t - nt * m_tiles) * 128 + quarter * 32;
+      if (j + 1 < mine) begin(t + int(gridDim.x));
+      if (p.splits == 1) fp8_store<kCols, 1, OUT>(acc, staged + (warp - 2) * 4096, tm_out, p, row0, nt * 128 + c0);
+    }
+    if (p.splits > 1) {  // (one tile per CTA) this CTA's part, where the operands were: row r's chunk j of four columns at j ^ (r & 31)
+      const int r = quarter * 32 + lane;
+#pragma unroll
+      for (int j = 0; j < kCols / 4; ++j)
+        *reinterpret_cast<uint4*>(smem + r * 512 + (((c0 / 4 + j) ^ lane) << 4)) = make_uint4(uint32_t(acc[2 * j]), uint32_t(acc[2 * j] >> 32), uint32_t(acc[2 * j + 1]), uint32_t(acc[2 * j + 1] >> 32));
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  } else if (warp == 0) {
+    const bool issuer = elect_one();
+    auto load_w = [&](int s, int n0, int b) {
+      mbar_expect_tx(&tail->full[s], kFp8TileStage);
+      tma_load_2d(smem + s * kFp8TileStage + kFp8OperandBytes, &tm_w, b * kScaleBlock, n0, &tail->full[s], kEvictNormal);
+    };
+    const int pre = p.early ? min(F, kFp8TileStages) : 0;
+    int s = 0, b = b0, t = blockIdx.x;
+    if (issuer)
+      for (int f = 0; f < pre; ++f) {
+        load_w(f, t / m_tiles * 128, b);
+        if (++b == b1) b = b0, t += gridDim.x;
+      }
+    griddep_wait();
+    b = b0;
+    t = blockIdx.x;
+    int n0 = t / m_tiles * 128, r0 = t % m_tiles * 128;
+    uint32_t phase = 1;
+    bool good = true;
+    for (int f = 0; f < F; ++f) {
+      if (f >= kFp8TileStages) good &= fp8_wait(&tail->done[s], phase, failed);
+      if (issuer && good) {
+        if (f >= pre) load_w(s, n0, b);
+        tma_load_2d(smem + s * kFp8TileStage, &tm_x, b * kScaleBlock, r0, &tail->full[s], kEvictLast);
+      }
+      if (++s == kFp8TileStages) s = 0, phase ^= 1;
+      if (++b == b1) {
+        b = b0;
+        t += gridDim.x;
+        n0 = t / m_tiles * 128;
+        r0 = t % m_tiles * 128;
+      }
+    }
+    __syncwarp();
+  } else {
+    const bool issuer = elect_one();
+    const uint32_t idesc = umma_idesc_e4m3(128, 128);
+    const uint64_t d0 = umma_desc_sw128(smem);
+    const uint32_t desc_hi = uint32_t(d0 >> 32), desc_lo = uint32_t(d0);  // (the low words alone count on)
+    int s = 0, buf = 0;
+    uint32_t phase = 0, acc_phase = 1;
+    bool good = true;
+    for (int f = 0; f < F; ++f) {
+      good &= fp8_wait(&tail->full[s], phase, failed);
+      good &= fp8_wait(&tail->tmem_empty[buf], acc_phase, failed);
+      tcgen05_fence_after();
+      if (issuer && good) {
+        const uint32_t at = desc_lo + uint32_t(s) * (kFp8TileStage >> 4);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_e4m3(tmem_base + uint32_t(buf * 128), umma_desc_of(at + kk * 2, desc_hi), umma_desc_of(at + (kFp8OperandBytes >> 4) + kk * 2, desc_hi), idesc, kk != 0);
+        umma_commit(&tail->done[s]);
+      }
+      if (++s == kFp8TileStages) s = 0, phase ^= 1;
+      if (++buf == NB) buf = 0, acc_phase ^= 1;
+    }
+    __syncwarp();
+  }
+  if (*failed) fp8_let_copies_land();
+  if (p.splits > 1) {
+    cluster_sync_all();
+    if (warp >= 2) {  // a warp adds a row, a lane four columns of it, all parts on their way at once
+      const int nt = blockIdx.x / m_tiles, row0 = (blockIdx.x - nt * m_tiles) * 128, n0 = nt * 128 + lane * 4, left = min(128, p.rows - row0), count = min(4, p.n - n0);
+      const uint32_t own = smem_u32(smem);
+      for (int r = part + (warp - 2) * p.splits; r < left; r += kFp8TileWarps * p.splits) {
+        float4 v[kFp8MaxSplits];
+#pragma unroll
+        for (int q = 0; q < kFp8MaxSplits; ++q)
+          if (q < p.splits) v[q] = ld_dsmem_f32x4(dsmem_addr(own + r * 512 + ((lane ^ (r & 31)) << 4), q));
+        float4 sum = v[0];
+#pragma unroll
+        for (int q = 1; q < kFp8MaxSplits; ++q)
+          if (q < p.splits) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
+        const float o[4] = {sum.x, sum.y, sum.z, sum.w};
+        OUT* to = static_cast<OUT*>(p.out) + (row0 + r) * p.ldo + n0;
+        if (count == 4 && p.tma_store) {  // (whole 16 bytes of a base and a pitch)
+          if (sizeof(OUT) == 4) *reinterpret_cast<float4*>(to) = sum;
+          else *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < count) to[i] = OUT(o[i]);
+        }
+      }
+      __syncwarp();
+    }
+    cluster_sync_all();  // the parts are read from the other CTAs until here
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, 512);
 }
 
 }  // namespace mtx
