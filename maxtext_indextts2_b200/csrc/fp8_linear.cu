@@ -99,9 +99,11 @@ constexpr int fp8_stream_most_stages() {
 
 // Parts of the sum that CTAs of a cluster share: as many as leave every CTA an SM to itself, all clusters at once (a cluster lies in one GPC, so that fewer
 // large ones fit than SMs).  64 rows of 5120 by 1280 columns: 16.9 us in one part, 8.8 in four, 7.8 in eight; with a CTA of 128 rows of 10240 by 2560 columns
-// (20 tiles) 14.6 in six, 24.0 in eight, whose clusters take turns.  More tiles than SMs: one part (64 x 2560 by 10240, 80 tiles: 11.3 us, 12.6 in two).
+// (20 tiles) 14.6 in six, 24.0 in eight, whose clusters take turns.  More than half as many tiles as SMs: one part (64 x 2560 by 10240, 80 tiles: 11.3 us, 12.6 in two).
+// Joining the parts takes as long as `worth` blocks; a sum that sharing shortens by less stays in one part (32 x 1280 by 1280 columns, 10 blocks, in one part 6.3 us,
+// in eight 5.7; 32 x 512 by 1280 4.3 and 5.1; 128 x 1280 by 1280 7.2 and 8.1, 128 x 2560 by 1280 10.0 and 8.6).
 template <class Kernel>
-int cluster_splits(Kernel kernel, int threads, size_t smem, std::atomic<int>* fit, long long tiles, int blocks) {  // fit[s]: clusters of s CTAs that run at once; 0: not asked yet
+int cluster_splits(Kernel kernel, int threads, size_t smem, std::atomic<int>* fit, long long tiles, int blocks, int worth) {  // fit[s]: clusters of s CTAs that run at once; 0: not asked yet
   for (int s = kFp8MaxSplits; s > 1; --s) {
     if (s > blocks || tiles * s > kSms) continue;
     int n = fit[s].load(std::memory_order_relaxed);
@@ -124,7 +126,7 @@ int cluster_splits(Kernel kernel, int threads, size_t smem, std::atomic<int>* fi
       }
       fit[s].store(n, std::memory_order_relaxed);
     }
-    if (tiles <= n) return s;
+    if (tiles <= n) return blocks - (blocks + s - 1) / s >= worth ? s : 1;
   }
   return 1;
 }
@@ -135,7 +137,7 @@ int stream_splits(long long tiles, int blocks, int* splits) {
   static std::atomic<uint64_t> done{0};
   const size_t smem = fp8_stream_smem_bytes<BN>(fp8_stream_most_stages<BN>());
   MTX_TRY(allow_smem(fp8_stream_kernel<BN>, smem, done));
-  *splits = cluster_splits(fp8_stream_kernel<BN>, 64 + 32 * fp8_stream_warps<BN>(), smem, fit, tiles, blocks);
+  *splits = cluster_splits(fp8_stream_kernel<BN>, 64 + 32 * fp8_stream_warps<BN>(), smem, fit, tiles, blocks, BN == 16 ? 5 : BN == 32 ? 7 : 6);
   return MTX_OK;
 }
 
@@ -144,7 +146,7 @@ int tile_splits(long long tiles, int blocks, int* splits) {
   static std::atomic<int> fit[kFp8MaxSplits + 1];
   static std::atomic<uint64_t> done{0};
   MTX_TRY(allow_smem(fp8_tile_kernel<OUT>, kFp8TileSmem, done));
-  *splits = cluster_splits(fp8_tile_kernel<OUT>, kFp8TileThreads, kFp8TileSmem, fit, tiles, blocks);
+  *splits = cluster_splits(fp8_tile_kernel<OUT>, kFp8TileThreads, kFp8TileSmem, fit, tiles, blocks, 12);
   return MTX_OK;
 }
 
