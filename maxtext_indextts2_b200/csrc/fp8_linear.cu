@@ -1,4 +1,6 @@
 // C entry points of the 8-bit products (fp8_linear.cuh).
+#include <climits>
+
 #include "host_util.cuh"
 #include "fp8_linear.cuh"
 #include "operator_args.cuh"
@@ -174,6 +176,13 @@ int launch_stream(const Fp8Call& c, cudaStream_t st) {
   return rc;
 }
 
+// A TMA store writes whole 16 bytes: of a box across the end of a row it would fill the values behind the last column, up to seven, with zeros.
+template <class OUT>
+int tma_columns(const Fp8LinearParams& p) {
+  if (!fits16(p.out, p.ldo * (long long)sizeof(OUT))) return 0;
+  return p.n % int(16 / sizeof(OUT)) == 0 ? INT_MAX : p.n;
+}
+
 template <class OUT>
 int launch_pair(const Fp8Call& c, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
@@ -182,12 +191,12 @@ int launch_pair(const Fp8Call& c, cudaStream_t st) {
   const long long tiles = (long long)((p.rows + kFp8PairRows - 1) / kFp8PairRows) * ((p.n + kFp8PairCols - 1) / kFp8PairCols);
   if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
   p.stages = kFp8PairStages;
-  p.tma_store = fits16(p.out, p.ldo * (long long)sizeof(OUT));
+  p.tma_cols = tma_columns<OUT>(p);
   MTX_TRY(allow_smem(fp8_pair_kernel<OUT>, kFp8PairSmem, done));
   CUtensorMap tw, tx, to;
   MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, kFp8PairCols / 2));
   MTX_TRY(make_map_e4m3(&tx, c.x, c.k, p.rows, c.ldx, 128));
-  if (p.tma_store) MTX_TRY(make_map_result(&to, p.out, p.out_f32, p.n, p.rows, p.ldo));
+  if (p.tma_cols > 0) MTX_TRY(make_map_result(&to, p.out, p.out_f32, p.n, p.rows, p.ldo));
   else to = tx;  // (not read)
   const unsigned pairs = unsigned(tiles < kSms / 2 ? tiles : kSms / 2);
   g_cluster_x = 2;
@@ -203,11 +212,11 @@ int launch_tile(const Fp8Call& c, cudaStream_t st) {
   const long long tiles = (long long)((p.rows + 127) / 128) * ((p.n + 127) / 128);
   if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
   MTX_TRY(tile_splits<OUT>(tiles, p.blocks, &p.splits));
-  p.tma_store = fits16(p.out, p.ldo * (long long)sizeof(OUT));
+  p.tma_cols = tma_columns<OUT>(p);
   CUtensorMap tw, tx, to;
   MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, 128));
   MTX_TRY(make_map_e4m3(&tx, c.x, c.k, p.rows, c.ldx, 128));
-  if (p.tma_store) MTX_TRY(make_map_result(&to, p.out, p.out_f32, p.n, p.rows, p.ldo));
+  if (p.tma_cols > 0) MTX_TRY(make_map_result(&to, p.out, p.out_f32, p.n, p.rows, p.ldo));
   else to = tx;  // (not read)
   g_cluster_y = p.splits;
   const int rc = launch(fp8_tile_kernel<OUT>, dim3(unsigned(tiles < kSms ? tiles : kSms), unsigned(p.splits)), dim3(kFp8TileThreads), kFp8TileSmem, st, tw, tx, to, p);

@@ -259,7 +259,7 @@ struct Fp8LinearParams {
   int splits;       // stream: CTAs of a cluster that share a tile's blocks
   int stages;
   int early;        // stream: the weights may be read before the kernel in front is done (it waited for everything before itself)
-  int tma_store;    // pair: the result's base and pitch are whole 16 bytes
+  int tma_cols;      // pair and tile: results leave by TMA in boxes that end by this column (0: none)
 };
 
 // Waits that run out (some 2 s: a protocol error) end the kernel instead of the GPU: the CTA's roles go through their loops without waiting and without
@@ -612,8 +612,8 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, const void* 
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(src)), "r"(c0), "r"(c1) : "memory");
 }
 
-// A warp's 32 rows from row0 on, COLS columns from col0 on, from registers (a thread has a row) to memory: 32 rows x 128 bytes at a time through shared memory (chunk j of row r at j ^ (r & 7): the 128-byte swizzle of the tensor map).  stage: BUFFERS
-// times 4096 bytes.
+// A warp's 32 rows from row0 on, COLS columns from col0 on, from registers (a thread has a row) to memory: 32 rows x 128 bytes at a time through shared memory
+// (chunk j of row r at j ^ (r & 7): the 128-byte swizzle of the tensor map).  stage: BUFFERS times 4096 bytes.
 template <int COLS, int BUFFERS, class OUT>
 __device__ __forceinline__ void fp8_store(const unsigned long long (&acc)[COLS / 2], uint8_t* stage, const CUtensorMap& tm_out, const Fp8LinearParams& p, int row0, int col0) {
   constexpr int kBox = 128 / int(sizeof(OUT));
@@ -622,7 +622,7 @@ __device__ __forceinline__ void fp8_store(const unsigned long long (&acc)[COLS /
   for (int c = 0; c < COLS; c += kBox) {
     if (col0 + c < p.n && row0 < p.rows) {
       uint8_t* to = stage + c / kBox % BUFFERS * 4096;
-      if (p.tma_store) {  // the buffer's last store has been read: one of the tile before, or of this one's box but BUFFERS
+      if (p.tma_cols > 0) {  // the buffer's last store has been read: one of the tile before, or of this one's box but BUFFERS
         if (lane == 0 && c == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         if (lane == 0 && c >= BUFFERS * kBox) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(BUFFERS - 1) : "memory");
         __syncwarp();
@@ -640,14 +640,14 @@ __device__ __forceinline__ void fp8_store(const unsigned long long (&acc)[COLS /
         }
         *reinterpret_cast<uint4*>(to + lane * 128 + ((j ^ (lane & 7)) << 4)) = u;
       }
-      if (p.tma_store) {
+      if (col0 + c + kBox <= p.tma_cols) {
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) {
           tma_store_2d(&tm_out, to, col0 + c, row0);
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
-      } else {  // results at odd places: a row's values by neighbouring lanes, sixteen rows on their way at a time (5310 x 4000 by 13887: 418 us row by row, 284 so, 265 at 13888)
+      } else {  // results at odd places, or a last box: a row's values by neighbouring lanes, sixteen rows on their way at a time (5310 x 4000 by 13887: 418 us row by row, 284 so, 265 at 13888)
         __syncwarp();
         const int rows = min(32, p.rows - row0), cols = min(kBox, p.n - col0 - c);
         OUT* o = static_cast<OUT*>(p.out) + row0 * p.ldo + col0 + c + lane;
@@ -1020,7 +1020,7 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
           if (q < p.splits) sum.x += v[q].x, sum.y += v[q].y, sum.z += v[q].z, sum.w += v[q].w;
         const float o[4] = {sum.x, sum.y, sum.z, sum.w};
         OUT* to = static_cast<OUT*>(p.out) + (row0 + r) * p.ldo + n0;
-        if (count == 4 && p.tma_store) {  // (whole 16 bytes of a base and a pitch)
+        if (count == 4 && p.tma_cols > 0) {  // (whole 16 bytes of a base and a pitch)
           if (sizeof(OUT) == 4) *reinterpret_cast<float4*>(to) = sum;
           else *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
         } else {

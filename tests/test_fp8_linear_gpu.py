@@ -141,6 +141,41 @@ def test_product(rows, n, k, out_dtype):
   close(out, *expected(xq, xs, values(wq, k), ws.double().cpu(), rows, n, k))
 
 
+# Sums that several CTAs share (two to eight, few rows and many), tiles in one wave and in several, pairs of CTAs in one wave and in two.
+LARGER = [(20, 1300, 2600), (32, 300, 1300), (80, 150, 2100), (257, 1000, 3200), (500, 1500, 2048), (300, 10240, 1280), (1030, 2200, 2570), (2500, 2901, 1280)]
+
+
+@pytest.mark.parametrize("rows,n,k", LARGER)
+def test_larger_product(rows, n, k):
+  """Both types of result, each at a pitch of whole 16 bytes and inside a wider matrix at an odd column whose other values stay."""
+  x, w = inputs(rows, n, k)
+  wq, ws = quantize(w.cuda(), 128)
+  xq, xs = ref.quantised(x, 1)
+  want = expected(xq, xs, values(wq, k), ws.double().cpu(), rows, n, k)
+  for out_dtype in (torch.bfloat16, torch.float32):
+    ldo = -(-n // 8) * 8
+    out = linear(x.cuda(), wq, ws, n, k, out_dtype, ldo=ldo)
+    close(out[:, :n], *want)
+    assert (out[:, n:] == 7.0).all()
+    whole = torch.full((rows + 3, ldo + 9), 7.0, dtype=out_dtype, device="cuda")
+    linear(x.cuda(), wq, ws, n, k, out=whole[:rows, 3 : 3 + n])
+    assert torch.equal(whole[:rows, 3 : 3 + n], out[:, :n])
+    whole[:rows, 3 : 3 + n] = 7.0
+    assert (whole == 7.0).all()
+
+
+@pytest.mark.parametrize("rows,n,k", [(30, 300, 1300), (100, 300, 2100), (1030, 2200, 2570)])
+def test_rows_of_larger_products_do_not_disturb_each_other(rows, n, k):
+  x, w = inputs(rows, n, k)
+  wq, ws = quantize(w.cuda(), 128)
+  plain = linear(x.cuda(), wq, ws, n, k, torch.float32)
+  x[1], x[2, 100], x[3, k - 1], x[4] = float("nan"), float("inf"), float("nan"), 0.0
+  out = linear(x.cuda(), wq, ws, n, k, torch.float32)
+  assert out[1:4].isnan().all() and (out[4] == 0).all()
+  keep = [0] + list(range(5, rows))
+  assert torch.equal(out[keep], plain[keep])
+
+
 @pytest.mark.parametrize("rows,n,k", [(1, 200, 200), (16, 128, 1280), (64, 640, 2000), (130, 300, 300), (513, 512, 1040)])
 def test_forms_of_the_activations_agree(rows, n, k):
   """Values that the call quantises and values that were quantised before give the same bits; the bytes behind a row's end are not read as values."""
