@@ -158,7 +158,7 @@ int launch_stream(const Fp8Call& c, cudaStream_t st) {
   constexpr int kLeast = BN == 32 ? 3 : 4;
   static_assert(kLeast >= fp8_stream_buffers<BN>(), "a stage's barrier would turn twice before the sums have seen it");
   Fp8LinearParams p = c.p;
-  const long long tiles = (long long)((p.n + 127) / 128) * ((p.rows + BN - 1) / BN);
+  const long long tiles = (p.n + 127) / 128;
   if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
   MTX_TRY(stream_splits<BN>(tiles, p.blocks, &p.splits));
   // an SM's shared memory in stages, whether one CTA has it or several: 64 KB in flight are too few for a CTA alone (16 x 2560 by 10240, 80 CTAs: 11.1 us, 8.8 with all)

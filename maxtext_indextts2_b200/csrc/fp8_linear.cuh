@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
 
 // ---- products ----------------------------------------------------------------------------------------------------------------------
 //
-// Both kernels multiply one block of 128 columns at a time on the tensor cores (kind::f8f6f4, four instructions of 32), each into an accumulator of its
+// The kernels multiply one block of 128 columns at a time on the tensor cores (kind::f8f6f4, four instructions of 32), each into an accumulator of its
 // own in TMEM, and add acc += d * (xs ws) in registers, so that the scales are applied once per block and sums are fp32 throughout.  (The block-scaled
 // MMAs take powers of two alone as scales.)  The way of an accumulator from the MMAs' barrier through registers and back to the next MMAs is what many rows are bound by.
 
@@ -256,10 +256,10 @@ struct Fp8LinearParams {
   long long ldo;
   int out_f32;
   int rows, n, blocks;
-  int splits;       // stream: CTAs of a cluster that share a tile's blocks
-  int stages;
-  int early;        // stream: the weights may be read before the kernel in front is done (it waited for everything before itself)
-  int tma_cols;      // pair and tile: results leave by TMA in boxes that end by this column (0: none)
+  int splits;       // stream and tile: CTAs of a cluster that share a tile's blocks
+  int stages;       // stream and pair
+  int early;        // stream and tile: the weights may be read before the kernel in front is done (it waited for everything before itself)
+  int tma_cols;     // pair and tile: results leave by TMA in boxes that end by this column (0: none)
 };
 
 // Waits that run out (some 2 s: a protocol error) end the kernel instead of the GPU: the CTA's roles go through their loops without waiting and without
@@ -354,7 +354,7 @@ struct Fp8SmemTail {
 
 // ---- few rows: the weights as they stream by ------------------------------------------------------------------------------------------
 //
-// The 128 rows of a weight tile are the MMA's M, BN activation rows its N: nothing is padded but the last few rows, and a CTA takes in 16 KB of weights
+// The 128 rows of a weight tile are the MMA's M, the activation rows, up to BN, its N: nothing is padded but the last few rows, and a CTA takes in 16 KB of weights
 // with BN * 128 bytes of activations per block.  An epilogue thread owns a weight row and BN sums.  Bound: the weights' bytes.
 // Few tiles are shared by the CTAs of a cluster, each with a part of the blocks, and the parts are added over distributed shared memory in
 // the order of the blocks (so that a result never depends on timing).  1 x 1280 by 264192 columns 52.1 us (the weights at 6.5 TB/s), 64 rows 67.4 (the
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
   volatile int* failed = &tail->failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.y;
   const int b0 = int((long long)part * p.blocks / p.splits), b1 = int((long long)(part + 1) * p.blocks / p.splits), per = b1 - b0;
-  const int tiles_n = (p.n + 127) / 128, tiles = tiles_n * ((p.rows + BN - 1) / BN);
+  const int tiles = (p.n + 127) / 128;
   const int mine = int(blockIdx.x) < tiles ? (tiles - 1 - int(blockIdx.x)) / int(gridDim.x) + 1 : 0, F = mine * per;
 
   if (warp == 0 && lane == 0) {
@@ -408,38 +408,31 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
 
   if (warp == 0) {
     const bool issuer = elect_one();
-    // (tile t: weight rows 128 (t % tiles_n) .., activation rows BN (t / tiles_n) ..)
     auto load_w = [&](int s, int n0, int b) {
       mbar_expect_tx(&tail->full[s], kStage);
-      tma_load_2d(smem + s * kStage, &tm_w, b * kScaleBlock, n0, &tail->full[s], p.rows <= BN ? kEvictFirst : kEvictNormal);
+      tma_load_2d(smem + s * kStage, &tm_w, b * kScaleBlock, n0, &tail->full[s], kEvictFirst);
     };
-    auto load_x = [&](int s, int r0, int b) { tma_load_2d(smem + s * kStage + kFp8OperandBytes, &tm_x, b * kScaleBlock, r0, &tail->full[s], kEvictLast); };
+    auto load_x = [&](int s, int b) { tma_load_2d(smem + s * kStage + kFp8OperandBytes, &tm_x, b * kScaleBlock, 0, &tail->full[s], kEvictLast); };
     const int pre = p.early ? min(F, p.stages) : 0;
     int s = 0, b = b0, t = blockIdx.x;
     if (issuer)
       for (int f = 0; f < pre; ++f) {
-        load_w(f, t % tiles_n * 128, b);
+        load_w(f, t * 128, b);
         if (++b == b1) b = b0, t += gridDim.x;
       }
     griddep_wait();
     b = b0;
     t = blockIdx.x;
-    int n0 = t % tiles_n * 128, r0 = t / tiles_n * BN;
     uint32_t phase = 1;
     bool good = true;
     for (int f = 0; f < F; ++f) {
       if (f >= p.stages) good &= fp8_wait(&tail->done[s], phase, failed);
       if (issuer && good) {
-        if (f >= pre) load_w(s, n0, b);
-        load_x(s, r0, b);
+        if (f >= pre) load_w(s, t * 128, b);
+        load_x(s, b);
       }
       if (++s == p.stages) s = 0, phase ^= 1;
-      if (++b == b1) {
-        b = b0;
-        t += gridDim.x;
-        n0 = t % tiles_n * 128;
-        r0 = t / tiles_n * BN;
-      }
+      if (++b == b1) b = b0, t += gridDim.x;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -481,9 +474,8 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
       ++next_w;
     };
     auto begin = [&](int tt) {
-      const int rt = tt / tiles_n;
-      next_x = p.x_scale + min(rt * BN + c0 + (lane & (kCols - 1)), p.rows - 1) * p.x_scale_row + b0 * p.x_scale_block;
-      next_w = p.w_scale + (tt - rt * tiles_n) * (long long)p.blocks + b0;
+      next_x = p.x_scale + min(c0 + (lane & (kCols - 1)), p.rows - 1) * p.x_scale_row + b0 * p.x_scale_block;
+      next_w = p.w_scale + tt * (long long)p.blocks + b0;
       fetch(0);
       if (per > 1) fetch(1);
     };
@@ -524,17 +516,17 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
       __syncwarp();  // (an odd number of blocks: the next tile's first factors go where the last ones were)
       if (j + 1 < mine) begin(t + int(gridDim.x));
       if (p.splits == 1) {
-        const int n = t % tiles_n * 128 + local, row0 = t / tiles_n * BN + c0, left = p.rows - row0;
+        const int n = t * 128 + local, left = p.rows - c0;
         if (n < p.n) {
           if (p.out_f32) {
-            float* o = static_cast<float*>(p.out) + row0 * p.ldo + n;
+            float* o = static_cast<float*>(p.out) + c0 * p.ldo + n;
 #pragma unroll
             for (int c = 0; c < kCols; ++c) {
               if (c < left) __stcs(o, c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]));
               o += p.ldo;
             }
           } else {
-            bf16* o = static_cast<bf16*>(p.out) + row0 * p.ldo + n;
+            bf16* o = static_cast<bf16*>(p.out) + c0 * p.ldo + n;
 #pragma unroll
             for (int c = 0; c < kCols; ++c) {
               if (c < left) *o = __float2bfloat16_rn(c & 1 ? pair_hi(acc[c / 2]) : pair_lo(acc[c / 2]));
@@ -555,9 +547,9 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
   if (p.splits > 1) {
     cluster_sync_all();
     if (warp >= 2) {  // a thread adds four neighbouring columns of the result, all parts on their way at once
-      const int t = blockIdx.x, n0 = t % tiles_n * 128 + lane * 4, row0 = t / tiles_n * BN, left = min(BN, p.rows - row0), count = min(4, p.n - n0);
+      const int n0 = blockIdx.x * 128 + lane * 4, count = min(4, p.n - n0);
       const uint32_t own = smem_u32(smem) + lane * 16;
-      for (int c = part + (warp - 2) * p.splits; c < left; c += kWarps * p.splits) {
+      for (int c = part + (warp - 2) * p.splits; c < p.rows; c += kWarps * p.splits) {
         float4 v[kFp8MaxSplits];
 #pragma unroll
         for (int q = 0; q < kFp8MaxSplits; ++q)
@@ -570,7 +562,7 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (i < count) {
-            const long long at = (row0 + c) * p.ldo + n0 + i;
+            const long long at = c * p.ldo + n0 + i;
             if (p.out_f32) static_cast<float*>(p.out)[at] = o[i];
             else static_cast<bf16*>(p.out)[at] = __float2bfloat16_rn(o[i]);
           }
@@ -591,14 +583,14 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
 // activations and half of the weight tile, so an SM takes in 32 KB per block for 2^22 multiply-adds.  A thread of the
 // epilogue warps owns one row and half of the columns: its scale of a block is ONE number, which the sums take in with packed fused
 // multiply-adds while the next block's MMAs run into another accumulator.
-// 4096 x 5376 by 21504: 400 us, 2.37 PFLOP/s.  A block of a tile takes 0.42 us where its MMAs take 0.28: TMEM holds two such accumulators, and one is
+// 4096 x 5376 by 21504: 395 us, 2.4 PFLOP/s.  A block of a tile takes 0.42 us where its MMAs take 0.28: TMEM holds two such accumulators, and one is
 // on its way (MMAs, barrier, 128 columns through registers in some 450 cycles, barriers of both CTAs) for two blocks.  (Without the sums in between: 342 us of 421.)
 
 constexpr int kFp8PairRows = 256, kFp8PairCols = 256;
 
 // Epilogue warps: 32 rows x half of the columns each.  (Sixteen with a quarter of the columns take longer, 532 us for 421 at 4096 x 5376 by 21504: every
 // arrival at the leader's barrier is on the way from one block's sums to the next MMAs into their accumulator.  So do registers moved from the
-// first warps to these, 482 us.)
+// first warps to these, 482 us, and MMAs and barriers for each half of the columns, 402 for 390.)
 constexpr int kFp8PairWarps = 8;
 constexpr int kFp8PairThreads = 64 + 32 * kFp8PairWarps;  // warp 0: copies, warp 1: MMAs, then the sums
 constexpr int kFp8PairStage = kFp8OperandBytes + kFp8PairCols / 2 * kScaleBlock;
