@@ -716,7 +716,7 @@ int mtx_quantize_fp8(const void* x, int x_type, long long ldx, int rows, int k, 
  * beside mtx_linear, with weights of mtx_quantize_fp8(block_rows = 128) and any number of rows.  x: MTX_E4M3 values with their x_scale
  * [rows, ceil(k / 128)] (block_rows = 1), or MTX_BF16 / MTX_F32 values, which the call quantises in the same way (x_scale is not read) in `scratch`:
  * mtx_linear_fp8_scratch_bytes(rows, k) bytes, 16-byte aligned, written by every call and so not for two calls at once.  8-bit
- * operands: base and pitch whole 16 bytes.  out: MTX_BF16 or MTX_F32, pitch ldo values; it may not overlap an input.
+ * operands: base and pitch whole 16 bytes (whole 128 are the fast ones).  out: MTX_BF16 or MTX_F32, pitch ldo values; it may not overlap an input.
  * rows, n, k <= 2^30.  A row of NaN or infinities leaves the other rows as they are; the same call gives the same bits every time. */
 size_t mtx_linear_fp8_scratch_bytes(int rows, int k);
 int mtx_linear_fp8(const void* x, int x_type, long long ldx, const float* x_scale, const void* wq, long long ldw, const float* w_scale, void* out, int out_type, long long ldo,

@@ -41,8 +41,8 @@ int quantize(const void* x, int x_type, long long ldx, int rows, int k, int bloc
   return x_type == MTX_BF16 ? launch_quantize<bf16>(p, block_rows, st) : launch_quantize<float>(p, block_rows, st);
 }
 
-// what a linear keeps of its quantised activations in the caller's scratch: the values at a pitch of whole 16 bytes, then a block's scales side by side
-size_t scratch_pitch(int k) { return align_up(size_t(k), 16); }
+// what a linear keeps of its quantised activations in the caller's scratch: the values in rows of whole L2 lines, then a block's scales side by side
+size_t scratch_pitch(int k) { return align_up(size_t(k), 128); }
 size_t scratch_scales_at(int rows, int k) { return align_up(size_t(rows) * scratch_pitch(k), 256); }
 
 // 8-bit rows [rows, k] in boxes of `box_rows` rows x 128 columns with the 128-byte swizzle; columns behind k and rows behind the last read as zeros
@@ -147,8 +147,8 @@ template <class OUT>
 int tile_splits(long long tiles, int blocks, int* splits) {
   static std::atomic<int> fit[kFp8MaxSplits + 1];
   static std::atomic<uint64_t> done{0};
-  MTX_TRY(allow_smem(fp8_tile_kernel<OUT>, kFp8TileSmem, done));
-  *splits = cluster_splits(fp8_tile_kernel<OUT>, kFp8TileThreads, kFp8TileSmem, fit, tiles, blocks, 12);
+  MTX_TRY(allow_smem(fp8_tile_kernel<128, OUT>, fp8_tile_smem<128>(), done));
+  *splits = cluster_splits(fp8_tile_kernel<128, OUT>, kFp8TileThreads, fp8_tile_smem<128>(), fit, tiles, blocks, 12);
   return MTX_OK;
 }
 
@@ -205,44 +205,59 @@ int launch_pair(const Fp8Call& c, cudaStream_t st) {
   return rc;
 }
 
-template <class OUT>
-int launch_tile(const Fp8Call& c, cudaStream_t st) {
-  static_assert(kFp8TileStages >= 4, "a stage's barrier would turn twice before the sums have seen it");
+template <int BN, class OUT>
+int launch_tile(const Fp8Call& c, int splits, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  static_assert(fp8_tile_stages<BN>() >= 512 / BN, "a stage's barrier would turn twice before the sums have seen it");
   Fp8LinearParams p = c.p;
-  const long long tiles = (long long)((p.rows + 127) / 128) * ((p.n + 127) / 128);
+  const long long tiles = (long long)((p.rows + 127) / 128) * ((p.n + BN - 1) / BN);
   if (tiles * p.blocks >= 1ll << 31) return fail(MTX_ERR_ARG, "too many tiles for one call");
-  MTX_TRY(tile_splits<OUT>(tiles, p.blocks, &p.splits));
+  p.stages = fp8_tile_stages<BN>();
+  p.splits = splits;
   p.tma_cols = tma_columns<OUT>(p);
+  MTX_TRY(allow_smem(fp8_tile_kernel<BN, OUT>, fp8_tile_smem<BN>(), done));
   CUtensorMap tw, tx, to;
-  MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, 128));
+  MTX_TRY(make_map_e4m3(&tw, c.w, c.k, p.n, c.ldw, BN));
   MTX_TRY(make_map_e4m3(&tx, c.x, c.k, p.rows, c.ldx, 128));
   if (p.tma_cols > 0) MTX_TRY(make_map_result(&to, p.out, p.out_f32, p.n, p.rows, p.ldo));
   else to = tx;  // (not read)
-  g_cluster_y = p.splits;
-  const int rc = launch(fp8_tile_kernel<OUT>, dim3(unsigned(tiles < kSms ? tiles : kSms), unsigned(p.splits)), dim3(kFp8TileThreads), kFp8TileSmem, st, tw, tx, to, p);
+  g_cluster_y = splits;
+  const int rc = launch(fp8_tile_kernel<BN, OUT>, dim3(unsigned(tiles < kSms ? tiles : kSms), unsigned(splits)), dim3(kFp8TileThreads), fp8_tile_smem<BN>(), st, tw, tx, to, p);
   g_cluster_y = 1;
   return rc;
 }
 
 // Which kernel: up to 64 rows the streamed weights.  Above, each form's time as it was measured, in ns: what a call takes besides its blocks, and in every wave of
-// tiles the blocks and the tile's end, which goes by the results' type and place.  (Measured and by this, us: 200 x 2560 by 10240 a tile per CTA 17.0 and 17.7, pairs 15.3 and 14.7;
-// 333 x 2560 by 10240 17.5 and 17.7, 25.2 and 25.1; 1000 x 2560 by 10240 37.3 and 37.2, 36.6 and 35.5; 333 x 5120 by 1280 10.7 and 10.8, 22.7 and 23.3; 2048 x 5120 by
-// 1280 28.3 and 29.7, 23.9 and 23.3; 419 x 425 by 15262 in fp32 17.2 and 19.1, 17.6 and 19.3.)
+// tiles the blocks (which take longer where rows of weights do not begin with a line of L2, and in CTAs of 256 columns with the SMs that take in as much) and the
+// tile's end, which goes by the results' type and place.  Measured, us:
+//                                    128 columns   256 columns   pairs
+//   333 x 5120 by 1280                      10.6          21.1    22.4
+//   128 x 2560 by 10240                     11.2          14.1    15.3
+//   333 x 2560 by 10240                     18.1          14.7    24.7
+//   128 x 5376 by 21504                     33.7          26.8    43.8
+//   333 x 5376 by 21504                     58.9          45.1    63.8
+//   1000 x 2560 by 10240                    38.4          34.1    35.6
+//   2048 x 5376 by 21504                   264.6         213.8   207.5
+//   4096 x 5376 by 21504                   527.0         418.4   398.2
+//   153 x 7306 by 10997, fp32               53.3          41.9    35.6
 int launch_linear(const Fp8Call& c, cudaStream_t st) {
   const int rows = c.p.rows;
   if (rows <= 16) return launch_stream<16>(c, st);
   if (rows <= 32) return launch_stream<32>(c, st);
   if (rows <= 64) return launch_stream<64>(c, st);
-  const bool f32 = c.p.out_f32, aligned = fits16(c.p.out, c.p.ldo * (f32 ? 4 : 2));
-  const long long blocks = c.p.blocks, tiles = (long long)((rows + 127) / 128) * ((c.p.n + 127) / 128);
-  const long long pairs = (long long)((rows + kFp8PairRows - 1) / kFp8PairRows) * ((c.p.n + kFp8PairCols - 1) / kFp8PairCols);
+  const bool f32 = c.p.out_f32, aligned = fits16(c.p.out, c.p.ldo * (f32 ? 4 : 2)), lines = c.ldw % 128 == 0;
+  const int end = (f32 ? 2 : 0) + (aligned ? 0 : 1);
+  const long long blocks = c.p.blocks, m = (rows + 127) / 128, tiles = m * ((c.p.n + 127) / 128), wide = m * ((c.p.n + 255) / 256), pairs = (m + 1) / 2 * ((c.p.n + 255) / 256);
   int splits;
   if (f32) MTX_TRY(tile_splits<float>(tiles, c.p.blocks, &splits));
   else MTX_TRY(tile_splits<bf16>(tiles, c.p.blocks, &splits));
-  const long long tile_end = f32 ? (aligned ? 1400 : 2400) : aligned ? 500 : 1100, pair_end = f32 ? (aligned ? 3850 : 5800) : aligned ? 1800 : 3700;
-  const long long tile = 4700 + (splits > 1 ? 2600 : 0) + (tiles * splits + kSms - 1) / kSms * ((blocks + splits - 1) / splits * 300 + tile_end);
-  const long long pair = 4300 + (pairs + kSms / 2 - 1) / (kSms / 2) * (blocks * 430 + pair_end);
-  if (tile <= pair) return f32 ? launch_tile<float>(c, st) : launch_tile<bf16>(c, st);
+  constexpr int kTileEnd[4] = {500, 1100, 1400, 2400}, kWideEnd[4] = {1800, 4900, 4100, 6000}, kPairEnd[4] = {1800, 3700, 3850, 5800};  // bf16 in place, at odd places, fp32 both
+  const long long waves = (wide + kSms - 1) / kSms;
+  const long long tile = 4700 + (splits > 1 ? 2600 : 0) + (tiles * splits + kSms - 1) / kSms * ((blocks + splits - 1) / splits * (lines ? 300 : 370) + kTileEnd[end]);
+  const long long wide_ns = 4300 + waves * (blocks * ((lines ? 360 : 450) + 90 * wide / (waves * kSms)) + kWideEnd[end]);
+  const long long pair = 4300 + (pairs + kSms / 2 - 1) / (kSms / 2) * (blocks * (lines ? 430 : 460) + kPairEnd[end]);
+  if (tile <= wide_ns && tile <= pair) return f32 ? launch_tile<128, float>(c, splits, st) : launch_tile<128, bf16>(c, splits, st);
+  if (wide_ns <= pair) return f32 ? launch_tile<256, float>(c, 1, st) : launch_tile<256, bf16>(c, 1, st);
   return f32 ? launch_pair<float>(c, st) : launch_pair<bf16>(c, st);
 }
 

@@ -825,38 +825,46 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
 
 // ---- some rows: a tile per CTA -------------------------------------------------------------------------------------------------------------
 //
-// 128 rows x 128 columns of a CTA's own, rows as the MMA's M like the pairs' (one scale per thread and block), the sum shared by a cluster's CTAs like the streamed
-// weights'.  TMEM holds four accumulators, and no barrier of another CTA is on an accumulator's way: a block takes 0.30 us.  333 x 2560 by 10240, 240 tiles, 17.5 us; 128 x 2560
-// by 10240 11.0; 333 x 5120 by 1280, 30 tiles in four parts each, 10.7.  (Pairs of CTAs with tiles of 128 columns, 26.1, 18.9 and 17.8, and 128 activation rows
-// as the N of streamed weights, 23.9, 13.7 and 12.1, which this replaces: the pairs for their barriers, the others for a scale per column.)
+// 128 rows x BN columns of a CTA's own, rows as the MMA's M like the pairs' (one scale per thread and block).  BN = 128: the sum may be shared by a cluster's CTAs
+// like the streamed weights', and TMEM holds four accumulators.  No barrier of another CTA is on an accumulator's way, and the bound is what an SM takes in from L2:
+// 32 KB of operands in 0.30 us, some 60 bytes a clock.  BN = 256: 48 KB in 0.36 to 0.45 us for twice the work, but half as many tiles.
+// 333 x 2560 by 10240: 240 tiles of 128 columns (two waves) 17.5 us, 120 of 256 (one) 14.7; 128 x 2560 by 10240 11.0 and 14.1; 333 x 5120 by 1280, 30 tiles in four
+// parts each, 10.7.  (Pairs of CTAs with tiles of 128 columns take 26.1, 18.9 and 17.8, and 128 activation rows as the N of streamed weights 23.9, 13.7
+// and 12.1: the pairs for their barriers, the others for a scale per column.)
 
-constexpr int kFp8TileWarps = 8;  // epilogue warps: 32 rows x 64 columns each
+constexpr int kFp8TileWarps = 8;  // epilogue warps: 32 rows x half of the columns each
 constexpr int kFp8TileThreads = 64 + 32 * kFp8TileWarps;
-constexpr int kFp8TileStage = 2 * kFp8OperandBytes;
-constexpr int kFp8TileStages = 6;
-constexpr int kFp8TileTailAt = kFp8TileStages * kFp8TileStage + kFp8TileWarps * 4096;
-constexpr size_t kFp8TileSmem = 1024 + kFp8TileTailAt + sizeof(Fp8SmemTail);
-static_assert(kFp8TileSmem <= 227 * 1024 && 128 * 128 * sizeof(float) <= kFp8TileStages * kFp8TileStage, "a CTA's part of a tile lies where the operands were");
+template <int BN>
+__host__ __device__ constexpr int fp8_tile_stage() { return kFp8OperandBytes + BN * kScaleBlock; }
+template <int BN>
+constexpr int fp8_tile_stages() { return BN == 128 ? 6 : 4; }  // (what shared memory holds; in the kernel from the call, like the pairs')
+template <int BN>
+__host__ __device__ constexpr int fp8_tile_tail_at(int stages) { return stages * fp8_tile_stage<BN>() + kFp8TileWarps * 4096; }
+template <int BN>
+constexpr size_t fp8_tile_smem() { return 1024 + fp8_tile_tail_at<BN>(fp8_tile_stages<BN>()) + sizeof(Fp8SmemTail); }
+static_assert(fp8_tile_smem<128>() <= 227 * 1024 && fp8_tile_smem<256>() <= 227 * 1024, "what an SM has");
+static_assert(128 * 128 * sizeof(float) <= fp8_tile_stages<128>() * fp8_tile_stage<128>(), "a CTA's part of a tile lies where the operands were");
 
-template <class OUT>
+template <int BN, class OUT>
 __global__ void __launch_bounds__(kFp8TileThreads, 1)
 fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_out, const Fp8LinearParams p) {
-  constexpr int NB = 4, kCols = 64;
+  constexpr int NB = 512 / BN, kCols = BN / 2, kStage = fp8_tile_stage<BN>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* staged = smem + kFp8TileStages * kFp8TileStage;
-  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(smem + kFp8TileTailAt);
+  uint8_t* staged = smem + p.stages * kStage;
+  Fp8SmemTail* tail = reinterpret_cast<Fp8SmemTail*>(smem + fp8_tile_tail_at<BN>(p.stages));
   volatile int* failed = &tail->failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.y;
+  const bool shared = BN == 128 && p.splits > 1;
   const int b0 = int((long long)part * p.blocks / p.splits), b1 = int((long long)(part + 1) * p.blocks / p.splits), per = b1 - b0;
-  const int m_tiles = (p.rows + 127) / 128, tiles = m_tiles * ((p.n + 127) / 128);
+  const int m_tiles = (p.rows + 127) / 128, tiles = m_tiles * ((p.n + BN - 1) / BN);
   const int mine = int(blockIdx.x) < tiles ? (tiles - 1 - int(blockIdx.x)) / int(gridDim.x) + 1 : 0, F = mine * per;
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tm_w);
     tma_prefetch_desc(&tm_x);
     tma_prefetch_desc(&tm_out);
-    for (int s = 0; s < kFp8TileStages; ++s) {
+    for (int s = 0; s < p.stages; ++s) {
       mbar_init(&tail->full[s], 1);
       mbar_init(&tail->done[s], 1);
     }
@@ -891,7 +899,7 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
     auto begin = [&](int tt) {
       const int nt = tt / m_tiles, r = (tt - nt * m_tiles) * 128 + quarter * 32 + lane;
       next_x = p.x_scale + min(r, p.rows - 1) * p.x_scale_row + b0 * p.x_scale_block;
-      next_w = p.w_scale + nt * (long long)p.blocks + b0;
+      next_w = p.w_scale + min(nt * BN + c0, p.n - 1) / kScaleBlock * (long long)p.blocks + b0;
       fetch(0);
       if (per > 1) fetch(1);
     };
@@ -904,7 +912,7 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
       asm volatile("mul.rn.f32 %0, %1, %2;" : "=f"(scale) : "f"(xs[i]), "f"(ws[i]));
       const unsigned long long by = pair_of(scale, scale);
       fp8_columns<kCols>(
-          lanes + uint32_t(buf * 128),
+          lanes + uint32_t(buf * BN),
           [&](int c, const uint32_t(&v)[16]) {
 #pragma unroll
             for (int x = 0; x < 16; x += 2) fma_pair(acc[(c + x) / 2], pair_of(v[x], v[x + 1]), by);
@@ -915,7 +923,7 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
             if (lane == 0) fp8_release(&tail->tmem_empty[buf]);
           });
       if (b + 2 < per) fetch(i);
-      if (++s == kFp8TileStages) s = 0, phase ^= 1;
+      if (++s == p.stages) s = 0, phase ^= 1;
       if (++buf == NB) buf = 0;
     };
     for (int j = 0; j < mine; ++j, t += gridDim.x) {
@@ -925,11 +933,10 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
         step(b, 0);
         if (b + 1 < per) step(b + 1, 1);
       }
-      const int nt = t / m_tiles, row0 = (t - nt * m_tiles) * 128 + quarter * 32;
       if (j + 1 < mine) begin(t + int(gridDim.x));
-      if (p.splits == 1) fp8_store<kCols, 1, OUT>(acc, staged + (warp - 2) * 4096, tm_out, p, row0, nt * 128 + c0);
+      if (!shared) fp8_store<kCols, 1, OUT>(acc, staged + (warp - 2) * 4096, tm_out, p, t % m_tiles * 128 + quarter * 32, t / m_tiles * BN + c0);
     }
-    if (p.splits > 1) {  // (one tile per CTA) this CTA's part, where the operands were: row r's chunk j of four columns at j ^ (r & 31)
+    if (shared) {  // (one tile per CTA) this CTA's part, where the operands were: row r's chunk j of four columns at j ^ (r & 31)
       const int r = quarter * 32 + lane;
 #pragma unroll
       for (int j = 0; j < kCols / 4; ++j)
@@ -940,40 +947,40 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
   } else if (warp == 0) {
     const bool issuer = elect_one();
     auto load_w = [&](int s, int n0, int b) {
-      mbar_expect_tx(&tail->full[s], kFp8TileStage);
-      tma_load_2d(smem + s * kFp8TileStage + kFp8OperandBytes, &tm_w, b * kScaleBlock, n0, &tail->full[s], kEvictNormal);
+      mbar_expect_tx(&tail->full[s], kStage);
+      tma_load_2d(smem + s * kStage + kFp8OperandBytes, &tm_w, b * kScaleBlock, n0, &tail->full[s], kEvictNormal);
     };
-    const int pre = p.early ? min(F, kFp8TileStages) : 0;
+    const int pre = p.early ? min(F, p.stages) : 0;
     int s = 0, b = b0, t = blockIdx.x;
     if (issuer)
       for (int f = 0; f < pre; ++f) {
-        load_w(f, t / m_tiles * 128, b);
+        load_w(f, t / m_tiles * BN, b);
         if (++b == b1) b = b0, t += gridDim.x;
       }
     griddep_wait();
     b = b0;
     t = blockIdx.x;
-    int n0 = t / m_tiles * 128, r0 = t % m_tiles * 128;
+    int n0 = t / m_tiles * BN, r0 = t % m_tiles * 128;
     uint32_t phase = 1;
     bool good = true;
     for (int f = 0; f < F; ++f) {
-      if (f >= kFp8TileStages) good &= fp8_wait(&tail->done[s], phase, failed);
+      if (f >= p.stages) good &= fp8_wait(&tail->done[s], phase, failed);
       if (issuer && good) {
         if (f >= pre) load_w(s, n0, b);
-        tma_load_2d(smem + s * kFp8TileStage, &tm_x, b * kScaleBlock, r0, &tail->full[s], kEvictLast);
+        tma_load_2d(smem + s * kStage, &tm_x, b * kScaleBlock, r0, &tail->full[s], kEvictLast);
       }
-      if (++s == kFp8TileStages) s = 0, phase ^= 1;
+      if (++s == p.stages) s = 0, phase ^= 1;
       if (++b == b1) {
         b = b0;
         t += gridDim.x;
-        n0 = t / m_tiles * 128;
+        n0 = t / m_tiles * BN;
         r0 = t % m_tiles * 128;
       }
     }
     __syncwarp();
   } else {
     const bool issuer = elect_one();
-    const uint32_t idesc = umma_idesc_e4m3(128, 128);
+    const uint32_t idesc = umma_idesc_e4m3(128, BN);
     const uint64_t d0 = umma_desc_sw128(smem);
     const uint32_t desc_hi = uint32_t(d0 >> 32), desc_lo = uint32_t(d0);  // (the low words alone count on)
     int s = 0, buf = 0;
@@ -984,19 +991,19 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
       good &= fp8_wait(&tail->tmem_empty[buf], acc_phase, failed);
       tcgen05_fence_after();
       if (issuer && good) {
-        const uint32_t at = desc_lo + uint32_t(s) * (kFp8TileStage >> 4);
+        const uint32_t at = desc_lo + uint32_t(s) * (kStage >> 4);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_e4m3(tmem_base + uint32_t(buf * 128), umma_desc_of(at + kk * 2, desc_hi), umma_desc_of(at + (kFp8OperandBytes >> 4) + kk * 2, desc_hi), idesc, kk != 0);
+          umma_e4m3(tmem_base + uint32_t(buf * BN), umma_desc_of(at + kk * 2, desc_hi), umma_desc_of(at + (kFp8OperandBytes >> 4) + kk * 2, desc_hi), idesc, kk != 0);
         umma_commit(&tail->done[s]);
       }
-      if (++s == kFp8TileStages) s = 0, phase ^= 1;
+      if (++s == p.stages) s = 0, phase ^= 1;
       if (++buf == NB) buf = 0, acc_phase ^= 1;
     }
     __syncwarp();
   }
   if (*failed) fp8_let_copies_land();
-  if (p.splits > 1) {
+  if (shared) {
     cluster_sync_all();
     if (warp >= 2) {  // a warp adds a row, a lane four columns of it, all parts on their way at once
       const int nt = blockIdx.x / m_tiles, row0 = (blockIdx.x - nt * m_tiles) * 128, n0 = nt * 128 + lane * 4, left = min(128, p.rows - row0), count = min(4, p.n - n0);

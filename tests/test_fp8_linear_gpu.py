@@ -141,8 +141,8 @@ def test_product(rows, n, k, out_dtype):
   close(out, *expected(xq, xs, values(wq, k), ws.double().cpu(), rows, n, k))
 
 
-# Sums that several CTAs share (two to eight, few rows and many), tiles in one wave and in several, pairs of CTAs in one wave and in two.
-LARGER = [(20, 1300, 2600), (32, 300, 1300), (80, 150, 2100), (257, 1000, 3200), (500, 1500, 2048), (300, 10240, 1280), (1030, 2200, 2570), (2500, 2901, 1280)]
+# Sums that several CTAs share (few rows and many), tiles of 128 and 256 columns in one wave and in several, pairs of CTAs in one wave and in two.
+LARGER = [(20, 1300, 2600), (32, 300, 1300), (80, 150, 2100), (257, 1000, 3200), (500, 1500, 2048), (300, 10240, 1280), (1100, 8190, 1280), (1030, 2200, 2570), (2500, 2901, 1280)]
 
 
 @pytest.mark.parametrize("rows,n,k", LARGER)
@@ -164,7 +164,7 @@ def test_larger_product(rows, n, k):
     assert (whole == 7.0).all()
 
 
-@pytest.mark.parametrize("rows,n,k", [(30, 300, 1300), (100, 300, 2100), (1030, 2200, 2570)])
+@pytest.mark.parametrize("rows,n,k", [(30, 300, 1300), (100, 300, 2100), (300, 10240, 1280), (1030, 2200, 2570)])
 def test_rows_of_larger_products_do_not_disturb_each_other(rows, n, k):
   x, w = inputs(rows, n, k)
   wq, ws = quantize(w.cuda(), 128)
