@@ -41,8 +41,8 @@ int quantize(const void* x, int x_type, long long ldx, int rows, int k, int bloc
   return x_type == MTX_BF16 ? launch_quantize<bf16>(p, block_rows, st) : launch_quantize<float>(p, block_rows, st);
 }
 
-// what a linear keeps of its quantised activations in the caller's scratch: the values in rows of whole L2 lines, then a block's scales side by side
-size_t scratch_pitch(int k) { return align_up(size_t(k), 128); }
+// what a linear keeps of its quantised activations in the caller's scratch: the values at a pitch of whole 16 bytes, then a block's scales side by side
+size_t scratch_pitch(int k) { return align_up(size_t(k), 16); }
 size_t scratch_scales_at(int rows, int k) { return align_up(size_t(rows) * scratch_pitch(k), 256); }
 
 // 8-bit rows [rows, k] in boxes of `box_rows` rows x 128 columns with the 128-byte swizzle; columns behind k and rows behind the last read as zeros
