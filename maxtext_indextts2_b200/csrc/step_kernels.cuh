@@ -622,8 +622,9 @@ __global__ void __launch_bounds__(kFinalizeThreads) finalize_kernel(const Finali
         if (a.log_prob_host != nullptr) a.log_prob_host[r] = logp;
       }
     } else if (a.mode == 3) {
-      a.first_token[r] = idx;
-      if (a.log_prob != nullptr) a.log_prob[r] = logp;
+      const bool none = idx == 0x7fffffff;  // nothing is above -infinity: a mask that leaves the row empty
+      a.first_token[r] = none ? -1 : idx;
+      if (a.log_prob != nullptr) a.log_prob[r] = none ? -INFINITY : logp;
     } else if (r == a.rows - 1) {
       a.first_token[0] = idx;
       if (a.log_prob != nullptr) a.log_prob[0] = logp;
