@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
     float val = x;
     if (by_mass) {
       keep = i < V;
-      if (x < cutoff) val = -1.0e7f;  // NEG_INF of inference_utils.py:20; still takes part, as in the reference
+      if (x < cutoff && x > -INFINITY) val = -1.0e7f;  // NEG_INF of inference_utils.py:20; still takes part, as in the reference, except what a mask has taken out
     } else {
       const bool eq = i < V && found && f32_order_key(x) == cut_key;
       // ordered rank among the entries equal to the cut-off

@@ -71,3 +71,18 @@ def test_a_row_of_nan(strategy):
   token, log_prob = drawn(logits, strategy)
   assert int(token[0]) == -1 and float(log_prob[0]) == float("-inf")
   assert 0 <= int(token[1]) < 300 and -20 < float(log_prob[1]) < 0
+
+
+@pytest.mark.parametrize("strategy", STRATEGIES)
+@pytest.mark.parametrize("low", [-2.0e7, -3.0e38])
+def test_what_a_mask_leaves_may_be_very_low(strategy, low):
+  """Allowed logits far below the value that a nucleus gives to what it cuts: no token that the mask forbids is drawn in their place."""
+  vocab = 700
+  allowed = torch.zeros(40, vocab, dtype=torch.bool)
+  allowed[:, 100:600:7] = True
+  logits = torch.full((40, vocab), low, device="cuda")
+  logits[:, 350] = low * 0.99  # (100 + 7 * 35 + 5: not allowed)
+  masked(logits, allowed)
+  token, log_prob = drawn(logits, strategy, temperature=1.0)
+  assert all(bool(allowed[r, t]) for r, t in enumerate(token.tolist()))
+  assert bool(log_prob.isfinite().all())
