@@ -436,6 +436,7 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
     }
     __syncwarp();
   } else if (warp == 1) {
+    griddep_wait();  // (no stage is full before; what the kernel in front takes is not counted in the waits' limit)
     const bool issuer = elect_one();
     const uint32_t idesc = umma_idesc_e4m3(128, BN);
     int s = 0, buf = 0;
@@ -980,6 +981,7 @@ fp8_tile_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
     }
     __syncwarp();
   } else {
+    griddep_wait();  // (no stage is full before; what the kernel in front takes is not counted in the waits' limit)
     const bool issuer = elect_one();
     const uint32_t idesc = umma_idesc_e4m3(128, BN);
     const uint64_t d0 = umma_desc_sw128(smem);
