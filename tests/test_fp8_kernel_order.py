@@ -30,3 +30,11 @@ def test_limited_waits_begin_behind_the_kernel_in_front(name):
   assert "fp8_wait(" not in front
   for part in parts:
     assert "griddep_wait();" in front or part.index("griddep_wait();") < part.index("fp8_wait("), part[:200]
+
+
+@pytest.mark.parametrize("file", ["fp8_linear.cuh", "logit_controls.cuh"])
+def test_nothing_is_read_by_the_read_only_path(file):
+  """That path is for what nobody writes while the kernel lives; the kernel in front may still write all that these read."""
+  with open(os.path.join(_lib.CSRC, file), encoding="utf-8") as f:
+    code = re.sub(r"//.*", "", f.read())
+  assert re.findall(r"__ldg\b|global\.nc|__restrict__", code) == []
