@@ -724,7 +724,7 @@ size_t mtx_linear_fp8_scratch_bytes(int rows, int k);
 int mtx_linear_fp8(const void* x, int x_type, long long ldx, const float* x_scale, const void* wq, long long ldw, const float* w_scale, void* out, int out_type, long long ldo,
                    int rows, int n, int k, void* scratch, size_t scratch_bytes, mtx_stream stream);
 /* Debug aid: waits inside mtx_linear_fp8's kernels that gave up after some two seconds, on the current device since the library was loaded (`count` is host
- * memory; synchronises).  Not 0: a protocol error, and the results of that call are wrong. */
+ * memory; waits for all of the device's streams, so not while one is captured).  Not 0: a protocol error, and the results of that call are wrong. */
 int mtx_linear_fp8_stalls(uint32_t* count);
 
 /* ---- controls of logits ---------------------------------------------------------------------- */

@@ -332,6 +332,7 @@ int mtx_linear_fp8(const void* x, int x_type, long long ldx, const float* x_scal
 
 int mtx_linear_fp8_stalls(uint32_t* count) {
   if (!count) return fail(MTX_ERR_ARG, "null argument");
+  MTX_CUDA(cudaDeviceSynchronize());  // (the copy below does not wait for streams that do not block)
   MTX_CUDA(cudaMemcpyFromSymbol(count, d_fp8_waits_failed, sizeof(uint32_t)));
   return MTX_OK;
 }

@@ -27,3 +27,17 @@ def pytest_collection_modifyitems(config, items):
   for item in items:
     if "gpu" in item.keywords:
       item.add_marker(skip)
+
+
+@pytest.fixture(autouse=True)
+def _no_stalled_products(request):
+  """Behind every test of 8-bit products: no wait in their kernels has run out (their results would be wrong without an error)."""
+  yield
+  if "gpu" in request.keywords and request.module.__name__.rpartition(".")[2] in ("test_fp8_linear_gpu", "test_answer_step_gpu", "test_far_offsets_gpu"):
+    import ctypes
+
+    from maxtext_indextts2_b200 import _lib
+
+    count = ctypes.c_uint32(1)
+    _lib.check(_lib.load().mtx_linear_fp8_stalls(ctypes.byref(count)))
+    assert count.value == 0

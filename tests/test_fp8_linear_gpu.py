@@ -299,3 +299,21 @@ def test_no_wait_ran_out():
   count = ctypes.c_uint32(7)
   _lib.check(_lib.load().mtx_linear_fp8_stalls(ctypes.byref(count)))
   assert count.value == 0
+
+
+def test_stalls_are_counted_behind_all_streams():
+  """The count is read once every product in flight is done, on a stream of the caller's own too; products of every kernel waited for nothing in vain."""
+  side, lib, count = torch.cuda.Stream(), _lib.load(), ctypes.c_uint32(7)
+  for rows, n, k, times in [(1, 1792, 1280, 50), (30, 40000, 384, 50), (64, 1280, 5120, 50), (100, 640, 2048, 50), (300, 10240, 1280, 50), (2048, 10240, 5120, 40)]:
+    x, w = torch.randn(rows, k, device="cuda").to(torch.bfloat16), torch.randn(n, k, device="cuda")
+    wq, ws = quantize(w, 128)
+    need = lib.mtx_linear_fp8_scratch_bytes(rows, k)
+    out, scratch = torch.empty(rows, n, device="cuda"), torch.empty(need, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+      for _ in range(times):
+        _lib.check(lib.mtx_linear_fp8(x.data_ptr(), _lib.BF16, k, None, wq.data_ptr(), wq.stride(0), ws.data_ptr(), out.data_ptr(), _lib.F32, n, rows, n, k, scratch.data_ptr(), need,
+                                      stream()))
+      done = side.record_event()
+    _lib.check(lib.mtx_linear_fp8_stalls(ctypes.byref(count)))
+    assert done.query() and count.value == 0
