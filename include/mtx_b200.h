@@ -741,9 +741,9 @@ typedef struct {
   long long ld_touched;
   const float* repetition;    /* [slots] or NULL: the logit of a seen token is divided by it where it is positive, else multiplied */
   const float* presence;      /* [slots] or NULL: taken off the logits of generated tokens */
-  const float* frequency;     /* [slots] or NULL: times a token's count taken off its logit */
+  const float* frequency;     /* [slots] or NULL: times a generated token's count taken off its logit; both may be infinite: the token then comes once */
   const int32_t* bias_off;    /* [rows + 1]: row r's biases are the entries [bias_off[r], bias_off[r + 1]) of the two arrays below, their */
-  const int32_t* bias_token;  /* tokens ascending; of entries with one token the first counts, tokens outside the vocabulary are skipped */
+  const int32_t* bias_token;  /* tokens ascending; of entries with one token the first counts, tokens outside the vocabulary are skipped. */
   const float* bias_value;
   int32_t allowed_rows;
   const int32_t* allowed_row; /* [rows]; NULL: row r has mask r.  A row whose mask is not in [0, allowed_rows) is not masked */

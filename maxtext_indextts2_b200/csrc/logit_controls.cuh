@@ -45,8 +45,7 @@ __device__ __forceinline__ float penalised(float l, uint32_t word, float repetit
   if (word == 0) return l;
   l = l > 0.0f ? __fdiv_rn(l, repetition) : __fmul_rn(l, repetition);
   const uint32_t count = word & 0x7fffu;
-  l = __fsub_rn(l, __fmul_rn(frequency, float(count)));
-  return count ? __fsub_rn(l, presence) : l;
+  return count ? __fsub_rn(__fsub_rn(l, __fmul_rn(frequency, float(count))), presence) : l;  // (a count of 0 takes nothing off, an infinite penalty's product neither)
 }
 
 // index of the first of the n ascending tokens that is at least t: each round 32 probes

@@ -254,3 +254,22 @@ def test_slots_by_order_and_a_record_without_bits():
   seen, _ = record(5, 100)
   note(seen, None, 100, [7, 8, -1, 9], None, False)
   assert (seen.cpu() != 0).nonzero().tolist() == [[0, 7], [1, 8], [3, 9]]
+
+
+@pytest.mark.parametrize("vocab", [256, 999, 1024])
+@pytest.mark.parametrize("which", ["frequency", "presence"])
+def test_infinite_penalties(vocab, which):
+  """A token that was generated is out; the prompt's tokens and all others stay as they are."""
+  b = Batch(6, vocab, history=0, biases=0, masks=0)
+  prompt, new = list(range(0, vocab, 5)), list(range(3, vocab, 7))
+  slots = b.seen.shape[0]
+  note(b.seen, b.touched, vocab, prompt * slots, [s for s in range(slots) for _ in prompt], True)
+  note(b.seen, b.touched, vocab, new * slots, [s for s in range(slots) for _ in new], False)
+  b.keep[which][:] = float("inf")
+  b.keep["presence" if which == "frequency" else "frequency"][:] = 0
+  b.keep["repetition"][:] = 1
+  out = torch.empty(6, vocab, device="cuda")
+  b.run(out)
+  want = b.logits.clone()
+  want[:3, new] = want[4:, new] = float("-inf")  # (row 3 has no penalties)
+  assert torch.equal(out, want)
