@@ -744,7 +744,7 @@ typedef struct {
   const float* frequency;     /* [slots] or NULL: times a generated token's count taken off its logit; both may be infinite: the token then comes once */
   const int32_t* bias_off;    /* [rows + 1]: row r's biases are the entries [bias_off[r], bias_off[r + 1]) of the two arrays below, their */
   const int32_t* bias_token;  /* tokens ascending; of entries with one token the first counts, tokens outside the vocabulary are skipped. */
-  const float* bias_value;
+  const float* bias_value;    /* The three are given together: for a batch without any bias all are NULL, or the lists are addresses that nothing is read from */
   int32_t allowed_rows;
   const int32_t* allowed_row; /* [rows]; NULL: row r has mask r.  A row whose mask is not in [0, allowed_rows) is not masked */
   const uint32_t* allowed;    /* [allowed_rows, ld_allowed]: token t is allowed by bit t % 32 of word t / 32 */

@@ -273,3 +273,17 @@ def test_infinite_penalties(vocab, which):
   want = b.logits.clone()
   want[:3, new] = want[4:, new] = float("-inf")  # (row 3 has no penalties)
   assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("lists", [True, False])
+def test_a_batch_without_any_bias(lists):
+  """Lists of no entries at all, at addresses that nothing is read from, and no lists."""
+  b = Batch(5, 700, biases=0)
+  out = torch.full((5, 700), 9.0, device="cuda")
+  if lists:
+    nothing = torch.empty(4, dtype=torch.int32, device="cuda")[4:]  # (of its own an empty tensor has no address)
+    place = nothing.untyped_storage().data_ptr()
+    b.run(out, bias_token=place, bias_value=place)
+  else:
+    b.run(out, bias_off=None, bias_token=None, bias_value=None)
+  close(out, b.want(), b)
