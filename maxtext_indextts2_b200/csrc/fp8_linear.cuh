@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
 // own in TMEM, and add acc += d * (xs ws) in registers, so that the scales are applied once per block and sums are fp32 throughout.  (The block-scaled
 // MMAs take powers of two alone as scales.)  The way of an accumulator from the MMAs' barrier through registers and back to the next MMAs is what many rows are bound by.
 // Scales come by ordinary loads: the kernels begin while the one in front still writes them, and the read-only path (__ldg) is for what nobody writes in a kernel's
-// life; a compiler may also move such loads in front of the wait for that kernel.  (4096 x 5376 by 21504: 401 us, by the read-only path 394; the other kernels as fast.)
+// life; a compiler may also move such loads in front of the wait for that kernel.  (4096 x 5376 by 21504: 407 us, by the read-only path 405; 5310 x 4000 by 13887 291 and 288; the other kernels are as fast.)
 
 struct Fp8LinearParams {
   const float* x_scale;
@@ -748,13 +748,13 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
           [&](int c, const uint32_t(&v)[16]) {
 #pragma unroll
             for (int x = 0; x < 16; x += 2) fma_pair(acc[(c + x) / 2], pair_of(v[x], v[x + 1]), by);
+            if (c == kCols - 32 && b + 2 < p.blocks) fetch(i);  // (beside the last columns' way from TMEM: 5310 x 4000 by 13887 291 us, behind them 295)
           },
           [&]() {
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) fp8_release_leader(&tail->tmem_empty[buf]);
           });
-      if (b + 2 < p.blocks) fetch(i);
       if (++s == p.stages) s = 0, phase ^= 1;
       if (++buf == NB) buf = 0;
     };
