@@ -752,7 +752,7 @@ typedef struct {
 } mtx_logit_controls;
 
 /* out = controlled logits, rows x vocab each: repetition, then frequency, then presence penalty, then the bias; the logits of tokens that are not
- * allowed are -infinity whatever they were (a row whose mask allows nothing is -infinity throughout).  Every operation is rounded to fp32.
+ * allowed are -infinity whatever they were (a row whose mask allows nothing is -infinity throughout, and mtx_sample_rows gives token -1 for it).  Every operation is rounded to fp32.
  * out == logits (with ldo == ld): in place, and then only what changes is read and written; otherwise the two may not overlap.  vocab <= 2^28. */
 int mtx_control_logits(const float* logits, long long ld, float* out, long long ldo, int rows, int vocab, const mtx_logit_controls* c, mtx_stream stream);
 

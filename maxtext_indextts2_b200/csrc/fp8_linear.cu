@@ -100,7 +100,7 @@ constexpr int fp8_stream_most_stages() {
 }
 
 // Parts of the sum that CTAs of a cluster share: as many as leave every CTA an SM to itself, all clusters at once (a cluster lies in one GPC, so that fewer
-// large ones fit than SMs).  64 rows of 5120 by 1280 columns: 16.9 us in one part, 8.8 in four, 7.8 in eight; with a CTA of 128 rows of 10240 by 2560 columns
+// large ones fit than SMs).  64 rows of 5120 by 1280 columns: 16.9 us in one part, 8.8 in four, 7.6 in eight; with a CTA of 128 rows of 10240 by 2560 columns
 // (20 tiles) 14.6 in six, 24.0 in eight, whose clusters take turns.  More than half as many tiles as SMs: one part (64 x 2560 by 10240, 80 tiles: 11.3 us, 12.6 in two).
 // Joining the parts takes as long as `worth` blocks; a sum that sharing shortens by less stays in one part (32 x 1280 by 1280 columns, 10 blocks, in one part 6.3 us,
 // in eight 5.7; 32 x 512 by 1280 4.3 and 5.1; 128 x 1280 by 1280 7.2 and 8.1, 128 x 2560 by 1280 10.0 and 8.6).
@@ -231,14 +231,14 @@ int launch_tile(const Fp8Call& c, int splits, cudaStream_t st) {
 // tiles the blocks (which take longer where rows of weights do not begin with a line of L2, and in CTAs of 256 columns with the SMs that take in as much) and the
 // tile's end, which goes by the results' type and place.  Measured, us:
 //                                    128 columns   256 columns   pairs
-//   333 x 5120 by 1280                      10.6          21.1    22.4
-//   128 x 2560 by 10240                     11.2          14.1    15.3
-//   333 x 2560 by 10240                     18.1          14.7    24.7
-//   128 x 5376 by 21504                     33.7          26.8    43.8
-//   333 x 5376 by 21504                     58.9          45.1    63.8
-//   1000 x 2560 by 10240                    38.4          34.1    35.6
-//   2048 x 5376 by 21504                   264.6         213.8   207.5
-//   4096 x 5376 by 21504                   527.0         418.4   398.2
+//   333 x 5120 by 1280                      10.1          21.2    22.6
+//   128 x 2560 by 10240                     11.3          14.2    15.3
+//   333 x 2560 by 10240                     18.1          14.9    25.5
+//   128 x 5376 by 21504                     34.6          27.1    44.9
+//   333 x 5376 by 21504                     60.7          44.8    63.7
+//   1000 x 2560 by 10240                    39.9          35.5    35.9
+//   2048 x 5376 by 21504                   271.6         213.9   210.4
+//   4096 x 5376 by 21504                   533.4         416.1   404.9
 //   153 x 7306 by 10997, fp32               53.3          41.9    35.6
 int launch_linear(const Fp8Call& c, cudaStream_t st) {
   const int rows = c.p.rows;

@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : 4) quantiz
 // own in TMEM, and add acc += d * (xs ws) in registers, so that the scales are applied once per block and sums are fp32 throughout.  (The block-scaled
 // MMAs take powers of two alone as scales.)  The way of an accumulator from the MMAs' barrier through registers and back to the next MMAs is what many rows are bound by.
 // Scales come by ordinary loads: the kernels begin while the one in front still writes them, and the read-only path (__ldg) is for what nobody writes in a kernel's
-// life; a compiler may also move such loads in front of the wait for that kernel.  (4096 x 5376 by 21504: 407 us, by the read-only path 405; 5310 x 4000 by 13887 291 and 288; the other kernels are as fast.)
+// life; a compiler may also move such loads in front of the wait for that kernel.  (4096 x 5376 by 21504: 407 us, by the read-only path 405; 5310 x 4000 by 13887 291
+// and 288; the other kernels are as fast.)
 
 struct Fp8LinearParams {
   const float* x_scale;
@@ -259,7 +260,7 @@ struct Fp8LinearParams {
   int out_f32;
   int rows, n, blocks;
   int splits;       // stream and tile: CTAs of a cluster that share a tile's blocks
-  int stages;       // stream and pair
+  int stages;       // of operands in shared memory
   int early;        // stream and tile: the weights may be read before the kernel in front is done (it waited for everything before itself)
   int tma_cols;     // pair and tile: results leave by TMA in boxes that end by this column (0: none)
 };
@@ -360,7 +361,7 @@ struct Fp8SmemTail {
 // with BN * 128 bytes of activations per block.  An epilogue thread owns a weight row and BN sums.  Bound: the weights' bytes.
 // Few tiles are shared by the CTAs of a cluster, each with a part of the blocks, and the parts are added over distributed shared memory in
 // the order of the blocks (so that a result never depends on timing).  1 x 1280 by 264192 columns 52.1 us (the weights at 6.5 TB/s), 64 rows 67.4 (the
-// logits, 68 MB, beside them); 64 x 5120 by 1280, ten tiles in eight parts each, 7.8: launch, fill and exchange, the weights are 1.0 of it.
+// logits, 68 MB, beside them); 64 x 5120 by 1280, ten tiles in eight parts each, 7.6: launch, fill and exchange, the weights are 1.0 of it.
 
 template <int BN>
 __host__ __device__ constexpr int fp8_stream_warps() { return BN <= 32 ? 4 : 8; }  // epilogue warps: 16 or 32 activation rows each
@@ -586,7 +587,7 @@ __global__ void __launch_bounds__(64 + 32 * fp8_stream_warps<BN>()) fp8_stream_k
 // activations and half of the weight tile, so an SM takes in 32 KB per block for 2^22 multiply-adds.  A thread of the
 // epilogue warps owns one row and half of the columns: its scale of a block is ONE number, which the sums take in with packed fused
 // multiply-adds while the next block's MMAs run into another accumulator.
-// 4096 x 5376 by 21504: 395 us, 2.4 PFLOP/s.  A block of a tile takes 0.42 us where its MMAs take 0.28: TMEM holds two such accumulators, and one is
+// 4096 x 5376 by 21504: 407 us, 2.3 PFLOP/s.  A block of a tile takes 0.42 us where its MMAs take 0.28: TMEM holds two such accumulators, and one is
 // on its way (MMAs, barrier, 128 columns through registers in some 450 cycles, barriers of both CTAs) for two blocks.  (Without the sums in between: 342 us of 421.)
 
 constexpr int kFp8PairRows = 256, kFp8PairCols = 256;
@@ -642,7 +643,7 @@ __device__ __forceinline__ void fp8_store(const unsigned long long (&acc)[COLS /
           tma_store_2d(&tm_out, to, col0 + c, row0);
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
-      } else {  // results at odd places, or a last box: a row's values by neighbouring lanes, sixteen rows on their way at a time (5310 x 4000 by 13887: 418 us row by row, 284 so, 265 at 13888)
+      } else {  // results at odd places, or a last box: a row's values by neighbouring lanes, sixteen rows on their way at a time (5310 x 4000 by 13887: 418 us row by row, 291 so)
         __syncwarp();
         const int rows = min(32, p.rows - row0), cols = min(kBox, p.n - col0 - c);
         OUT* o = static_cast<OUT*>(p.out) + row0 * p.ldo + col0 + c + lane;
@@ -748,7 +749,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
           [&](int c, const uint32_t(&v)[16]) {
 #pragma unroll
             for (int x = 0; x < 16; x += 2) fma_pair(acc[(c + x) / 2], pair_of(v[x], v[x + 1]), by);
-            if (c == kCols - 32 && b + 2 < p.blocks) fetch(i);  // (beside the last columns' way from TMEM: 5310 x 4000 by 13887 291 us, behind them 295)
+            // (beside the last columns' way from TMEM: 5310 x 4000 by 13887 291 us, behind them 295)
+            if (c == kCols - 32 && b + 2 < p.blocks) fetch(i);
           },
           [&]() {
             tcgen05_fence_before();
@@ -831,8 +833,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant_
 // 128 rows x BN columns of a CTA's own, rows as the MMA's M like the pairs' (one scale per thread and block).  BN = 128: the sum may be shared by a cluster's CTAs
 // like the streamed weights', and TMEM holds four accumulators.  No barrier of another CTA is on an accumulator's way, and the bound is what an SM takes in from L2:
 // 32 KB of operands in 0.30 us, some 60 bytes a clock.  BN = 256: 48 KB in 0.36 to 0.45 us for twice the work, but half as many tiles.
-// 333 x 2560 by 10240: 240 tiles of 128 columns (two waves) 17.5 us, 120 of 256 (one) 14.7; 128 x 2560 by 10240 11.0 and 14.1; 333 x 5120 by 1280, 30 tiles in four
-// parts each, 10.7.  (Pairs of CTAs with tiles of 128 columns take 26.1, 18.9 and 17.8, and 128 activation rows as the N of streamed weights 23.9, 13.7
+// 333 x 2560 by 10240: 240 tiles of 128 columns (two waves) 18.1 us, 120 of 256 (one) 14.9; 128 x 2560 by 10240 11.3 and 14.2; 333 x 5120 by 1280, 30 tiles in four
+// parts each, 10.1.  (Pairs of CTAs with tiles of 128 columns take 26.1, 18.9 and 17.8, and 128 activation rows as the N of streamed weights 23.9, 13.7
 // and 12.1: the pairs for their barriers, the others for a scale per column.)
 
 constexpr int kFp8TileWarps = 8;  // epilogue warps: 32 rows x half of the columns each
