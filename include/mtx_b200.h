@@ -762,6 +762,100 @@ int mtx_control_logits(const float* logits, long long ld, float* out, long long 
 int mtx_note_tokens(uint16_t* seen, long long ld_seen, uint32_t* touched, long long ld_touched, int slots, int vocab, const int32_t* token, const int32_t* slot, int n, int prompt,
                     mtx_stream stream);
 
+/* ---- a step of drafted tokens over shared prefixes ------------------------------------------- */
+
+/* The residual stream's sum, its RMS norm and the next product's operand in one pass, beside mtx_rmsnorm:
+ *   h = x + residual, rounded to residual_type and stored in `sum` (NULL: it is not kept);  residual NULL: h = x;
+ *   out = h * (weight_offset + weight) / sqrt(mean(h^2) + eps);  weight NULL: without that factor.
+ * x, residual (and sum, of its type), weight [width]: MTX_BF16 or MTX_F32 each; out: MTX_BF16, MTX_F32, or MTX_E4M3 with out_scale
+ * [rows, ceil(width / 128)], as mtx_quantize_fp8(block_rows = 1) gives them for out's fp32 values (8-bit values: base and pitch whole 16 bytes; the bytes behind a
+ * row's last value stay).  Pitches in values; width <= 32768; other values at any multiple of their types' sizes, with any pitch.  sum may be residual or x, and out any
+ * input, where type and pitch are the same; nothing else may overlap.  A row with a NaN is NaN throughout, one with an infinity 0 but for NaN in its place. */
+int mtx_add_rmsnorm(const void* x, int x_type, long long ldx, const void* residual, int residual_type, long long ld_residual, void* sum, long long ld_sum, const void* weight,
+                    int weight_type, float weight_offset, float eps, void* out, int out_type, long long ldo, float* out_scale, int rows, int width, mtx_stream stream);
+
+/* Frequencies of rotary positions, radians per position of pair i of rot_dims / 2, and the factor on cosine and sine; freq and amplitude are HOST memory.  f = base^(-2i / rot_dims), and
+ *   MTX_ROTARY_LINEAR  f / factor;
+ *   MTX_ROTARY_BANDS   turns = original_len f / 2 pi: f from `high` turns on, f / factor up to `low`, linear in the turns between;
+ *   MTX_ROTARY_YARN    f for the pairs in front of the one with `high` turns, f / factor behind the one with `low`, linear in i between; amplitude 0.1 ln(factor) + 1. */
+#define MTX_ROTARY_PLAIN 0
+#define MTX_ROTARY_LINEAR 1
+#define MTX_ROTARY_BANDS 2
+#define MTX_ROTARY_YARN 3
+int mtx_rotary_frequencies(int rot_dims, double base, int scaling, double factor, double original_len, double low, double high, double* freq, float* amplitude);
+
+/* Rotary positions for projected queries and keys, and the way of keys and values into the pages of mtx_paged_attention, for any number of rows of any sequences (beside
+ * mtx_qkv_rope_append and mtx_paged_append). */
+typedef struct {
+  int32_t rows;
+  int32_t heads, kv_heads;  /* either may be 0 */
+  int32_t dim;              /* channels of a head, up to 1024 */
+  int32_t rot_dims;         /* the first of them are rotated: even, 0 .. dim; the others pass */
+  int32_t rot_half;         /* 1: channel i < rot_dims / 2 is paired with channel i + rot_dims / 2, 0: 2i with 2i + 1 */
+  float amplitude;          /* factor on cosine and sine; 0 = 1 */
+  int32_t type, out_type;   /* MTX_BF16 or MTX_F32: of q, k, v, and of q_out, k_out */
+  const double* freq;       /* [rot_dims / 2] radians per position; angles are formed in 64 bits */
+  const int32_t* pos;       /* [rows] */
+  const void* q;            /* [rows, heads * dim] at pitch ldq (values), and so on: parts of one projection's row, or matrices of their own */
+  const void* k;
+  const void* v;            /* read for pages alone */
+  long long ldq, ldk, ldv;
+  void* q_out;              /* may be q, with its type and pitch */
+  long long ldq_out;
+  void* k_out;              /* NULL, or rotated keys [rows, kv_heads * dim]; may be k, with its type and pitch */
+  long long ldk_out;
+  void* k_pages;            /* NULL, or [kv_heads, num_pages, tokens_per_page, dim] bfloat16: the rotated keys go there, */
+  void* v_pages;            /* and the values; given together with page_map.  A (group, position) comes once in a call */
+  int32_t groups, num_pages, tokens_per_page, max_pages_per_group;
+  const int32_t* group;     /* [rows]; NULL: row r is group r.  With pages a row whose group is not in [0, groups) or whose position is negative is left as it is, results too; */
+  const int32_t* page_map;  /* [groups, max_pages_per_group].  keys and values whose page is not in [0, num_pages) are not stored */
+} mtx_rotary_batch;
+int mtx_rotary(const mtx_rotary_batch* b, mtx_stream stream);
+
+/* Attention of the last rows of each sequence over its pages, where neighbouring sequences share the first tokens of their contexts: mtx_paged_attention for several rows per
+ * sequence, which reads the keys and values of a shared prefix once for all its sequences. */
+typedef struct {
+  int32_t rows, sequences;
+  const int32_t* row0;        /* [sequences + 1] ascending: sequence s has the rows [row0[s], row0[s + 1]), its last tokens (none: it is left out) */
+  const int32_t* lengths;     /* [sequences] tokens in the pages, the rows' own among them: row i of n sees the first lengths - n + i + 1 */
+  const int32_t* page_map;    /* [sequences, max_pages_per_group] */
+  int32_t prefixes;           /* 0: no prefix is shared */
+  const int32_t* prefix_seq0; /* [prefixes + 1] ascending: prefix p belongs to the sequences [prefix_seq0[p], prefix_seq0[p + 1]), whose first */
+  const int32_t* prefix_len;  /* [prefixes] tokens are the same: they are read through the page map of the first of these sequences.  A sequence of which a row does not see the
+                                 whole prefix reads its own pages throughout */
+} mtx_prefix_batch;
+/* q, out [rows, num_q_heads * head_dim] bf16 at pitches ldq, ldo; k_pages, v_pages [num_kv_heads, num_pages, tokens_per_page, head_dim] bf16, tokens_per_page a power of two >= 8;
+ * head_dim 64, 128 or 256; up to 16 query heads per key head.  out = softmax(cap(scale * <q, k>)) v, cap(x) = softcap * tanh(x / softcap) (0: off).  A row that sees no token, and rows
+ * outside the sequences, are left as they were.  Page numbers outside the pool are read as page 0, lengths end with the page map.  All bases and pitches whole 16 bytes.
+ * scratch: written by every call, so one per stream (or graph) that runs at the same time; base on 256 bytes.  The same call gives the same bits every time. */
+size_t mtx_prefix_attention_scratch_bytes(int rows, int sequences, int prefixes, int num_q_heads, int num_kv_heads, int head_dim);
+int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, const void* v_pages, const mtx_prefix_batch* batch, void* out, long long ldo, int num_q_heads,
+                         int num_kv_heads, int head_dim, int num_pages, int tokens_per_page, int max_pages_per_group, float scale, float softcap, void* scratch,
+                         size_t scratch_bytes, mtx_stream stream);
+
+/* Verification of drafted tokens, beside mtx_sample_rows: the step's rows of a sequence are its last token and the drafted ones, so that row r's logits decide on token[r + 1], and the
+ * last row's on a token behind all drafts.  With p, q the softmax of the target's and the draft's logits over their temperatures and x the drafted token: x stays when
+ * accept_u * q(x) < p(x).  At the first that does not, the sequence goes on with a token drawn from max(p - q, 0) (over its sum); behind the last draft with one drawn from p.  Drawn is the
+ * first token at which the sum of the weights in the tokens' order exceeds pick_u times their whole sum. */
+typedef struct {
+  int32_t rows, sequences, vocab;  /* vocab <= 2^28 */
+  const int32_t* row0;             /* [sequences + 1] ascending, as in mtx_prefix_batch */
+  const int32_t* token;            /* [rows]: the tokens of the step's rows; a drafted token outside the vocabulary does not stay */
+  const float* target;             /* [rows, vocab] logits; NaN counts as -infinity, infinity as the largest number */
+  long long ld_target;
+  const float* draft;              /* [rows, vocab]: row r's are those that token[r + 1] was drawn from (a sequence's last row is not read).  NULL: q(x) = 1 (drafts that were looked up) */
+  long long ld_draft;
+  const float* temperature;        /* [sequences] or NULL: 1.  0: greedy, x stays when it is the largest logit, of equal ones the first */
+  const float* draft_temperature;  /* [sequences] or NULL: the target's.  0: q(x) = 1 */
+  const float* accept_u;           /* [rows] in [0, 1): row r's decides on token[r + 1] */
+  const float* pick_u;             /* [sequences] in [0, 1) */
+} mtx_draft_batch;
+/* accepted [sequences]: drafts that stay; emitted [rows]: a sequence's new tokens, those drafts and the drawn token, then -1 (as mtx_note_tokens skips it).  Rows outside the sequences
+ * are left as they were.  A row that leaves nothing to draw (no logit above -infinity) gives -1 as mtx_sample_rows does.
+ * scratch: written by every call, so one per stream (or graph) that runs at the same time; base on 16 bytes. */
+size_t mtx_verify_drafts_scratch_bytes(int rows, int sequences, int vocab);
+int mtx_verify_drafts(const mtx_draft_batch* b, int32_t* accepted, int32_t* emitted, void* scratch, size_t scratch_bytes, mtx_stream stream);
+
 /* ---- misc ---------------------------------------------------------------------------------- */
 
 /* Measurement aid: grid-barrier timeline of the persistent step kernel.  While a device buffer of

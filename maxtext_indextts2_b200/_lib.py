@@ -225,6 +225,39 @@ class LogitControls(ctypes.Structure):
               ("allowed_row", ctypes.c_void_p), ("allowed", ctypes.c_void_p), ("ld_allowed", ctypes.c_longlong)]
 
 
+ROTARY = {"plain": 0, "linear": 1, "bands": 2, "yarn": 3}  # MTX_ROTARY_*
+
+
+class RotaryBatch(ctypes.Structure):
+  """mtx_rotary_batch."""
+
+  _fields_ = (
+      [(n, ctypes.c_int32) for n in ("rows", "heads", "kv_heads", "dim", "rot_dims", "rot_half")]
+      + [("amplitude", ctypes.c_float), ("type", ctypes.c_int32), ("out_type", ctypes.c_int32)]
+      + [(n, ctypes.c_void_p) for n in ("freq", "pos", "q", "k", "v")]
+      + [(n, ctypes.c_longlong) for n in ("ldq", "ldk", "ldv")]
+      + [("q_out", ctypes.c_void_p), ("ldq_out", ctypes.c_longlong), ("k_out", ctypes.c_void_p), ("ldk_out", ctypes.c_longlong)]
+      + [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p)]
+      + [(n, ctypes.c_int32) for n in ("groups", "num_pages", "tokens_per_page", "max_pages_per_group")]
+      + [("group", ctypes.c_void_p), ("page_map", ctypes.c_void_p)]
+  )
+
+
+class PrefixBatch(ctypes.Structure):
+  """mtx_prefix_batch."""
+
+  _fields_ = [("rows", ctypes.c_int32), ("sequences", ctypes.c_int32), ("row0", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("page_map", ctypes.c_void_p),
+              ("prefixes", ctypes.c_int32), ("prefix_seq0", ctypes.c_void_p), ("prefix_len", ctypes.c_void_p)]
+
+
+class DraftBatch(ctypes.Structure):
+  """mtx_draft_batch."""
+
+  _fields_ = [("rows", ctypes.c_int32), ("sequences", ctypes.c_int32), ("vocab", ctypes.c_int32), ("row0", ctypes.c_void_p), ("token", ctypes.c_void_p),
+              ("target", ctypes.c_void_p), ("ld_target", ctypes.c_longlong), ("draft", ctypes.c_void_p), ("ld_draft", ctypes.c_longlong), ("temperature", ctypes.c_void_p),
+              ("draft_temperature", ctypes.c_void_p), ("accept_u", ctypes.c_void_p), ("pick_u", ctypes.c_void_p)]
+
+
 def sources() -> list[str]:
   return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".cc"))) + [HEADER]
 
@@ -243,7 +276,7 @@ def _jaxlib_include() -> list[str]:
     return []
 
 
-UNITS = ("engine.cu", "layered.cu", "fp8_linear.cu", "logit_controls.cu", "mtx_jax_ffi.cc")  # translation units of the library, compiled separately and linked
+UNITS = ("engine.cu", "layered.cu", "fp8_linear.cu", "logit_controls.cu", "row_operators.cu", "prefix_attention.cu", "verify_drafts.cu", "mtx_jax_ffi.cc")  # translation units of the library, compiled separately and linked
 
 
 def _unit_deps(path: str, seen=None) -> set:
@@ -421,6 +454,20 @@ def _declare(lib) -> None:
   lib.mtx_control_logits.argtypes = [vp, i64, vp, i64, i32, i32, c.POINTER(LogitControls), vp]
   lib.mtx_note_tokens.restype = i32
   lib.mtx_note_tokens.argtypes = [vp, i64, vp, i64, i32, i32, vp, vp, i32, i32, vp]
+  lib.mtx_add_rmsnorm.restype = i32
+  lib.mtx_add_rmsnorm.argtypes = [vp, i32, i64, vp, i32, i64, vp, i64, vp, i32, f32, f32, vp, i32, i64, vp, i32, i32, vp]
+  lib.mtx_rotary_frequencies.restype = i32
+  lib.mtx_rotary_frequencies.argtypes = [i32, c.c_double, i32, c.c_double, c.c_double, c.c_double, c.c_double, c.POINTER(c.c_double), c.POINTER(f32)]
+  lib.mtx_rotary.restype = i32
+  lib.mtx_rotary.argtypes = [c.POINTER(RotaryBatch), vp]
+  lib.mtx_prefix_attention_scratch_bytes.restype = sz
+  lib.mtx_prefix_attention_scratch_bytes.argtypes = [i32] * 6
+  lib.mtx_prefix_attention.restype = i32
+  lib.mtx_prefix_attention.argtypes = [vp, i64, vp, vp, c.POINTER(PrefixBatch), vp, i64] + [i32] * 6 + [f32, f32, vp, sz, vp]
+  lib.mtx_verify_drafts_scratch_bytes.restype = sz
+  lib.mtx_verify_drafts_scratch_bytes.argtypes = [i32] * 3
+  lib.mtx_verify_drafts.restype = i32
+  lib.mtx_verify_drafts.argtypes = [c.POINTER(DraftBatch), vp, vp, vp, sz, vp]
   lib.mtx_engine_rebind_state.restype = i32
   lib.mtx_engine_rebind_state.argtypes = [vp, c.POINTER(DecodeState)]
 

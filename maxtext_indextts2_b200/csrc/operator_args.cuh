@@ -1,4 +1,4 @@
-// Checks of the arguments of the operators that stand alone (fp8_linear.cu, logit_controls.cu).
+// Checks of the arguments of the operators that stand alone (fp8_linear.cu, logit_controls.cu, row_operators.cu, prefix_attention.cu, verify_drafts.cu).
 #pragma once
 
 #include <initializer_list>

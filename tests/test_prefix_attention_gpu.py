@@ -1,0 +1,279 @@
+"""Attention over shared prefixes against the definition in 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from maxtext_indextts2_b200 import _lib
+from tests import draft_helpers as ref
+
+pytestmark = pytest.mark.gpu
+
+
+class Case:
+  """Sequences with `rows` rows each; `lengths` tokens; `prefixes`: (first sequence, sequences, tokens) whose whole pages are shared and whose rest is a copy."""
+
+  def __init__(self, rows, lengths, prefixes=(), heads=4, kv=2, dim=64, page=16, seed=0, lead=0, behind=0, spare=3, more_pages=0, spread=2.0, wide=0):
+    g = torch.Generator().manual_seed(seed)
+    self.heads, self.kv, self.dim, self.page = heads, kv, dim, page
+    self.lengths, self.sequences = list(lengths), len(lengths)
+    self.row0 = [lead]
+    for n in rows:
+      self.row0.append(self.row0[-1] + n)
+    self.rows = self.row0[-1] + behind
+    used = [-(-max(0, l) // page) for l in self.lengths]
+    most = max(1, max(used, default=1)) + more_pages
+    self.num_pages = sum(used) + spare
+    order = torch.randperm(self.num_pages, generator=g).tolist()
+    maps, at = torch.zeros(max(1, self.sequences), most, dtype=torch.int32), 0
+    for s, n in enumerate(used):
+      maps[s, :n] = torch.tensor(order[at : at + n], dtype=torch.int32)
+      at += n
+    k = torch.randn(kv, self.num_pages, page, dim, generator=g)
+    v = torch.randn(kv, self.num_pages, page, dim, generator=g)
+    for first, count, tokens in prefixes:
+      whole = tokens // page
+      for s in range(first + 1, first + count):
+        maps[s, : min(whole, used[s])] = maps[first, : min(whole, used[s])]
+        if tokens % page and used[s] > whole:
+          k[:, maps[s, whole], : tokens % page] = k[:, maps[first, whole], : tokens % page]
+          v[:, maps[s, whole], : tokens % page] = v[:, maps[first, whole], : tokens % page]
+    self.bounds, self.prefix_len = [0], []
+    for first, count, tokens in prefixes:
+      while self.bounds[-1] < first:  # sequences that share nothing
+        self.bounds.append(self.bounds[-1] + 1)
+        self.prefix_len.append(0)
+      self.bounds.append(first + count)
+      self.prefix_len.append(tokens)
+    self.prefixes = len(self.prefix_len)
+    self.maps = maps
+    self.k, self.v = k.to(torch.bfloat16).cuda(), v.to(torch.bfloat16).cuda()
+    self.store = torch.full((max(1, self.rows), heads * dim + wide), 7.0, dtype=torch.bfloat16)
+    self.store[:, : heads * dim] = spread * torch.randn(max(1, self.rows), heads * dim, generator=g)
+    self.q = self.store.cuda()[:, : heads * dim]
+    self.out = torch.full((max(1, self.rows), heads * dim + 2 * wide), 7.0, dtype=torch.bfloat16, device="cuda")[:, : heads * dim]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    self.dev = dict(row0=ints(self.row0), lengths=ints(self.lengths), page_map=maps.cuda(), prefix_seq0=ints(self.bounds), prefix_len=ints(self.prefix_len or [0]))
+    self.scale = dim**-0.5
+    self.need = _lib.load().mtx_prefix_attention_scratch_bytes(self.rows, self.sequences, self.prefixes, heads, kv, dim)
+    self.scratch = torch.full((max(256, self.need),), 255, dtype=torch.uint8, device="cuda")  # (every word a NaN)
+
+  def batch(self):
+    d = {k: v.data_ptr() for k, v in self.dev.items()}
+    if not self.prefixes:
+      d["prefix_seq0"] = d["prefix_len"] = None
+    return _lib.PrefixBatch(rows=self.rows, sequences=self.sequences, prefixes=self.prefixes, **d)
+
+  def run(self, softcap=0.0, scratch=None, out=None, stream=None):
+    out = self.out if out is None else out
+    scratch = self.scratch if scratch is None else scratch
+    _lib.check(_lib.load().mtx_prefix_attention(
+        self.q.data_ptr(), self.q.stride(0), self.k.data_ptr(), self.v.data_ptr(), self.batch(), out.data_ptr(), out.stride(0), self.heads, self.kv, self.dim, self.num_pages, self.page,
+        self.maps.shape[1], self.scale, softcap, scratch.data_ptr(), scratch.numel(), torch.cuda.current_stream().cuda_stream if stream is None else stream))
+    return out
+
+  def want(self, softcap=0.0):
+    return ref.attention(self.q, self.k, self.v, self.row0, self.lengths, self.dev["page_map"], self.heads, self.scale, softcap)
+
+  def check(self, softcap=0.0):
+    got = self.run(softcap)
+    want, bound = self.want(softcap)
+    got = got.double().view(max(1, self.rows), self.heads, self.dim)[: want.shape[0]]
+    there = ~want.isnan()
+    off = ((got - want).abs() - bound)[there]
+    assert off.numel() == 0 or float(off.max()) <= 0, (float(off.max()), int((off > 0).sum()), off.numel())
+    assert bool((got[~there] == 7).all())  # rows that see nothing, or belong to nobody
+    return got
+
+
+@pytest.mark.parametrize("length", [1, 2, 7, 8, 15, 16, 17, 31, 63, 64, 65, 127, 128, 129, 300, 1000, 4097])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_one_sequence(length, dim):
+  Case([1], [length], dim=dim, seed=length).check()
+  Case([min(4, length)], [length], dim=dim, seed=length, page=8).check()
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (3, 1), (5, 1), (16, 1), (20, 4), (8, 8), (14, 2), (33, 3)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 8)])
+def test_heads(heads, kv, dim, page):
+  Case([1, 3, 2], [200, 333, 261], [(0, 3, 192)], heads=heads, kv=kv, dim=dim, page=page, seed=heads).check()
+  Case([1, 5], [100, 70], heads=heads, kv=kv, dim=dim, page=page, seed=heads + 1).check()
+
+
+@pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("tokens", [1, 8, 63, 64, 65, 100, 128, 200, 511, 1000])
+def test_prefix_lengths(page, tokens):
+  """Prefixes that end anywhere in a page or a tile."""
+  Case([1, 2, 1, 4], [tokens + 1, tokens + 60, tokens + 129, tokens + 4], [(0, 4, tokens)], page=page, seed=tokens).check()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_rows_of_a_prefix(dim):
+  """More rows than a tile holds, tails from none to long ones."""
+  g = torch.Generator().manual_seed(dim)
+  rows = torch.randint(0, 9, (70,), generator=g).tolist()
+  lengths = [700 + max(n, int(t)) for n, t in zip(rows, torch.randint(0, 300, (70,), generator=g))]
+  Case(rows, lengths, [(0, 70, 700)], heads=10, kv=2, dim=dim, page=32, seed=dim).check()
+
+
+def test_several_prefixes():
+  g = torch.Generator().manual_seed(3)
+  rows = torch.randint(1, 4, (24,), generator=g).tolist()
+  of = [300] * 5 + [0] * 3 + [1100] * 10 + [64] * 2 + [0] * 4
+  lengths = [p + n + int(t) for p, n, t in zip(of, rows, torch.randint(0, 200, (24,), generator=g))]
+  Case(rows, lengths, [(0, 5, 300), (8, 10, 1100), (18, 2, 64)], heads=8, kv=2, dim=128, page=64, seed=5).check()
+
+
+def test_rows_that_see_nothing():
+  """Sequences without rows or tokens, rows in front of their sequence's first token, rows of nobody in front of the first sequence and behind the last."""
+  Case([0, 2, 3, 1, 0], [50, 0, 2, 7, 0], lead=2, behind=5, seed=1).check()
+  Case([2, 0, 6, 1, 1], [70, 100, 66, 90, 3], [(0, 5, 64)], lead=1, behind=200, heads=6, kv=3, seed=2).check()
+  Case([3], [-4], seed=1).check()
+
+
+def test_no_sequences():
+  c = Case([1], [5])
+  c.sequences = 0
+  assert bool((c.run() == 7).all())
+  c = Case([0, 0], [5, 9], [(0, 2, 4)], behind=3)
+  assert bool((c.run() == 7).all())
+
+
+def test_sequences_inside_a_prefix():
+  """Rows whose position lies within the prefix, beside sequences that go on behind it."""
+  Case([4, 2, 3, 1, 5], [130, 200, 60, 129, 140], [(0, 5, 129)], seed=4).check()
+  Case([2, 2], [64, 65], [(0, 2, 64)], seed=4).check()
+
+
+@pytest.mark.parametrize("softcap", [5.0, 30.0])
+def test_softcap(softcap):
+  for dim in (64, 128, 256):
+    Case([2, 1, 3], [300, 258, 400], [(0, 3, 256)], dim=dim, seed=7, spread=6.0).check(softcap)
+
+
+def test_peaky_scores():
+  """Scores of some hundred: one key has it all, and it may come last."""
+  for dim in (64, 128, 256):
+    c = Case([1, 2, 1], [600, 700, 520], [(0, 3, 512)], dim=dim, seed=11, spread=60.0)
+    c.check()
+
+
+def test_pitches():
+  Case([1, 4, 2], [100, 300, 212], [(0, 3, 96)], dim=128, wide=24, seed=6).check()
+  c = Case([1, 4, 2], [100, 300, 212], [(0, 3, 96)], dim=64, wide=8, seed=6)
+  c.check()
+  base = c.out._base if c.out._base is not None else c.out
+  assert bool((base[:, 256:] == 7).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_values_that_nobody_sees(dim, bad):
+  """Whatever stands behind a sequence's tokens, in pages of nobody and in the later rows' own keys and values, changes nothing for the rows that do not see it."""
+  c = Case([1, 4, 2, 1], [301, 333, 260, 257], [(0, 4, 250)], dim=dim, page=32, seed=dim, spare=9)
+  clean = c.check().clone()
+  for s in range(4):
+    last = c.lengths[s] - 1
+    page, at = int(c.maps[s, last // 32]), last % 32
+    c.k[:, page, at + 1 :] = bad
+    c.v[:, page, at + 1 :] = bad
+  owned = set(c.maps.flatten().tolist())
+  for page in range(c.num_pages):
+    if page not in owned:
+      c.k[:, page], c.v[:, page] = bad, bad
+  assert torch.equal(c.check(), clean)
+  # the last row of a sequence sees its own value, the rows in front of it do not
+  for s, n in ((1, 4), (2, 2)):
+    last = c.lengths[s] - 1
+    c.v[:, int(c.maps[s, last // 32]), last % 32, ::3] = bad
+  got = c.run().double().view(c.rows, c.heads, dim)
+  mine = [c.row0[2] - 1, c.row0[3] - 1]
+  others = [r for r in range(c.rows) if r not in mine]
+  assert torch.equal(got[others], clean[others])
+  for r in mine:
+    assert not bool(got[r, :, ::3].isfinite().any()) and torch.equal(got[r, :, 1::3], clean[r, :, 1::3])
+
+
+def test_numbers_that_a_prefix_has():
+  """An infinite value or a NaN in a shared token reaches every row that sees it, and its channel alone."""
+  c = Case([1, 2], [300, 310], [(0, 2, 256)], dim=64, seed=1)
+  clean = c.check().clone()
+  c.v[0, int(c.maps[0, 3]), 5, 7] = math.inf
+  got = c.run().double().view(c.rows, c.heads, 64)
+  assert bool(got[:, :2, 7].isinf().all())
+  clean[:, :2, 7] = got[:, :2, 7]
+  assert torch.equal(got, clean)
+
+
+def test_pages_outside_the_pool():
+  """They are read as page 0, and a length ends with the page map."""
+  c = Case([1, 2], [90, 80], dim=64, page=16, seed=3)
+  c.dev["page_map"][0, 2], c.dev["page_map"][1, 1] = -5, c.num_pages
+  c.check()
+  c.lengths[0] = 5000
+  c.dev["lengths"][0] = 5000
+  c.check()
+
+
+def test_the_same_bits():
+  """Every call, and every place of a sequence in the scratch, with whatever a scratch held."""
+  c = Case([3, 1, 5, 2] * 8, [1100 + 37 * i for i in range(32)], [(0, 32, 1024)], heads=8, kv=2, dim=128, page=64, seed=5)
+  first = c.run().clone()
+  for fill in (0, 255, 127):
+    c.scratch.fill_(fill)
+    c.out.fill_(3)
+    assert torch.equal(c.run(), first)
+
+
+def test_streams_and_graphs():
+  """Two captured calls with a scratch each, replayed at the same time on two streams while their lengths change."""
+  cases = [Case([2, 1, 3], [400, 300, 350], [(0, 3, 256)], dim=128, page=32, seed=i, more_pages=2, spare=40) for i in range(2)]
+  graphs, streams = [torch.cuda.CUDAGraph() for _ in cases], [torch.cuda.Stream() for _ in cases]
+  torch.cuda.synchronize()
+  for c, graph, stream in zip(cases, graphs, streams):
+    with torch.cuda.graph(graph, stream=stream):
+      c.run()
+  for step in range(3):
+    for c in cases:
+      c.lengths = [l - 3 * step for l in c.lengths]
+      c.dev["lengths"].copy_(torch.tensor(c.lengths, dtype=torch.int32))
+      c.out.fill_(7)
+    torch.cuda.synchronize()
+    for _ in range(3):
+      for graph, stream in zip(graphs, streams):
+        with torch.cuda.stream(stream):
+          graph.replay()
+    torch.cuda.synchronize()
+    for c in cases:
+      want, bound = c.want()
+      assert bool(((c.out.double().view_as(want) - want).abs() <= bound).all())
+
+
+def test_far_pages():
+  """A pool of more than 2^31 values, its ends in use."""
+  kv, num_pages, page, dim = 2, 140000, 64, 128
+  c = Case([2, 1], [200, 190], [(0, 2, 128)], kv=kv, dim=dim, page=page, seed=1)
+  k, v = c.k, c.v
+  c.k, c.v = (torch.zeros(kv, num_pages, page, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+  far = torch.arange(c.num_pages) * ((num_pages - 1) // (c.num_pages - 1)) + (num_pages - 1) % (c.num_pages - 1)
+  c.k[:, far], c.v[:, far] = k, v
+  c.maps = far[c.maps.long()].int()
+  c.dev["page_map"].copy_(c.maps)
+  c.num_pages = num_pages
+  c.check()
+
+
+def test_as_paged_attention():
+  """One row per sequence and no prefix: what mtx_paged_attention gives, within both roundings."""
+  lib = _lib.load()
+  c = Case([1] * 6, [70, 1, 300, 129, 64, 500], heads=8, kv=2, dim=128, page=16, seed=2)
+  c.scale = 1.0
+  c.q.mul_(0.1)
+  got = c.run().double()
+  need = lib.mtx_paged_attention_scratch_bytes(6, 2, 8, 128, c.maps.shape[1] * 16)
+  scratch, out = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.empty(6, 1024, dtype=torch.bfloat16, device="cuda")
+  _lib.check(lib.mtx_paged_attention(c.q.contiguous().data_ptr(), c.k.data_ptr(), c.v.data_ptr(), c.dev["lengths"].data_ptr(), c.dev["page_map"].data_ptr(), out.data_ptr(), 6, 8, 2, 128,
+                                     c.num_pages, 16, c.maps.shape[1], 0.0, scratch.data_ptr(), torch.cuda.current_stream().cuda_stream))
+  _, bound = c.want()
+  assert bool(((out.double() - got).abs().view_as(bound) <= 2 * bound).all())
