@@ -833,6 +833,9 @@ int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, cons
                          int num_kv_heads, int head_dim, int num_pages, int tokens_per_page, int max_pages_per_group, float scale, float softcap, void* scratch,
                          size_t scratch_bytes, mtx_stream stream);
 
+/* Debug aid, as mtx_linear_fp8_stalls: waits inside mtx_prefix_attention's kernels that gave up. */
+int mtx_prefix_attention_stalls(uint32_t* count);
+
 /* Verification of drafted tokens, beside mtx_sample_rows: the step's rows of a sequence are its last token and the drafted ones, so that row r's logits decide on token[r + 1], and the
  * last row's on a token behind all drafts.  With p, q the softmax of the target's and the draft's logits over their temperatures and x the drafted token: x stays when
  * accept_u * q(x) < p(x).  At the first that does not, the sequence goes on with a token drawn from max(p - q, 0) (over its sum); behind the last draft with one drawn from p.  Drawn is the
@@ -845,8 +848,8 @@ typedef struct {
   long long ld_target;
   const float* draft;              /* [rows, vocab]: row r's are those that token[r + 1] was drawn from (a sequence's last row is not read).  NULL: q(x) = 1 (drafts that were looked up) */
   long long ld_draft;
-  const float* temperature;        /* [sequences] or NULL: 1.  0: greedy, x stays when it is the largest logit, of equal ones the first */
-  const float* draft_temperature;  /* [sequences] or NULL: the target's.  0: q(x) = 1 */
+  const float* temperature;        /* [sequences] or NULL: 1.  Not above 0: greedy, x stays when it is the largest logit, of equal ones the first.  Below 2^-20: 2^-20 */
+  const float* draft_temperature;  /* [sequences] or NULL: the target's.  Not above 0: q(x) = 1 */
   const float* accept_u;           /* [rows] in [0, 1): row r's decides on token[r + 1] */
   const float* pick_u;             /* [sequences] in [0, 1) */
 } mtx_draft_batch;

@@ -464,6 +464,8 @@ def _declare(lib) -> None:
   lib.mtx_prefix_attention_scratch_bytes.argtypes = [i32] * 6
   lib.mtx_prefix_attention.restype = i32
   lib.mtx_prefix_attention.argtypes = [vp, i64, vp, vp, c.POINTER(PrefixBatch), vp, i64] + [i32] * 6 + [f32, f32, vp, sz, vp]
+  lib.mtx_prefix_attention_stalls.restype = i32
+  lib.mtx_prefix_attention_stalls.argtypes = [c.POINTER(c.c_uint32)]
   lib.mtx_verify_drafts_scratch_bytes.restype = sz
   lib.mtx_verify_drafts_scratch_bytes.argtypes = [i32] * 3
   lib.mtx_verify_drafts.restype = i32

@@ -71,19 +71,6 @@ int make_map_result(CUtensorMap* m, void* base, bool f32, long long n, long long
 
 constexpr int kSms = 148;
 
-// a kernel's opt-in to more shared memory, once per device
-template <class Kernel>
-int allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
-  int device;
-  MTX_CUDA(cudaGetDevice(&device));
-  const uint64_t bit = 1ull << (device & 63);
-  if ((done.load(std::memory_order_relaxed) & bit) == 0) {
-    MTX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
-    done.fetch_or(bit, std::memory_order_relaxed);
-  }
-  return MTX_OK;
-}
-
 struct Fp8Call {
   Fp8LinearParams p;
   const void* x;

@@ -3,11 +3,50 @@
 #include "operator_args.cuh"
 #include "prefix_attention.cuh"
 
+namespace {
+
+constexpr int kPrefixWorkers = 2 * 148;  // two CTAs per SM
+
+// the scratch: the entries, a maximum and a sum per slot and pair, weighted values
+struct PrefixLayout {
+  size_t stat, part, bytes;
+
+  PrefixLayout(int rows, int sequences, int prefixes, int heads, int kv_heads, int dim) {
+    const size_t group = size_t(heads / kv_heads), entries = size_t(prefixes) + size_t(sequences);
+    // items: every row belongs to one tail and at most one prefix, and each entry has a last block that is not full
+    const size_t items = 2 * (size_t(rows) * group / kPrefixPairs) + entries, slots = items * size_t(kv_heads) + kPrefixWorkers;
+    stat = align_up((entries + 1) * sizeof(PrefixEntry), 256);
+    part = stat + align_up(slots * kPrefixPairs * sizeof(float2), 256);
+    bytes = part + slots * kPrefixPairs * size_t(dim) * sizeof(float);
+  }
+};
+
+template <int D>
+int launch_prefix(PrefixAttnParams p, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int KT = PrefixShape<D>::KT;
+  const size_t smem = prefix_smem_bytes<D>();
+  MTX_TRY(allow_smem(prefix_units_kernel<D>, smem, done));
+  p.box = p.tokens_per_page < KT ? p.tokens_per_page : KT;
+  p.workers = kPrefixWorkers;
+  p.tabled = p.prefixes + p.sequences > kPrefixCached;
+  CUtensorMap tk, tv;
+  const uint64_t pool = uint64_t(p.kv_heads) * p.num_pages * p.tokens_per_page;
+  MTX_TRY(make_map(&tk, p.k, D, pool, p.box));
+  MTX_TRY(make_map(&tv, p.v, D, pool, p.box));
+  if (p.tabled) MTX_TRY(launch(prefix_plan_kernel, dim3(1), dim3(1024), 0, st, p, KT));
+  MTX_TRY(launch(prefix_units_kernel<D>, dim3(p.workers), dim3(kPrefixThreads), smem, st, tk, tv, p));
+  const int threads = p.heads * (D / 4);
+  return launch(prefix_join_kernel<D>, dim3(p.rows), dim3(threads < 512 ? (threads + 31) / 32 * 32 : 512), 0, st, p);
+}
+
+}  // namespace
+
 extern "C" {
 
 size_t mtx_prefix_attention_scratch_bytes(int rows, int sequences, int prefixes, int num_q_heads, int num_kv_heads, int head_dim) {
   if (rows < 1 || sequences < 1 || prefixes < 0 || num_kv_heads < 1 || num_q_heads < num_kv_heads || head_dim < 1) return 0;
-  return 1024;
+  return PrefixLayout(rows, sequences, prefixes, num_q_heads, num_kv_heads, head_dim).bytes;
 }
 
 int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, const void* v_pages, const mtx_prefix_batch* b, void* out, long long ldo, int num_q_heads,
@@ -49,13 +88,26 @@ int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, cons
   p.prefix_len = b->prefix_len;
   p.heads = num_q_heads;
   p.kv_heads = num_kv_heads;
+  p.group = num_q_heads / num_kv_heads;
   p.num_pages = num_pages;
   p.tokens_per_page = tokens_per_page;
   p.max_pages = max_pages_per_group;
   p.scale = scale;
   p.softcap = softcap;
-  return launch(head_dim == 64 ? prefix_simple_kernel<64> : head_dim == 128 ? prefix_simple_kernel<128> : prefix_simple_kernel<256>, dim3(p.rows, p.heads), dim3(128), 0,
-                static_cast<cudaStream_t>(stream), p);
+  const PrefixLayout at(b->rows, b->sequences, b->prefixes, num_q_heads, num_kv_heads, head_dim);
+  uint8_t* base = static_cast<uint8_t*>(scratch);
+  p.table = reinterpret_cast<PrefixEntry*>(base);
+  p.stat = reinterpret_cast<float2*>(base + at.stat);
+  p.part = reinterpret_cast<float*>(base + at.part);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return head_dim == 64 ? launch_prefix<64>(p, st) : head_dim == 128 ? launch_prefix<128>(p, st) : launch_prefix<256>(p, st);
+}
+
+int mtx_prefix_attention_stalls(uint32_t* count) {
+  if (!count) return fail(MTX_ERR_ARG, "null argument");
+  MTX_CUDA(cudaDeviceSynchronize());  // (the copy below does not wait for streams that do not block)
+  MTX_CUDA(cudaMemcpyFromSymbol(count, d_prefix_waits_failed, sizeof(uint32_t)));
+  return MTX_OK;
 }
 
 }  // extern "C"

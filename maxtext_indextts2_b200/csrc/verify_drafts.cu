@@ -6,6 +6,32 @@
 namespace {
 
 constexpr int kMaxVocab = 1 << 28;
+constexpr int kMostSequences = 65535;  // (a grid's second dimension)
+
+// tokens per thread of a chunk: few where chunks of 4096 would leave SMs without one
+int verify_each(int rows, int vocab) { return (long long)rows * (vocab / 4096 + 1) < 4 * 148 ? 4 : 16; }
+int verify_chunks(int each, int vocab) { return (vocab + 3 - 1) / (each * kVerifyThreads) + 1; }  // (rows begin up to three tokens behind a chunk's)
+
+// the scratch: sums of chunks of either side, of the differences, tasks, counters
+struct VerifyLayout {
+  size_t draft, left, task, done, bytes;
+
+  VerifyLayout(int rows, int sequences, int vocab) {
+    const size_t chunks = size_t(verify_chunks(verify_each(rows, vocab), vocab));
+    draft = size_t(rows) * chunks * sizeof(VerifySum);
+    left = 2 * draft;
+    task = left + size_t(sequences) * chunks * sizeof(double);
+    done = task + size_t(sequences) * sizeof(VerifyTask);
+    bytes = align_up(done + size_t(sequences) * sizeof(int), 256);
+  }
+};
+
+template <int E>
+int launch_verify(const VerifyParams& p, cudaStream_t st) {
+  if (p.rows > 0) MTX_TRY(launch(verify_sums_kernel<E>, dim3(unsigned(p.rows) * unsigned(p.chunks)), dim3(kVerifyThreads), 0, st, p));
+  MTX_TRY(launch(verify_settle_kernel<E>, dim3(p.sequences), dim3(kVerifyThreads), 0, st, p));
+  return p.task != nullptr ? launch(verify_difference_kernel<E>, dim3(p.chunks, p.sequences), dim3(kVerifyThreads), 0, st, p) : MTX_OK;
+}
 
 }  // namespace
 
@@ -13,13 +39,15 @@ extern "C" {
 
 size_t mtx_verify_drafts_scratch_bytes(int rows, int sequences, int vocab) {
   if (rows < 1 || sequences < 1 || vocab < 1) return 0;
-  return 1024;
+  return VerifyLayout(rows, sequences, vocab).bytes;
 }
 
 int mtx_verify_drafts(const mtx_draft_batch* b, int32_t* accepted, int32_t* emitted, void* scratch, size_t scratch_bytes, mtx_stream stream) {
   if (!b) return fail(MTX_ERR_ARG, "null batch");
-  if (b->rows < 0 || b->rows > 1 << 20 || b->sequences < 0 || b->sequences > 1 << 16 || b->vocab < 1 || b->vocab > kMaxVocab || b->ld_target < b->vocab || (b->draft && b->ld_draft < b->vocab))
+  if (b->rows < 0 || b->rows > 1 << 20 || b->sequences < 0 || b->sequences > kMostSequences || b->vocab < 1 || b->vocab > kMaxVocab || b->ld_target < b->vocab || (b->draft && b->ld_draft < b->vocab))
     return fail(MTX_ERR_ARG, "bad rows / sequences / vocab / pitches");
+  const int each = verify_each(b->rows, b->vocab), chunks = verify_chunks(each, b->vocab);
+  if ((long long)b->rows * chunks >= 1ll << 31) return fail(MTX_ERR_ARG, "rows * vocab is too large for one call");
   if (b->sequences == 0) return MTX_OK;
   if (!accepted || !b->row0 || (b->rows && (!emitted || !b->token || !b->target || !b->accept_u)) || !b->pick_u) return fail(MTX_ERR_ARG, "null argument");
   if (!lie_on(4, {accepted, emitted, b->row0, b->token, b->target, b->draft, b->temperature, b->draft_temperature, b->accept_u, b->pick_u})) return fail(MTX_ERR_ARG, "a batch's arrays lie on 4 bytes");
@@ -43,7 +71,18 @@ int mtx_verify_drafts(const mtx_draft_batch* b, int32_t* accepted, int32_t* emit
   p.pick_u = b->pick_u;
   p.accepted = accepted;
   p.emitted = emitted;
-  return launch(verify_simple_kernel, dim3(p.sequences), dim3(kVerifyThreads), 0, static_cast<cudaStream_t>(stream), p);
+  p.chunks = chunks;
+  if (b->rows > 0) {
+    const VerifyLayout at(b->rows, b->sequences, b->vocab);
+    uint8_t* base = static_cast<uint8_t*>(scratch);
+    p.target_sum = reinterpret_cast<VerifySum*>(base);
+    p.draft_sum = reinterpret_cast<VerifySum*>(base + at.draft);
+    p.left = reinterpret_cast<double*>(base + at.left);
+    if (b->draft) p.task = reinterpret_cast<VerifyTask*>(base + at.task);
+    p.done = reinterpret_cast<int*>(base + at.done);
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return each == 4 ? launch_verify<4>(p, st) : launch_verify<16>(p, st);
 }
 
 }  // extern "C"

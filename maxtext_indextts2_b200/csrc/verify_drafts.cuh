@@ -1,12 +1,38 @@
-// Drafted tokens against the target's probabilities (simple form).
+// Drafted tokens against the target's probabilities.
+//
+//   row r, drafted token x = token[r + 1]:  x stays when u q(x) < p(x);  p = softmax(target / T), q = softmax(draft / T'), or q(x) = 1
+//   the first row whose draft does not stay draws from max(p - q, 0), the row behind the last draft from p: the first token at which the weights' sum in the tokens' order
+//   exceeds pick_u times their whole sum
+//
+// Three kernels.  The first goes through all rows in chunks and leaves every chunk's largest logit and its sum of 2^((l - largest) / T log2 e).  The second, a CTA per sequence, joins
+// the chunks, settles which drafts stay and draws where the target's own weights are drawn from: the chunks' sums say which chunk, which is then read once more.  The third goes
+// through the rows that draw from a difference, a chunk per CTA; the last CTA of a sequence draws.  Bound: bytes, every row once and those of the third kernel twice.
+//
+// Weights are 32-bit powers of two of an exponent that is rounded twice, relative to itself; sums of a thread's tokens are 32-bit, all others 64-bit: a border between two tokens
+// lies within 2^-19.5 of the whole sum of where it belongs, and the same call always draws the same token.
 #pragma once
 
 #include "common.cuh"
 
 namespace mtx {
 
+constexpr int kVerifyThreads = 256;
+
+// A chunk of a row, or a row: the largest logit, and the weights relative to it
+struct VerifySum {
+  double sum;
+  float top;   // -infinity: nothing, and the sum is 0
+  int best;    // the first token with that logit (greedy sequences)
+};
+
+// What the third kernel goes through: rows that draw from max(p - q, 0)
+struct VerifyTask {
+  int row;  // -1: nothing to do
+  VerifySum target, draft;
+};
+
 struct VerifyParams {
-  int rows, sequences, vocab;
+  int rows, sequences, vocab, chunks;
   const int *row0, *token;
   const float* target;
   long long ld_target;
@@ -14,125 +40,445 @@ struct VerifyParams {
   long long ld_draft;
   const float *temperature, *draft_temperature, *accept_u, *pick_u;
   int *accepted, *emitted;
+  VerifySum *target_sum, *draft_sum;  // [rows, chunks]
+  double* left;                       // [sequences, chunks]: sums of max(p - q, 0)
+  VerifyTask* task;                   // [sequences]
+  int* done;                          // [sequences]: chunks that are through
 };
 
-constexpr int kVerifyThreads = 1024;
+// A logit as it counts: NaN as -infinity, infinity as the largest number
+__device__ __forceinline__ float verify_logit(float l) { return fminf(fmaxf(l, -INFINITY), 3.402823466e38f); }
 
-// a logit as it counts: NaN as -infinity, infinity as the largest number
-__device__ __forceinline__ float verify_logit(float l) { return l != l ? -INFINITY : fminf(l, 3.402823466e38f); }
+// 2^(l c - base) with c = log2 e / T in two parts: both products are exact in their sums, so that the exponent has two roundings of its own size and none of the logit's
+struct VerifyScale {
+  float hi, lo;
+
+  __device__ __forceinline__ explicit VerifyScale(float heat) {
+    const double c = 1.4426950408889634074 / double(fmaxf(heat, 9.5367431640625e-07f));  // (2^-20: products with any logit's lower part stay finite)
+    hi = float(c);
+    lo = float(c - double(hi));
+  }
+  __device__ __forceinline__ double exact() const { return double(hi) + double(lo); }
+  __device__ __forceinline__ float base(float top) const { return float(double(top) * exact()); }
+};
+
+struct VerifyWeight {
+  VerifyScale scale;
+  float top, base;
+  bool far;  // logits next to the largest number: an exponent would overflow, and what is not the largest logit weighs nothing
+
+  __device__ __forceinline__ VerifyWeight(const VerifyScale& s, float t) : scale(s), top(t), base(t == -INFINITY ? 0.0f : s.base(t)), far(!(fabsf(base) < 1e30f)) {}
+  __device__ __forceinline__ float operator()(float l) const {
+    if (far) return l == top ? 1.0f : 0.0f;
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(l, scale.lo, fmaf(l, scale.hi, -base))));
+    return l == -INFINITY ? 0.0f : y;  // (its two products may be infinite to either side)
+  }
+  __device__ __forceinline__ double precise(float l) const {
+    if (l == -INFINITY || top == -INFINITY) return 0.0;
+    if (far) return l == top ? 1.0 : 0.0;
+    return exp2(fma(double(l), scale.exact(), -double(base)));
+  }
+};
+
+// how much of one sum's unit another's is: 2^(a's base - b's base)
+__device__ __forceinline__ double verify_rescale(const VerifyScale& s, float a, float b) {
+  if (a == -INFINITY) return 0.0;
+  if (a == b) return 1.0;
+  const VerifyWeight x(s, a), y(s, b);
+  if (x.far || y.far) return exp2((double(a) - double(b)) * s.exact());
+  return exp2(double(x.base) - double(y.base));
+}
 
 template <class T, class F>
-__device__ __forceinline__ T verify_reduce(T v, F&& join, T* shared) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = shared[threadIdx.x & 31];
+__device__ __forceinline__ T verify_warp(T v, F&& join) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
+// over the CTA; `shared`: a value per warp
+template <class T, class F>
+__device__ __forceinline__ T verify_block(T v, F&& join, T* shared) {
+  v = verify_warp(v, join);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = shared[0];
+#pragma unroll
+  for (int w = 1; w < kVerifyThreads / 32; ++w) v = join(v, shared[w]);
+  return v;
+}
 
-// CTA = sequence
-__global__ void __launch_bounds__(kVerifyThreads) verify_simple_kernel(const VerifyParams p) {
-  __shared__ double sums[32];
-  __shared__ int ints[32];
+struct VerifyMax {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
+};
+struct VerifyMin {
+  __device__ __forceinline__ int operator()(int a, int b) const { return min(a, b); }
+};
+struct VerifyAdd {
+  __device__ __forceinline__ double operator()(double a, double b) const { return a + b; }
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+
+// the first token of a row's chunk: rows lie anywhere, chunks begin on 16 bytes (the first up to three tokens in front of the row)
+template <int E>
+__device__ __forceinline__ int verify_begin(const float* row, int chunk) { return chunk * (E * kVerifyThreads) - int(reinterpret_cast<uintptr_t>(row) >> 2 & 3); }
+
+// A thread's E tokens of a chunk, four neighbours of every 4 x 256; -infinity outside the row.
+template <int E>
+__device__ __forceinline__ void verify_load(const float* row, int begin, int vocab, float (&l)[E]) {
+  const bool aligned = (reinterpret_cast<uintptr_t>(row + begin) & 15) == 0;
+#pragma unroll
+  for (int j = 0; j < E / 4; ++j) {
+    const int t = begin + (j * kVerifyThreads + int(threadIdx.x)) * 4;
+    if (aligned && t >= 0 && t + 4 <= vocab) {
+      const float4 u = *reinterpret_cast<const float4*>(row + t);
+      l[4 * j] = u.x, l[4 * j + 1] = u.y, l[4 * j + 2] = u.z, l[4 * j + 3] = u.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[4 * j + i] = t + i >= 0 && t + i < vocab ? row[t + i] : -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) l[i] = verify_logit(l[i]);
+}
+
+// The sequence of a row, in all threads: -1 for nobody's.
+__device__ __forceinline__ int verify_sequence(const VerifyParams& p, int row, int* shared) {
+  if (threadIdx.x == 0) *shared = -1;
+  __syncthreads();
+  for (int s = threadIdx.x; s < p.sequences; s += kVerifyThreads)
+    if (p.row0[s] <= row && row < p.row0[s + 1]) *shared = s;
+  __syncthreads();
+  return *shared;
+}
+
+__device__ __forceinline__ float verify_heat(const VerifyParams& p, int s) { return p.temperature != nullptr ? p.temperature[s] : 1.0f; }
+__device__ __forceinline__ float verify_draft_heat(const VerifyParams& p, int s) { return p.draft_temperature != nullptr ? p.draft_temperature[s] : verify_heat(p, s); }
+
+// a row's chunk: its largest logit and its sum
+template <int E>
+__device__ __forceinline__ void verify_chunk(const float (&l)[E], int begin, float heat, VerifySum* out, float* floats, double* doubles, int* ints) {
+  float top = l[0];
+#pragma unroll
+  for (int i = 1; i < E; ++i) top = fmaxf(top, l[i]);
+  top = verify_block(top, VerifyMax(), floats);
+  VerifySum r;
+  r.top = top;
+  r.sum = 0.0;
+  r.best = 0x7fffffff;
+  if (top != -INFINITY) {
+    if (heat > 0.0f) {
+      const VerifyWeight weight(VerifyScale(heat), top);
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < E; ++i) sum[i & 3] += weight(l[i]);
+      r.sum = verify_block(double((sum[0] + sum[1]) + (sum[2] + sum[3])), VerifyAdd(), doubles);
+    } else {
+      int best = 0x7fffffff;
+#pragma unroll
+      for (int j = 0; j < E / 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (l[4 * j + i] == top) best = min(best, begin + (j * kVerifyThreads + int(threadIdx.x)) * 4 + i);
+      r.best = verify_block(best, VerifyMin(), ints);
+    }
+  }
+  if (threadIdx.x == 0) *out = r;
+}
+
+// CTA = (row, chunk)
+template <int E>
+__global__ void __launch_bounds__(kVerifyThreads) verify_sums_kernel(const VerifyParams p) {
+  __shared__ float floats[8];
+  __shared__ double doubles[8];
+  __shared__ int ints[8], sequence;
   griddep_launch_dependents();
   griddep_wait();
-  const int s = blockIdx.x, tid = threadIdx.x, V = p.vocab;
+  const int row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
+  if (blockIdx.x == 0)
+    for (int s = threadIdx.x; s < p.sequences; s += kVerifyThreads) p.done[s] = 0;
+  const float* target = p.target + row * p.ld_target;
+  float l[E], d[E];
+  verify_load<E>(target, verify_begin<E>(target, chunk), p.vocab, l);
+  const int s = verify_sequence(p, row, &sequence);
+  if (s < 0) return;
+  const float heat = verify_heat(p, s), draft_heat = verify_draft_heat(p, s);
+  const bool drafted = p.draft != nullptr && heat > 0.0f && draft_heat > 0.0f && row + 1 < p.row0[s + 1];
+  const float* draft = p.draft + row * p.ld_draft;
+  if (drafted) verify_load<E>(draft, verify_begin<E>(draft, chunk), p.vocab, d);
+  const long long at = (long long)row * p.chunks + chunk;
+  verify_chunk<E>(l, verify_begin<E>(target, chunk), heat, p.target_sum + at, floats, doubles, ints);
+  if (drafted) verify_chunk<E>(d, 0, draft_heat, p.draft_sum + at, floats, doubles, ints);
+}
+
+// a row's chunks joined, by a warp
+__device__ __forceinline__ VerifySum verify_join(const VerifySum* part, int chunks, float heat) {
+  const int lane = threadIdx.x & 31;
+  VerifySum r;
+  r.top = -INFINITY;
+  r.best = 0x7fffffff;
+  for (int c = lane; c < chunks; c += 32) {
+    const VerifySum x = part[c];
+    if (x.top > r.top) r.top = x.top, r.best = x.best;  // (of equal ones the first chunk's)
+  }
+  const float top = verify_warp(r.top, VerifyMax());
+  r.best = verify_warp(r.top == top ? r.best : 0x7fffffff, VerifyMin());
+  r.top = top;
+  double sum = 0.0;
+  if (top != -INFINITY && heat > 0.0f) {
+    const VerifyScale scale(heat);
+    for (int c = lane; c < chunks; c += 32) sum += part[c].sum * verify_rescale(scale, part[c].top, top);
+  }
+  r.sum = verify_warp(sum, VerifyAdd());
+  return r;
+}
+
+// The first of `chunks` at which sums exceed `want` (in the order of the chunks; else the last one whose sum is not 0) and what is left of want in it; by a warp.  of(c): its sum.
+template <class Of>
+__device__ __forceinline__ int verify_find_chunk(Of&& of, int chunks, double& want) {
+  const int lane = threadIdx.x & 31;
+  double before = 0.0, left = 0.0;
+  int found = -1;
+  for (int c0 = 0; c0 < chunks; c0 += 32) {
+    const double x = c0 + lane < chunks ? of(c0 + lane) : 0.0;
+    double up = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double t = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += t;
+    }
+    const uint32_t over = __ballot_sync(0xffffffffu, x > 0.0 && before + up > want), some = __ballot_sync(0xffffffffu, x > 0.0);
+    const int at = over != 0 ? __ffs(over) - 1 : some != 0 ? 31 - __clz(some) : -1;
+    const double front = __shfl_sync(0xffffffffu, before + (up - x), at < 0 ? 0 : at);
+    if (at >= 0) {
+      found = c0 + at;
+      left = over != 0 ? want - front : INFINITY;
+    }
+    if (over != 0) break;
+    before += __shfl_sync(0xffffffffu, up, 31);
+  }
+  want = left;
+  return found;
+}
+
+// The first token of [begin, begin + E * 256) at which the weights' sum exceeds `want`, else the last one with a weight; by the CTA.  weight(t): of token t, 0 outside the row.
+template <int E, class Weight>
+__device__ __forceinline__ int verify_find_token(Weight&& weight, int begin, double want, double* doubles, int* ints) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t0 = begin + int(threadIdx.x) * E;
+  float w[E];
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    w[i] = weight(t0 + i);
+    sum += double(w[i]);
+  }
+  double up = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double t = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += t;
+  }
+  __syncthreads();
+  if (lane == 31) doubles[warp] = up;
+  __syncthreads();
+  double before = up - sum;
+  for (int v = 0; v < warp; ++v) before += doubles[v];
+  int found = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    before += double(w[i]);
+    if (w[i] > 0.0f) {
+      last = t0 + i;
+      if (before > want && found == 0x7fffffff) found = t0 + i;
+    }
+  }
+  found = verify_block(found, VerifyMin(), ints);
+  last = verify_block(last, VerifyMax(), ints);
+  return found != 0x7fffffff ? found : last;
+}
+
+// A token drawn from the target's own weights of a row; `without`: a token that is not drawn (-1: none).  By the CTA.  -1: nothing to draw.
+template <int E>
+__device__ int verify_draw_target(const VerifyParams& p, int row, float heat, float pick, int without, double* doubles, int* ints) {
+  __shared__ double want_in;
+  __shared__ int chunk_in;
+  __syncthreads();
+  const float* target = p.target + row * p.ld_target;
+  const VerifySum* part = p.target_sum + (long long)row * p.chunks;
+  const VerifyScale scale(heat);
+  const VerifySum all = verify_join(part, p.chunks, heat);  // (every warp)
+  if (all.top == -INFINITY) return -1;
+  // the chunk without its token: anew, for a difference would leave the rounding of what may be nearly all of it
+  int chunk_of = -1;
+  double rest = 0.0;
+  if (without >= 0) {
+    chunk_of = (without - verify_begin<E>(target, 0)) / (E * kVerifyThreads);
+    const int begin = verify_begin<E>(target, chunk_of);
+    float l[E];
+    verify_load<E>(target, begin, p.vocab, l);
+    const VerifyWeight weight(scale, part[chunk_of].top);
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (part[chunk_of].top != -INFINITY) {
+#pragma unroll
+      for (int j = 0; j < E / 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (begin + (j * kVerifyThreads + int(threadIdx.x)) * 4 + i != without) sum[i] += weight(l[4 * j + i]);
+    }
+    rest = verify_block(double((sum[0] + sum[1]) + (sum[2] + sum[3])), VerifyAdd(), doubles);
+  }
+  auto of = [&](int c) { return (c == chunk_of ? rest : part[c].sum) * verify_rescale(scale, part[c].top, all.top); };
+  if (threadIdx.x < 32) {
+    double total = 0.0;
+    for (int c = threadIdx.x; c < p.chunks; c += 32) total += of(c);
+    total = verify_warp(total, VerifyAdd());
+    double want = double(pick) * total;
+    int chunk = verify_find_chunk(of, p.chunks, want);
+    if (chunk >= 0) want /= verify_rescale(scale, part[chunk].top, all.top);
+    if (threadIdx.x == 0) want_in = want, chunk_in = chunk;
+  }
+  __syncthreads();
+  const int chunk = chunk_in;
+  if (chunk < 0) return -1;
+  const VerifyWeight weight(scale, part[chunk].top);
+  return verify_find_token<E>([&](int t) { return t >= 0 && t < p.vocab && t != without ? weight(verify_logit(target[t])) : 0.0f; }, verify_begin<E>(target, chunk), want_in, doubles, ints);
+}
+
+// CTA = sequence
+template <int E>
+__global__ void __launch_bounds__(kVerifyThreads) verify_settle_kernel(const VerifyParams p) {
+  __shared__ double doubles[8];
+  __shared__ int ints[8], first_stop;
+  griddep_launch_dependents();
+  const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) first_stop = 0x7fffffff;
+  griddep_wait();
   const int first = max(p.row0[s], 0), end = min(p.row0[s + 1], p.rows);
+  if (threadIdx.x == 0 && p.task != nullptr) p.task[s].row = -1;
   if (end <= first) {
-    if (tid == 0) p.accepted[s] = 0;
+    if (threadIdx.x == 0) p.accepted[s] = 0;
     return;
   }
-  const float heat = p.temperature != nullptr ? p.temperature[s] : 1.0f, draft_heat = p.draft_temperature != nullptr ? p.draft_temperature[s] : heat;
+  const float heat = verify_heat(p, s), draft_heat = verify_draft_heat(p, s);
   const bool greedy = !(heat > 0.0f), sure = p.draft == nullptr || !(draft_heat > 0.0f);
-  auto add = [](double a, double b) { return a + b; };
-  auto more = [](double a, double b) { return a > b ? a : b; };
-  auto less = [](int a, int b) { return a < b ? a : b; };
-  auto later = [](int a, int b) { return a > b ? a : b; };
-  struct Stat { double top, sum; };
-  auto stat = [&](const float* l, float t) {
-    double top = -INFINITY, sum = 0.0;
-    for (int i = tid; i < V; i += kVerifyThreads) top = more(top, double(verify_logit(l[i])));
-    top = verify_reduce(top, more, sums);
-    if (top == -INFINITY || !(t > 0.0f)) return Stat{top, 0.0};
-    for (int i = tid; i < V; i += kVerifyThreads) sum += exp((double(verify_logit(l[i])) - top) / t);
-    return Stat{top, verify_reduce(sum, add, sums)};
-  };
-  int row = first;
-  for (;; ++row) {
-    const float *l = p.target + row * p.ld_target, *d = sure ? nullptr : p.draft + row * p.ld_draft;
+  __syncthreads();
+  for (int row = first + warp; row < end; row += kVerifyThreads / 32) {
     const bool final = row == end - 1;
-    const int x = final ? -1 : p.token[row + 1];
-    const Stat a = stat(l, heat);
-    const bool known = x >= 0 && x < V;
-    if (greedy) {
-      int best = V;
-      if (a.top != -INFINITY)
-        for (int i = tid; i < V; i += kVerifyThreads)
-          if (double(verify_logit(l[i])) == a.top) best = min(best, i);
-      best = verify_reduce(best, less, ints);
-      if (!final && known && best == x) {
-        if (tid == 0) p.emitted[row] = x;
-        continue;
-      }
-      if (tid == 0) p.emitted[row] = best < V ? best : -1;
-      break;
-    }
-    const Stat b = final || sure ? Stat{0.0, 0.0} : stat(d, draft_heat);
-    auto prob = [&](int i) { return a.top == -INFINITY ? 0.0 : exp((double(verify_logit(l[i])) - a.top) / heat) / a.sum; };
-    auto drafted = [&](int i) { return b.top == -INFINITY ? 0.0 : exp((double(verify_logit(d[i])) - b.top) / draft_heat) / b.sum; };
-    if (!final && known && double(p.accept_u[row]) * (sure ? 1.0 : drafted(x)) < prob(x)) {
-      if (tid == 0) p.emitted[row] = x;
-      continue;
-    }
-    int out = -1;
-    for (int plain = 0; plain < 2 && out < 0; ++plain) {  // (what is left may be nothing: then the target's own)
-      auto weight = [&](int i) {
-        const double w = prob(i);
-        if (plain || final) return w;
-        if (sure) return i == x ? 0.0 : w;
-        return w > drafted(i) ? w - drafted(i) : 0.0;
-      };
-      // a thread has neighbouring tokens
-      const int each = (V + kVerifyThreads - 1) / kVerifyThreads, i0 = min(tid * each, V), i1 = min(i0 + each, V);
-      double sum = 0.0;
-      for (int i = i0; i < i1; ++i) sum += weight(i);
-      double before = sum;  // inclusive sums over the threads
-      for (int o = 1; o < 32; o <<= 1) {
-        const double t = __shfl_up_sync(0xffffffffu, before, o);
-        if ((tid & 31) >= o) before += t;
-      }
-      __syncthreads();
-      if ((tid & 31) == 31) sums[tid >> 5] = before;
-      __syncthreads();
-      double base = 0.0, total = 0.0;
-      for (int w = 0; w < 32; ++w) {
-        if (w < tid >> 5) base += sums[w];
-        total += sums[w];
-      }
-      before = base + before - sum;
-      const double want = double(p.pick_u[s]) * total;
-      int found = V, last = -1;
-      for (int i = i0; i < i1; ++i) {
-        const double w = weight(i);
-        before += w;
-        if (w > 0.0) {
-          last = i;
-          if (before > want) found = min(found, i);
+    bool stays = false;
+    if (!final) {
+      const int x = p.token[row + 1];
+      if (x >= 0 && x < p.vocab) {
+        const VerifySum a = verify_join(p.target_sum + (long long)row * p.chunks, p.chunks, heat);
+        if (greedy) {
+          stays = a.top != -INFINITY && a.best == x;
+        } else if (a.top != -INFINITY) {
+          const double here = VerifyWeight(VerifyScale(heat), a.top).precise(verify_logit(p.target[row * p.ld_target + x])) / a.sum;
+          double there = 1.0;
+          if (!sure) {
+            const VerifySum b = verify_join(p.draft_sum + (long long)row * p.chunks, p.chunks, draft_heat);
+            there = b.top == -INFINITY ? 0.0 : VerifyWeight(VerifyScale(draft_heat), b.top).precise(verify_logit(p.draft[row * p.ld_draft + x])) / b.sum;
+          }
+          stays = double(p.accept_u[row]) * there < here;
         }
       }
-      found = verify_reduce(found, less, ints);
-      last = verify_reduce(last, later, ints);
-      out = found < V ? found : last;
     }
-    if (tid == 0) p.emitted[row] = out;
-    break;
+    if (!stays) {
+      if (lane == 0) atomicMin(&first_stop, row);
+      break;
+    }
   }
-  if (tid == 0) p.accepted[s] = row - first;
-  for (int r = row + 1 + tid; r < end; r += kVerifyThreads) p.emitted[r] = -1;
+  __syncthreads();
+  const int stop = first_stop;
+  for (int row = first + threadIdx.x; row < end; row += kVerifyThreads)
+    if (row != stop) p.emitted[row] = row < stop ? p.token[row + 1] : -1;
+  if (threadIdx.x == 0) p.accepted[s] = stop - first;
+  const bool final = stop == end - 1;
+  if (greedy) {
+    if (warp == 0) {
+      const VerifySum a = verify_join(p.target_sum + (long long)stop * p.chunks, p.chunks, heat);
+      if (lane == 0) p.emitted[stop] = a.top == -INFINITY ? -1 : a.best;
+    }
+    return;
+  }
+  if (final || sure) {
+    const int x = final ? -1 : p.token[stop + 1];
+    int drawn = verify_draw_target<E>(p, stop, heat, p.pick_u[s], x >= 0 && x < p.vocab ? x : -1, doubles, ints);
+    if (drawn < 0 && !final) drawn = verify_draw_target<E>(p, stop, heat, p.pick_u[s], -1, doubles, ints);  // (the draft is all that the target may say)
+    if (threadIdx.x == 0) p.emitted[stop] = drawn;
+    return;
+  }
+  if (warp == 0) {
+    VerifyTask t;
+    t.row = stop;
+    t.target = verify_join(p.target_sum + (long long)stop * p.chunks, p.chunks, heat);
+    t.draft = verify_join(p.draft_sum + (long long)stop * p.chunks, p.chunks, draft_heat);
+    if (lane == 0) {
+      p.emitted[stop] = -1;
+      if (t.target.top != -INFINITY) p.task[s] = t;
+    }
+  }
+}
+
+// max(p - q, 0) of a row's tokens
+struct VerifyDifference {
+  VerifyWeight target, draft;
+  float by_target, by_draft;
+
+  __device__ __forceinline__ VerifyDifference(const VerifyTask& t, float heat, float draft_heat)
+      : target(VerifyScale(heat), t.target.top), draft(VerifyScale(draft_heat), t.draft.top), by_target(float(1.0 / t.target.sum)),
+        by_draft(t.draft.top == -INFINITY ? 0.0f : float(1.0 / t.draft.sum)) {}
+  __device__ __forceinline__ float operator()(float l, float d) const { return fmaxf(target(l) * by_target - draft(d) * by_draft, 0.0f); }
+};
+
+// CTA = (chunk, sequence), the last sequences first: their rows are what the first kernel has left in L2
+template <int E>
+__global__ void __launch_bounds__(kVerifyThreads) verify_difference_kernel(const VerifyParams p) {
+  __shared__ double doubles[8], want_in;
+  __shared__ int ints[8], is_last, chunk_in;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int s = p.sequences - 1 - int(blockIdx.y), chunk = blockIdx.x;
+  const VerifyTask task = p.task[s];
+  if (task.row < 0) return;
+  const float heat = verify_heat(p, s), draft_heat = verify_draft_heat(p, s);
+  const float *target = p.target + task.row * p.ld_target, *draft = p.draft + task.row * p.ld_draft;
+  const VerifyDifference weight(task, heat, draft_heat);
+  {
+    const int begin = verify_begin<E>(target, chunk);
+    float l[E], d[E], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    verify_load<E>(target, begin, p.vocab, l);
+    verify_load<E>(draft, begin, p.vocab, d);
+#pragma unroll
+    for (int i = 0; i < E; ++i) sum[i & 3] += weight(l[i], d[i]);
+    const double all = verify_block(double((sum[0] + sum[1]) + (sum[2] + sum[3])), VerifyAdd(), doubles);
+    if (threadIdx.x == 0) {
+      p.left[(long long)s * p.chunks + chunk] = all;
+      __threadfence();
+      is_last = atomicAdd(&p.done[s], 1) == p.chunks - 1;
+      __threadfence();
+    }
+  }
+  __syncthreads();
+  if (!is_last) return;
+  const double* left = p.left + (long long)s * p.chunks;
+  if (threadIdx.x < 32) {
+    double total = 0.0;
+    for (int c = threadIdx.x; c < p.chunks; c += 32) total += __ldcg(left + c);
+    total = verify_warp(total, VerifyAdd());
+    double want = double(p.pick_u[s]) * total;
+    const int found = verify_find_chunk([&](int c) { return __ldcg(left + c); }, p.chunks, want);
+    if (threadIdx.x == 0) want_in = want, chunk_in = found;
+  }
+  __syncthreads();
+  int drawn;
+  if (chunk_in >= 0)
+    drawn = verify_find_token<E>([&](int t) { return t >= 0 && t < p.vocab ? weight(verify_logit(target[t]), verify_logit(draft[t])) : 0.0f; }, verify_begin<E>(target, chunk_in), want_in,
+                                 doubles, ints);
+  else  // (no difference that 32 bits show: the target's own)
+    drawn = verify_draw_target<E>(p, task.row, heat, p.pick_u[s], -1, doubles, ints);
+  if (threadIdx.x == 0) p.emitted[task.row] = drawn;
 }
 
 }  // namespace mtx

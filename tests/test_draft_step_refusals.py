@@ -140,6 +140,10 @@ def test_attention_without_a_batch(lib):
   refused(lib.mtx_prefix_attention(*ATTEND.values()), "null batch")
 
 
+def test_stalls(lib):
+  refused(lib.mtx_prefix_attention_stalls(None), "null")
+
+
 def test_scratch_of_an_attention(lib):
   size = lib.mtx_prefix_attention_scratch_bytes
   assert size(0, 1, 0, 4, 2, 64) == 0 and size(4, 0, 0, 4, 2, 64) == 0 and size(4, 1, -1, 4, 2, 64) == 0

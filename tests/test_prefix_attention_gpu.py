@@ -1,5 +1,6 @@
 """Attention over shared prefixes against the definition in 64 bits."""
 
+import ctypes
 import math
 
 import pytest
@@ -9,6 +10,15 @@ from maxtext_indextts2_b200 import _lib
 from tests import draft_helpers as ref
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _no_stalls():
+  """No wait in the kernels has run out (their results would be wrong without an error)."""
+  yield
+  count = ctypes.c_uint32(1)
+  _lib.check(_lib.load().mtx_prefix_attention_stalls(ctypes.byref(count)))
+  assert count.value == 0
 
 
 class Case:
@@ -248,6 +258,17 @@ def test_streams_and_graphs():
     for c in cases:
       want, bound = c.want()
       assert bool(((c.out.double().view_as(want) - want).abs() <= bound).all())
+
+
+def test_many_sequences():
+  """More sequences than a CTA keeps entries of, with and without prefixes."""
+  g = torch.Generator().manual_seed(8)
+  rows = torch.randint(0, 3, (300,), generator=g).tolist()
+  lengths = [40 + n + int(t) for n, t in zip(rows, torch.randint(0, 60, (300,), generator=g))]
+  Case(rows, lengths, [(0, 100, 40), (150, 120, 33)], seed=8).check()
+  Case(rows, lengths, seed=9).check()
+  Case([1] * 128, [20] * 128, seed=10).check()
+  Case([1] * 127, [50] * 127, [(0, 127, 32)], seed=11).check()
 
 
 def test_far_pages():
