@@ -4,7 +4,11 @@
 //   y = h (offset + weight) / sqrt(mean(h^2) + eps)
 //   out = y, or blocks of 128 values as 8 bits: A = max(max |y|, 2^-96), scale = A / 448, e4m3(y (448 / A))
 //
-// A row lives in the registers of its threads, eight neighbouring values of every 8 T (T threads), so that the sixteen lanes of half a warp hold a block of 128.
+// A row lives in the registers of its threads, eight neighbouring values of every 8 T (T threads), so that the sixteen lanes of half a warp hold a block of 128.  
+//
+// The mean (of sums of eight), the norm's factor and the scales' fractions are 64-bit, so that scales and 8-bit values are those of the definition; what 64 bits cost is spent
+// once per row and block, by one warp.  A value that 32 bits bring next to a border of two 8-bit values (one in 60,000) is formed again in 64.  Other results have two
+// roundings in 32 bits and their type's own.
 #pragma once
 
 #include "fp8_linear.cuh"
@@ -22,6 +26,7 @@ struct AddNormParams {
   const void* weight;
   int weight_f32;
   float weight_offset, eps;
+  double by_width;  // 1 / width
   void* out;
   int out_type;  // MTX_BF16, MTX_F32 or MTX_E4M3
   long long ldo;
@@ -37,128 +42,242 @@ template <class TX, class TR>
 struct AddNormRow {
   typedef typename std::conditional<std::is_same<TR, NoResidual>::value, TX, TR>::type TH;  // h's type
   static constexpr bool kAdd = !std::is_same<TR, NoResidual>::value;
-
-  const TX* x;
-  const TH* r;
-  TH* s;
-  uintptr_t xb, xe, rb, re;
-
-  __device__ __forceinline__ AddNormRow(const AddNormParams& p, int row) {
-    const TX* x0 = static_cast<const TX*>(p.x);
-    x = x0 + row * p.ldx;
-    xb = reinterpret_cast<uintptr_t>(x0), xe = reinterpret_cast<uintptr_t>(x0 + (p.rows - 1) * p.ldx + p.width);
-    if (kAdd) {
-      const TH* r0 = static_cast<const TH*>(p.residual);
-      r = r0 + row * p.ldr;
-      rb = reinterpret_cast<uintptr_t>(r0), re = reinterpret_cast<uintptr_t>(r0 + (p.rows - 1) * p.ldr + p.width);
-      s = p.sum != nullptr ? static_cast<TH*>(p.sum) + row * p.lds : nullptr;
-    }
-  }
 };
 
-template <class TX, class TR, int J>
-__global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const AddNormParams p) {
+// x + r as it is stored
+template <class TX, class TR>
+__device__ __forceinline__ float norm_sum(TX x, float r) {
+  const float h = static_cast<float>(x) + r;
+  return std::is_same<TR, bf16>::value ? bf16r(h) : h;
+}
+
+// offset + weight of a thread's eight values
+__device__ __forceinline__ void norm_weights(const AddNormParams& p, int c, float (&w)[8]) {
+  const int n = p.width - c;
+  if (p.weight == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 1.0f;
+    return;
+  }
+  if (p.weight_f32) {
+    const float* w0 = static_cast<const float*>(p.weight);
+    uint32_t u[8];
+    load_piece<float>(w0 + c, n, reinterpret_cast<uintptr_t>(w0), reinterpret_cast<uintptr_t>(w0 + p.width), u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = piece_value<float>(u, i);
+  } else {
+    const bf16* w0 = static_cast<const bf16*>(p.weight);
+    uint32_t u[4];
+    load_piece<bf16>(w0 + c, n, reinterpret_cast<uintptr_t>(w0), reinterpret_cast<uintptr_t>(w0 + p.width), u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = piece_value<bf16>(u, i);
+  }
+  if (p.weight_offset != 0.0f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] += p.weight_offset;
+  }
+}
+
+// a product in 64 bits as the fp32 number that rounds to any shorter format as the product would: towards zero, and odd where something was cut
+__device__ __forceinline__ float norm_odd(double v) {
+  const float t = __double2float_rz(v);
+  return double(t) == v || !(fabsf(t) < INFINITY) ? t : __uint_as_float(__float_as_uint(t) | 1u);
+}
+
+// Borders of 8-bit values: from 2^-6 on the numbers whose last 20 bits are 2^19, below (where 8-bit values are 2^-9 apart) some of those whose last 19 are 0.
+// At most 8: the number is a border or up to four last bits away from one.
+__device__ __forceinline__ uint32_t norm_off_border(float v) { return (__float_as_uint(v) + 0x80004u) & 0xfffffu; }
+__device__ __forceinline__ bool norm_next_to_border(float v) {
+  if (fabsf(v) >= 0x1p-6f) return norm_off_border(v) <= 8;
+  return ((__float_as_uint(v) + 4) & 0x7ffffu) <= 8 && fabsf(v) >= 0x1p-11f;  // (less is 0)
+}
+
+// CTA = a row, or eight rows of a warp each.  VEC: all rows lie on 16 bytes and end with whole eight values.
+template <class TX, class TR, bool E4M3, bool VEC, int J, int T>
+__global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 512 ? 1536 / T : 1) add_rmsnorm_kernel(const AddNormParams p) {
   typedef AddNormRow<TX, TR> Row;
   typedef typename Row::TH TH;
-  __shared__ float part[32];
+  __shared__ double part[32], inv_of_row;
+  __shared__ float block_top[256], block_low[256], block_f[256], block_by[256];  // of a row; of the warps' rows four blocks each
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31, threads = blockDim.x;  // of a row; rows of a warp each lie along threadIdx.y
-  const int row = blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= p.rows) return;  // (whole warps; the block waits for one another only where it has one row)
-  const Row at(p, row);
-  uint32_t rx[J][kPieceWords<TX>], rr[J][kPieceWords<TH>];
+  const int row = blockIdx.x * blockDim.y + threadIdx.y, block0 = threadIdx.y * 4;
+  const bool single = threads == 32;
+  if (row >= p.rows) return;  // (whole warps; the CTA's threads wait for one another only where it has one row)
+  const TX* x0 = static_cast<const TX*>(p.x);
+  const TH* r0 = static_cast<const TH*>(p.residual);
+  auto load = [&](auto* base, long long ld, int c, auto& w) {
+    typedef typename std::remove_const<typename std::remove_pointer<decltype(base)>::type>::type V;
+    if (VEC) {
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int c = (threadIdx.x + j * threads) * 8;
-    load_piece<TX>(at.x + c, p.width - c, at.xb, at.xe, rx[j]);
-    if (Row::kAdd) load_piece<TH>(at.r + c, p.width - c, at.rb, at.re, rr[j]);
-  }
-  float h[J][8], sum = 0.0f;
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int c = (threadIdx.x + j * threads) * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[j][i] = piece_value<TX>(rx[j], i) + (Row::kAdd ? piece_value<TH>(rr[j], i) : 0.0f);
-    if (Row::kAdd) {
-      pack_piece<TH>(h[j], rr[j]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[j][i] = piece_value<TH>(rr[j], i);
-      if (at.s != nullptr) store_piece<TH>(at.s + c, p.width - c, rr[j]);
+      for (int i = 0; i < kPieceWords<V> / 4; ++i) {
+        const uint4 u = c < p.width ? reinterpret_cast<const uint4*>(base + row * ld + c)[i] : make_uint4(0, 0, 0, 0);
+        w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+      }
+    } else {
+      load_piece<V>(base + row * ld + c, p.width - c, reinterpret_cast<uintptr_t>(base), reinterpret_cast<uintptr_t>(base + (p.rows - 1) * ld + p.width), w);
     }
-    float local = 0.0f;
+  };
+  auto store = [&](auto* base, long long ld, int c, const auto& w) {
+    typedef typename std::remove_pointer<decltype(base)>::type V;
+    if (VEC) {
+      if (c < p.width) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) local = fmaf(h[j][i], h[j][i], local);
-    sum += local;
+        for (int i = 0; i < kPieceWords<V> / 4; ++i) reinterpret_cast<uint4*>(base + row * ld + c)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+      }
+    } else {
+      store_piece<V>(base + row * ld + c, p.width - c, w);
+    }
+  };
+  uint32_t x[J][kPieceWords<TX>], r[J][kPieceWords<TH>];
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int c = (threadIdx.x + j * threads) * 8;
+    load(x0, p.ldx, c, x[j]);
+    if (Row::kAdd) load(r0, p.ldr, c, r[j]);
+  }
+  double sum = 0.0;
+  float v[J][8];  // h times the weight
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const int c = (threadIdx.x + j * threads) * 8;
+    float h[8], w[8], local[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = piece_value<TX>(x[j], i) + (Row::kAdd ? piece_value<TH>(r[j], i) : 0.0f);
+    if (Row::kAdd) {
+      pack_piece<TH>(h, r[j]);
+      if (p.sum != nullptr) store(static_cast<TH*>(p.sum), p.lds, c, r[j]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = piece_value<TH>(r[j], i);
+    }
+    norm_weights(p, c, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      local[i & 1] = fmaf(h[i], h[i], local[i & 1]);
+      v[j][i] = h[i] * w[i];
+    }
+    sum += double(local[0] + local[1]);
+    if (E4M3) {  // 16 lanes have a block: its largest product, and what that product's rounding took off
+      float mine = 0.0f, low = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine = fmaxf(mine, fabsf(v[j][i]));
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (fabsf(v[j][i]) == mine) low = fmaf(fabsf(h[i]), fabsf(w[i]), -mine);
+      float top = mine;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (mine != top) low = -INFINITY;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) low = fmaxf(low, __shfl_xor_sync(0xffffffffu, low, o));
+      if ((lane & 15) == 0 && c < p.width) block_top[block0 + c / kScaleBlock] = top, block_low[block0 + c / kScaleBlock] = low;
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (threads > 32) {
+  double inv;
+  auto whole = [&]() {
+    if (!single) {
+      sum = lane < threads / 32 ? part[lane] : 0.0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    return sum * p.by_width + double(p.eps);
+  };
+  if (!single) {
     if (lane == 0) part[threadIdx.x >> 5] = sum;
     __syncthreads();
-    sum = lane < threads / 32 ? part[lane] : 0.0f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  } else {
+    __syncwarp();
   }
-  const float inv = __frsqrt_rn(__fadd_rn(__fdiv_rn(sum, float(p.width)), p.eps));
+  if (!E4M3) {
+    const float f = __frsqrt_rn(float(whole()));
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = (threadIdx.x + j * threads) * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] *= f;
+      if (p.out_type == MTX_F32) {
+        uint32_t o[8];
+        pack_piece<float>(v[j], o);
+        store(static_cast<float*>(p.out), p.ldo, c, o);
+      } else {
+        uint32_t o[4];
+        pack_piece<bf16>(v[j], o);
+        store(static_cast<bf16*>(p.out), p.ldo, c, o);
+      }
+    }
+    return;
+  }
+  // one warp has the row's factor and the blocks' fractions, a lane a block
+  if (threadIdx.x < 32) {
+    inv = rsqrt(whole());
+    for (int b = lane; b < p.blocks; b += 32) {
+      const float top = block_top[block0 + b], low = block_low[block0 + b];
+      double largest = (double(top) + double(fabsf(low) < INFINITY ? low : 0.0f)) * inv;
+      if (largest < 0x1p-96) largest = 0x1p-96;
+      const double rough = double(__frcp_rn(float(largest))), off = fma(-largest, rough, 1.0), recip = fma(rough, fma(off, off, off), rough);
+      const float by = float(448.0 * recip);
+      block_by[block0 + b] = by;
+      block_f[block0 + b] = float(inv * double(by));
+      p.scale[(long long)row * p.blocks + b] = float(largest * (1.0 / 448.0));
+    }
+    if (!single && lane == 0) inv_of_row = inv;
+  }
+  if (!single) __syncthreads();
+  else __syncwarp();
+  int again = 0;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int c = (threadIdx.x + j * threads) * 8, n = p.width - c;
-    if (p.weight != nullptr) {
-      float w[8];
-      if (p.weight_f32) {
-        const float* w0 = static_cast<const float*>(p.weight);
-        uint32_t u[8];
-        load_piece<float>(w0 + c, n, reinterpret_cast<uintptr_t>(w0), reinterpret_cast<uintptr_t>(w0 + p.width), u);
+    if (n <= 0) continue;
+    const float f = block_f[block0 + c / kScaleBlock];
+    uint32_t near = f < INFINITY ? 0xfffffu : 0u;
+    float least = INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = piece_value<float>(u, i);
-      } else {
-        const bf16* w0 = static_cast<const bf16*>(p.weight);
-        uint32_t u[4];
-        load_piece<bf16>(w0 + c, n, reinterpret_cast<uintptr_t>(w0), reinterpret_cast<uintptr_t>(w0 + p.width), u);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = piece_value<bf16>(u, i);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[j][i] *= p.weight_offset + w[i];
+    for (int i = 0; i < 8; ++i) {
+      v[j][i] *= f;  // within four last bits
+      near = min(near, norm_off_border(v[j][i]));
+      least = fminf(least, fabsf(v[j][i]));
     }
-    if (p.out_type == MTX_E4M3) {
-      // the block's largest |y| by its bits, so that a NaN stays
-      uint32_t top = 0;
+    if (near <= 8 || least < 0x1p-6f) {
+      bool border = !(f < INFINITY);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) top = max(top, __float_as_uint(h[j][i] * inv) & 0x7fffffffu);
+      for (int i = 0; i < 8; ++i) border = border || norm_next_to_border(v[j][i]);
+      if (border) again |= 1 << j;
+    }
+    uint32_t e[4];
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float largest = __uint_as_float(max(top, kLeastLargest)), up = __fdiv_rn(448.0f, largest);
-      const bool apart = !(inv * up < INFINITY);                          // (rows next to zero with an eps next to it)
-      const float by = apart ? up : inv * up, first = apart ? inv : 1.0f;  // one factor for both steps: one rounding less per value
-      if (n > 0) {
-        if ((lane & 15) == 0) p.scale[(long long)row * p.blocks + c / kScaleBlock] = __fdiv_rn(largest, 448.0f);
-        uint32_t e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = e4m3_pair(h[j][2 * i] * first * by, h[j][2 * i + 1] * first * by);
-        uint8_t* to = static_cast<uint8_t*>(p.out) + row * p.ldo + c;
-        if (n >= 8) {
-          *reinterpret_cast<uint2*>(to) = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < n) to[i] = uint8_t(e[i / 2] >> (i % 2 * 8));
-        }
-      }
+    for (int i = 0; i < 4; ++i) e[i] = e4m3_pair(v[j][2 * i], v[j][2 * i + 1]);
+    uint8_t* to = static_cast<uint8_t*>(p.out) + row * p.ldo + c;
+    if (VEC || n >= 8) {
+      *reinterpret_cast<uint2*>(to) = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[j][i] *= inv;
-      if (p.out_type == MTX_F32) {
-        uint32_t w[8];
-        pack_piece<float>(h[j], w);
-        store_piece<float>(static_cast<float*>(p.out) + row * p.ldo + c, n, w);
-      } else {
-        uint32_t w[4];
-        pack_piece<bf16>(h[j], w);
-        store_piece<bf16>(static_cast<bf16*>(p.out) + row * p.ldo + c, n, w);
-      }
+      for (int i = 0; i < 8; ++i)
+        if (i < n) to[i] = uint8_t(e[i / 2] >> (i % 2 * 8));
+    }
+  }
+  // values next to a border once more, from memory (registers for this would be every row's)
+  __syncwarp();  // (a sum may have been stored by the next lane)
+  if (again == 0) return;
+  const double row_inv = single ? inv : inv_of_row;
+#pragma unroll 1
+  for (int j = 0; j < J; ++j) {
+    if (!(again >> j & 1)) continue;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const int c = (threadIdx.x + j * threads) * 8 + i;
+      if (c >= p.width) break;
+      float h;
+      if (Row::kAdd && p.sum != nullptr) h = static_cast<float>(static_cast<const TH*>(p.sum)[row * p.lds + c]);
+      else h = norm_sum<TX, TR>(x0[row * p.ldx + c], Row::kAdd ? static_cast<float>(r0[row * p.ldr + c]) : 0.0f);
+      const float w = p.weight == nullptr ? 1.0f : (p.weight_f32 ? static_cast<const float*>(p.weight)[c] : static_cast<float>(static_cast<const bf16*>(p.weight)[c])) + p.weight_offset;
+      const int b = block0 + c / kScaleBlock;
+      const float first = h * w * block_f[b];
+      if (block_f[b] < INFINITY && !norm_next_to_border(first)) continue;
+      static_cast<uint8_t*>(p.out)[row * p.ldo + c] = uint8_t(e4m3_pair(norm_odd(double(h) * double(w) * (row_inv * double(block_by[b]))), 0.0f));
     }
   }
 }

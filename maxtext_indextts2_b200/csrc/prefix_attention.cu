@@ -5,39 +5,69 @@
 
 namespace {
 
-constexpr int kPrefixWorkers = 2 * 148;  // two CTAs per SM
+constexpr int kPrefixSms = 148;
+constexpr int kPrefixWorkers = 2 * kPrefixSms;  // two CTAs of prefix_units_kernel per SM
+constexpr int kPrefixTcPairs = 256;             // most pairs of an item of prefix_tc_kernel
 
-// the scratch: the entries, a maximum and a sum per slot and pair, weighted values
+// Prefixes go to the tensor cores' kernel when their sequences bring at least 64 pairs on the average.
+bool prefix_on_tc(int rows, int prefixes, int group) { return prefixes > 0 && (long long)rows * group >= 64ll * prefixes; }
+
+// the scratch: the entries, a maximum, a sum and weighted values per place; where prefixes have a kernel of their own, the same for them
 struct PrefixLayout {
-  size_t stat, part, bytes;
+  size_t table[2], stat[2], part[2], bytes;
 
   PrefixLayout(int rows, int sequences, int prefixes, int heads, int kv_heads, int dim) {
-    const size_t group = size_t(heads / kv_heads), entries = size_t(prefixes) + size_t(sequences);
-    // items: every row belongs to one tail and at most one prefix, and each entry has a last block that is not full
-    const size_t items = 2 * (size_t(rows) * group / kPrefixPairs) + entries, slots = items * size_t(kv_heads) + kPrefixWorkers;
-    stat = align_up((entries + 1) * sizeof(PrefixEntry), 256);
-    part = stat + align_up(slots * kPrefixPairs * sizeof(float2), 256);
-    bytes = part + slots * kPrefixPairs * size_t(dim) * sizeof(float);
+    const size_t group = size_t(heads / kv_heads), all = size_t(rows) * group;
+    const bool tc = prefix_on_tc(rows, prefixes, int(group));
+    bytes = 0;
+    for (int k = 0; k < 2; ++k) {  // prefixes, tails
+      // every pair has a place in one tail and at most one prefix, and another in every CTA that shares its item with the CTA before
+      const size_t entries = k == 0 ? size_t(prefixes) : size_t(sequences) + (tc ? 0 : size_t(prefixes));
+      const size_t extra = k == 0 ? size_t(dim == 256 ? 128 : kPrefixTcPairs) * kPrefixSms : size_t(kPrefixPairs) * kPrefixWorkers;
+      const size_t places = k == 0 && !tc ? 0 : all * size_t(kv_heads) * (k == 0 || tc ? 1 : 2) + extra;
+      table[k] = bytes;
+      stat[k] = table[k] + align_up((entries + 1) * sizeof(PrefixEntry), 256);
+      part[k] = stat[k] + align_up(places * sizeof(float2), 256);
+      bytes = part[k] + align_up(places * size_t(dim) * sizeof(float), 256);
+    }
   }
 };
 
 template <int D>
-int launch_prefix(PrefixAttnParams p, cudaStream_t st) {
-  static std::atomic<uint64_t> done{0};
+int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0}, tc_done{0};
   constexpr int KT = PrefixShape<D>::KT;
-  const size_t smem = prefix_smem_bytes<D>();
-  MTX_TRY(allow_smem(prefix_units_kernel<D>, smem, done));
-  p.box = p.tokens_per_page < KT ? p.tokens_per_page : KT;
-  p.workers = kPrefixWorkers;
-  p.tabled = p.prefixes + p.sequences > kPrefixCached;
+  typedef PrefixTcShape<D> Tc;
+  const bool tc = prefix_on_tc(p.rows, p.prefixes, p.group);
+  const PrefixLayout at(p.rows, p.sequences, p.prefixes, p.heads, p.kv_heads, D);
+  const int box = KT < Tc::KT ? KT : Tc::KT;
+  p.box = p.tokens_per_page < box ? p.tokens_per_page : box;
+  PrefixWork w[2];
+  memset(w, 0, sizeof(w));
+  for (int k = 0; k < 2; ++k) {
+    w[k].first = k == 1 && tc ? p.prefixes : 0;
+    w[k].count = k == 0 ? p.prefixes : p.sequences + (tc ? 0 : p.prefixes);
+    w[k].kt = k == 0 ? Tc::KT : KT;
+    w[k].pairs = k == 0 ? Tc::kPairs : kPrefixPairs;
+    w[k].workers = k == 0 ? kPrefixSms : kPrefixWorkers;
+    w[k].tabled = (k == 1 || tc) && w[k].count > kPrefixCached;
+    w[k].table = reinterpret_cast<PrefixEntry*>(scratch + at.table[k]);
+    w[k].stat = reinterpret_cast<float2*>(scratch + at.stat[k]);
+    w[k].part = reinterpret_cast<float*>(scratch + at.part[k]);
+  }
   CUtensorMap tk, tv;
   const uint64_t pool = uint64_t(p.kv_heads) * p.num_pages * p.tokens_per_page;
   MTX_TRY(make_map(&tk, p.k, D, pool, p.box));
   MTX_TRY(make_map(&tv, p.v, D, pool, p.box));
-  if (p.tabled) MTX_TRY(launch(prefix_plan_kernel, dim3(1), dim3(1024), 0, st, p, KT));
-  MTX_TRY(launch(prefix_units_kernel<D>, dim3(p.workers), dim3(kPrefixThreads), smem, st, tk, tv, p));
+  if (w[0].tabled || w[1].tabled) MTX_TRY(launch(prefix_plan_kernel, dim3(1), dim3(1024), 0, st, p, w[0], w[1]));
+  if (tc) {
+    MTX_TRY(allow_smem(prefix_tc_kernel<D>, prefix_tc_smem_bytes<D>(), tc_done));
+    MTX_TRY(launch(prefix_tc_kernel<D>, dim3(w[0].workers), dim3(Tc::kThreads), prefix_tc_smem_bytes<D>(), st, tk, tv, p, w[0]));
+  }
+  MTX_TRY(allow_smem(prefix_units_kernel<D>, prefix_smem_bytes<D>(), done));
+  MTX_TRY(launch(prefix_units_kernel<D>, dim3(w[1].workers), dim3(kPrefixThreads), prefix_smem_bytes<D>(), st, tk, tv, p, w[1]));
   const int threads = p.heads * (D / 4);
-  return launch(prefix_join_kernel<D>, dim3(p.rows), dim3(threads < 512 ? (threads + 31) / 32 * 32 : 512), 0, st, p);
+  return launch(prefix_join_kernel<D>, dim3(p.rows), dim3(threads < 512 ? (threads + 31) / 32 * 32 : 512), 0, st, p, tc ? w[0] : w[1], w[1]);
 }
 
 }  // namespace
@@ -94,13 +124,9 @@ int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, cons
   p.max_pages = max_pages_per_group;
   p.scale = scale;
   p.softcap = softcap;
-  const PrefixLayout at(b->rows, b->sequences, b->prefixes, num_q_heads, num_kv_heads, head_dim);
-  uint8_t* base = static_cast<uint8_t*>(scratch);
-  p.table = reinterpret_cast<PrefixEntry*>(base);
-  p.stat = reinterpret_cast<float2*>(base + at.stat);
-  p.part = reinterpret_cast<float*>(base + at.part);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return head_dim == 64 ? launch_prefix<64>(p, st) : head_dim == 128 ? launch_prefix<128>(p, st) : launch_prefix<256>(p, st);
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  return head_dim == 64 ? launch_prefix<64>(p, at, st) : head_dim == 128 ? launch_prefix<128>(p, at, st) : launch_prefix<256>(p, at, st);
 }
 
 int mtx_prefix_attention_stalls(uint32_t* count) {

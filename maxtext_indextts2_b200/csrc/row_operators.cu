@@ -12,18 +12,29 @@ constexpr int kMostWidth = 32768;  // four times eight values in each of 1024 th
 
 int value_bytes(int type) { return type == MTX_F32 ? 4 : type == MTX_BF16 ? 2 : 1; }
 
-// Threads of a row, each with J times eight of its values: a warp up to 512 values (no barrier, eight rows in a CTA), then as many warps as have eight values for each
-// lane, from 4096 values on twice eight, from 16384 on four times.
-template <class TX, class TR>
-int launch_add_rmsnorm(const AddNormParams& p, cudaStream_t st) {
+// Threads of a row, each with J times eight of its values: a warp up to 512 values (no barrier, eight rows in a CTA), then as many warps as have eight values for each lane, from 4096
+// values on twice eight, from 16384 on four times.
+template <class TX, class TR, bool E4M3, bool VEC>
+int launch_norm_rows(const AddNormParams& p, cudaStream_t st) {
   const int lanes = (p.width + 7) / 8;
   if (lanes <= 64) {
-    const dim3 block(32, kNormWarpRows), grid((p.rows + kNormWarpRows - 1) / kNormWarpRows);
-    return launch(lanes <= 32 ? add_rmsnorm_kernel<TX, TR, 1> : add_rmsnorm_kernel<TX, TR, 2>, grid, block, 0, st, p);
+    const dim3 grid((p.rows + kNormWarpRows - 1) / kNormWarpRows), block(32, kNormWarpRows);
+    return launch(lanes <= 32 ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 1, 256> : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 2, 256>, grid, block, 0, st, p);
   }
   const int each = lanes <= 512 ? 1 : lanes <= 2048 ? 2 : 4, threads = ((lanes + each - 1) / each + 31) / 32 * 32;
-  return launch(each == 1 ? add_rmsnorm_kernel<TX, TR, 1> : each == 2 ? add_rmsnorm_kernel<TX, TR, 2> : add_rmsnorm_kernel<TX, TR, 4>, dim3(p.rows), dim3(threads), 0, st, p);
+  return launch(each == 1 ? (threads <= 256 ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 1, 256> : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 1, 512>)
+                : each == 2 ? (threads <= 512 ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 2, 512> : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 2, 1024>)
+                            : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 4, 1024>, dim3(p.rows), dim3(threads), 0, st, p);
 }
+
+template <class TX, class TR>
+int launch_add_rmsnorm(const AddNormParams& p, bool vec, cudaStream_t st) {
+  if (p.out_type == MTX_E4M3) return vec ? launch_norm_rows<TX, TR, true, true>(p, st) : launch_norm_rows<TX, TR, true, false>(p, st);
+  return vec ? launch_norm_rows<TX, TR, false, true>(p, st) : launch_norm_rows<TX, TR, false, false>(p, st);
+}
+
+// whether rows lie on 16 bytes
+bool rows_on_16(const void* base, long long pitch, int size) { return ((reinterpret_cast<uintptr_t>(base) | uintptr_t(pitch * size)) & 15) == 0; }
 
 template <class TI, class TO>
 int launch_rotary(const RotaryParams& p, bool vec, cudaStream_t st) {
@@ -80,11 +91,14 @@ int mtx_add_rmsnorm(const void* x, int x_type, long long ldx, const void* residu
   p.scale = out_scale;
   p.rows = rows;
   p.width = width;
+  p.by_width = 1.0 / width;
   p.blocks = (width + kScaleBlock - 1) / kScaleBlock;
+  const bool vec = width % 8 == 0 && rows_on_16(x, ldx, value_bytes(x_type)) && (!residual || rows_on_16(residual, ld_residual, value_bytes(residual_type))) &&
+                   (!sum || rows_on_16(sum, ld_sum, value_bytes(residual_type))) && rows_on_16(out, ldo, value_bytes(out_type));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!residual) return x_type == MTX_F32 ? launch_add_rmsnorm<float, NoResidual>(p, st) : launch_add_rmsnorm<bf16, NoResidual>(p, st);
-  if (residual_type == MTX_F32) return x_type == MTX_F32 ? launch_add_rmsnorm<float, float>(p, st) : launch_add_rmsnorm<bf16, float>(p, st);
-  return x_type == MTX_F32 ? launch_add_rmsnorm<float, bf16>(p, st) : launch_add_rmsnorm<bf16, bf16>(p, st);
+  if (!residual) return x_type == MTX_F32 ? launch_add_rmsnorm<float, NoResidual>(p, vec, st) : launch_add_rmsnorm<bf16, NoResidual>(p, vec, st);
+  if (residual_type == MTX_F32) return x_type == MTX_F32 ? launch_add_rmsnorm<float, float>(p, vec, st) : launch_add_rmsnorm<bf16, float>(p, vec, st);
+  return x_type == MTX_F32 ? launch_add_rmsnorm<float, bf16>(p, vec, st) : launch_add_rmsnorm<bf16, bf16>(p, vec, st);
 }
 
 int mtx_rotary_frequencies(int rot_dims, double base, int scaling, double factor, double original_len, double low, double high, double* freq, float* amplitude) {
@@ -160,9 +174,8 @@ int mtx_rotary(const mtx_rotary_batch* b, mtx_stream stream) {
     p.page_map = b->page_map;
   }
   MTX_TRY(on_this_device({p.freq, p.pos, p.q, p.k, p.v, p.q_out, p.k_out, p.k_pages, p.v_pages, p.group, p.page_map}));
-  auto on16 = [](const void* base, long long pitch, int size) { return ((reinterpret_cast<uintptr_t>(base) | uintptr_t(pitch * size)) & 15) == 0; };
-  const bool vec = p.dim % 8 == 0 && p.pairs % 8 == 0 && on16(p.q, p.ldq, in) && on16(p.k, p.ldk, in) && on16(p.v, p.ldv, in) && on16(p.q_out, p.ldq_out, out) &&
-                   on16(p.k_out, p.ldk_out, out) && on16(p.k_pages, 0, 2) && on16(p.v_pages, 0, 2);
+  const bool vec = p.dim % 8 == 0 && p.pairs % 8 == 0 && rows_on_16(p.q, p.ldq, in) && rows_on_16(p.k, p.ldk, in) && rows_on_16(p.v, p.ldv, in) && rows_on_16(p.q_out, p.ldq_out, out) &&
+                   rows_on_16(p.k_out, p.ldk_out, out) && rows_on_16(p.k_pages, 0, 2) && rows_on_16(p.v_pages, 0, 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (b->type == MTX_F32) return b->out_type == MTX_F32 ? launch_rotary<float, float>(p, vec, st) : launch_rotary<float, bf16>(p, vec, st);
   return b->out_type == MTX_F32 ? launch_rotary<bf16, float>(p, vec, st) : launch_rotary<bf16, bf16>(p, vec, st);
