@@ -6,7 +6,7 @@
 namespace {
 
 constexpr int kPrefixSms = 148;
-constexpr int kPrefixWorkers = 2 * kPrefixSms;  // two CTAs of prefix_units_kernel per SM
+constexpr int kPrefixWorkers = 2 * kPrefixSms;  // most CTAs of prefix_units_kernel
 constexpr int kPrefixTcPairs = 256;             // most pairs of an item of prefix_tc_kernel
 
 // Prefixes go to the tensor cores' kernel when their sequences bring at least 64 pairs on the average.
@@ -35,7 +35,7 @@ struct PrefixLayout {
 
 template <int D>
 int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
-  static std::atomic<uint64_t> done{0}, tc_done{0};
+  static std::atomic<uint64_t> done{0}, cap_done{0}, tc_done{0};
   constexpr int KT = PrefixShape<D>::KT;
   typedef PrefixTcShape<D> Tc;
   const bool tc = prefix_on_tc(p.rows, p.prefixes, p.group);
@@ -49,7 +49,7 @@ int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
     w[k].count = k == 0 ? p.prefixes : p.sequences + (tc ? 0 : p.prefixes);
     w[k].kt = k == 0 ? Tc::KT : KT;
     w[k].pairs = k == 0 ? Tc::kPairs : kPrefixPairs;
-    w[k].workers = k == 0 ? kPrefixSms : kPrefixWorkers;
+    w[k].workers = k == 0 ? kPrefixSms : PrefixShape<D>::kCtas * kPrefixSms;
     w[k].tabled = (k == 1 || tc) && w[k].count > kPrefixCached;
     w[k].table = reinterpret_cast<PrefixEntry*>(scratch + at.table[k]);
     w[k].stat = reinterpret_cast<float2*>(scratch + at.stat[k]);
@@ -64,10 +64,11 @@ int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
     MTX_TRY(allow_smem(prefix_tc_kernel<D>, prefix_tc_smem_bytes<D>(), tc_done));
     MTX_TRY(launch(prefix_tc_kernel<D>, dim3(w[0].workers), dim3(Tc::kThreads), prefix_tc_smem_bytes<D>(), st, tk, tv, p, w[0]));
   }
-  MTX_TRY(allow_smem(prefix_units_kernel<D>, prefix_smem_bytes<D>(), done));
-  MTX_TRY(launch(prefix_units_kernel<D>, dim3(w[1].workers), dim3(kPrefixThreads), prefix_smem_bytes<D>(), st, tk, tv, p, w[1]));
-  const int threads = p.heads * (D / 4);
-  return launch(prefix_join_kernel<D>, dim3(p.rows), dim3(threads < 512 ? (threads + 31) / 32 * 32 : 512), 0, st, p, tc ? w[0] : w[1], w[1]);
+  auto units = p.softcap > 0.0f ? prefix_units_kernel<D, true> : prefix_units_kernel<D, false>;
+  MTX_TRY(allow_smem(units, prefix_smem_bytes<D>(), p.softcap > 0.0f ? cap_done : done));
+  MTX_TRY(launch(units, dim3(w[1].workers), dim3(kPrefixThreads), prefix_smem_bytes<D>(), st, tk, tv, p, w[1]));
+  const int threads = p.group * (D / 4) < 256 ? (p.group * (D / 4) + 31) / 32 * 32 : 256;
+  return launch(prefix_join_kernel<D>, dim3(p.rows, p.kv_heads), dim3(threads < 64 ? 64 : threads), 0, st, p, tc ? w[0] : w[1], w[1]);
 }
 
 }  // namespace
@@ -91,6 +92,8 @@ int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, cons
   if ((long long)num_kv_heads * num_pages * tokens_per_page >= 1ll << 31) return fail(MTX_ERR_UNSUPPORTED, "the page pool has too many rows for one tensor map");
   if (b->rows < 0 || b->rows > 1 << 20 || b->sequences < 0 || b->sequences > 1 << 16 || b->prefixes < 0 || b->prefixes > b->sequences) return fail(MTX_ERR_ARG, "bad rows / sequences / prefixes");
   const long long wide = (long long)num_q_heads * head_dim;
+  const double blocks = 2.0 * b->rows * (num_q_heads / num_kv_heads) / kPrefixPairs + b->sequences + b->prefixes, tiles = double(max_pages_per_group) * tokens_per_page * head_dim / 4096 + 1;
+  if (blocks * num_kv_heads * tiles >= double(1ll << 31)) return fail(MTX_ERR_ARG, "rows * tokens is too large for one call");
   if (ldq < wide || ldo < wide) return fail(MTX_ERR_ARG, "bad pitches");
   if (!(scale > 0.0f && scale < INFINITY) || !(softcap >= 0.0f && softcap < INFINITY)) return fail(MTX_ERR_ARG, "scale is positive, softcap not negative");
   if (b->rows == 0 || b->sequences == 0) return MTX_OK;

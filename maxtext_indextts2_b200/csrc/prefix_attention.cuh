@@ -38,46 +38,19 @@ struct PrefixWork {
 };
 
 // What a CTA needs of an entry.  The one behind the last holds the sums.
-struct PrefixEntry {
-  int row, rows;        // the first, and how many
-  int key0, key1;       // its tokens
-  int first_seen;       // tokens that the first row sees (the next row one more, at most key1)
-  int map;              // the page map's row
-  int pairs;            // pairs of one key head in the entries before
-  int prefix;           // a tail's prefix where it begins behind one, else -1
-  long long units;      // units of one key head in the entries before
+struct alignas(16) PrefixEntry {
+  int row, rows;     // the first, and how many
+  int key0, key1;    // its tokens
+  int first_seen;    // tokens that the first row sees (the next row one more, at most key1)
+  int map;           // the page map's row
+  int prefix;        // a tail's prefix where it begins behind one, else -1
+  int first, tiles;  // the first tile's first token: key0 rounded down to where a copy may begin; tiles of an item
+  int pairs, units;  // of one key head in the entries before
+  int unused;
 };
 
 constexpr float kPrefixLog2e = 1.4426950408889634f;
-constexpr int kPrefixPairs = 32;      // pairs of an item: two MMA tiles
-constexpr int kPrefixCached = 128;    // entries that a CTA keeps in shared memory
-constexpr int kPrefixWarps = 4;       // that compute; one more copies
-constexpr int kPrefixThreads = 32 * (kPrefixWarps + 1);
-constexpr int kPrefixPieces = 5;      // K or V tiles in flight, 16 KB each
-constexpr int kPrefixPieceBytes = 16384;
-
-template <int D>
-struct PrefixShape {
-  static constexpr int KT = 8192 / D;               // tokens of a tile
-  static constexpr int CH = D / 64;                 // 64-channel chunks of a row
-  static constexpr int kKeys = KT / kPrefixWarps;   // a warp's tokens of a tile (its part of S)
-  static constexpr int kCols = D / kPrefixWarps;    // a warp's channels (its part of P V)
-  static constexpr int kPRow = KT * 2 + 16;         // bytes of a row of P: 16 more than its values, so that eight rows lie in different banks
-};
-
-struct PrefixTail {
-  PrefixEntry entry[kPrefixCached + 1];
-  uint64_t full[kPrefixPieces], empty[kPrefixPieces];
-  alignas(16) float top[2][kPrefixPairs][kPrefixWarps];
-  alignas(16) float sum[kPrefixPairs][kPrefixWarps];
-  int not_finite[2];
-  int failed;
-};
-
-template <int D>
-constexpr size_t prefix_smem_bytes() {
-  return 1024 + size_t(kPrefixPieces) * kPrefixPieceBytes + kPrefixPairs * D * 2 + kPrefixPairs * PrefixShape<D>::kPRow + sizeof(PrefixTail) + 16;
-}
+constexpr int kPrefixCached = 128;  // entries that a CTA keeps in shared memory
 
 // ---- waits -----------------------------------------------------------------------------------------------------------------------
 // A wait that lasts some two seconds is a protocol error: it gives up, then so does every other wait of the CTA, and the counter (mtx_prefix_attention_stalls) says that results are wrong.
@@ -100,31 +73,29 @@ __device__ __forceinline__ bool prefix_wait(uint64_t* bar, uint32_t parity, vola
 
 // ---- the entries -----------------------------------------------------------------------------------------------------------------
 
-// entry e without its sums; `kt` tokens a tile
-__device__ __forceinline__ PrefixEntry prefix_entry(const PrefixAttnParams& p, int e) {
+// entry e without its sums; bounds, lens: the batch's prefix_seq0 and prefix_len, or copies of them
+__device__ __forceinline__ PrefixEntry prefix_entry(const PrefixAttnParams& p, int kt, int e, const int* bounds, const int* lens) {
   const int most = p.max_pages * p.tokens_per_page;
   auto row_of = [&](int s) { return min(max(p.row0[s], 0), p.rows); };
-  auto seq_of = [&](int i) { return min(max(p.prefix_seq0[i], 0), p.sequences); };
+  auto seq_of = [&](int i) { return min(max(bounds[i], 0), p.sequences); };
   PrefixEntry x;
-  x.pairs = 0;
-  x.units = 0;
+  x.pairs = x.units = x.unused = 0;
   x.prefix = -1;
   if (e < p.prefixes) {
     const int s0 = seq_of(e), s1 = max(seq_of(e + 1), s0);
     x.row = row_of(s0);
     x.rows = s1 > s0 ? max(row_of(s1) - x.row, 0) : 0;
     x.key0 = 0;
-    x.key1 = min(max(p.prefix_len[e], 0), most);
+    x.key1 = min(max(lens[e], 0), most);
     x.first_seen = x.key1;
     x.map = s0 < p.sequences ? s0 : 0;
   } else {
     const int s = e - p.prefixes;
-    x.row = row_of(s);
-    x.rows = max(row_of(s + 1) - x.row, 0);
-    const int length = p.lengths[s];
+    const int r0 = row_of(s), r1 = row_of(s + 1), length = p.lengths[s];
+    x.row = r0;
+    x.rows = max(r1 - r0, 0);
     x.key1 = min(max(length, 0), most);
-    x.first_seen = length - x.rows + 1;  // (lengths and rows are far from 2^31 together: a length below -2^30 counts as none)
-    if (length < 0) x.first_seen = -(1 << 30);
+    x.first_seen = length < 0 ? -(1 << 30) : length - x.rows + 1;
     x.map = s;
     x.key0 = 0;
     // the prefix: the last one that begins at s or in front of it
@@ -135,112 +106,115 @@ __device__ __forceinline__ PrefixEntry prefix_entry(const PrefixAttnParams& p, i
       else hi = mid;
     }
     if (lo > 0 && s < seq_of(lo)) {
-      const int shared = min(max(p.prefix_len[lo - 1], 0), most);
+      const int shared = min(max(lens[lo - 1], 0), most);
       if (shared > 0 && x.first_seen > shared) x.key0 = shared, x.prefix = lo - 1;  // every row lies behind the prefix; otherwise the sequence reads its own pages throughout
     }
   }
-  
+  x.first = x.key0 & ~(p.box - 1);
+  x.tiles = x.rows > 0 && x.key1 > x.key0 ? (x.key1 - x.first + kt - 1) / kt : 0;
   return x;
 }
 
-// a tile begins where a copy may: at key0 rounded down to one
-__device__ __forceinline__ int prefix_first(const PrefixEntry& x, int box) { return x.key0 & ~(box - 1); }
-__device__ __forceinline__ int prefix_tiles(const PrefixEntry& x, int kt, int box) { return x.rows > 0 && x.key1 > x.key0 ? (x.key1 - prefix_first(x, box) + kt - 1) / kt : 0; }
+constexpr int kPrefixKnown = 64;  // prefixes whose bounds and lengths a CTA copies
 
-// All of a work's entries with their sums, by `threads` threads (whole warps, at most 1024) of a CTA; carry: two words of shared memory per warp.
-__device__ __forceinline__ void prefix_build_table(const PrefixAttnParams& p, const PrefixWork& k, PrefixEntry* table, long long* carry, int tid, int threads) {
+struct PrefixBuild {
+  int carry[64];
+  int bounds[kPrefixKnown + 1], lens[kPrefixKnown];
+};
+
+// All of a work's entries with their sums, by `threads` threads (whole warps, at most 1024) of a CTA.
+__device__ __forceinline__ void prefix_build_table(const PrefixAttnParams& p, const PrefixWork& k, PrefixEntry* table, PrefixBuild* build, int tid, int threads) {
   const int lane = tid & 31, warp = tid >> 5, total = k.count;
-  long long units = 0;
-  int pairs = 0;
+  const int *bounds = p.prefix_seq0, *lens = p.prefix_len;
+  if (p.prefixes <= kPrefixKnown) {
+    for (int i = tid; i <= p.prefixes && p.prefixes > 0; i += threads) {
+      build->bounds[i] = bounds[i];
+      if (i < p.prefixes) build->lens[i] = lens[i];
+    }
+    bounds = build->bounds;
+    lens = build->lens;
+    __syncthreads();
+  }
+  int units = 0, pairs = 0;
   for (int e0 = 0; e0 <= total; e0 += threads) {
     const int e = e0 + tid;
     PrefixEntry x;
-    long long u = 0;
-    int b = 0;
+    int u = 0, b = 0;
     if (e < total) {
-      x = prefix_entry(p, k.first + e);
-      const int tiles = prefix_tiles(x, k.kt, p.box);
-      b = tiles > 0 ? x.rows * p.group : 0;
-      u = (long long)tiles * ((b + k.pairs - 1) / k.pairs);
+      x = prefix_entry(p, k.kt, k.first + e, bounds, lens);
+      b = x.tiles > 0 ? x.rows * p.group : 0;
+      u = x.tiles * ((b + k.pairs - 1) / k.pairs);
     } else {
-      x.row = x.rows = x.key0 = x.key1 = x.first_seen = x.map = 0;
+      memset(&x, 0, sizeof(x));
       x.prefix = -1;
     }
-    long long us = u;
-    int bs = b;
+    int us = u, bs = b;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long t = __shfl_up_sync(0xffffffffu, us, o);
-      const int w = __shfl_up_sync(0xffffffffu, bs, o);
+      const int t = __shfl_up_sync(0xffffffffu, us, o), w = __shfl_up_sync(0xffffffffu, bs, o);
       if (lane >= o) us += t, bs += w;
     }
     __syncthreads();
-    if (lane == 31) carry[2 * warp] = us, carry[2 * warp + 1] = bs;
+    if (lane == 31) build->carry[2 * warp] = us, build->carry[2 * warp + 1] = bs;
     __syncthreads();
-    long long before = units, sum_u = 0;
-    int before_b = pairs, sum_b = 0;
+    int before = units, before_b = pairs;
     for (int w = 0; w < threads / 32; ++w) {
-      if (w < warp) before += carry[2 * w], before_b += int(carry[2 * w + 1]);
-      sum_u += carry[2 * w], sum_b += int(carry[2 * w + 1]);
+      const int cu = build->carry[2 * w], cb = build->carry[2 * w + 1];
+      if (w < warp) before += cu, before_b += cb;
+      units += cu, pairs += cb;
     }
     if (e <= total) {
       x.units = before + us - u;
       x.pairs = before_b + bs - b;
       table[e] = x;
     }
-    units += sum_u;
-    pairs += sum_b;
   }
   __syncthreads();
 }
 
 // for batches of more entries than a CTA keeps: one CTA in front of the others
 __global__ void __launch_bounds__(1024) prefix_plan_kernel(const PrefixAttnParams p, const PrefixWork a, const PrefixWork b) {
-  __shared__ long long carry[64];
+  __shared__ PrefixBuild build;
   griddep_wait();
   griddep_launch_dependents();
-  if (a.tabled) prefix_build_table(p, a, a.table, carry, threadIdx.x, 1024);
-  if (b.tabled) prefix_build_table(p, b, b.table, carry, threadIdx.x, 1024);
+  if (a.tabled) prefix_build_table(p, a, a.table, &build, threadIdx.x, 1024);
+  if (b.tabled) prefix_build_table(p, b, b.table, &build, threadIdx.x, 1024);
 }
 
-// A CTA's run of units: worker c of W has those from begin(c) on.
+// A CTA's run of units: worker c has those from begin(c) on, the first workers one more than the others.  (All numbers of units stay below 2^31: the call's sizes say so.)
 struct PrefixShare {
-  long long units;  // of all key heads
-  int workers;
+  int workers, each, more;
 
-  __device__ __forceinline__ PrefixShare(long long u, int most) : units(u), workers(u < most ? int(u) : most) {}
-  __device__ __forceinline__ long long begin(int c) const { return units / workers * c + units % workers * c / workers; }
-  __device__ __forceinline__ int of(long long u) const {  // the worker that has unit u
-    int c = int(double(u) * workers / double(units));
-    c = min(max(c, 0), workers - 1);
-    while (c > 0 && begin(c) > u) --c;
-    while (c + 1 < workers && begin(c + 1) <= u) ++c;
-    return c;
+  __device__ __forceinline__ PrefixShare(int units, int most) {
+    workers = min(units, most);
+    each = workers > 0 ? units / workers : 0;
+    more = units - each * workers;
+  }
+  __device__ __forceinline__ int begin(int c) const { return each * c + min(c, more); }
+  __device__ __forceinline__ int of(int u) const {  // the worker that has unit u
+    const int longer = more * (each + 1);
+    return u < longer ? u / (each + 1) : more + (u - longer) / each;
   }
 };
 
 // One item of a CTA's run: its tiles [tile0, tile1).
 struct PrefixSegment {
   PrefixEntry x;
-  int e, kvh, block, tiles, tile0, tile1;
-  int first;        // the first tile's first token
+  int e, kvh, block, tile0, tile1;
   long long place;  // of its first pair's results
 };
 
 // Goes through a CTA's run item by item; all threads of a warp alike.
 struct PrefixWalk {
   const PrefixEntry* table;
-  int total, kt, box, most, worker;
-  long long per_head, at, end;
-  int e, kvh;
+  int total, most, worker, per_head, at, end, e, kvh;
 
-  __device__ __forceinline__ PrefixWalk(const PrefixAttnParams& p, const PrefixWork& k, const PrefixEntry* t, const PrefixShare& share, int c)
-      : table(t), total(k.count), kt(k.kt), box(p.box), most(k.pairs), worker(c) {
+  __device__ __forceinline__ PrefixWalk(const PrefixWork& k, const PrefixEntry* t, const PrefixShare& share, int c) : table(t), total(k.count), most(k.pairs), worker(c) {
     per_head = t[total].units;
     at = share.begin(c);
     end = share.begin(c + 1);
-    kvh = int(at / per_head);
-    const long long rest = at - kvh * per_head;
+    kvh = at / per_head;
+    const int rest = at - kvh * per_head;
     int lo = 0, hi = total;  // the last entry whose units begin at `rest` or before (entries without units are in front of it)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -251,54 +225,102 @@ struct PrefixWalk {
   }
   __device__ __forceinline__ bool next(PrefixSegment& s) {
     if (at >= end) return false;
-    long long rest = at - kvh * per_head;
+    int rest = at - kvh * per_head;
     if (rest >= per_head) ++kvh, rest = 0, e = 0;
     while (table[e + 1].units <= rest) ++e;
     s.x = table[e];
     s.e = e;
     s.kvh = kvh;
-    s.tiles = prefix_tiles(s.x, kt, box);
-    s.first = prefix_first(s.x, box);
-    const long long in = rest - s.x.units;
-    s.block = int(in / s.tiles);
-    s.tile0 = int(in - (long long)s.block * s.tiles);
-    s.tile1 = int(min((long long)s.tiles, s.tile0 + (end - at)));
+    const int in = rest - s.x.units;
+    s.block = in / s.x.tiles;
+    s.tile0 = in - s.block * s.x.tiles;
+    s.tile1 = min(s.x.tiles, s.tile0 + (end - at));
     s.place = (long long)kvh * table[total].pairs + s.x.pairs + (long long)(s.block + worker) * most;  // (every step to the next one goes to another item, another CTA or both)
     at += s.tile1 - s.tile0;
     return true;
   }
 };
 
-__device__ __forceinline__ bool prefix_whole(const PrefixSegment& s) { return s.x.key0 == 0 && s.tile0 == 0 && s.tile1 == s.tiles; }
+__device__ __forceinline__ bool prefix_whole(const PrefixSegment& s) { return s.x.key0 == 0 && s.tile0 == 0 && s.tile1 == s.x.tiles; }
 
 // ---- units on the warps' MMAs ------------------------------------------------------------------------------------------------------
+//
+// Tails, and prefixes whose sequences bring few pairs.  Warp 4 copies K and V tiles of 8 KB each.  Warps 0 to 3 compute, each a tile of its own for 16 of the item's pairs, with S, P and O
+// in its registers: an item of up to 16 pairs has every fourth tile in a warp, one of up to 32 every second, one of up to 64 all.  Where several warps have parts of the
+// same pairs, they are joined in shared memory at the item's end.
+// Bound: the tails' bytes, each read once.
+
+constexpr int kPrefixPairs = 64;    // pairs of an item: four MMA tiles
+constexpr int kPrefixWarps = 4;     // that compute; one more copies
+constexpr int kPrefixThreads = 32 * (kPrefixWarps + 1);
+constexpr int kPrefixPieceBytes = 8192;
+
+template <int D>
+struct PrefixShape {
+  static constexpr int KT = kPrefixPieceBytes / 2 / D;  // tokens of a tile
+  static constexpr int CH = D / 64;                     // 64-channel chunks of a row
+  static constexpr int kCtas = D == 256 ? 1 : 2;        // per SM (registers: Q and O of 16 pairs are 3/8 D per thread)
+  static constexpr int kPieces = D == 64 ? 12 : D == 128 ? 10 : 16;
+};
+
+struct PrefixTail {
+  PrefixEntry entry[kPrefixCached + 1];
+  uint64_t full[16], empty[16];
+  int armed[16];  // the tile that a piece is for
+  PrefixBuild build;
+  float2 stat[2][16];
+  int failed;
+};
+
+template <int D>
+constexpr size_t prefix_smem_bytes() {
+  return 1024 + size_t(PrefixShape<D>::kPieces) * kPrefixPieceBytes + 2 * 16 * (D + 4) * 4 + sizeof(PrefixTail) + 16;
+}
 
 __device__ __forceinline__ void prefix_bar() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kPrefixWarps) : "memory"); }
+// Waits for a piece of tile n.  A warp does not see every tile of a piece, and copies end in any order: by its parity alone a barrier that still waits for the tile before (another warp's)
+// looks as if tile n were there.  So the copying warp says which tile a piece is for, once the one before is used up.
+__device__ __forceinline__ void prefix_wait_tile(volatile int* armed, int n, uint64_t* full, uint32_t phase, volatile int* failed) {
+  if (*armed != n) {
+    const long long t0 = clock64();
+    while (*armed != n && *failed == 0)
+      if (clock64() - t0 > 4000000000LL) {
+        atomicAdd(&d_prefix_waits_failed, 1u);
+        *failed = 1;
+      }
+  }
+  prefix_wait(full, phase, failed);
+}
+// `count` of a barrier's four arrivals
+__device__ __forceinline__ void prefix_arrive(uint64_t* bar, int count) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory"); }
 
-// Warp 4 copies K and V tiles, warps 0 to 3 compute: of every tile each has a quarter of the tokens for S = Q K^T and a quarter of the channels for P V, so that no accumulators
-// have to be joined; maxima and P pass through shared memory, two barriers a tile.
-template <int D>
-__global__ void __launch_bounds__(kPrefixThreads, 2)
+__device__ __forceinline__ float prefix_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(kPrefixThreads, PrefixShape<D>::kCtas)
 prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PrefixAttnParams p, const PrefixWork k) {
   typedef PrefixShape<D> F;
-  constexpr int KT = F::KT, CH = F::CH, NS = F::kKeys / 8, NO = F::kCols / 8, MT = kPrefixPairs / 16;
+  constexpr int KT = F::KT, CH = F::CH, NS = KT / 8, NO = D / 8, P = F::kPieces;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // piece: [CH][KT tokens][128 B], swizzled
-  uint8_t* sq = ring + kPrefixPieces * kPrefixPieceBytes;                        // [CH][pairs][128 B], swizzled alike
-  uint8_t* sp = sq + kPrefixPairs * D * 2;                                       // [pairs][kPRow]
-  PrefixTail* tail = reinterpret_cast<PrefixTail*>(sp + kPrefixPairs * F::kPRow);
+  float* joint = reinterpret_cast<float*>(ring + P * kPrefixPieceBytes);         // [2][16 pairs][D + 4]
+  PrefixTail* tail = reinterpret_cast<PrefixTail*>(joint + 2 * 16 * (D + 4));
   volatile int* failed = &tail->failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
-    for (int i = 0; i < kPrefixPieces; ++i) {
+    for (int i = 0; i < P; ++i) {
       mbar_init(&tail->full[i], 1);
       mbar_init(&tail->empty[i], kPrefixWarps);
+      tail->armed[i] = -1;
     }
     tail->failed = 0;
-    tail->not_finite[0] = tail->not_finite[1] = 0;
     fence_barrier_init();
   }
   // (behind the prefixes' kernel: that one has waited for what is in front of it, and the join waits for this one, which waits for that one before it ends)
@@ -306,7 +328,7 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   griddep_launch_dependents();
   const PrefixEntry* table = k.table;
   if (!k.tabled) {
-    prefix_build_table(p, k, tail->entry, reinterpret_cast<long long*>(sp), threadIdx.x, kPrefixThreads);
+    prefix_build_table(p, k, tail->entry, &tail->build, threadIdx.x, kPrefixThreads);
     table = tail->entry;
     if (blockIdx.x == 0)  // for the join
       for (int e = threadIdx.x; e <= k.count; e += kPrefixThreads) k.table[e] = table[e];
@@ -318,39 +340,47 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     griddep_wait();
     return;
   }
-  PrefixWalk walk(p, k, table, share, blockIdx.x);
+  PrefixWalk walk(k, table, share, blockIdx.x);
   PrefixSegment s;
 
   if (warp == kPrefixWarps) {
     const bool issuer = elect_one();
     const int boxes = KT / p.box, tpp = p.tokens_per_page;
-    int piece = 0;
+    int piece = 0, tile = 0;  // (of all that the CTA goes through)
     uint32_t phase = 1;
     bool good = true;
     while (walk.next(s)) {
       const int* pages = p.page_map + (long long)s.x.map * p.max_pages;
-      const long long head_row = (long long)s.kvh * p.num_pages * tpp;
-      // lane i: the pool's row where box i of the tile begins; boxes behind the last token: that token's page
+      const int head_row = s.kvh * p.num_pages * tpp;
+      // lane i: the pool's row where box i of the item's tiles begins, counted from `tile`; boxes behind the last token: that token's page
       auto row_of = [&](int tile) {
-        const int key = min(s.first + tile * KT + (lane < boxes ? lane : 0) * p.box, s.x.key1 - 1);
+        const int key = min(s.x.first + tile * KT + lane * p.box, s.x.key1 - 1);
         const int page = pages[key / tpp];
-        return int(head_row + (long long)(page >= 0 && page < p.num_pages ? page : 0) * tpp + key % tpp / p.box * p.box);
+        return head_row + (page >= 0 && page < p.num_pages ? page : 0) * tpp + key % tpp / p.box * p.box;
       };
-      int row = row_of(s.tile0);
-      for (int t = s.tile0; t < s.tile1; ++t) {
-        const int next = t + 1 < s.tile1 ? row_of(t + 1) : 0;
+      // the 32 lanes look up as many boxes at a time, one round ahead
+      const int per = 32 / boxes;  // tiles of a round
+      int row = row_of(s.tile0), ahead = s.tile0 + per < s.tile1 ? row_of(s.tile0 + per) : 0;
+      for (int t = s.tile0, i = 0; t < s.tile1; ++t, ++tile) {
         for (int kv = 0; kv < 2; ++kv) {
           good = good && prefix_wait(&tail->empty[piece], phase, failed);
           uint8_t* to = ring + piece * kPrefixPieceBytes;
-          if (issuer && good) mbar_expect_tx(&tail->full[piece], kPrefixPieceBytes);
+          if (issuer && good) {
+            mbar_expect_tx(&tail->full[piece], kPrefixPieceBytes);
+            *const_cast<volatile int*>(&tail->armed[piece]) = tile;
+          }
           for (int b = 0; b < boxes; ++b) {
-            const int from = __shfl_sync(0xffffffffu, row, b);
+            const int from = __shfl_sync(0xffffffffu, row, i * boxes + b);
             if (issuer && good)
               for (int c = 0; c < CH; ++c) tma_load_2d(to + c * KT * 128 + b * p.box * 128, kv == 0 ? &tm_k : &tm_v, c * 64, from, &tail->full[piece], kEvictNormal);
           }
-          if (++piece == kPrefixPieces) piece = 0, phase ^= 1;
+          if (++piece == P) piece = 0, phase ^= 1;
         }
-        row = next;
+        if (++i == per) {
+          i = 0;
+          row = ahead;
+          ahead = t + 1 + per < s.tile1 ? row_of(t + 1 + per) : 0;
+        }
       }
     }
     if (!good) {  // copies in flight have a millisecond to end
@@ -361,247 +391,265 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     return;
   }
 
-  const float mul = p.softcap > 0.0f ? p.scale / p.softcap : p.scale * kPrefixLog2e, cap = p.softcap * kPrefixLog2e;
-  const int r = lane >> 2;  // this lane's pairs of an MMA tile: r and r + 8
-  const uint32_t sq_addr = smem_u32(sq), sp_addr = smem_u32(sp), ring_addr = smem_u32(ring);
-  int piece = 0;
-  uint32_t phase = 0;
-  int turn = 0;  // which buffer of maxima
-  while (walk.next(s)) {
-    const int pair0 = s.block * kPrefixPairs, pairs = min(kPrefixPairs, s.x.rows * p.group - pair0), mts = (pairs + 15) / 16;
-    prefix_bar();  // (the item before has left Q and the sums)
-    for (int i = threadIdx.x; i < mts * 16 * (D / 8); i += 32 * kPrefixWarps) {
-      const int pair = i / (D / 8), c = i - pair * (D / 8), at = pair0 + pair;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (pair < pairs) v = *reinterpret_cast<const uint4*>(p.q + (s.x.row + at / p.group) * p.ldq + (s.kvh * p.group + at % p.group) * D + c * 8);
-      *reinterpret_cast<uint4*>(sq + (c >> 3) * kPrefixPairs * 128 + pair * 128 + (((c & 7) ^ (pair & 7)) << 4)) = v;
+  const float mul = CAP ? p.scale / p.softcap : p.scale * kPrefixLog2e, cap = p.softcap * kPrefixLog2e;
+  const int r = lane >> 2, q2 = (lane & 3) * 2;  // this lane's pairs of an MMA tile: r and r + 8; its columns
+  const uint32_t ring_addr = smem_u32(ring);
+  int piece0 = 0, tile0 = 0;  // the item's first tile: its piece, its number
+  uint32_t phase0 = 0;
+  uint32_t q[D / 16][4];
+  int wm, mt;  // MMA tiles of the item, this warp's
+  auto load_q = [&]() {
+    const int left = s.x.rows * p.group - s.block * kPrefixPairs;
+    wm = left > 32 ? 4 : left > 16 ? 2 : 1;
+    mt = warp & (wm - 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int pair = mt * 16 + r + 8 * h, at = s.block * kPrefixPairs + pair;
+      const bf16* from = p.q + (s.x.row + at / p.group) * p.ldq + (s.kvh * p.group + at % p.group) * D + q2;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        q[kk][h] = pair < left ? *reinterpret_cast<const uint32_t*>(from + kk * 16) : 0u;
+        q[kk][2 + h] = pair < left ? *reinterpret_cast<const uint32_t*>(from + kk * 16 + 8) : 0u;
+      }
     }
-    int seen[MT][2];
+  };
+  bool more = walk.next(s);
+  if (more) load_q();
+  while (more) {
+    const int pair0 = s.block * kPrefixPairs + mt * 16, left = s.x.rows * p.group - pair0;  // (pairs from this warp's first on)
+    const int groups = kPrefixWarps / wm;  // of warps, with a tile each; a barrier has as many arrivals of each of a tile's warps
+    const bool prefix = k.first + s.e < p.prefixes;
+    int seen[2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int h = 0; h < 2; ++h) seen[h] = prefix ? s.x.key1 : min(s.x.first_seen + (pair0 + r + 8 * h) / p.group, s.x.key1);
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[NO][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) seen[mt][h] = k.first + s.e < p.prefixes ? s.x.key1 : min(s.x.first_seen + (pair0 + mt * 16 + r + 8 * h) / p.group, s.x.key1);
-    float m[MT][2], l[MT][2], o[MT][NO][4];
+    for (int n = 0; n < NO; ++n)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) m[mt][h] = -INFINITY, l[mt][h] = 0.0f;
-#pragma unroll
-      for (int n = 0; n < NO; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[mt][n][i] = 0.0f;
-    }
-    prefix_bar();
-    for (int t = s.tile0; t < s.tile1; ++t) {
-      const int key = s.first + t * KT;  // the tile's first token
+      for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+    const int mine = warp / wm;  // of the groups
+    int piece = piece0 + 2 * mine;
+    uint32_t phase = phase0;
+    if (piece >= P) piece -= P, phase ^= 1;
+    for (int t = s.tile0 + mine, number = tile0 + mine; t < s.tile1; t += groups, number += groups) {
+      const int key = s.x.first + t * KT;  // the tile's first token
       const bool masked = key < s.x.key0 || key + KT > min(s.x.first_seen, s.x.key1);
-      // S of this warp's tokens
-      prefix_wait(&tail->full[piece], phase, failed);
-      float x[MT][NS][4];
+      int v_piece = piece + 1;
+      uint32_t v_phase = phase;
+      if (v_piece == P) v_piece = 0, v_phase ^= 1;
+      float x[NS][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = 0.0f;
+      prefix_wait_tile(&tail->armed[piece], number, &tail->full[piece], phase, failed);
+      {
+        // ldmatrix: lanes 0-7 and 8-15 the two halves of 16 channels of eight tokens, lanes 16-31 of the next eight
+        const int token = (lane & 7) + (lane >> 4) * 8;
+        const uint32_t k_addr = ring_addr + piece * kPrefixPieceBytes + token * 128;
+        const int half = lane >> 3 & 1, turn = lane & 7;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+          for (int n = 0; n < NS; n += 2) {
+            uint32_t b[4];
+            ldmatrix_x4(k_addr + kk / 4 * KT * 128 + n * 1024 + (((kk % 4 * 2 + half) ^ turn) << 4), b[0], b[1], b[2], b[3]);
+            mma_m16n8k16_bf16(x[n], q[kk], b[0], b[1]);
+            mma_m16n8k16_bf16(x[n + 1], q[kk], b[2], b[3]);
+          }
+      }
+      __syncwarp();
+      if (lane == 0) prefix_arrive(&tail->empty[piece], groups);
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[n][i] *= mul;
+          if (CAP) x[n][i] = cap * tanhf(x[n][i]);
+        }
+      if (masked) {
 #pragma unroll
         for (int n = 0; n < NS; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[mt][n][i] = 0.0f;
-      const uint32_t k_addr = ring_addr + piece * kPrefixPieceBytes;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t a[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-          if (mt < mts) {
-            const int pair = mt * 16 + (lane & 15), c = kk % 4 * 2 + (lane >> 4);
-            ldmatrix_x4(sq_addr + kk / 4 * kPrefixPairs * 128 + pair * 128 + ((c ^ (pair & 7)) << 4), a[mt][0], a[mt][1], a[mt][2], a[mt][3]);
+          for (int i = 0; i < 4; ++i) {
+            const int j = key + n * 8 + q2 + (i & 1);
+            if (j < s.x.key0 || j >= seen[i >> 1]) x[n][i] = -INFINITY;
           }
+      }
 #pragma unroll
-        for (int n = 0; n < NS; n += 2) {
-          uint32_t b[4];
-          if (NS == 1) {  // eight tokens: the two halves of 16 channels
-            const int token = warp * F::kKeys + (lane & 7), c = kk % 4 * 2 + (lane >> 3 & 1);
-            asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(b[0]), "=r"(b[1]) : "r"(k_addr + kk / 4 * KT * 128 + token * 128 + ((c ^ (token & 7)) << 4)) : "memory");
-            b[2] = b[3] = 0;
-          } else {
-            const int token = warp * F::kKeys + n * 8 + (lane & 7) + (lane >> 4) * 8, c = kk % 4 * 2 + (lane >> 3 & 1);
-            ldmatrix_x4(k_addr + kk / 4 * KT * 128 + token * 128 + ((c ^ (token & 7)) << 4), b[0], b[1], b[2], b[3]);
-          }
+      for (int n = 0; n < NS; ++n)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-            if (mt < mts) {
-              mma_m16n8k16_bf16(x[mt][n], a[mt], b[0], b[1]);
-              if (NS > 1) mma_m16n8k16_bf16(x[mt][n + (NS > 1)], a[mt], b[2], b[3]);
-            }
+        for (int i = 0; i < 4; ++i) top[i >> 1] = fmaxf(top[i >> 1], x[n][i]);
+      float base[2];
+      bool grown = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+        top[h] = fmaxf(top[h], m[h]);
+        grown = grown || top[h] > m[h];
+        base[h] = top[h] == -INFINITY ? 0.0f : top[h];
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float fix = prefix_ex2(m[h] - base[h]);
+          m[h] = top[h];
+          l[h] *= fix;
+#pragma unroll
+          for (int n = 0; n < NO; ++n) o[n][2 * h] *= fix, o[n][2 * h + 1] *= fix;
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tail->empty[piece]);
-      if (++piece == kPrefixPieces) piece = 0, phase ^= 1;
+      uint32_t a[KT / 16][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        if (mt < mts) {
-          float top[2] = {-INFINITY, -INFINITY};
+      for (int n = 0; n < NS; ++n)
 #pragma unroll
-          for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float& v = x[mt][n][i];
-              v *= mul;
-              if (p.softcap > 0.0f) v = cap * tanhf(v);
-              if (masked) {
-                const int j = key + warp * F::kKeys + n * 8 + (lane & 3) * 2 + (i & 1);
-                if (j < s.x.key0 || j >= seen[mt][i >> 1]) v = -INFINITY;
-              }
-              top[i >> 1] = fmaxf(top[i >> 1], v);
-            }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-            if ((lane & 3) == 0) tail->top[turn][mt * 16 + r + 8 * h][warp] = top[h];
-          }
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w = pack_bf16x2(prefix_ex2(x[n][2 * h] - base[h]), prefix_ex2(x[n][2 * h + 1] - base[h]));
+          l[h] += bf16_lo(w) + bf16_hi(w);  // (of the rounded weights: where one key has nearly all, its rounding cancels)
+          a[n / 2][n % 2 * 2 + h] = w;
         }
-      // V: tokens outside the entry's count 0 whatever they hold.  So do numbers that are none, in tokens that some rows see and others do not (0 times them is none either); the rows that see them
-      // add them behind the products
-      prefix_wait(&tail->full[piece], phase, failed);
-      uint8_t* v = ring + piece * kPrefixPieceBytes;
-      const int some = max(s.x.first_seen - key, 0), hi = s.x.key1 - key;  // of the tile, tokens that not all rows see
+      prefix_wait_tile(&tail->armed[v_piece], number, &tail->full[v_piece], v_phase, failed);
+      bool odd = false;
+      int some = 0, hi = 0;
       if (masked) {
+        // V: tokens outside the entry's count 0 whatever they hold.  So do numbers that are none, in tokens that some rows see and others do not (0 times them is none either); the rows
+        // that see them add them behind the products
+        uint8_t* v = ring + v_piece * kPrefixPieceBytes;
         const int lo = s.x.key0 - key;
-        bool odd = false;
-        for (int i = threadIdx.x; i < KT * (D / 8); i += 32 * kPrefixWarps) {
+        some = max(s.x.first_seen - key, 0), hi = min(s.x.key1 - key, KT);
+        uint32_t gone = 0;
+        for (int i = lane; i < KT * (D / 8); i += 32) {
           const int token = i / (D / 8), c = i - token * (D / 8);
-          uint4* at = reinterpret_cast<uint4*>(v + (c >> 3) * KT * 128 + token * 128 + ((c & 7) << 4));  // (any order of a row's pieces)
+          if (token < some || token >= hi) continue;
+          const uint4 u = *reinterpret_cast<const uint4*>(v + (c >> 3) * KT * 128 + token * 128 + ((c & 7) << 4));  // (any order of a row's pieces)
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int b = 0; b < 4; ++b) gone |= (w[b] & 0x7f80u) == 0x7f80u || (w[b] & 0x7f800000u) == 0x7f800000u;
+        }
+        odd = __any_sync(0xffffffffu, gone != 0);
+        if (wm > 1) asm volatile("bar.sync %0, %1;" ::"r"(2 + mine), "r"(32 * wm) : "memory");  // (the tile's other warps have looked too)
+        for (int i = lane; i < KT * (D / 8); i += 32) {
+          const int token = i / (D / 8), c = i - token * (D / 8);
+          uint4* at = reinterpret_cast<uint4*>(v + (c >> 3) * KT * 128 + token * 128 + ((c & 7) << 4));
           if (token < lo || token >= hi) {
             *at = make_uint4(0, 0, 0, 0);
-          } else if (token >= some) {
-            const uint4 u = *at;
-            uint32_t w[4] = {u.x, u.y, u.z, u.w}, gone = 0;
+          } else if (odd && token >= some) {
+            uint4 u = *at;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              const uint32_t none = ((w[b] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w[b] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
-              w[b] &= ~none;
-              gone |= none;
-            }
-            if (gone != 0) {
-              *at = make_uint4(w[0], w[1], w[2], w[3]);
-              odd = true;
-            }
+            for (int b = 0; b < 4; ++b) w[b] &= ~(((w[b] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w[b] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u));
+            *at = u;
           }
         }
-        if (odd) tail->not_finite[turn] = 1;
+        __syncwarp();
       }
-      prefix_bar();
-      const bool odd_tile = masked && *reinterpret_cast<volatile int*>(&tail->not_finite[turn]) != 0;
-      if (threadIdx.x == 0) tail->not_finite[turn ^ 1] = 0;
+      {
+        const uint32_t v_addr = ring_addr + v_piece * kPrefixPieceBytes + (lane & 15) * 128;
+        const int half = lane >> 4, turn = lane & 7;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        if (mt < mts) {
-          float base[2], fix[2];
+        for (int kk = 0; kk < KT / 16; ++kk)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 u = *reinterpret_cast<const float4*>(tail->top[turn][mt * 16 + r + 8 * h]);
-            const float now = fmaxf(m[mt][h], fmaxf(fmaxf(u.x, u.y), fmaxf(u.z, u.w)));
-            base[h] = now == -INFINITY ? 0.0f : now;
-            fix[h] = exp2f(m[mt][h] - base[h]);
-            m[mt][h] = now;
-            l[mt][h] *= fix[h];
+          for (int n = 0; n < NO; n += 2) {
+            uint32_t b[4];
+            ldmatrix_x4_trans(v_addr + n / 8 * KT * 128 + kk * 2048 + (((n % 8 + half) ^ turn) << 4), b[0], b[1], b[2], b[3]);
+            mma_m16n8k16_bf16(o[n], a[kk], b[0], b[1]);
+            mma_m16n8k16_bf16(o[n + 1], a[kk], b[2], b[3]);
           }
-#pragma unroll
-          for (int n = 0; n < NS; ++n) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float p0 = exp2f(x[mt][n][2 * h] - base[h]), p1 = exp2f(x[mt][n][2 * h + 1] - base[h]);
-              l[mt][h] += p0 + p1;
-              *reinterpret_cast<uint32_t*>(sp + (mt * 16 + r + 8 * h) * F::kPRow + (warp * F::kKeys + n * 8 + (lane & 3) * 2) * 2) = pack_bf16x2(p0, p1);
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NO; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[mt][n][i] *= fix[i >> 1];
-        }
-      prefix_bar();
-      // P V: this warp's channels
-      const uint32_t v_addr = ring_addr + piece * kPrefixPieceBytes;
-#pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk) {
-        uint32_t a[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-          if (mt < mts) ldmatrix_x4(sp_addr + (mt * 16 + (lane & 15)) * F::kPRow + kk * 32 + (lane >> 4) * 16, a[mt][0], a[mt][1], a[mt][2], a[mt][3]);
-#pragma unroll
-        for (int n = 0; n < NO; n += 2) {
-          const int token = kk * 16 + (lane & 15), c = warp * (F::kCols / 8) + n + (lane >> 4);
-          uint32_t b[4];
-          ldmatrix_x4_trans(v_addr + (c >> 3) * KT * 128 + token * 128 + (((c & 7) ^ (token & 7)) << 4), b[0], b[1], b[2], b[3]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-            if (mt < mts) {
-              mma_m16n8k16_bf16(o[mt][n], a[mt], b[0], b[1]);
-              mma_m16n8k16_bf16(o[mt][n + 1], a[mt], b[2], b[3]);
-            }
-        }
       }
-      if (odd_tile) {  // the sum is none either, whatever the token's weight
+      if (masked) {
+        if (odd) {  // the sum is none either, whatever the token's weight
 #pragma unroll 1
-        for (int i = some; i < min(hi, KT); ++i) {
-          const int page = p.page_map[(long long)s.x.map * p.max_pages + (key + i) / p.tokens_per_page];
-          const bf16* y = p.v + (((long long)s.kvh * p.num_pages + (page >= 0 && page < p.num_pages ? page : 0)) * p.tokens_per_page + (key + i) % p.tokens_per_page) * D +
-                          warp * F::kCols + (lane & 3) * 2;
+          for (int i = some; i < hi; ++i) {
+            const int page = p.page_map[(long long)s.x.map * p.max_pages + (key + i) / p.tokens_per_page];
+            const bf16* y = p.v + (((long long)s.kvh * p.num_pages + (page >= 0 && page < p.num_pages ? page : 0)) * p.tokens_per_page + (key + i) % p.tokens_per_page) * D + q2;
 #pragma unroll
-          for (int n = 0; n < NO; ++n)
+            for (int n = 0; n < NO; ++n)
 #pragma unroll
-            for (int f = 0; f < 2; ++f) {
-              const float value = __bfloat162float(y[n * 8 + f]);
-              if (!(fabsf(value) < INFINITY))
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+              for (int f = 0; f < 2; ++f) {
+                const float value = __bfloat162float(y[n * 8 + f]);
+                if (!(fabsf(value) < INFINITY)) {
 #pragma unroll
                   for (int h = 0; h < 2; ++h)
-                    if (key + i < seen[mt][h]) o[mt][n][2 * h + f] += value;
-            }
+                    if (key + i < seen[h]) o[n][2 * h + f] += value;
+                }
+              }
+          }
         }
+        fence_proxy_async();  // (zeros in a piece that the next copy overwrites)
       }
-      if (masked) fence_proxy_async();  // (zeros in a piece that the next copy overwrites)
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tail->empty[piece]);
-      if (++piece == kPrefixPieces) piece = 0, phase ^= 1;
-      turn ^= 1;
+      if (lane == 0) prefix_arrive(&tail->empty[v_piece], groups);
+      piece += 2 * groups;
+      if (piece >= P) piece -= P, phase ^= 1;
     }
-    // the item's results: as they are where no other part joins them
+    // the next item's queries are on their way while this one's warps are joined
+    const PrefixSegment done = s;
+    const int pieces = 2 * (s.tile1 - s.tile0), here = mt;
+    tile0 += s.tile1 - s.tile0;
+    piece0 += pieces % P;
+    phase0 ^= pieces / P & 1;
+    if (piece0 >= P) piece0 -= P, phase0 ^= 1;
+    more = walk.next(s);
+    const int was = wm;
+    if (more) load_q();
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+    // warps w and w + n have the same pairs: the upper ones leave their part, the lower ones add it, n = 2, 1 (for 32 pairs 2 alone, for 64 none)
+    for (int n = 2; n >= was; n >>= 1) {
+      prefix_bar();  // (the buffers are free)
+      if (warp >= n && warp < 2 * n) {
+        float* to = joint + (warp - n) * 16 * (D + 4);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
-        l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
-        if (mt < mts && (lane & 3) == 0) tail->sum[mt * 16 + r + 8 * h][warp] = l[mt][h];
-      }
-    prefix_bar();
-    const bool whole = prefix_whole(s) && k.first + s.e >= p.prefixes;
+        for (int h = 0; h < 2; ++h) {
+          if ((lane & 3) == 0) tail->stat[warp - n][r + 8 * h] = make_float2(m[h], l[h]);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int pair = mt * 16 + r + 8 * h, at = pair0 + pair;
-        if (pair >= pairs) continue;
-        const float4 u = *reinterpret_cast<const float4*>(tail->sum[pair]);
-        const float sum = (u.x + u.y) + (u.z + u.w);
-        const int col0 = warp * F::kCols + (lane & 3) * 2;
-        if (whole) {
-          if (seen[mt][h] <= 0) continue;  // a row that sees nothing
-          const float inv = 1.0f / sum;
-          bf16* out = p.out + (s.x.row + at / p.group) * p.ldo + (s.kvh * p.group + at % p.group) * D + col0;
-#pragma unroll
-          for (int n = 0; n < NO; ++n) *reinterpret_cast<uint32_t*>(out + n * 8) = pack_bf16x2(o[mt][n][2 * h] * inv, o[mt][n][2 * h + 1] * inv);
-        } else {
-          const long long place = s.place + pair;
-          float* out = k.part + place * D + col0;
-#pragma unroll
-          for (int n = 0; n < NO; ++n) *reinterpret_cast<float2*>(out + n * 8) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
-          if (warp == 0 && (lane & 3) == 0) k.stat[place] = make_float2(m[mt][h], sum);
+          for (int c = 0; c < NO; ++c) *reinterpret_cast<float2*>(to + (r + 8 * h) * (D + 4) + c * 8 + q2) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
         }
       }
+      prefix_bar();
+      if (warp < n) {
+        const float* from = joint + warp * 16 * (D + 4);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 st = tail->stat[warp][r + 8 * h];
+          const float now = fmaxf(m[h], st.x), base = now == -INFINITY ? 0.0f : now, f0 = prefix_ex2(m[h] - base), f1 = prefix_ex2(st.x - base);
+          m[h] = now;
+          l[h] = l[h] * f0 + st.y * f1;
+#pragma unroll
+          for (int c = 0; c < NO; ++c) {
+            const float2 u = *reinterpret_cast<const float2*>(from + (r + 8 * h) * (D + 4) + c * 8 + q2);
+            o[c][2 * h] = o[c][2 * h] * f0 + u.x * f1;
+            o[c][2 * h + 1] = o[c][2 * h + 1] * f0 + u.y * f1;
+          }
+        }
+      }
+    }
+    if (warp >= was) continue;
+    // the item's results: as they are where no other part joins them
+    const bool whole = prefix_whole(done) && !prefix;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = pair0 + r + 8 * h;
+      if (r + 8 * h >= left) continue;
+      if (whole) {
+        if (seen[h] <= 0) continue;  // a row that sees nothing
+        const float inv = 1.0f / l[h];
+        bf16* out = p.out + (done.x.row + at / p.group) * p.ldo + (done.kvh * p.group + at % p.group) * D + q2;
+#pragma unroll
+        for (int n = 0; n < NO; ++n) *reinterpret_cast<uint32_t*>(out + n * 8) = pack_bf16x2(o[n][2 * h] * inv, o[n][2 * h + 1] * inv);
+      } else {
+        const long long place = done.place + here * 16 + r + 8 * h;
+        float* out = k.part + place * D + q2;
+#pragma unroll
+        for (int n = 0; n < NO; ++n) *reinterpret_cast<float2*>(out + n * 8) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+        if ((lane & 3) == 0) k.stat[place] = make_float2(m[h], l[h]);
+      }
+    }
   }
   griddep_wait();
 }
@@ -628,7 +676,7 @@ struct PrefixTcTail {
   PrefixEntry entry[kPrefixCached + 1];
   uint64_t full[8], empty[8];
   uint64_t q_ready, s_full[2], p_ready[2], o_done[2];
-  long long carry[20];
+  PrefixBuild build;
   uint32_t tmem_base;
   int failed;
 };
@@ -637,12 +685,6 @@ template <int D>
 constexpr size_t prefix_tc_smem_bytes() {
   typedef PrefixTcShape<D> F;
   return 1024 + size_t(F::NQ) * F::kQBytes + size_t(F::kPieces) * F::kPieceBytes + sizeof(PrefixTcTail) + 16;
-}
-
-__device__ __forceinline__ float prefix_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 template <int D>
@@ -682,7 +724,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   const PrefixEntry* table = k.table;
   tcgen05_fence_before();
   if (!k.tabled) {
-    prefix_build_table(p, k, tail->entry, tail->carry, threadIdx.x, F::kThreads);
+    prefix_build_table(p, k, tail->entry, &tail->build, threadIdx.x, F::kThreads);
     table = tail->entry;
     if (blockIdx.x == 0)  // for the join
       for (int e = threadIdx.x; e <= k.count; e += F::kThreads) k.table[e] = table[e];
@@ -697,7 +739,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 
   if (!mine) {
   } else if (warp == 0) {
-    PrefixWalk walk(p, k, table, share, blockIdx.x);
+    PrefixWalk walk(k, table, share, blockIdx.x);
     const bool issuer = elect_one();
     const int boxes = KT / p.box, tpp = p.tokens_per_page;
     int piece = 0;
@@ -707,7 +749,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const int* pages = p.page_map + (long long)s.x.map * p.max_pages;
       const long long head_row = (long long)s.kvh * p.num_pages * tpp;
       auto row_of = [&](int tile) {  // as in prefix_units_kernel
-        const int key = min(s.first + tile * KT + (lane < boxes ? lane : 0) * p.box, s.x.key1 - 1);
+        const int key = min(s.x.first + tile * KT + (lane < boxes ? lane : 0) * p.box, s.x.key1 - 1);
         const int page = pages[key / tpp];
         return int(head_row + (long long)(page >= 0 && page < p.num_pages ? page : 0) * tpp + key % tpp / p.box * p.box);
       };
@@ -737,7 +779,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       while (clock64() - t0 < 2000000) __nanosleep(1000);
     }
   } else if (warp == 1) {
-    PrefixWalk walk(p, k, table, share, blockIdx.x);
+    PrefixWalk walk(k, table, share, blockIdx.x);
     const bool issuer = elect_one();
     const uint32_t idesc_s = umma_idesc_bf16(128, KT), idesc_o = umma_idesc_bf16(128, D) | kIdescBMajorMN;
     const uint64_t dq = umma_desc_sw128(sq), dk = umma_desc_sw128(ring);
@@ -779,7 +821,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         const bool more = j + 1 < s.tile1;
         good = good && prefix_wait(&tail->full[piece], phase, failed);
         const int v_at = advance();
-        const int beyond = s.x.key1 - (s.first + j * KT);  // the tile's first token that the prefix does not have
+        const int beyond = s.x.key1 - (s.x.first + j * KT);  // the tile's first token that the prefix does not have
         if (beyond < KT) {                                 // it may hold anything, and 0 * NaN is not 0
           uint8_t* v = ring + v_at * F::kPieceBytes;
           for (int c = 0; c < CH; ++c)
@@ -808,7 +850,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     }
     __syncwarp();
   } else {
-    PrefixWalk walk(p, k, table, share, blockIdx.x);
+    PrefixWalk walk(k, table, share, blockIdx.x);
     const int t = (warp - 2) >> 2, quarter = warp & 3, own = quarter * 32 + lane;
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), acc = lanes + F::kOCol + t * D, scores = lanes + t * KT;
     const float mul = p.softcap > 0.0f ? 1.0f : p.scale * kPrefixLog2e, cap = p.softcap * kPrefixLog2e, by_cap = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
@@ -852,7 +894,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 #pragma unroll
           for (int c = 0; c < KT; ++c) x[c] = cap * tanhf(x[c] * by_cap);
         }
-        const int beyond = s.x.key1 - (s.first + j * KT);
+        const int beyond = s.x.key1 - (s.x.first + j * KT);
         if (beyond < KT) {
 #pragma unroll
           for (int c = 0; c < KT; ++c)
@@ -924,73 +966,80 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 
 // ---- the join ----------------------------------------------------------------------------------------------------------------------
 
-// CTA = row; a thread has four channels of a head.  A row's parts: its prefix's (of `a`), then its tail's (of `b`), in the tokens' order.
+// CTA = (row, key head); a thread has four channels of a head.  A row's parts: its prefix's (of `a`), then its tail's (of `b`), in the tokens' order.
 template <int D>
-__global__ void __launch_bounds__(512) prefix_join_kernel(const PrefixAttnParams p, const PrefixWork a, const PrefixWork b) {
+__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixAttnParams p, const PrefixWork a, const PrefixWork b) {
+  __shared__ PrefixEntry found[4];  // the row's prefix and tail, the sums of both works
+  __shared__ int is;
+  if (threadIdx.x == 0) is = 0;
+  __syncthreads();
   griddep_launch_dependents();
   griddep_wait();
-  const int row = blockIdx.x, lane = threadIdx.x & 31;
+  const int row = blockIdx.x, kvh = blockIdx.y;
   const PrefixEntry* sequences = b.table + (p.prefixes - b.first);
-  // the last sequence that begins at the row or in front of it: 32 probes at a time
-  int lo = 0, hi = p.sequences;
-  while (lo < hi) {
-    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-    const bool below = at < hi && sequences[at].row <= row;
-    const int c = __popc(__ballot_sync(0xffffffffu, below));
-    if (c == 0) break;
-    hi = min(hi, lo + c * step);
-    lo = lo + (c - 1) * step + 1;
+  if (threadIdx.x == 0) found[2] = a.table[a.count], found[3] = b.table[b.count];
+  for (int s = threadIdx.x; s < p.sequences; s += blockDim.x) {
+    const PrefixEntry x = sequences[s];
+    if (x.row <= row && row < x.row + x.rows) {
+      found[1] = x;
+      if (x.prefix >= 0) found[0] = a.table[x.prefix];
+      is = 1;
+    }
   }
-  if (lo == 0) return;
-  const PrefixEntry tail = sequences[lo - 1];
-  if (row >= tail.row + tail.rows) return;
+  __syncthreads();
+  if (is == 0) return;
+  const PrefixEntry &front = found[0], &tail = found[1];
   if (min(tail.first_seen + row - tail.row, tail.key1) <= 0) return;
-  const PrefixEntry front = a.table[max(tail.prefix, 0)];
-  const PrefixEntry last[2] = {a.table[a.count], b.table[b.count]};
-  for (int i = threadIdx.x; i < p.heads * (D / 4); i += blockDim.x) {
-    const int head = i / (D / 4), c = (i - head * (D / 4)) * 4, kvh = head / p.group, g = head - kvh * p.group;
+  for (int i = threadIdx.x; i < p.group * (D / 4); i += blockDim.x) {
+    const int g = i / (D / 4), c = (i - g * (D / 4)) * 4;
     long long place[2];
     int parts[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       place[k] = parts[k] = 0;
       const PrefixWork& w = k == 0 ? a : b;
-      const PrefixEntry& x = k == 0 ? front : tail;
-      const int tiles = prefix_tiles(x, w.kt, p.box);
-      if ((k == 0 && tail.prefix < 0) || tiles == 0) continue;
-      const long long at = (long long)(row - x.row) * p.group + g;
-      const int block = int(at / w.pairs);
-      const long long first = kvh * last[k].units + x.units + (long long)block * tiles;
-      const PrefixShare share(last[k].units * p.kv_heads, w.workers);
-      const int c0 = share.of(first), c1 = share.of(first + tiles - 1);
-      place[k] = (long long)kvh * last[k].pairs + x.pairs + at + (long long)c0 * w.pairs;
+      const PrefixEntry &x = k == 0 ? front : tail, &last = found[2 + k];
+      if ((k == 0 && tail.prefix < 0) || x.tiles == 0) continue;
+      const int at = (row - x.row) * p.group + g, first = kvh * last.units + x.units + at / w.pairs * x.tiles;
+      const PrefixShare share(last.units * p.kv_heads, w.workers);
+      const int c0 = share.of(first), c1 = share.of(first + x.tiles - 1);
+      place[k] = (long long)kvh * last.pairs + x.pairs + at + (long long)c0 * w.pairs;
       parts[k] = c1 - c0 + 1;
     }
     if (tail.key0 == 0 && parts[1] == 1) continue;  // written already
-    float top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const PrefixWork& w = k == 0 ? a : b;
-      for (int j = 0; j < parts[k]; ++j) top = fmaxf(top, w.stat[place[k] + (long long)j * w.pairs].x);
-    }
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
+    float top = -INFINITY, sum = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const PrefixWork& w = k == 0 ? a : b;
-      for (int j = 0; j < parts[k]; ++j) {
-        const long long at = place[k] + (long long)j * w.pairs;
-        const float2 st = w.stat[at];
-        const float4 v = *reinterpret_cast<const float4*>(w.part + at * D + c);
-        const float f = exp2f(st.x - base);
-        if (st.x == -INFINITY) continue;  // (a part of which the row sees nothing)
-        sum = fmaf(st.y, f, sum);
-        o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
+      constexpr int N = 8;  // parts in flight
+      for (int j0 = 0; j0 < parts[k]; j0 += N) {
+        float2 st[N];
+        float4 v[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const long long at = place[k] + (long long)min(j0 + n, parts[k] - 1) * w.pairs;
+          st[n] = w.stat[at];
+          v[n] = *reinterpret_cast<const float4*>(w.part + at * D + c);
+        }
+        float now = top;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          if (j0 + n < parts[k]) now = fmaxf(now, st[n].x);
+        const float base = now == -INFINITY ? 0.0f : now, fix = exp2f(top - base);
+        top = now;
+        sum *= fix, o.x *= fix, o.y *= fix, o.z *= fix, o.w *= fix;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (j0 + n >= parts[k] || st[n].x == -INFINITY) continue;  // (-infinity: a part of which the row sees nothing)
+          const float f = exp2f(st[n].x - base);
+          sum = fmaf(st[n].y, f, sum);
+          o.x = fmaf(v[n].x, f, o.x), o.y = fmaf(v[n].y, f, o.y), o.z = fmaf(v[n].z, f, o.z), o.w = fmaf(v[n].w, f, o.w);
+        }
       }
     }
     const float inv = 1.0f / sum;
-    *reinterpret_cast<uint2*>(p.out + row * p.ldo + head * D + c) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    *reinterpret_cast<uint2*>(p.out + row * p.ldo + (kvh * p.group + g) * D + c) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
   }
 }
 
