@@ -38,10 +38,14 @@ bool rows_on_16(const void* base, long long pitch, int size) { return ((reinterp
 
 template <class TI, class TO>
 int launch_rotary(const RotaryParams& p, bool vec, cudaStream_t st) {
-  const int units = vec ? (p.heads + p.kv_heads) * (p.dim / 8 - p.pairs / 8) : (p.heads + p.kv_heads) * (p.dim - p.pairs);
-  int threads = (units + 31) / 32 * 32;
-  if (threads > kRotaryThreads) threads = kRotaryThreads;
-  return launch(vec ? rotary_kernel<TI, TO, true> : rotary_kernel<TI, TO, false>, dim3(p.rows), dim3(threads), 0, st, p);
+  const int step = vec ? 8 : 1;
+  const long long units = (long long)(p.heads + p.kv_heads) * (p.dim - p.pairs) / step + (p.k_pages != nullptr ? (long long)p.kv_heads * p.dim / step : 0);
+  // as many tokens per CTA as leave every SM some
+  int tokens = p.rows / (4 * 148);
+  tokens = tokens < 1 ? 1 : tokens > kRotaryTokens ? kRotaryTokens : tokens;
+  const int threads = units < kRotaryThreads ? int(units + 31) / 32 * 32 : kRotaryThreads;
+  return launch(vec ? rotary_kernel<TI, TO, true> : rotary_kernel<TI, TO, false>, dim3((p.rows + tokens - 1) / tokens), dim3(threads), size_t(tokens) * p.pairs * sizeof(float2), st,
+                p, tokens);
 }
 
 // a result in an input's place, but not value by value
