@@ -62,13 +62,24 @@ int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
   if (w[0].tabled || w[1].tabled) MTX_TRY(launch(prefix_plan_kernel, dim3(1), dim3(1024), 0, st, p, w[0], w[1]));
   if (tc) {
     MTX_TRY(allow_smem(prefix_tc_kernel<D>, prefix_tc_smem_bytes<D>(), tc_done));
+    if (Tc::NQ == 2) {  // (the split of its registers: with fewer at launch it would wait for good)
+      static std::atomic<int> regs{0};
+      if (regs.load(std::memory_order_relaxed) == 0) {
+        cudaFuncAttributes attr;
+        MTX_CUDA(cudaFuncGetAttributes(&attr, prefix_tc_kernel<D>));
+        regs.store(attr.numRegs, std::memory_order_relaxed);
+      }
+      if (regs.load(std::memory_order_relaxed) < Tc::kRegs) return fail(MTX_ERR_CUDA, "prefix_tc_kernel has %d registers, not %d", regs.load(), Tc::kRegs);
+    }
     MTX_TRY(launch(prefix_tc_kernel<D>, dim3(w[0].workers), dim3(Tc::kThreads), prefix_tc_smem_bytes<D>(), st, tk, tv, p, w[0]));
   }
   auto units = p.softcap > 0.0f ? prefix_units_kernel<D, true> : prefix_units_kernel<D, false>;
   MTX_TRY(allow_smem(units, prefix_smem_bytes<D>(), p.softcap > 0.0f ? cap_done : done));
   MTX_TRY(launch(units, dim3(w[1].workers), dim3(kPrefixThreads), prefix_smem_bytes<D>(), st, tk, tv, p, w[1]));
-  const int threads = p.group * (D / 4) < 256 ? (p.group * (D / 4) + 31) / 32 * 32 : 256;
-  return launch(prefix_join_kernel<D>, dim3(p.rows, p.kv_heads), dim3(threads < 64 ? 64 : threads), 0, st, p, tc ? w[0] : w[1], w[1]);
+  // the join: where rows and key heads are few, several threads share a place's parts
+  const int lanes = p.group * (D / 8) < 128 ? (p.group * (D / 8) + 31) / 32 * 32 : 128;
+  const int shares = (long long)p.rows * p.kv_heads < 2 * kPrefixSms ? kPrefixJoinMost / lanes : 1;
+  return launch(prefix_join_kernel<D>, dim3(p.rows, p.kv_heads), dim3(lanes, shares), 0, st, p, tc ? w[0] : w[1], w[1]);
 }
 
 }  // namespace

@@ -517,30 +517,28 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // V: tokens outside the entry's count 0 whatever they hold.  So do numbers that are none, in tokens that some rows see and others do not (0 times them is none either); the rows
         // that see them add them behind the products
         uint8_t* v = ring + v_piece * kPrefixPieceBytes;
-        const int lo = s.x.key0 - key;
-        some = max(s.x.first_seen - key, 0), hi = min(s.x.key1 - key, KT);
+        const int lo = min(max(s.x.key0 - key, 0), KT);
+        hi = min(s.x.key1 - key, KT);
+        some = min(max(s.x.first_seen - key, lo), hi);
+        auto piece_of = [&](int token, int i) { return reinterpret_cast<uint4*>(v + (i >> 3) * KT * 128 + token * 128 + ((i & 7) << 4)); };  // (any order of a row's pieces)
         uint32_t gone = 0;
-        for (int i = lane; i < KT * (D / 8); i += 32) {
-          const int token = i / (D / 8), c = i - token * (D / 8);
-          if (token < some || token >= hi) continue;
-          const uint4 u = *reinterpret_cast<const uint4*>(v + (c >> 3) * KT * 128 + token * 128 + ((c & 7) << 4));  // (any order of a row's pieces)
+        for (int i = some * (D / 8) + lane; i < hi * (D / 8); i += 32) {
+          const uint4 u = *piece_of(i / (D / 8), i % (D / 8));
           const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
           for (int b = 0; b < 4; ++b) gone |= (w[b] & 0x7f80u) == 0x7f80u || (w[b] & 0x7f800000u) == 0x7f800000u;
         }
         odd = __any_sync(0xffffffffu, gone != 0);
         if (wm > 1) asm volatile("bar.sync %0, %1;" ::"r"(2 + mine), "r"(32 * wm) : "memory");  // (the tile's other warps have looked too)
-        for (int i = lane; i < KT * (D / 8); i += 32) {
-          const int token = i / (D / 8), c = i - token * (D / 8);
-          uint4* at = reinterpret_cast<uint4*>(v + (c >> 3) * KT * 128 + token * 128 + ((c & 7) << 4));
-          if (token < lo || token >= hi) {
-            *at = make_uint4(0, 0, 0, 0);
-          } else if (odd && token >= some) {
-            uint4 u = *at;
+        for (int i = lane; i < lo * (D / 8); i += 32) *piece_of(i / (D / 8), i % (D / 8)) = make_uint4(0, 0, 0, 0);
+        for (int i = hi * (D / 8) + lane; i < KT * (D / 8); i += 32) *piece_of(i / (D / 8), i % (D / 8)) = make_uint4(0, 0, 0, 0);
+        if (odd) {
+          for (int i = some * (D / 8) + lane; i < hi * (D / 8); i += 32) {
+            uint4 u = *piece_of(i / (D / 8), i % (D / 8));
             uint32_t* w = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
             for (int b = 0; b < 4; ++b) w[b] &= ~(((w[b] & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w[b] & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u));
-            *at = u;
+            *piece_of(i / (D / 8), i % (D / 8)) = u;
           }
         }
         __syncwarp();
@@ -668,8 +666,11 @@ struct PrefixTcShape {
   static constexpr int kPairs = NQ * 128;
   static constexpr int kPieceBytes = KT * D * 2, kPieces = 131072 / kPieceBytes;
   static constexpr int kQBytes = 128 * D * 2;
-  static constexpr int kThreads = 64 + NQ * 128;
+  static constexpr int kThreads = 128 + NQ * 128;  // a warpgroup of which two warps work, one or two of the softmax
   static constexpr int kOCol = NQ * KT;
+  // registers at launch and after the split (two softmax warpgroups: 128 x 80 + 256 x 208 of 384 x 168)
+  static constexpr int kRegs = 168, kRegsCopy = 80, kRegsSoftmax = 208;
+  static_assert(NQ == 1 || 128 * kRegsCopy + NQ * 128 * kRegsSoftmax <= kThreads * kRegs, "a warpgroup would wait for registers for good");
 };
 
 struct PrefixTcTail {
@@ -685,6 +686,152 @@ template <int D>
 constexpr size_t prefix_tc_smem_bytes() {
   typedef PrefixTcShape<D> F;
   return 1024 + size_t(F::NQ) * F::kQBytes + size_t(F::kPieces) * F::kPieceBytes + sizeof(PrefixTcTail) + 16;
+}
+
+// two fp32 operations at a time
+__device__ __forceinline__ float2 prefix_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 prefix_add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// umma_desc_sw128 of a shared address
+__device__ __forceinline__ uint64_t prefix_desc(uint32_t addr) { return uint64_t((addr & 0x3FFFFu) >> 4) | uint64_t(1) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61; }
+
+// What the softmax warps do with a CTA's run.
+template <int D>
+__device__ __forceinline__ void prefix_softmax(const PrefixAttnParams& p, const PrefixWork& k, PrefixTcTail* tail, uint8_t* sq, uint32_t tmem, const PrefixEntry* table, const PrefixShare& share) {
+  typedef PrefixTcShape<D> F;
+  constexpr int KT = F::KT;
+  volatile int* failed = &tail->failed;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  PrefixSegment s;
+  PrefixWalk walk(k, table, share, blockIdx.x);
+  const int t = (warp - 4) >> 2, quarter = warp & 3, own = quarter * 32 + lane;
+  const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), acc = lanes + F::kOCol + t * D, scores = lanes + t * KT;
+  const float mul = p.softcap > 0.0f ? 1.0f : p.scale * kPrefixLog2e, cap = p.softcap * kPrefixLog2e, by_cap = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
+  uint32_t turn = 0, done = 0;
+  int segment = 0;
+  while (walk.next(s)) {
+    const int pair0 = s.block * F::kPairs + t * 128, pairs = s.x.rows * p.group - pair0;
+    // Q: a thread brings its pair's row
+    {
+      uint4 v[D / 8];
+      const int at = pair0 + own;
+      const bf16* from = p.q + (s.x.row + at / p.group) * p.ldq + (s.kvh * p.group + at % p.group) * D;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) v[c] = own < pairs ? reinterpret_cast<const uint4*>(from)[c] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(sq + t * F::kQBytes + (c >> 3) * 16384 + own * 128 + (((c & 7) ^ (own & 7)) << 4)) = v[c];
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tail->q_ready);
+    }
+    const int now_segment = segment++;
+    if (pairs <= 0) {  // (not two arrivals for one item)
+      prefix_wait(&tail->q_ready, now_segment & 1, failed);
+      continue;
+    }
+    float m = -INFINITY, l = 0.0f;  // the maximum that the accumulator stands at (times log2 e), the sum
+    for (int j = s.tile0; j < s.tile1; ++j) {
+      prefix_wait(&tail->s_full[t], turn, failed);
+      turn ^= 1;
+      tcgen05_fence_after();
+      float x[KT];
+      {
+        uint32_t raw[KT / 32][32];
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) tmem_ld_x32(scores + c * 32, raw[c]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < KT; ++c) x[c] = __uint_as_float(raw[c / 32][c % 32]);
+      }
+      if (p.softcap > 0.0f) {
+#pragma unroll
+        for (int c = 0; c < KT; ++c) x[c] = cap * tanhf(x[c] * by_cap);
+      }
+      const int beyond = s.x.key1 - (s.x.first + j * KT);
+      if (beyond < KT) {
+#pragma unroll
+        for (int c = 0; c < KT; ++c)
+          if (c >= beyond) x[c] = -INFINITY;
+      }
+      float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+      for (int c = 4; c + 7 < KT + 4; c += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = c + 4 + i < KT ? fmaxf(mx[i], fmaxf(x[c + i], x[c + 4 + i])) : fmaxf(mx[i], x[c + i]);
+      const float now = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul);
+      if (__any_sync(0xffffffffu, now > m + 8.0f)) {  // (m = -inf: the first tile)
+        const float fix = now == -INFINITY ? 1.0f : prefix_ex2(m - now);
+        l *= fix;
+        m = now;
+        if (j > s.tile0) {  // the accumulator holds the tiles before: they are complete (s_full came behind them)
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld_x32(acc + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
+            tmem_st_x32(acc + c, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+      const float2 mul2 = make_float2(mul, mul), base2 = make_float2(-base, -base);
+      float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+      for (int c = 0; c < KT; c += 32) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float2 w = prefix_fma2(make_float2(x[c + 2 * e], x[c + 2 * e + 1]), mul2, base2);
+          w.x = prefix_ex2(w.x);
+          w.y = prefix_ex2(w.y);
+          sums[e & 1] = prefix_add2(sums[e & 1], w);
+          pk[e] = pack_bf16x2(w.x, w.y);
+        }
+        tmem_st_x16(scores + c / 2, pk);
+      }
+      l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+      tmem_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tail->p_ready[t]);
+    }
+    prefix_wait(&tail->o_done[t], done, failed);
+    done ^= 1;
+    tcgen05_fence_after();
+    const long long place = s.place + t * 128 + own;
+#pragma unroll 1
+    for (int c = 0; c < D; c += 32) {
+      uint32_t o[32];
+      tmem_ld_x32(acc + c, o);
+      tmem_wait_ld();
+      if (own < pairs) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(k.part + place * D + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+      }
+    }
+    if (own < pairs) k.stat[place] = make_float2(m, l);
+    tcgen05_fence_before();
+  }
 }
 
 template <int D>
@@ -737,8 +884,10 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   const bool mine = int(blockIdx.x) < share.workers;
   PrefixSegment s;
 
-  if (!mine) {
-  } else if (warp == 0) {
+  if (warp < 4) {
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::kRegsCopy));
+    if (!mine || warp >= 2) {
+    } else if (warp == 0) {
     PrefixWalk walk(k, table, share, blockIdx.x);
     const bool issuer = elect_one();
     const int boxes = KT / p.box, tpp = p.tokens_per_page;
@@ -778,12 +927,14 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       const long long t0 = clock64();
       while (clock64() - t0 < 2000000) __nanosleep(1000);
     }
-  } else if (warp == 1) {
+    } else {
     PrefixWalk walk(k, table, share, blockIdx.x);
     const bool issuer = elect_one();
+    // numbers that the compiler takes for the same in all lanes: otherwise it brings every operand of every MMA to where the MMA reads it by itself (16 MMAs 1550 cycles, 950 so)
+    auto same = [](int x) { return __reduce_max_sync(0xffffffffu, x); };
+    const uint32_t tmem_at = uint32_t(same(int(tmem))), ring_addr = uint32_t(same(int(smem_u32(ring))));
     const uint32_t idesc_s = umma_idesc_bf16(128, KT), idesc_o = umma_idesc_bf16(128, D) | kIdescBMajorMN;
-    const uint64_t dq = umma_desc_sw128(sq), dk = umma_desc_sw128(ring);
-    const uint32_t ring_addr = smem_u32(ring);
+    const uint64_t dq = prefix_desc(uint32_t(same(int(smem_u32(sq))))), dk = prefix_desc(ring_addr);
     bool good = true;
     auto issue_s = [&](int t, int piece) {
       if (!issuer || !good) return;
@@ -791,7 +942,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_bf16(tmem + t * KT, dq + uint64_t((t * F::kQBytes + c * 16384 + kk * 32) >> 4), dk + uint64_t((piece * F::kPieceBytes + c * KT * 128 + kk * 32) >> 4), idesc_s,
+          umma_bf16(tmem_at + t * KT, dq + uint64_t((t * F::kQBytes + c * 16384 + kk * 32) >> 4), dk + uint64_t((piece * F::kPieceBytes + c * KT * 128 + kk * 32) >> 4), idesc_s,
                     uint32_t((c | kk) != 0));
       umma_commit(&tail->s_full[t]);
     };
@@ -799,7 +950,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       if (!issuer || !good) return;
 #pragma unroll
       for (int kk = 0; kk < KT / 16; ++kk)
-        umma_bf16_ts(tmem + F::kOCol + t * D, tmem + t * KT + kk * 8, umma_desc_sw128_mn(ring_addr + piece * F::kPieceBytes + kk * 2048, KT * 128), idesc_o, uint32_t(!start || kk != 0));
+        umma_bf16_ts(tmem_at + F::kOCol + t * D, tmem_at + t * KT + kk * 8, umma_desc_sw128_mn(ring_addr + piece * F::kPieceBytes + kk * 2048, KT * 128), idesc_o, uint32_t(!start || kk != 0));
     };
     int piece = 0, segment = 0;  // pieces: K, V, K, V ..
     uint32_t phase = 0, turn[2] = {0, 0};
@@ -809,19 +960,19 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       return at;
     };
     while (walk.next(s)) {
-      const int halves = NQ == 2 && s.x.rows * p.group - s.block * F::kPairs > 128 ? 2 : 1;
-      good = good && prefix_wait(&tail->q_ready, segment & 1, failed);
+      const int halves = same(NQ == 2 && s.x.rows * p.group - s.block * F::kPairs > 128 ? 2 : 1), tile0 = same(s.tile0), tile1 = same(s.tile1), key1 = same(s.x.key1), first = same(s.x.first);
+      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->q_ready, segment & 1, failed));
       ++segment;
-      good = good && prefix_wait(&tail->full[piece], phase, failed);
+      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->full[piece], phase, failed));
       tcgen05_fence_after();
       int at = advance();
       for (int t = 0; t < halves; ++t) issue_s(t, at);
       if (issuer && good) umma_commit(&tail->empty[at]);
-      for (int j = s.tile0; j < s.tile1; ++j) {
-        const bool more = j + 1 < s.tile1;
-        good = good && prefix_wait(&tail->full[piece], phase, failed);
+      for (int j = tile0; j < tile1; ++j) {
+        const bool more = j + 1 < tile1;
+        good = __all_sync(0xffffffffu, good && prefix_wait(&tail->full[piece], phase, failed));
         const int v_at = advance();
-        const int beyond = s.x.key1 - (s.x.first + j * KT);  // the tile's first token that the prefix does not have
+        const int beyond = key1 - (first + j * KT);  // the tile's first token that the prefix does not have
         if (beyond < KT) {                                 // it may hold anything, and 0 * NaN is not 0
           uint8_t* v = ring + v_at * F::kPieceBytes;
           for (int c = 0; c < CH; ++c)
@@ -831,14 +982,14 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
         }
         int k_at = 0;
         if (more) {
-          good = good && prefix_wait(&tail->full[piece], phase, failed);
+          good = __all_sync(0xffffffffu, good && prefix_wait(&tail->full[piece], phase, failed));
           k_at = advance();
         }
         for (int t = 0; t < halves; ++t) {
-          good = good && prefix_wait(&tail->p_ready[t], turn[t], failed);
+          good = __all_sync(0xffffffffu, good && prefix_wait(&tail->p_ready[t], turn[t], failed));
           turn[t] ^= 1;
           tcgen05_fence_after();
-          issue_o(t, v_at, j == s.tile0);
+          issue_o(t, v_at, j == tile0);
           if (more) issue_s(t, k_at);
           else if (issuer && good) umma_commit(&tail->o_done[t]);
         }
@@ -849,114 +1000,10 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
       }
     }
     __syncwarp();
-  } else {
-    PrefixWalk walk(k, table, share, blockIdx.x);
-    const int t = (warp - 2) >> 2, quarter = warp & 3, own = quarter * 32 + lane;
-    const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), acc = lanes + F::kOCol + t * D, scores = lanes + t * KT;
-    const float mul = p.softcap > 0.0f ? 1.0f : p.scale * kPrefixLog2e, cap = p.softcap * kPrefixLog2e, by_cap = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
-    uint32_t turn = 0, done = 0;
-    int segment = 0;
-    while (walk.next(s)) {
-      const int pair0 = s.block * F::kPairs + t * 128, pairs = s.x.rows * p.group - pair0;
-      // Q: a thread brings its pair's row
-      {
-        uint4 v[D / 8];
-        const int at = pair0 + own;
-        const bf16* from = p.q + (s.x.row + at / p.group) * p.ldq + (s.kvh * p.group + at % p.group) * D;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) v[c] = own < pairs ? reinterpret_cast<const uint4*>(from)[c] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(sq + t * F::kQBytes + (c >> 3) * 16384 + own * 128 + (((c & 7) ^ (own & 7)) << 4)) = v[c];
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tail->q_ready);
-      }
-      const int now_segment = segment++;
-      if (pairs <= 0) {  // (not two arrivals for one item)
-        prefix_wait(&tail->q_ready, now_segment & 1, failed);
-        continue;
-      }
-      float m = -INFINITY, l = 0.0f;  // the maximum that the accumulator stands at (times log2 e), the sum
-      for (int j = s.tile0; j < s.tile1; ++j) {
-        prefix_wait(&tail->s_full[t], turn, failed);
-        turn ^= 1;
-        tcgen05_fence_after();
-        float x[KT];
-        {
-          uint32_t raw[KT / 32][32];
-#pragma unroll
-          for (int c = 0; c < KT / 32; ++c) tmem_ld_x32(scores + c * 32, raw[c]);
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < KT; ++c) x[c] = __uint_as_float(raw[c / 32][c % 32]);
-        }
-        if (p.softcap > 0.0f) {
-#pragma unroll
-          for (int c = 0; c < KT; ++c) x[c] = cap * tanhf(x[c] * by_cap);
-        }
-        const int beyond = s.x.key1 - (s.x.first + j * KT);
-        if (beyond < KT) {
-#pragma unroll
-          for (int c = 0; c < KT; ++c)
-            if (c >= beyond) x[c] = -INFINITY;
-        }
-        float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int c = 4; c < KT; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-        const float now = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul);
-        if (__any_sync(0xffffffffu, now > m + 8.0f)) {  // (m = -inf: the first tile)
-          const float fix = now == -INFINITY ? 1.0f : prefix_ex2(m - now);
-          l *= fix;
-          m = now;
-          if (j > s.tile0) {  // the accumulator holds the tiles before: they are complete (s_full came behind them)
-#pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld_x32(acc + c, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
-              tmem_st_x32(acc + c, o);
-            }
-          }
-        }
-        const float base = m == -INFINITY ? 0.0f : m;
-        float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-        for (int c = 0; c < KT; c += 32) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float p0 = prefix_ex2(fmaf(x[c + 2 * e], mul, -base)), p1 = prefix_ex2(fmaf(x[c + 2 * e + 1], mul, -base));
-            l0 += p0;
-            l1 += p1;
-            pk[e] = pack_bf16x2(p0, p1);
-          }
-          tmem_st_x16(scores + c / 2, pk);
-        }
-        l += l0 + l1;
-        tmem_wait_st();
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&tail->p_ready[t]);
-      }
-      prefix_wait(&tail->o_done[t], done, failed);
-      done ^= 1;
-      tcgen05_fence_after();
-      const long long place = s.place + t * 128 + own;
-#pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        tmem_ld_x32(acc + c, o);
-        tmem_wait_ld();
-        if (own < pairs) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(k.part + place * D + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        }
-      }
-      if (own < pairs) k.stat[place] = make_float2(m, l);
-      tcgen05_fence_before();
     }
+  } else {
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::kRegsSoftmax));
+    if (mine) prefix_softmax<D>(p, k, tail, sq, tmem, table, share);
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -966,19 +1013,24 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
 
 // ---- the join ----------------------------------------------------------------------------------------------------------------------
 
-// CTA = (row, key head); a thread has four channels of a head.  A row's parts: its prefix's (of `a`), then its tail's (of `b`), in the tokens' order.
+// CTA = (row, key head); a thread has eight channels of a head, and every blockDim.y-th part of the row's: its prefix's (of `a`), then its tail's (of `b`), in the tokens' order.
+constexpr int kPrefixJoinMost = 256;  // threads
+
 template <int D>
-__global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixAttnParams p, const PrefixWork a, const PrefixWork b) {
+__global__ void __launch_bounds__(kPrefixJoinMost) prefix_join_kernel(const PrefixAttnParams p, const PrefixWork a, const PrefixWork b) {
   __shared__ PrefixEntry found[4];  // the row's prefix and tail, the sums of both works
   __shared__ int is;
-  if (threadIdx.x == 0) is = 0;
+  __shared__ float joint[kPrefixJoinMost][10];
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y;
+  if (tid == 0) is = 0;
   __syncthreads();
   griddep_launch_dependents();
   griddep_wait();
   const int row = blockIdx.x, kvh = blockIdx.y;
   const PrefixEntry* sequences = b.table + (p.prefixes - b.first);
-  if (threadIdx.x == 0) found[2] = a.table[a.count], found[3] = b.table[b.count];
-  for (int s = threadIdx.x; s < p.sequences; s += blockDim.x) {
+  if (tid == 0) found[2] = a.table[a.count];
+  if (tid == 1) found[3] = b.table[b.count];
+  for (int s = tid; s < p.sequences; s += threads) {
     const PrefixEntry x = sequences[s];
     if (x.row <= row && row < x.row + x.rows) {
       found[1] = x;
@@ -990,8 +1042,10 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixAttnParams
   if (is == 0) return;
   const PrefixEntry &front = found[0], &tail = found[1];
   if (min(tail.first_seen + row - tail.row, tail.key1) <= 0) return;
-  for (int i = threadIdx.x; i < p.group * (D / 4); i += blockDim.x) {
-    const int g = i / (D / 4), c = (i - g * (D / 4)) * 4;
+  const int lanes = D / 8, most = p.group * lanes;
+  for (int i0 = 0; i0 < most; i0 += blockDim.x) {  // (one round where blockDim.x threads have all heads)
+    const int i = i0 + threadIdx.x, g = min(i / lanes, p.group - 1), c = i % lanes * 8;
+    const bool mine = i < most;
     long long place[2];
     int parts[2];
 #pragma unroll
@@ -1006,40 +1060,68 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(const PrefixAttnParams
       place[k] = (long long)kvh * last.pairs + x.pairs + at + (long long)c0 * w.pairs;
       parts[k] = c1 - c0 + 1;
     }
-    if (tail.key0 == 0 && parts[1] == 1) continue;  // written already
-    float top = -INFINITY, sum = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const bool written = tail.key0 == 0 && parts[1] == 1;  // already
+    float top = -INFINITY, sum = 0.0f, o[8] = {};
+    constexpr int N = 4;  // parts in flight
+    const int all = mine && !written ? parts[0] + parts[1] : 0;
+    for (int j0 = threadIdx.y; j0 < all; j0 += N * blockDim.y) {
+      float2 st[N];
+      float4 v[N][2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const PrefixWork& w = k == 0 ? a : b;
-      constexpr int N = 8;  // parts in flight
-      for (int j0 = 0; j0 < parts[k]; j0 += N) {
-        float2 st[N];
-        float4 v[N];
+      for (int n = 0; n < N; ++n) {
+        const int j = min(j0 + n * int(blockDim.y), all - 1);
+        const bool of_tail = j >= parts[0];
+        const long long at = of_tail ? place[1] + (long long)(j - parts[0]) * b.pairs : place[0] + (long long)j * a.pairs;
+        const float4* from = reinterpret_cast<const float4*>((of_tail ? b.part : a.part) + at * D + c);
+        st[n] = (of_tail ? b.stat : a.stat)[at];
+        v[n][0] = from[0];
+        v[n][1] = from[1];
+      }
+      float now = top;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const long long at = place[k] + (long long)min(j0 + n, parts[k] - 1) * w.pairs;
-          st[n] = w.stat[at];
-          v[n] = *reinterpret_cast<const float4*>(w.part + at * D + c);
-        }
-        float now = top;
+      for (int n = 0; n < N; ++n)
+        if (j0 + n * int(blockDim.y) < all) now = fmaxf(now, st[n].x);
+      const float base = now == -INFINITY ? 0.0f : now, fix = exp2f(top - base);
+      top = now;
+      sum *= fix;
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-          if (j0 + n < parts[k]) now = fmaxf(now, st[n].x);
-        const float base = now == -INFINITY ? 0.0f : now, fix = exp2f(top - base);
-        top = now;
-        sum *= fix, o.x *= fix, o.y *= fix, o.z *= fix, o.w *= fix;
+      for (int e = 0; e < 8; ++e) o[e] *= fix;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          if (j0 + n >= parts[k] || st[n].x == -INFINITY) continue;  // (-infinity: a part of which the row sees nothing)
-          const float f = exp2f(st[n].x - base);
-          sum = fmaf(st[n].y, f, sum);
-          o.x = fmaf(v[n].x, f, o.x), o.y = fmaf(v[n].y, f, o.y), o.z = fmaf(v[n].z, f, o.z), o.w = fmaf(v[n].w, f, o.w);
-        }
+      for (int n = 0; n < N; ++n) {
+        if (j0 + n * int(blockDim.y) >= all || st[n].x == -INFINITY) continue;  // (-infinity: a part of which the row sees nothing)
+        const float f = exp2f(st[n].x - base);
+        sum = fmaf(st[n].y, f, sum);
+        o[0] = fmaf(v[n][0].x, f, o[0]), o[1] = fmaf(v[n][0].y, f, o[1]), o[2] = fmaf(v[n][0].z, f, o[2]), o[3] = fmaf(v[n][0].w, f, o[3]);
+        o[4] = fmaf(v[n][1].x, f, o[4]), o[5] = fmaf(v[n][1].y, f, o[5]), o[6] = fmaf(v[n][1].z, f, o[6]), o[7] = fmaf(v[n][1].w, f, o[7]);
       }
     }
+    if (blockDim.y > 1) {  // the threads of one place, in order
+      __syncthreads();
+      joint[tid][8] = top;
+      joint[tid][9] = sum;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) joint[tid][e] = o[e];
+      __syncthreads();
+      if (threadIdx.y > 0) continue;
+      float now = top;
+      for (int y = 1; y < int(blockDim.y); ++y) now = fmaxf(now, joint[y * blockDim.x + threadIdx.x][8]);
+      const float base = now == -INFINITY ? 0.0f : now, fix = exp2f(top - base);
+      sum *= fix;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= fix;
+      for (int y = 1; y < int(blockDim.y); ++y) {
+        const float* other = joint[y * blockDim.x + threadIdx.x];
+        if (other[8] == -INFINITY) continue;
+        const float f = exp2f(other[8] - base);
+        sum = fmaf(other[9], f, sum);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = fmaf(other[e], f, o[e]);
+      }
+    }
+    if (all == 0) continue;
     const float inv = 1.0f / sum;
-    *reinterpret_cast<uint2*>(p.out + row * p.ldo + (kvh * p.group + g) * D + c) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    *reinterpret_cast<uint4*>(p.out + row * p.ldo + (kvh * p.group + g) * D + c) =
+        make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv), pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
   }
 }
 
