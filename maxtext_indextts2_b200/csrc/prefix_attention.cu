@@ -33,49 +33,71 @@ struct PrefixLayout {
   }
 };
 
+// bf16 rows [rows, ld] that hold `heads` vectors of `dim` side by side, box [64, box_heads, box_rows] with the 128-byte swizzle; what is behind the last row reads as zeros
+int make_map_heads(CUtensorMap* m, const void* base, int dim, int heads, int rows, long long ld, int box_heads, int box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return fail(MTX_ERR_CUDA, "cuTensorMapEncodeTiled is not available (no CUDA driver?)");
+  const cuuint64_t dims[3] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(rows)}, strides[2] = {cuuint64_t(dim) * 2, cuuint64_t(ld) * 2};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_heads), cuuint32_t(box_rows)}, estr[3] = {1, 1, 1};
+  CUresult rc = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(MTX_ERR_CUDA, "cuTensorMapEncodeTiled (heads) failed with CUresult %d", int(rc));
+  return MTX_OK;
+}
+
+// a pool [rows, dim] in chunks of 64 channels, box [64, box_rows, chunks] with the 128-byte swizzle
+int make_map_pool(CUtensorMap* m, const void* base, int dim, uint64_t rows, int box_rows, int chunks) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return fail(MTX_ERR_CUDA, "cuTensorMapEncodeTiled is not available (no CUDA driver?)");
+  const cuuint64_t dims[3] = {64, rows, cuuint64_t(dim / 64)}, strides[2] = {cuuint64_t(dim) * 2, 128};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), cuuint32_t(chunks)}, estr[3] = {1, 1, 1};
+  CUresult rc = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(MTX_ERR_CUDA, "cuTensorMapEncodeTiled (pool) failed with CUresult %d", int(rc));
+  return MTX_OK;
+}
+
 template <int D>
 int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
-  static std::atomic<uint64_t> done{0}, cap_done{0}, tc_done{0};
+  static std::atomic<uint64_t> done{0}, cap_done{0}, tc_done{0}, tc_cap_done{0};
   constexpr int KT = PrefixShape<D>::KT;
   typedef PrefixTcShape<D> Tc;
   const bool tc = prefix_on_tc(p.rows, p.prefixes, p.group);
   const PrefixLayout at(p.rows, p.sequences, p.prefixes, p.heads, p.kv_heads, D);
-  const int box = KT < Tc::KT ? KT : Tc::KT;
-  p.box = p.tokens_per_page < box ? p.tokens_per_page : box;
+  p.box = p.tokens_per_page < KT ? p.tokens_per_page : KT;
   PrefixWork w[2];
   memset(w, 0, sizeof(w));
   for (int k = 0; k < 2; ++k) {
     w[k].first = k == 1 && tc ? p.prefixes : 0;
     w[k].count = k == 0 ? p.prefixes : p.sequences + (tc ? 0 : p.prefixes);
     w[k].kt = k == 0 ? Tc::KT : KT;
-    w[k].pairs = k == 0 ? Tc::kPairs : kPrefixPairs;
+    w[k].pairs = k == 0 ? Tc::NQ * (128 / p.group * p.group) : kPrefixPairs;
+    w[k].mixed = k == 0;
+    w[k].box = p.tokens_per_page < w[k].kt ? p.tokens_per_page : w[k].kt;
     w[k].workers = k == 0 ? kPrefixSms : PrefixShape<D>::kCtas * kPrefixSms;
     w[k].tabled = (k == 1 || tc) && w[k].count > kPrefixCached;
     w[k].table = reinterpret_cast<PrefixEntry*>(scratch + at.table[k]);
     w[k].stat = reinterpret_cast<float2*>(scratch + at.stat[k]);
     w[k].part = reinterpret_cast<float*>(scratch + at.part[k]);
   }
-  CUtensorMap tk, tv;
+  CUtensorMap tk[2], tv[2];
   const uint64_t pool = uint64_t(p.kv_heads) * p.num_pages * p.tokens_per_page;
-  MTX_TRY(make_map(&tk, p.k, D, pool, p.box));
-  MTX_TRY(make_map(&tv, p.v, D, pool, p.box));
+  for (int k = tc ? 0 : 1; k < 2; ++k) {
+    const int chunks = w[k].box == w[k].kt ? D / 64 : 1;
+    MTX_TRY(make_map_pool(&tk[k], p.k, D, pool, w[k].box, chunks));
+    MTX_TRY(make_map_pool(&tv[k], p.v, D, pool, w[k].box, chunks));
+  }
   if (w[0].tabled || w[1].tabled) MTX_TRY(launch(prefix_plan_kernel, dim3(1), dim3(1024), 0, st, p, w[0], w[1]));
   if (tc) {
-    MTX_TRY(allow_smem(prefix_tc_kernel<D>, prefix_tc_smem_bytes<D>(), tc_done));
-    if (Tc::NQ == 2) {  // (the split of its registers: with fewer at launch it would wait for good)
-      static std::atomic<int> regs{0};
-      if (regs.load(std::memory_order_relaxed) == 0) {
-        cudaFuncAttributes attr;
-        MTX_CUDA(cudaFuncGetAttributes(&attr, prefix_tc_kernel<D>));
-        regs.store(attr.numRegs, std::memory_order_relaxed);
-      }
-      if (regs.load(std::memory_order_relaxed) < Tc::kRegs) return fail(MTX_ERR_CUDA, "prefix_tc_kernel has %d registers, not %d", regs.load(), Tc::kRegs);
-    }
-    MTX_TRY(launch(prefix_tc_kernel<D>, dim3(w[0].workers), dim3(Tc::kThreads), prefix_tc_smem_bytes<D>(), st, tk, tv, p, w[0]));
+    CUtensorMap tq;
+    MTX_TRY(make_map_heads(&tq, p.q, D, p.heads, p.rows, p.ldq, p.group, 128 / p.group));
+    auto kernel = p.softcap > 0.0f ? prefix_tc_kernel<D, true> : prefix_tc_kernel<D, false>;
+    MTX_TRY(allow_smem(kernel, prefix_tc_smem_bytes<D>(), p.softcap > 0.0f ? tc_cap_done : tc_done));
+    MTX_TRY(launch(kernel, dim3(w[0].workers), dim3(Tc::kThreads), prefix_tc_smem_bytes<D>(), st, tq, tk[0], tv[0], p, w[0]));
   }
   auto units = p.softcap > 0.0f ? prefix_units_kernel<D, true> : prefix_units_kernel<D, false>;
   MTX_TRY(allow_smem(units, prefix_smem_bytes<D>(), p.softcap > 0.0f ? cap_done : done));
-  MTX_TRY(launch(units, dim3(w[1].workers), dim3(kPrefixThreads), prefix_smem_bytes<D>(), st, tk, tv, p, w[1]));
+  MTX_TRY(launch(units, dim3(w[1].workers), dim3(kPrefixThreads), prefix_smem_bytes<D>(), st, tk[1], tv[1], p, w[1]));
   // the join: where rows and key heads are few, several threads share a place's parts
   const int lanes = p.group * (D / 8) < 128 ? (p.group * (D / 8) + 31) / 32 * 32 : 128;
   const int shares = (long long)p.rows * p.kv_heads < 2 * kPrefixSms ? kPrefixJoinMost / lanes : 1;

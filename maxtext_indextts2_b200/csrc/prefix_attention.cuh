@@ -23,15 +23,17 @@ struct PrefixAttnParams {
   const int *row0, *lengths, *page_map, *prefix_seq0, *prefix_len;
   int heads, kv_heads, group, num_pages, tokens_per_page, max_pages;
   float scale, softcap;
-  int box;  // tokens of a copy: a page, or a part of one, at most a tile
+  int box;  // tokens of a copy of the tails' kernel: a page, or a part of one, at most a tile (tiles begin at its multiples)
 };
 
 // Entries that one kernel goes through, and where its results are.
 struct PrefixWork {
   int first, count;  // the entries: prefixes, then sequences
   int kt, pairs;     // tokens of a tile, pairs of an item
+  int box;           // tokens of a copy
   int workers;       // CTAs that share the units, at most
   int tabled;        // the table is there already (more entries than a CTA keeps)
+  int mixed;         // an item's weighted values lie as [D / 4][pairs][4], not [pairs][D]
   float* part;       // [place][D]: weighted values
   float2* stat;      // [place]: maximum (of the scores times log2 e) and sum
   struct PrefixEntry* table;  // [count + 1], for the join
@@ -243,6 +245,48 @@ struct PrefixWalk {
 
 __device__ __forceinline__ bool prefix_whole(const PrefixSegment& s) { return s.x.key0 == 0 && s.tile0 == 0 && s.tile1 == s.x.tiles; }
 
+// ---- copies of tiles ---------------------------------------------------------------------------------------------------------------
+
+// Where the boxes of an item's tiles lie in the pool: the 32 lanes look up as many boxes at a time.
+struct PrefixRows {
+  const int* pages;
+  int head_row, num_pages, tpp, box, boxes, per, first, last, lane;
+
+  __device__ __forceinline__ PrefixRows(const PrefixAttnParams& p, const PrefixWork& k, const PrefixSegment& s, int kt)
+      : pages(p.page_map + (long long)s.x.map * p.max_pages), head_row(s.kvh * p.num_pages * p.tokens_per_page), num_pages(p.num_pages), tpp(p.tokens_per_page), box(k.box), boxes(kt / k.box),
+        per(32 / boxes), first(s.x.first + s.tile0 * kt), last(s.x.key1 - 1), lane(threadIdx.x & 31) {}
+  // round r: lane i has box i of the tiles from r * per on; boxes behind the last token: that token's page
+  __device__ __forceinline__ int look_up(int r) const {
+    const int key = min(first + (r * 32 + lane) * box, last), page = pages[key / tpp];
+    return head_row + (page >= 0 && page < num_pages ? page : 0) * tpp + key % tpp / box * box;
+  }
+  // of a round: the row of tile t's box b, the same in all lanes as the compiler sees it
+  __device__ __forceinline__ int row(int round, int t, int b) const { return __reduce_max_sync(0xffffffffu, lane == t % per * boxes + b ? round : int(0x80000000)); }
+};
+
+// A box [CH][box tokens][128 B], or one chunk of channels of it
+__device__ __forceinline__ void prefix_load_box(void* dst, const CUtensorMap* tm, int row, int c, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;"
+      :
+      : "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(c), "l"(kEvictNormal)
+      : "memory");
+}
+
+// Tile t of K or V into a piece [CH][kt tokens][128 B]: one copy where a box is a whole tile, else one for each box and chunk.
+template <int CH>
+__device__ __forceinline__ void prefix_load_tile(const PrefixRows& rows, int round, int t, int kt, uint8_t* to, const CUtensorMap* tm, uint64_t* bar, bool issue) {
+  for (int b = 0; b < rows.boxes; ++b) {
+    const int from = rows.row(round, t, b);
+    if (!issue) continue;
+    if (rows.boxes == 1) {
+      prefix_load_box(to, tm, from, 0, bar);
+    } else {
+      for (int c = 0; c < CH; ++c) prefix_load_box(to + c * kt * 128 + b * rows.box * 128, tm, from, c, bar);
+    }
+  }
+}
+
 // ---- units on the warps' MMAs ------------------------------------------------------------------------------------------------------
 //
 // Tails, and prefixes whose sequences bring few pairs.  Warp 4 copies K and V tiles of 8 KB each.  Warps 0 to 3 compute, each a tile of its own for 16 of the item's pairs, with S, P and O
@@ -345,41 +389,23 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 
   if (warp == kPrefixWarps) {
     const bool issuer = elect_one();
-    const int boxes = KT / p.box, tpp = p.tokens_per_page;
     int piece = 0, tile = 0;  // (of all that the CTA goes through)
     uint32_t phase = 1;
     bool good = true;
     while (walk.next(s)) {
-      const int* pages = p.page_map + (long long)s.x.map * p.max_pages;
-      const int head_row = s.kvh * p.num_pages * tpp;
-      // lane i: the pool's row where box i of the item's tiles begins, counted from `tile`; boxes behind the last token: that token's page
-      auto row_of = [&](int tile) {
-        const int key = min(s.x.first + tile * KT + lane * p.box, s.x.key1 - 1);
-        const int page = pages[key / tpp];
-        return head_row + (page >= 0 && page < p.num_pages ? page : 0) * tpp + key % tpp / p.box * p.box;
-      };
-      // the 32 lanes look up as many boxes at a time, one round ahead
-      const int per = 32 / boxes;  // tiles of a round
-      int row = row_of(s.tile0), ahead = s.tile0 + per < s.tile1 ? row_of(s.tile0 + per) : 0;
-      for (int t = s.tile0, i = 0; t < s.tile1; ++t, ++tile) {
+      const PrefixRows rows(p, k, s, KT);
+      const int n = s.tile1 - s.tile0;
+      int round = rows.look_up(0), ahead = rows.look_up(1);
+      for (int i = 0; i < n; ++i, ++tile) {
+        if (i > 0 && i % rows.per == 0) round = ahead, ahead = rows.look_up(i / rows.per + 1);
         for (int kv = 0; kv < 2; ++kv) {
-          good = good && prefix_wait(&tail->empty[piece], phase, failed);
-          uint8_t* to = ring + piece * kPrefixPieceBytes;
+          good = __all_sync(0xffffffffu, good && prefix_wait(&tail->empty[piece], phase, failed));
           if (issuer && good) {
             mbar_expect_tx(&tail->full[piece], kPrefixPieceBytes);
             *const_cast<volatile int*>(&tail->armed[piece]) = tile;
           }
-          for (int b = 0; b < boxes; ++b) {
-            const int from = __shfl_sync(0xffffffffu, row, i * boxes + b);
-            if (issuer && good)
-              for (int c = 0; c < CH; ++c) tma_load_2d(to + c * KT * 128 + b * p.box * 128, kv == 0 ? &tm_k : &tm_v, c * 64, from, &tail->full[piece], kEvictNormal);
-          }
+          prefix_load_tile<CH>(rows, round, i, KT, ring + piece * kPrefixPieceBytes, kv == 0 ? &tm_k : &tm_v, &tail->full[piece], issuer && good);
           if (++piece == P) piece = 0, phase ^= 1;
-        }
-        if (++i == per) {
-          i = 0;
-          row = ahead;
-          ahead = t + 1 + per < s.tile1 ? row_of(t + 1 + per) : 0;
         }
       }
     }
@@ -654,29 +680,27 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 
 // ---- units of many rows on the tensor cores ------------------------------------------------------------------------------------------
 //
-// Prefixes whose sequences bring some hundred pairs.  Warp 0 copies K and V tiles, warp 1 issues the MMAs, four softmax warps have each 128 pairs of the item:
-//   S = Q K^T    tcgen05.mma, M = 128, N = KT, fp32 in TMEM
+// Prefixes whose sequences bring some hundred pairs.  Warp 0 copies queries and tiles of 64 tokens, warp 1 issues the MMAs, four softmax warps have each half of the item:
+//   S = Q K^T    tcgen05.mma, M = 128, N = 64, fp32 in TMEM
 //   P = exp2(..) a thread owns a pair: it reads its row of S, keeps maximum and sum in registers and writes P as bf16 over S
 //   O += P V     tcgen05.mma with P as the TMEM operand and V as an MN-major one, fp32 in TMEM
-// With two times 128 pairs the MMAs of one half run under the softmax of the other.  The accumulator is brought to a new maximum only when a pair's grew by more than 2^8.
+// Each half has two places for S: the next tile's is there before a softmax ends, so that neither waits for the other in turn (with one place of 128 tokens an item's tile of
+// 128 tokens took 3450 cycles: 2000 of softmax, 1000 of MMAs, the rest signals).  The accumulator is brought to a new maximum only when a pair's grew by more than 2^8.
+// Bound: MMAs, whose operands come from shared memory at 128 bytes a clock (of 256 pairs, 64 tokens and 128 channels 1280 cycles), and the special-function units (1024).
 
 template <int D>
 struct PrefixTcShape {
-  static constexpr int NQ = D == 256 ? 1 : 2, KT = D == 256 ? 64 : 128, CH = D / 64;
-  static constexpr int kPairs = NQ * 128;
+  static constexpr int NQ = D == 256 ? 1 : 2, KT = 64, CH = D / 64;
   static constexpr int kPieceBytes = KT * D * 2, kPieces = 131072 / kPieceBytes;
   static constexpr int kQBytes = 128 * D * 2;
-  static constexpr int kThreads = 128 + NQ * 128;  // a warpgroup of which two warps work, one or two of the softmax
-  static constexpr int kOCol = NQ * KT;
-  // registers at launch and after the split (two softmax warpgroups: 128 x 80 + 256 x 208 of 384 x 168)
-  static constexpr int kRegs = 168, kRegsCopy = 80, kRegsSoftmax = 208;
-  static_assert(NQ == 1 || 128 * kRegsCopy + NQ * 128 * kRegsSoftmax <= kThreads * kRegs, "a warpgroup would wait for registers for good");
+  static constexpr int kThreads = 64 + NQ * 128;
+  static constexpr int kOCol = NQ * 2 * KT;
 };
 
 struct PrefixTcTail {
   PrefixEntry entry[kPrefixCached + 1];
-  uint64_t full[8], empty[8];
-  uint64_t q_ready, s_full[2], p_ready[2], o_done[2];
+  uint64_t full[16], empty[16];
+  uint64_t q_full, q_empty, s_full[2][2], p_ready[2][2], o_done[2][2];
   PrefixBuild build;
   uint32_t tmem_base;
   int failed;
@@ -710,133 +734,23 @@ __device__ __forceinline__ float2 prefix_add2(float2 a, float2 b) {
   return d;
 }
 
+__device__ __forceinline__ void prefix_load_heads(void* dst, const CUtensorMap* tm, int c, int head, int row, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;"
+      :
+      : "r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(c), "r"(head), "r"(row), "l"(kEvictNormal)
+      : "memory");
+}
+
 // umma_desc_sw128 of a shared address
 __device__ __forceinline__ uint64_t prefix_desc(uint32_t addr) { return uint64_t((addr & 0x3FFFFu) >> 4) | uint64_t(1) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61; }
 
-// What the softmax warps do with a CTA's run.
-template <int D>
-__device__ __forceinline__ void prefix_softmax(const PrefixAttnParams& p, const PrefixWork& k, PrefixTcTail* tail, uint8_t* sq, uint32_t tmem, const PrefixEntry* table, const PrefixShare& share) {
-  typedef PrefixTcShape<D> F;
-  constexpr int KT = F::KT;
-  volatile int* failed = &tail->failed;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  PrefixSegment s;
-  PrefixWalk walk(k, table, share, blockIdx.x);
-  const int t = (warp - 4) >> 2, quarter = warp & 3, own = quarter * 32 + lane;
-  const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), acc = lanes + F::kOCol + t * D, scores = lanes + t * KT;
-  const float mul = p.softcap > 0.0f ? 1.0f : p.scale * kPrefixLog2e, cap = p.softcap * kPrefixLog2e, by_cap = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
-  uint32_t turn = 0, done = 0;
-  int segment = 0;
-  while (walk.next(s)) {
-    const int pair0 = s.block * F::kPairs + t * 128, pairs = s.x.rows * p.group - pair0;
-    // Q: a thread brings its pair's row
-    {
-      uint4 v[D / 8];
-      const int at = pair0 + own;
-      const bf16* from = p.q + (s.x.row + at / p.group) * p.ldq + (s.kvh * p.group + at % p.group) * D;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) v[c] = own < pairs ? reinterpret_cast<const uint4*>(from)[c] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(sq + t * F::kQBytes + (c >> 3) * 16384 + own * 128 + (((c & 7) ^ (own & 7)) << 4)) = v[c];
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tail->q_ready);
-    }
-    const int now_segment = segment++;
-    if (pairs <= 0) {  // (not two arrivals for one item)
-      prefix_wait(&tail->q_ready, now_segment & 1, failed);
-      continue;
-    }
-    float m = -INFINITY, l = 0.0f;  // the maximum that the accumulator stands at (times log2 e), the sum
-    for (int j = s.tile0; j < s.tile1; ++j) {
-      prefix_wait(&tail->s_full[t], turn, failed);
-      turn ^= 1;
-      tcgen05_fence_after();
-      float x[KT];
-      {
-        uint32_t raw[KT / 32][32];
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c) tmem_ld_x32(scores + c * 32, raw[c]);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < KT; ++c) x[c] = __uint_as_float(raw[c / 32][c % 32]);
-      }
-      if (p.softcap > 0.0f) {
-#pragma unroll
-        for (int c = 0; c < KT; ++c) x[c] = cap * tanhf(x[c] * by_cap);
-      }
-      const int beyond = s.x.key1 - (s.x.first + j * KT);
-      if (beyond < KT) {
-#pragma unroll
-        for (int c = 0; c < KT; ++c)
-          if (c >= beyond) x[c] = -INFINITY;
-      }
-      float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-      for (int c = 4; c + 7 < KT + 4; c += 8)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = c + 4 + i < KT ? fmaxf(mx[i], fmaxf(x[c + i], x[c + 4 + i])) : fmaxf(mx[i], x[c + i]);
-      const float now = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul);
-      if (__any_sync(0xffffffffu, now > m + 8.0f)) {  // (m = -inf: the first tile)
-        const float fix = now == -INFINITY ? 1.0f : prefix_ex2(m - now);
-        l *= fix;
-        m = now;
-        if (j > s.tile0) {  // the accumulator holds the tiles before: they are complete (s_full came behind them)
-#pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_ld_x32(acc + c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fix);
-            tmem_st_x32(acc + c, o);
-          }
-        }
-      }
-      const float base = m == -INFINITY ? 0.0f : m;
-      const float2 mul2 = make_float2(mul, mul), base2 = make_float2(-base, -base);
-      float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-      for (int c = 0; c < KT; c += 32) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 w = prefix_fma2(make_float2(x[c + 2 * e], x[c + 2 * e + 1]), mul2, base2);
-          w.x = prefix_ex2(w.x);
-          w.y = prefix_ex2(w.y);
-          sums[e & 1] = prefix_add2(sums[e & 1], w);
-          pk[e] = pack_bf16x2(w.x, w.y);
-        }
-        tmem_st_x16(scores + c / 2, pk);
-      }
-      l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-      tmem_wait_st();
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tail->p_ready[t]);
-    }
-    prefix_wait(&tail->o_done[t], done, failed);
-    done ^= 1;
-    tcgen05_fence_after();
-    const long long place = s.place + t * 128 + own;
-#pragma unroll 1
-    for (int c = 0; c < D; c += 32) {
-      uint32_t o[32];
-      tmem_ld_x32(acc + c, o);
-      tmem_wait_ld();
-      if (own < pairs) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(k.part + place * D + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-      }
-    }
-    if (own < pairs) k.stat[place] = make_float2(m, l);
-    tcgen05_fence_before();
-  }
-}
+// pairs of a half of an item: as many whole rows as fit
+__device__ __forceinline__ int prefix_half(int group) { return 128 / group * group; }
 
-template <int D>
+template <int D, bool CAP>
 __global__ void __launch_bounds__(PrefixTcShape<D>::kThreads, 1)
-prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PrefixAttnParams p, const PrefixWork k) {
+prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PrefixAttnParams p, const PrefixWork k) {
   typedef PrefixTcShape<D> F;
   constexpr int NQ = F::NQ, KT = F::KT, CH = F::CH;
   extern __shared__ uint8_t smem_raw[];
@@ -844,20 +758,24 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   uint8_t* ring = sq + NQ * F::kQBytes;                                         // piece: [CH][KT tokens][128 B]
   PrefixTcTail* tail = reinterpret_cast<PrefixTcTail*>(ring + F::kPieces * F::kPieceBytes);
   volatile int* failed = &tail->failed;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = prefix_half(p.group);
 
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
     for (int i = 0; i < F::kPieces; ++i) {
       mbar_init(&tail->full[i], 1);
       mbar_init(&tail->empty[i], 1);
     }
-    mbar_init(&tail->q_ready, NQ * 4);
+    mbar_init(&tail->q_full, 1);
+    mbar_init(&tail->q_empty, 1);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&tail->s_full[t], 1);
-      mbar_init(&tail->p_ready[t], 4);  // one arrival per softmax warp
-      mbar_init(&tail->o_done[t], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&tail->s_full[t][b], 1);
+        mbar_init(&tail->p_ready[t][b], 4);  // one arrival per softmax warp
+        mbar_init(&tail->o_done[t][b], 1);   // (two: a wait for a tile's products may come while those of the tile before are not done)
+      }
     }
     tail->failed = 0;
     fence_barrier_init();
@@ -884,50 +802,52 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
   const bool mine = int(blockIdx.x) < share.workers;
   PrefixSegment s;
 
-  if (warp < 4) {
-    if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::kRegsCopy));
-    if (!mine || warp >= 2) {
-    } else if (warp == 0) {
+  if (!mine) {
+  } else if (warp == 0) {
     PrefixWalk walk(k, table, share, blockIdx.x);
     const bool issuer = elect_one();
-    const int boxes = KT / p.box, tpp = p.tokens_per_page;
     int piece = 0;
-    uint32_t phase = 1;
+    uint32_t phase = 1, q_phase = 1;
     bool good = true;
+    auto advance = [&]() {
+      if (++piece == F::kPieces) piece = 0, phase ^= 1;
+    };
     while (walk.next(s)) {
-      const int* pages = p.page_map + (long long)s.x.map * p.max_pages;
-      const long long head_row = (long long)s.kvh * p.num_pages * tpp;
-      auto row_of = [&](int tile) {  // as in prefix_units_kernel
-        const int key = min(s.x.first + tile * KT + (lane < boxes ? lane : 0) * p.box, s.x.key1 - 1);
-        const int page = pages[key / tpp];
-        return int(head_row + (long long)(page >= 0 && page < p.num_pages ? page : 0) * tpp + key % tpp / p.box * p.box);
+      const PrefixRows rows(p, k, s, KT);
+      const int n = s.tile1 - s.tile0, halves = NQ == 2 && s.x.rows * p.group - s.block * k.pairs > half ? 2 : 1;
+      int round[3] = {rows.look_up(0), rows.look_up(1), rows.look_up(2)};  // of V's tile, and the next two
+      auto load = [&](const CUtensorMap* tm, int at, int tile) {
+        good = __all_sync(0xffffffffu, good && prefix_wait(&tail->empty[piece], phase, failed));
+        if (issuer && good) mbar_expect_tx(&tail->full[piece], F::kPieceBytes);
+        prefix_load_tile<CH>(rows, at, tile, KT, ring + piece * F::kPieceBytes, tm, &tail->full[piece], issuer && good);
+        advance();
       };
-      int row = row_of(s.tile0);
-      for (int t = s.tile0; t < s.tile1; ++t) {
-        const int next = t + 1 < s.tile1 ? row_of(t + 1) : 0;
-        for (int kv = 0; kv < 2; ++kv) {
-          good = good && prefix_wait(&tail->empty[piece], phase, failed);
-          uint8_t* to = ring + piece * F::kPieceBytes;
-          if (issuer && good) mbar_expect_tx(&tail->full[piece], F::kPieceBytes);
-          for (int b = 0; b < boxes; ++b) {
-            const int from = __shfl_sync(0xffffffffu, row, b);
-            if (issuer && good)
-              for (int c = 0; c < CH; ++c) tma_load_2d(to + c * KT * 128 + b * p.box * 128, kv == 0 ? &tm_k : &tm_v, c * 64, from, &tail->full[piece], kEvictNormal);
-          }
-          if (++piece == F::kPieces) piece = 0, phase ^= 1;
-        }
-        row = next;
+      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->q_empty, q_phase, failed));
+      q_phase ^= 1;
+      if (issuer && good) {
+        mbar_expect_tx(&tail->q_full, uint32_t(halves * CH * half * 128));
+        for (int t = 0; t < halves; ++t)
+          for (int c = 0; c < CH; ++c)
+            prefix_load_heads(sq + t * F::kQBytes + c * 16384, &tm_q, c * 64, s.kvh * p.group, s.x.row + (s.block * k.pairs + t * half) / p.group, &tail->q_full);
+      }
+      load(&tm_k, round[0], 0);
+      if (n > 1) load(&tm_k, round[0], 1);
+      for (int i = 0; i < n; ++i) {  // as the MMAs take them: V of a tile, then K of the next but one
+        if (i > 0 && i % rows.per == 0) round[0] = round[1], round[1] = round[2], round[2] = rows.look_up(i / rows.per + 2);
+        load(&tm_v, round[0], i);
+        if (i + 2 < n) load(&tm_k, (i + 2) / rows.per == i / rows.per ? round[0] : round[1], i + 2);
       }
     }
     for (int i = 0; i < F::kPieces; ++i) {  // the MMAs' arrivals have to be in before the CTA may leave
       good = good && prefix_wait(&tail->empty[piece], phase, failed);
-      if (++piece == F::kPieces) piece = 0, phase ^= 1;
+      advance();
     }
+    good = good && prefix_wait(&tail->q_empty, q_phase, failed);
     if (!good) {  // copies and MMAs in flight have a millisecond to end
       const long long t0 = clock64();
       while (clock64() - t0 < 2000000) __nanosleep(1000);
     }
-    } else {
+  } else if (warp == 1) {
     PrefixWalk walk(k, table, share, blockIdx.x);
     const bool issuer = elect_one();
     // numbers that the compiler takes for the same in all lanes: otherwise it brings every operand of every MMA to where the MMA reads it by itself (16 MMAs 1550 cycles, 950 so)
@@ -936,74 +856,177 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant
     const uint32_t idesc_s = umma_idesc_bf16(128, KT), idesc_o = umma_idesc_bf16(128, D) | kIdescBMajorMN;
     const uint64_t dq = prefix_desc(uint32_t(same(int(smem_u32(sq))))), dk = prefix_desc(ring_addr);
     bool good = true;
-    auto issue_s = [&](int t, int piece) {
+    int piece = 0;
+    uint32_t phase = 0, q_phase = 0, p_phase = 0;  // p_phase: bit 2 t + b
+    auto issue_s = [&](int t, int b, int from) {
       if (!issuer || !good) return;
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_bf16(tmem_at + t * KT, dq + uint64_t((t * F::kQBytes + c * 16384 + kk * 32) >> 4), dk + uint64_t((piece * F::kPieceBytes + c * KT * 128 + kk * 32) >> 4), idesc_s,
+          umma_bf16(tmem_at + (t * 2 + b) * KT, dq + uint64_t((t * F::kQBytes + c * 16384 + kk * 32) >> 4), dk + uint64_t((from * F::kPieceBytes + c * KT * 128 + kk * 32) >> 4), idesc_s,
                     uint32_t((c | kk) != 0));
-      umma_commit(&tail->s_full[t]);
+      umma_commit(&tail->s_full[t][b]);
     };
-    auto issue_o = [&](int t, int piece, bool start) {
+    auto issue_o = [&](int t, int b, int from, bool start) {
       if (!issuer || !good) return;
 #pragma unroll
       for (int kk = 0; kk < KT / 16; ++kk)
-        umma_bf16_ts(tmem_at + F::kOCol + t * D, tmem_at + t * KT + kk * 8, umma_desc_sw128_mn(ring_addr + piece * F::kPieceBytes + kk * 2048, KT * 128), idesc_o, uint32_t(!start || kk != 0));
+        umma_bf16_ts(tmem_at + F::kOCol + t * D, tmem_at + (t * 2 + b) * KT + kk * 8, umma_desc_sw128_mn(ring_addr + from * F::kPieceBytes + kk * 2048, KT * 128), idesc_o,
+                     uint32_t(!start || kk != 0));
+      umma_commit(&tail->o_done[t][b]);
     };
-    int piece = 0, segment = 0;  // pieces: K, V, K, V ..
-    uint32_t phase = 0, turn[2] = {0, 0};
-    auto advance = [&]() {
+    auto arrived = [&]() {  // the next piece is there
+      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->full[piece], phase, failed));
       const int at = piece;
       if (++piece == F::kPieces) piece = 0, phase ^= 1;
       return at;
     };
+    auto used = [&](uint64_t* bar) {
+      if (issuer && good) umma_commit(bar);
+    };
     while (walk.next(s)) {
-      const int halves = same(NQ == 2 && s.x.rows * p.group - s.block * F::kPairs > 128 ? 2 : 1), tile0 = same(s.tile0), tile1 = same(s.tile1), key1 = same(s.x.key1), first = same(s.x.first);
-      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->q_ready, segment & 1, failed));
-      ++segment;
-      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->full[piece], phase, failed));
-      tcgen05_fence_after();
-      int at = advance();
-      for (int t = 0; t < halves; ++t) issue_s(t, at);
-      if (issuer && good) umma_commit(&tail->empty[at]);
-      for (int j = tile0; j < tile1; ++j) {
-        const bool more = j + 1 < tile1;
-        good = __all_sync(0xffffffffu, good && prefix_wait(&tail->full[piece], phase, failed));
-        const int v_at = advance();
-        const int beyond = key1 - (first + j * KT);  // the tile's first token that the prefix does not have
-        if (beyond < KT) {                                 // it may hold anything, and 0 * NaN is not 0
+      const int halves = same(NQ == 2 && s.x.rows * p.group - s.block * k.pairs > half ? 2 : 1), n = same(s.tile1 - s.tile0), beyond = same(s.x.key1 - s.x.first - s.tile0 * KT);
+      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->q_full, q_phase, failed));
+      q_phase ^= 1;
+      for (int i = 0; i < 2 && i < n; ++i) {
+        const int at = arrived();
+        tcgen05_fence_after();
+        for (int t = 0; t < halves; ++t) issue_s(t, i, at);
+        used(&tail->empty[at]);
+      }
+      if (n <= 2) used(&tail->q_empty);
+      for (int i = 0; i < n; ++i) {
+        const int b = i & 1, v_at = arrived();
+        if (beyond - i * KT < KT) {  // tokens that the prefix does not have: V may hold anything, and 0 * NaN is not 0
           uint8_t* v = ring + v_at * F::kPieceBytes;
           for (int c = 0; c < CH; ++c)
-            for (int b = beyond * 128 + lane * 16; b < KT * 128; b += 512) *reinterpret_cast<uint4*>(v + c * KT * 128 + b) = make_uint4(0, 0, 0, 0);
+            for (int at = (beyond - i * KT) * 128 + lane * 16; at < KT * 128; at += 512) *reinterpret_cast<uint4*>(v + c * KT * 128 + at) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
           __syncwarp();
         }
-        int k_at = 0;
-        if (more) {
-          good = __all_sync(0xffffffffu, good && prefix_wait(&tail->full[piece], phase, failed));
-          k_at = advance();
-        }
+        const bool more = i + 2 < n;
+        const int k_at = more ? arrived() : 0;
         for (int t = 0; t < halves; ++t) {
-          good = __all_sync(0xffffffffu, good && prefix_wait(&tail->p_ready[t], turn[t], failed));
-          turn[t] ^= 1;
+          const int bit = t * 2 + b;
+          good = __all_sync(0xffffffffu, good && prefix_wait(&tail->p_ready[t][b], p_phase >> bit & 1, failed));
+          p_phase ^= 1u << bit;
           tcgen05_fence_after();
-          issue_o(t, v_at, j == tile0);
-          if (more) issue_s(t, k_at);
-          else if (issuer && good) umma_commit(&tail->o_done[t]);
+          issue_o(t, b, v_at, i == 0);
+          if (more) issue_s(t, b, k_at);
         }
-        if (issuer && good) {
-          umma_commit(&tail->empty[v_at]);
-          if (more) umma_commit(&tail->empty[k_at]);
-        }
+        used(&tail->empty[v_at]);
+        if (more) used(&tail->empty[k_at]);
+        if (i + 3 == n) used(&tail->q_empty);
       }
     }
     __syncwarp();
-    }
   } else {
-    if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::kRegsSoftmax));
-    if (mine) prefix_softmax<D>(p, k, tail, sq, tmem, table, share);
+    PrefixWalk walk(k, table, share, blockIdx.x);
+    const int t = (warp - 2) >> 2, quarter = warp & 3, own = quarter * 32 + lane;
+    const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), acc = lanes + F::kOCol + t * D;
+    const float mul = CAP ? 1.0f : p.scale * kPrefixLog2e, cap = p.softcap * kPrefixLog2e, by_cap = CAP ? p.scale / p.softcap : 0.0f;
+    const float2 mul2 = make_float2(mul, mul);
+    uint32_t s_phase = 0;  // bit b
+    uint32_t o_phase = 0;  // the same of the products
+    while (walk.next(s)) {
+      const int all = min(k.pairs, s.x.rows * p.group - s.block * k.pairs), pairs = min(half, all - t * half);  // of the item, of this half
+      if (pairs <= 0) continue;
+      const bool valid = own < pairs;
+      float m = -INFINITY, l = 0.0f;  // the maximum that the accumulator stands at (times log2 e), the sum
+      const int n = s.tile1 - s.tile0;
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const int b = i & 1;
+        const uint32_t scores = lanes + (t * 2 + b) * KT;
+        prefix_wait(&tail->s_full[t][b], s_phase >> b & 1, failed);
+        s_phase ^= 1u << b;
+        tcgen05_fence_after();
+        float x[KT];
+        {
+          uint32_t raw[KT / 32][32];
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c) tmem_ld_x32(scores + c * 32, raw[c]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < KT; ++c) x[c] = __uint_as_float(raw[c / 32][c % 32]);
+        }
+        if (CAP) {
+#pragma unroll
+          for (int c = 0; c < KT; ++c) x[c] = cap * tanhf(x[c] * by_cap);
+        }
+        const int beyond = s.x.key1 - s.x.first - (s.tile0 + i) * KT;
+        if (beyond < KT) {
+#pragma unroll
+          for (int c = 0; c < KT; ++c)
+            if (c >= beyond) x[c] = -INFINITY;
+        }
+        float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int c = 4; c + 8 <= KT; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(x[c + e], x[c + 4 + e]));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[KT - 4 + e]);
+        const float now = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul);
+        if (__any_sync(0xffffffffu, valid && now > m + 8.0f)) {  // (m = -inf: the first tile)
+          const float fix = now == -INFINITY ? 1.0f : prefix_ex2(m - now);
+          l *= fix;
+          m = now;
+          if (i > 0) {  // the accumulator holds the tiles before
+            prefix_wait(&tail->o_done[t][b ^ 1], ~o_phase >> (b ^ 1) & 1, failed);
+            tcgen05_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld_x32(acc + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fix);
+              tmem_st_x32(acc + c, o);
+            }
+          }
+        }
+        o_phase ^= 1u << b;
+        const float base = m == -INFINITY ? 0.0f : m;
+        const float2 base2 = make_float2(-base, -base);
+        float2 sums[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for (int c = 0; c < KT; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float2 w = prefix_fma2(make_float2(x[c + 2 * e], x[c + 2 * e + 1]), mul2, base2);
+            w.x = prefix_ex2(w.x);
+            w.y = prefix_ex2(w.y);
+            sums[e & 1] = prefix_add2(sums[e & 1], w);
+            pk[e] = pack_bf16x2(w.x, w.y);
+          }
+          tmem_st_x16(scores + c / 2, pk);
+        }
+        l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+        tmem_wait_st();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tail->p_ready[t][b]);
+      }
+      prefix_wait(&tail->o_done[t][(n - 1) & 1], ~o_phase >> ((n - 1) & 1) & 1, failed);
+      tcgen05_fence_after();
+      // the item's results [D / 4][pairs][4]: neighbouring lanes store side by side (a row of each lane of its own took 7200 cycles, most of them the stores' 128-byte lines)
+      float* out = k.part + s.place * D + (t * half + own) * 4;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_ld_x32(acc + c, o);
+        tmem_wait_ld();
+        if (valid) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(out + (long long)(c + e) * all) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      if (valid) k.stat[s.place + t * half + own] = make_float2(m, l);
+      tcgen05_fence_before();
+    }
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -1046,11 +1069,11 @@ __global__ void __launch_bounds__(kPrefixJoinMost) prefix_join_kernel(const Pref
   for (int i0 = 0; i0 < most; i0 += blockDim.x) {  // (one round where blockDim.x threads have all heads)
     const int i = i0 + threadIdx.x, g = min(i / lanes, p.group - 1), c = i % lanes * 8;
     const bool mine = i < most;
-    long long place[2];
-    int parts[2];
+    long long place[2], value[2];  // of the first part's statistics, and of its values from channel c on
+    int parts[2], step[2];         // between those and the next four channels
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      place[k] = parts[k] = 0;
+      place[k] = value[k] = parts[k] = 0, step[k] = 4;
       const PrefixWork& w = k == 0 ? a : b;
       const PrefixEntry &x = k == 0 ? front : tail, &last = found[2 + k];
       if ((k == 0 && tail.prefix < 0) || x.tiles == 0) continue;
@@ -1058,6 +1081,12 @@ __global__ void __launch_bounds__(kPrefixJoinMost) prefix_join_kernel(const Pref
       const PrefixShare share(last.units * p.kv_heads, w.workers);
       const int c0 = share.of(first), c1 = share.of(first + x.tiles - 1);
       place[k] = (long long)kvh * last.pairs + x.pairs + at + (long long)c0 * w.pairs;
+      value[k] = place[k] * D + c;
+      if (w.mixed) {
+        const int pair = at % w.pairs, all = min(w.pairs, x.rows * p.group - (at - pair));
+        value[k] = (place[k] - pair) * D + pair * 4 + (long long)c * all;
+        step[k] = 4 * all;
+      }
       parts[k] = c1 - c0 + 1;
     }
     const bool written = tail.key0 == 0 && parts[1] == 1;  // already
@@ -1071,11 +1100,11 @@ __global__ void __launch_bounds__(kPrefixJoinMost) prefix_join_kernel(const Pref
       for (int n = 0; n < N; ++n) {
         const int j = min(j0 + n * int(blockDim.y), all - 1);
         const bool of_tail = j >= parts[0];
-        const long long at = of_tail ? place[1] + (long long)(j - parts[0]) * b.pairs : place[0] + (long long)j * a.pairs;
-        const float4* from = reinterpret_cast<const float4*>((of_tail ? b.part : a.part) + at * D + c);
-        st[n] = (of_tail ? b.stat : a.stat)[at];
-        v[n][0] = from[0];
-        v[n][1] = from[1];
+        const long long off = of_tail ? (long long)(j - parts[0]) * b.pairs : (long long)j * a.pairs;
+        const float* from = of_tail ? b.part + value[1] + off * D : a.part + value[0] + off * D;
+        st[n] = of_tail ? b.stat[place[1] + off] : a.stat[place[0] + off];
+        v[n][0] = *reinterpret_cast<const float4*>(from);
+        v[n][1] = *reinterpret_cast<const float4*>(from + (of_tail ? step[1] : step[0]));
       }
       float now = top;
 #pragma unroll

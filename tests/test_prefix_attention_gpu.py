@@ -298,3 +298,14 @@ def test_as_paged_attention():
                                      c.num_pages, 16, c.maps.shape[1], 0.0, scratch.data_ptr(), torch.cuda.current_stream().cuda_stream))
   _, bound = c.want()
   assert bool(((out.double() - got).abs().view_as(bound) <= 2 * bound).all())
+
+
+@pytest.mark.parametrize("dim,heads,kv", [(64, 20, 4), (128, 16, 4), (256, 8, 4), (128, 6, 1), (64, 32, 2)])
+def test_long_prefixes(dim, heads, kv):
+  """Many tiles of each item in a CTA, several items of it, halves that are not full; more than once, since what is not waited for may come in time by chance."""
+  g = torch.Generator().manual_seed(heads)
+  rows = torch.randint(1, 6, (48,), generator=g).tolist()
+  c = Case(rows, [5001 + n + int(t) for n, t in zip(rows, torch.randint(0, 90, (48,), generator=g))], [(0, 48, 5001)], heads=heads, kv=kv, dim=dim, page=64, seed=dim)
+  first = c.check()
+  for _ in range(5):
+    assert torch.equal(c.run().double().view_as(first), first)
