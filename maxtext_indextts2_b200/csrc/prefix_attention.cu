@@ -9,6 +9,8 @@ constexpr int kPrefixSms = 148;
 constexpr int kPrefixWorkers = 2 * kPrefixSms;  // most CTAs of prefix_units_kernel
 constexpr int kPrefixTcPairs = 256;             // most pairs of an item of prefix_tc_kernel
 
+int bits_of(int power_of_two) { return __builtin_ctz(unsigned(power_of_two)); }
+
 // Prefixes go to the tensor cores' kernel when their sequences bring at least 64 pairs on the average.
 bool prefix_on_tc(int rows, int prefixes, int group) { return prefixes > 0 && (long long)rows * group >= 64ll * prefixes; }
 
@@ -73,7 +75,9 @@ int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
     w[k].kt = k == 0 ? Tc::KT : KT;
     w[k].pairs = k == 0 ? Tc::NQ * (128 / p.group * p.group) : kPrefixPairs;
     w[k].mixed = k == 0;
-    w[k].box = p.tokens_per_page < w[k].kt ? p.tokens_per_page : w[k].kt;
+    const int box = p.tokens_per_page < w[k].kt ? p.tokens_per_page : w[k].kt;
+    w[k].box_bits = bits_of(box);
+    w[k].round_bits = bits_of(32 * box / w[k].kt);
     w[k].workers = k == 0 ? kPrefixSms : PrefixShape<D>::kCtas * kPrefixSms;
     w[k].tabled = (k == 1 || tc) && w[k].count > kPrefixCached;
     w[k].table = reinterpret_cast<PrefixEntry*>(scratch + at.table[k]);
@@ -83,9 +87,9 @@ int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
   CUtensorMap tk[2], tv[2];
   const uint64_t pool = uint64_t(p.kv_heads) * p.num_pages * p.tokens_per_page;
   for (int k = tc ? 0 : 1; k < 2; ++k) {
-    const int chunks = w[k].box == w[k].kt ? D / 64 : 1;
-    MTX_TRY(make_map_pool(&tk[k], p.k, D, pool, w[k].box, chunks));
-    MTX_TRY(make_map_pool(&tv[k], p.v, D, pool, w[k].box, chunks));
+    const int box = 1 << w[k].box_bits, chunks = box == w[k].kt ? D / 64 : 1;
+    MTX_TRY(make_map_pool(&tk[k], p.k, D, pool, box, chunks));
+    MTX_TRY(make_map_pool(&tv[k], p.v, D, pool, box, chunks));
   }
   if (w[0].tabled || w[1].tabled) MTX_TRY(launch(prefix_plan_kernel, dim3(1), dim3(1024), 0, st, p, w[0], w[1]));
   if (tc) {
@@ -157,6 +161,7 @@ int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, cons
   p.group = num_q_heads / num_kv_heads;
   p.num_pages = num_pages;
   p.tokens_per_page = tokens_per_page;
+  p.page_bits = bits_of(tokens_per_page);
   p.max_pages = max_pages_per_group;
   p.scale = scale;
   p.softcap = softcap;

@@ -21,7 +21,7 @@ struct PrefixAttnParams {
   long long ldo;
   int rows, sequences, prefixes;
   const int *row0, *lengths, *page_map, *prefix_seq0, *prefix_len;
-  int heads, kv_heads, group, num_pages, tokens_per_page, max_pages;
+  int heads, kv_heads, group, num_pages, tokens_per_page, page_bits, max_pages;
   float scale, softcap;
   int box;  // tokens of a copy of the tails' kernel: a page, or a part of one, at most a tile (tiles begin at its multiples)
 };
@@ -30,7 +30,8 @@ struct PrefixAttnParams {
 struct PrefixWork {
   int first, count;  // the entries: prefixes, then sequences
   int kt, pairs;     // tokens of a tile, pairs of an item
-  int box;           // tokens of a copy
+  int box_bits;      // log2 of the tokens of a copy
+  int round_bits;    // log2 of the tiles whose copies 32 lanes look up
   int workers;       // CTAs that share the units, at most
   int tabled;        // the table is there already (more entries than a CTA keeps)
   int mixed;         // an item's weighted values lie as [D / 4][pairs][4], not [pairs][D]
@@ -250,18 +251,20 @@ __device__ __forceinline__ bool prefix_whole(const PrefixSegment& s) { return s.
 // Where the boxes of an item's tiles lie in the pool: the 32 lanes look up as many boxes at a time.
 struct PrefixRows {
   const int* pages;
-  int head_row, num_pages, tpp, box, boxes, per, first, last, lane;
+  int head_row, num_pages, page_bits, box_bits, boxes, per, first, last, lane;  // (pages, boxes, boxes of a tile and tiles of a round are powers of two: a division in a tile's way takes 100 cycles)
 
   __device__ __forceinline__ PrefixRows(const PrefixAttnParams& p, const PrefixWork& k, const PrefixSegment& s, int kt)
-      : pages(p.page_map + (long long)s.x.map * p.max_pages), head_row(s.kvh * p.num_pages * p.tokens_per_page), num_pages(p.num_pages), tpp(p.tokens_per_page), box(k.box), boxes(kt / k.box),
-        per(32 / boxes), first(s.x.first + s.tile0 * kt), last(s.x.key1 - 1), lane(threadIdx.x & 31) {}
-  // round r: lane i has box i of the tiles from r * per on; boxes behind the last token: that token's page
+      : pages(p.page_map + (long long)s.x.map * p.max_pages), head_row(s.kvh * p.num_pages * p.tokens_per_page), num_pages(p.num_pages), page_bits(p.page_bits),
+        box_bits(k.box_bits), boxes(kt >> k.box_bits), per(k.round_bits), first(s.x.first + s.tile0 * kt), last(s.x.key1 - 1), lane(threadIdx.x & 31) {}
+  __device__ __forceinline__ int round_of(int t) const { return t >> per; }
+  __device__ __forceinline__ bool begins_round(int t) const { return (t & ((1 << per) - 1)) == 0; }
+  // round r: lane i has box i of the round's tiles; boxes behind the last token: that token's page
   __device__ __forceinline__ int look_up(int r) const {
-    const int key = min(first + (r * 32 + lane) * box, last), page = pages[key / tpp];
-    return head_row + (page >= 0 && page < num_pages ? page : 0) * tpp + key % tpp / box * box;
+    const int key = min(first + ((r * 32 + lane) << box_bits), last), page = pages[key >> page_bits], in = key & ((1 << page_bits) - 1);
+    return head_row + ((page >= 0 && page < num_pages ? page : 0) << page_bits) + (in >> box_bits << box_bits);
   }
   // of a round: the row of tile t's box b, the same in all lanes as the compiler sees it
-  __device__ __forceinline__ int row(int round, int t, int b) const { return __reduce_max_sync(0xffffffffu, lane == t % per * boxes + b ? round : int(0x80000000)); }
+  __device__ __forceinline__ int row(int round, int t, int b) const { return __reduce_max_sync(0xffffffffu, lane == (t & ((1 << per) - 1)) * boxes + b ? round : int(0x80000000)); }
 };
 
 // A box [CH][box tokens][128 B], or one chunk of channels of it
@@ -282,7 +285,7 @@ __device__ __forceinline__ void prefix_load_tile(const PrefixRows& rows, int rou
     if (rows.boxes == 1) {
       prefix_load_box(to, tm, from, 0, bar);
     } else {
-      for (int c = 0; c < CH; ++c) prefix_load_box(to + c * kt * 128 + b * rows.box * 128, tm, from, c, bar);
+      for (int c = 0; c < CH; ++c) prefix_load_box(to + c * kt * 128 + (b << rows.box_bits) * 128, tm, from, c, bar);
     }
   }
 }
@@ -397,7 +400,7 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       const int n = s.tile1 - s.tile0;
       int round = rows.look_up(0), ahead = rows.look_up(1);
       for (int i = 0; i < n; ++i, ++tile) {
-        if (i > 0 && i % rows.per == 0) round = ahead, ahead = rows.look_up(i / rows.per + 1);
+        if (i > 0 && rows.begins_round(i)) round = ahead, ahead = rows.look_up(rows.round_of(i) + 1);
         for (int kv = 0; kv < 2; ++kv) {
           good = __all_sync(0xffffffffu, good && prefix_wait(&tail->empty[piece], phase, failed));
           if (issuer && good) {
@@ -693,7 +696,7 @@ struct PrefixTcShape {
   static constexpr int NQ = D == 256 ? 1 : 2, KT = 64, CH = D / 64;
   static constexpr int kPieceBytes = KT * D * 2, kPieces = 131072 / kPieceBytes;
   static constexpr int kQBytes = 128 * D * 2;
-  static constexpr int kThreads = 64 + NQ * 128;
+  static constexpr int kThreads = 32 * (1 + NQ + 4 * NQ);  // a warp that copies, one that issues MMAs for each half, four of the softmax for each
   static constexpr int kOCol = NQ * 2 * KT;
 };
 
@@ -742,6 +745,19 @@ __device__ __forceinline__ void prefix_load_heads(void* dst, const CUtensorMap* 
       : "memory");
 }
 
+// whether a phase is over, without waiting for it
+__device__ __forceinline__ bool prefix_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // umma_desc_sw128 of a shared address
 __device__ __forceinline__ uint64_t prefix_desc(uint32_t addr) { return uint64_t((addr & 0x3FFFFu) >> 4) | uint64_t(1) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61; }
 
@@ -766,10 +782,10 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     tma_prefetch_desc(&tm_v);
     for (int i = 0; i < F::kPieces; ++i) {
       mbar_init(&tail->full[i], 1);
-      mbar_init(&tail->empty[i], 1);
+      mbar_init(&tail->empty[i], NQ);
     }
     mbar_init(&tail->q_full, 1);
-    mbar_init(&tail->q_empty, 1);
+    mbar_init(&tail->q_empty, NQ);
     for (int t = 0; t < 2; ++t) {
       for (int b = 0; b < 2; ++b) {
         mbar_init(&tail->s_full[t][b], 1);
@@ -833,9 +849,9 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       load(&tm_k, round[0], 0);
       if (n > 1) load(&tm_k, round[0], 1);
       for (int i = 0; i < n; ++i) {  // as the MMAs take them: V of a tile, then K of the next but one
-        if (i > 0 && i % rows.per == 0) round[0] = round[1], round[1] = round[2], round[2] = rows.look_up(i / rows.per + 2);
+        if (i > 0 && rows.begins_round(i)) round[0] = round[1], round[1] = round[2], round[2] = rows.look_up(rows.round_of(i) + 2);
         load(&tm_v, round[0], i);
-        if (i + 2 < n) load(&tm_k, (i + 2) / rows.per == i / rows.per ? round[0] : round[1], i + 2);
+        if (i + 2 < n) load(&tm_k, rows.round_of(i + 2) == rows.round_of(i) ? round[0] : round[1], i + 2);
       }
     }
     for (int i = 0; i < F::kPieces; ++i) {  // the MMAs' arrivals have to be in before the CTA may leave
@@ -847,57 +863,73 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const long long t0 = clock64();
       while (clock64() - t0 < 2000000) __nanosleep(1000);
     }
-  } else if (warp == 1) {
+  } else if (warp <= NQ) {
     PrefixWalk walk(k, table, share, blockIdx.x);
     const bool issuer = elect_one();
     // numbers that the compiler takes for the same in all lanes: otherwise it brings every operand of every MMA to where the MMA reads it by itself (16 MMAs 1550 cycles, 950 so)
     auto same = [](int x) { return __reduce_max_sync(0xffffffffu, x); };
-    const uint32_t tmem_at = uint32_t(same(int(tmem))), ring_addr = uint32_t(same(int(smem_u32(ring))));
+    const int t = same(warp - 1);
+    const uint32_t tmem_at = uint32_t(same(int(tmem))), ring_addr = uint32_t(same(int(smem_u32(ring)))), s_at = tmem_at + t * 2 * KT, o_at = tmem_at + F::kOCol + t * D;
     const uint32_t idesc_s = umma_idesc_bf16(128, KT), idesc_o = umma_idesc_bf16(128, D) | kIdescBMajorMN;
-    const uint64_t dq = prefix_desc(uint32_t(same(int(smem_u32(sq))))), dk = prefix_desc(ring_addr);
+    const uint64_t dq = prefix_desc(uint32_t(same(int(smem_u32(sq)))) + t * F::kQBytes), dk = prefix_desc(ring_addr);
     bool good = true;
     int piece = 0;
-    uint32_t phase = 0, q_phase = 0, p_phase = 0;  // p_phase: bit 2 t + b
-    auto issue_s = [&](int t, int b, int from) {
-      if (!issuer || !good) return;
+    uint32_t phase = 0, q_phase = 0, p_phase = 0;  // p_phase: bit b
+    // by the issuing lane
+    auto issue_s = [&](int b, int from) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_bf16(tmem_at + (t * 2 + b) * KT, dq + uint64_t((t * F::kQBytes + c * 16384 + kk * 32) >> 4), dk + uint64_t((from * F::kPieceBytes + c * KT * 128 + kk * 32) >> 4), idesc_s,
-                    uint32_t((c | kk) != 0));
+          umma_bf16(s_at + b * KT, dq + uint64_t((c * 16384 + kk * 32) >> 4), dk + uint64_t((from * F::kPieceBytes + c * KT * 128 + kk * 32) >> 4), idesc_s, uint32_t((c | kk) != 0));
       umma_commit(&tail->s_full[t][b]);
+      umma_commit(&tail->empty[from]);
     };
-    auto issue_o = [&](int t, int b, int from, bool start) {
-      if (!issuer || !good) return;
+    auto issue_o = [&](int b, int from, bool start) {
 #pragma unroll
       for (int kk = 0; kk < KT / 16; ++kk)
-        umma_bf16_ts(tmem_at + F::kOCol + t * D, tmem_at + (t * 2 + b) * KT + kk * 8, umma_desc_sw128_mn(ring_addr + from * F::kPieceBytes + kk * 2048, KT * 128), idesc_o,
-                     uint32_t(!start || kk != 0));
+        umma_bf16_ts(o_at, s_at + b * KT + kk * 8, umma_desc_sw128_mn(ring_addr + from * F::kPieceBytes + kk * 2048, KT * 128), idesc_o, uint32_t(!start || kk != 0));
       umma_commit(&tail->o_done[t][b]);
+      umma_commit(&tail->empty[from]);
     };
-    auto arrived = [&]() {  // the next piece is there
-      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->full[piece], phase, failed));
+    auto next = [&](uint32_t& at_phase) {  // the next piece
       const int at = piece;
+      at_phase = phase;
       if (++piece == F::kPieces) piece = 0, phase ^= 1;
       return at;
     };
-    auto used = [&](uint64_t* bar) {
-      if (issuer && good) umma_commit(bar);
-    };
+    auto wait = [&](uint64_t* bar, uint32_t par) { good = __all_sync(0xffffffffu, good && prefix_wait(bar, par, failed)); };
     while (walk.next(s)) {
       const int halves = same(NQ == 2 && s.x.rows * p.group - s.block * k.pairs > half ? 2 : 1), n = same(s.tile1 - s.tile0), beyond = same(s.x.key1 - s.x.first - s.tile0 * KT);
-      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->q_full, q_phase, failed));
+      uint32_t v_phase, k_phase = 0;
+      wait(&tail->q_full, q_phase);
       q_phase ^= 1;
-      for (int i = 0; i < 2 && i < n; ++i) {
-        const int at = arrived();
-        tcgen05_fence_after();
-        for (int t = 0; t < halves; ++t) issue_s(t, i, at);
-        used(&tail->empty[at]);
+      if (t >= halves) {  // nothing of this half: the pieces go back as they come
+        if (issuer && good) mbar_arrive(&tail->q_empty);
+        for (int i = 0; i < 2 * n; ++i) {
+          const int at = next(v_phase);
+          wait(&tail->full[at], v_phase);
+          if (issuer && good) mbar_arrive(&tail->empty[at]);
+        }
+        continue;
       }
-      if (n <= 2) used(&tail->q_empty);
+      for (int i = 0; i < 2 && i < n; ++i) {
+        const int at = next(v_phase);
+        wait(&tail->full[at], v_phase);
+        tcgen05_fence_after();
+        if (issuer && good) {
+          issue_s(i, at);
+          if (n <= 2 && i == n - 1) umma_commit(&tail->q_empty);
+        }
+      }
       for (int i = 0; i < n; ++i) {
-        const int b = i & 1, v_at = arrived();
+        const int b = i & 1, v_at = next(v_phase);
+        const bool more = i + 2 < n;
+        const int k_at = more ? next(k_phase) : v_at;
+        // all that this tile needs is asked for at once: a wait in which nothing is waited for takes 150 cycles
+        const bool there = prefix_test(&tail->full[v_at], v_phase) & (!more || prefix_test(&tail->full[k_at], k_phase)) & prefix_test(&tail->p_ready[t][b], p_phase >> b & 1);
+        const bool go = __all_sync(0xffffffffu, there);
+        if (!go) wait(&tail->full[v_at], v_phase);
         if (beyond - i * KT < KT) {  // tokens that the prefix does not have: V may hold anything, and 0 * NaN is not 0
           uint8_t* v = ring + v_at * F::kPieceBytes;
           for (int c = 0; c < CH; ++c)
@@ -905,25 +937,23 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           fence_proxy_async();
           __syncwarp();
         }
-        const bool more = i + 2 < n;
-        const int k_at = more ? arrived() : 0;
-        for (int t = 0; t < halves; ++t) {
-          const int bit = t * 2 + b;
-          good = __all_sync(0xffffffffu, good && prefix_wait(&tail->p_ready[t][b], p_phase >> bit & 1, failed));
-          p_phase ^= 1u << bit;
-          tcgen05_fence_after();
-          issue_o(t, b, v_at, i == 0);
-          if (more) issue_s(t, b, k_at);
+        if (!go) {
+          if (more) wait(&tail->full[k_at], k_phase);
+          wait(&tail->p_ready[t][b], p_phase >> b & 1);
         }
-        used(&tail->empty[v_at]);
-        if (more) used(&tail->empty[k_at]);
-        if (i + 3 == n) used(&tail->q_empty);
+        p_phase ^= 1u << b;
+        tcgen05_fence_after();
+        if (issuer && good) {
+          issue_o(b, v_at, i == 0);
+          if (more) issue_s(b, k_at);
+          if (i + 3 == n) umma_commit(&tail->q_empty);
+        }
       }
     }
     __syncwarp();
   } else {
     PrefixWalk walk(k, table, share, blockIdx.x);
-    const int t = (warp - 2) >> 2, quarter = warp & 3, own = quarter * 32 + lane;
+    const int t = (warp - 1 - NQ) >> 2, quarter = warp & 3, own = quarter * 32 + lane;
     const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), acc = lanes + F::kOCol + t * D;
     const float mul = CAP ? 1.0f : p.scale * kPrefixLog2e, cap = p.softcap * kPrefixLog2e, by_cap = CAP ? p.scale / p.softcap : 0.0f;
     const float2 mul2 = make_float2(mul, mul);
