@@ -694,7 +694,7 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 template <int D>
 struct PrefixTcShape {
   static constexpr int NQ = D == 256 ? 1 : 2, KT = 64, CH = D / 64;
-  static constexpr int kPieceBytes = KT * D * 2, kPieces = 131072 / kPieceBytes;
+  static constexpr int kTileBytes = KT * D * 2, kStages = 65536 / kTileBytes;  // a stage: V of a tile and K of the next but one (an item's first: K of two tiles)
   static constexpr int kQBytes = 128 * D * 2;
   static constexpr int kThreads = 32 * (1 + NQ + 4 * NQ);  // a warp that copies, one that issues MMAs for each half, four of the softmax for each
   static constexpr int kOCol = NQ * 2 * KT;
@@ -702,7 +702,7 @@ struct PrefixTcShape {
 
 struct PrefixTcTail {
   PrefixEntry entry[kPrefixCached + 1];
-  uint64_t full[16], empty[16];
+  uint64_t full[8], empty[8];
   uint64_t q_full, q_empty, s_full[2][2], p_ready[2][2], o_done[2][2];
   PrefixBuild build;
   uint32_t tmem_base;
@@ -712,7 +712,7 @@ struct PrefixTcTail {
 template <int D>
 constexpr size_t prefix_tc_smem_bytes() {
   typedef PrefixTcShape<D> F;
-  return 1024 + size_t(F::NQ) * F::kQBytes + size_t(F::kPieces) * F::kPieceBytes + sizeof(PrefixTcTail) + 16;
+  return 1024 + size_t(F::NQ) * F::kQBytes + size_t(F::kStages) * 2 * F::kTileBytes + sizeof(PrefixTcTail) + 16;
 }
 
 // two fp32 operations at a time
@@ -745,19 +745,6 @@ __device__ __forceinline__ void prefix_load_heads(void* dst, const CUtensorMap* 
       : "memory");
 }
 
-// whether a phase is over, without waiting for it
-__device__ __forceinline__ bool prefix_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
 // umma_desc_sw128 of a shared address
 __device__ __forceinline__ uint64_t prefix_desc(uint32_t addr) { return uint64_t((addr & 0x3FFFFu) >> 4) | uint64_t(1) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61; }
 
@@ -771,8 +758,8 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   constexpr int NQ = F::NQ, KT = F::KT, CH = F::CH;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sq = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // [NQ][CH][128 pairs][128 B], swizzled
-  uint8_t* ring = sq + NQ * F::kQBytes;                                         // piece: [CH][KT tokens][128 B]
-  PrefixTcTail* tail = reinterpret_cast<PrefixTcTail*>(ring + F::kPieces * F::kPieceBytes);
+  uint8_t* ring = sq + NQ * F::kQBytes;                                         // stage: two tiles [CH][KT tokens][128 B]
+  PrefixTcTail* tail = reinterpret_cast<PrefixTcTail*>(ring + F::kStages * 2 * F::kTileBytes);
   volatile int* failed = &tail->failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = prefix_half(p.group);
 
@@ -780,7 +767,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
-    for (int i = 0; i < F::kPieces; ++i) {
+    for (int i = 0; i < F::kStages; ++i) {
       mbar_init(&tail->full[i], 1);
       mbar_init(&tail->empty[i], NQ);
     }
@@ -822,23 +809,15 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   } else if (warp == 0) {
     PrefixWalk walk(k, table, share, blockIdx.x);
     const bool issuer = elect_one();
-    int piece = 0;
+    int stage = 0;
     uint32_t phase = 1, q_phase = 1;
     bool good = true;
-    auto advance = [&]() {
-      if (++piece == F::kPieces) piece = 0, phase ^= 1;
-    };
+    auto wait = [&](uint64_t* bar, uint32_t par) { good = __all_sync(0xffffffffu, good && prefix_wait(bar, par, failed)); };
     while (walk.next(s)) {
       const PrefixRows rows(p, k, s, KT);
       const int n = s.tile1 - s.tile0, halves = NQ == 2 && s.x.rows * p.group - s.block * k.pairs > half ? 2 : 1;
       int round[3] = {rows.look_up(0), rows.look_up(1), rows.look_up(2)};  // of V's tile, and the next two
-      auto load = [&](const CUtensorMap* tm, int at, int tile) {
-        good = __all_sync(0xffffffffu, good && prefix_wait(&tail->empty[piece], phase, failed));
-        if (issuer && good) mbar_expect_tx(&tail->full[piece], F::kPieceBytes);
-        prefix_load_tile<CH>(rows, at, tile, KT, ring + piece * F::kPieceBytes, tm, &tail->full[piece], issuer && good);
-        advance();
-      };
-      good = __all_sync(0xffffffffu, good && prefix_wait(&tail->q_empty, q_phase, failed));
+      wait(&tail->q_empty, q_phase);
       q_phase ^= 1;
       if (issuer && good) {
         mbar_expect_tx(&tail->q_full, uint32_t(halves * CH * half * 128));
@@ -846,17 +825,21 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           for (int c = 0; c < CH; ++c)
             prefix_load_heads(sq + t * F::kQBytes + c * 16384, &tm_q, c * 64, s.kvh * p.group, s.x.row + (s.block * k.pairs + t * half) / p.group, &tail->q_full);
       }
-      load(&tm_k, round[0], 0);
-      if (n > 1) load(&tm_k, round[0], 1);
-      for (int i = 0; i < n; ++i) {  // as the MMAs take them: V of a tile, then K of the next but one
+      for (int i = -1; i < n; ++i) {  // as the MMAs take them
         if (i > 0 && rows.begins_round(i)) round[0] = round[1], round[1] = round[2], round[2] = rows.look_up(rows.round_of(i) + 2);
-        load(&tm_v, round[0], i);
-        if (i + 2 < n) load(&tm_k, rows.round_of(i + 2) == rows.round_of(i) ? round[0] : round[1], i + 2);
+        const int first = i < 0 ? 0 : i, second = i + 2;  // V of `first` (K where i < 0), K of `second`
+        const bool more = second < n;
+        wait(&tail->empty[stage], phase);
+        uint8_t* to = ring + stage * 2 * F::kTileBytes;
+        if (issuer && good) mbar_expect_tx(&tail->full[stage], (more ? 2 : 1) * F::kTileBytes);
+        prefix_load_tile<CH>(rows, round[0], first, KT, to, i < 0 ? &tm_k : &tm_v, &tail->full[stage], issuer && good);
+        if (more) prefix_load_tile<CH>(rows, rows.round_of(second) == rows.round_of(first) ? round[0] : round[1], second, KT, to + F::kTileBytes, &tm_k, &tail->full[stage], issuer && good);
+        if (++stage == F::kStages) stage = 0, phase ^= 1;
       }
     }
-    for (int i = 0; i < F::kPieces; ++i) {  // the MMAs' arrivals have to be in before the CTA may leave
-      good = good && prefix_wait(&tail->empty[piece], phase, failed);
-      advance();
+    for (int i = 0; i < F::kStages; ++i) {  // the MMAs' arrivals have to be in before the CTA may leave
+      wait(&tail->empty[stage], phase);
+      if (++stage == F::kStages) stage = 0, phase ^= 1;
     }
     good = good && prefix_wait(&tail->q_empty, q_phase, failed);
     if (!good) {  // copies and MMAs in flight have a millisecond to end
@@ -873,79 +856,71 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const uint32_t idesc_s = umma_idesc_bf16(128, KT), idesc_o = umma_idesc_bf16(128, D) | kIdescBMajorMN;
     const uint64_t dq = prefix_desc(uint32_t(same(int(smem_u32(sq)))) + t * F::kQBytes), dk = prefix_desc(ring_addr);
     bool good = true;
-    int piece = 0;
+    int stage = 0;
     uint32_t phase = 0, q_phase = 0, p_phase = 0;  // p_phase: bit b
     // by the issuing lane
-    auto issue_s = [&](int b, int from) {
+    auto issue_s = [&](int b, uint32_t from) {
+      const uint64_t d = dk + (from >> 4);
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          umma_bf16(s_at + b * KT, dq + uint64_t((c * 16384 + kk * 32) >> 4), dk + uint64_t((from * F::kPieceBytes + c * KT * 128 + kk * 32) >> 4), idesc_s, uint32_t((c | kk) != 0));
+          umma_bf16(s_at + b * KT, dq + uint64_t((c * 16384 + kk * 32) >> 4), d + uint64_t((c * KT * 128 + kk * 32) >> 4), idesc_s, uint32_t((c | kk) != 0));
       umma_commit(&tail->s_full[t][b]);
-      umma_commit(&tail->empty[from]);
     };
-    auto issue_o = [&](int b, int from, bool start) {
+    auto issue_o = [&](int b, uint32_t from, bool start) {
+      const uint64_t d = umma_desc_sw128_mn(ring_addr, KT * 128) + (from >> 4);
 #pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk)
-        umma_bf16_ts(o_at, s_at + b * KT + kk * 8, umma_desc_sw128_mn(ring_addr + from * F::kPieceBytes + kk * 2048, KT * 128), idesc_o, uint32_t(!start || kk != 0));
+      for (int kk = 0; kk < KT / 16; ++kk) umma_bf16_ts(o_at, s_at + b * KT + kk * 8, d + uint64_t(kk * 2048 >> 4), idesc_o, uint32_t(!start || kk != 0));
       umma_commit(&tail->o_done[t][b]);
-      umma_commit(&tail->empty[from]);
     };
-    auto next = [&](uint32_t& at_phase) {  // the next piece
-      const int at = piece;
-      at_phase = phase;
-      if (++piece == F::kPieces) piece = 0, phase ^= 1;
-      return at;
+    auto wait = [&](uint64_t* bar, uint32_t par) {
+      if (__all_sync(0xffffffffu, mbar_try_wait(bar, par))) return;
+      good = __all_sync(0xffffffffu, good && prefix_wait(bar, par, failed));
     };
-    auto wait = [&](uint64_t* bar, uint32_t par) { good = __all_sync(0xffffffffu, good && prefix_wait(bar, par, failed)); };
+    auto used = [&]() {  // a stage
+      if (++stage == F::kStages) stage = 0, phase ^= 1;
+    };
     while (walk.next(s)) {
       const int halves = same(NQ == 2 && s.x.rows * p.group - s.block * k.pairs > half ? 2 : 1), n = same(s.tile1 - s.tile0), beyond = same(s.x.key1 - s.x.first - s.tile0 * KT);
-      uint32_t v_phase, k_phase = 0;
       wait(&tail->q_full, q_phase);
       q_phase ^= 1;
-      if (t >= halves) {  // nothing of this half: the pieces go back as they come
+      if (t >= halves) {  // nothing of this half: the stages go back as they come
         if (issuer && good) mbar_arrive(&tail->q_empty);
-        for (int i = 0; i < 2 * n; ++i) {
-          const int at = next(v_phase);
-          wait(&tail->full[at], v_phase);
-          if (issuer && good) mbar_arrive(&tail->empty[at]);
+        for (int i = -1; i < n; ++i, used()) {
+          wait(&tail->full[stage], phase);
+          if (issuer && good) mbar_arrive(&tail->empty[stage]);
         }
         continue;
       }
-      for (int i = 0; i < 2 && i < n; ++i) {
-        const int at = next(v_phase);
-        wait(&tail->full[at], v_phase);
-        tcgen05_fence_after();
-        if (issuer && good) {
-          issue_s(i, at);
-          if (n <= 2 && i == n - 1) umma_commit(&tail->q_empty);
-        }
+      wait(&tail->full[stage], phase);
+      tcgen05_fence_after();
+      if (issuer && good) {
+        const uint32_t from = stage * 2 * F::kTileBytes;
+        issue_s(0, from);
+        if (n > 1) issue_s(1, from + F::kTileBytes);
+        umma_commit(&tail->empty[stage]);
+        if (n <= 2) umma_commit(&tail->q_empty);
       }
-      for (int i = 0; i < n; ++i) {
-        const int b = i & 1, v_at = next(v_phase);
-        const bool more = i + 2 < n;
-        const int k_at = more ? next(k_phase) : v_at;
-        // all that this tile needs is asked for at once: a wait in which nothing is waited for takes 150 cycles
-        const bool there = prefix_test(&tail->full[v_at], v_phase) & (!more || prefix_test(&tail->full[k_at], k_phase)) & prefix_test(&tail->p_ready[t][b], p_phase >> b & 1);
-        const bool go = __all_sync(0xffffffffu, there);
-        if (!go) wait(&tail->full[v_at], v_phase);
+      used();
+      for (int i = 0; i < n; ++i, used()) {
+        const int b = i & 1;
+        const uint32_t from = stage * 2 * F::kTileBytes;
+        wait(&tail->full[stage], phase);
         if (beyond - i * KT < KT) {  // tokens that the prefix does not have: V may hold anything, and 0 * NaN is not 0
-          uint8_t* v = ring + v_at * F::kPieceBytes;
+          uint8_t* v = ring + from;
           for (int c = 0; c < CH; ++c)
             for (int at = (beyond - i * KT) * 128 + lane * 16; at < KT * 128; at += 512) *reinterpret_cast<uint4*>(v + c * KT * 128 + at) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
           __syncwarp();
         }
-        if (!go) {
-          if (more) wait(&tail->full[k_at], k_phase);
-          wait(&tail->p_ready[t][b], p_phase >> b & 1);
-        }
+        wait(&tail->p_ready[t][b], p_phase >> b & 1);
         p_phase ^= 1u << b;
         tcgen05_fence_after();
         if (issuer && good) {
-          issue_o(b, v_at, i == 0);
-          if (more) issue_s(b, k_at);
+          issue_o(b, from, i == 0);
+          if (i + 2 < n) issue_s(b, from + F::kTileBytes);
+          umma_commit(&tail->empty[stage]);
           if (i + 3 == n) umma_commit(&tail->q_empty);
         }
       }
