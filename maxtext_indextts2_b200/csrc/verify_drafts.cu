@@ -28,9 +28,11 @@ struct VerifyLayout {
 
 template <int E>
 int launch_verify(const VerifyParams& p, cudaStream_t st) {
-  if (p.rows > 0) MTX_TRY(launch(verify_sums_kernel<E>, dim3(unsigned(p.rows) * unsigned(p.chunks)), dim3(kVerifyThreads), 0, st, p));
+  constexpr int kWarps = kVerifyThreads / 32;
+  const long long ctas = ((long long)p.rows * p.chunks * (p.draft != nullptr ? 2 : 1) + kWarps - 1) / kWarps;
+  if (p.rows > 0) MTX_TRY(launch(verify_sums_kernel<E>, dim3(unsigned(ctas < 4 * 148 ? ctas : 4 * 148)), dim3(kVerifyThreads), 0, st, p));
   MTX_TRY(launch(verify_settle_kernel<E>, dim3(p.sequences), dim3(kVerifyThreads), 0, st, p));
-  return p.task != nullptr ? launch(verify_difference_kernel<E>, dim3(p.chunks, p.sequences), dim3(kVerifyThreads), 0, st, p) : MTX_OK;
+  return p.task != nullptr ? launch(verify_difference_kernel<E>, dim3((p.chunks + kWarps - 1) / kWarps, p.sequences), dim3(kVerifyThreads), 0, st, p) : MTX_OK;
 }
 
 }  // namespace

@@ -4,9 +4,9 @@
 //   the first row whose draft does not stay draws from max(p - q, 0), the row behind the last draft from p: the first token at which the weights' sum in the tokens' order
 //   exceeds pick_u times their whole sum
 //
-// Three kernels.  The first goes through all rows in chunks and leaves every chunk's largest logit and its sum of 2^((l - largest) / T log2 e).  The second, a CTA per sequence, joins
-// the chunks, settles which drafts stay and draws where the target's own weights are drawn from: the chunks' sums say which chunk, which is then read once more.  The third goes
-// through the rows that draw from a difference, a chunk per CTA; the last CTA of a sequence draws.  Bound: bytes, every row once and those of the third kernel twice.
+// Three kernels.  The first goes through all rows in chunks, a warp each, and leaves every chunk's largest logit and its sum of 2^((l - largest) / T log2 e).  The second, a CTA per
+// sequence, joins the chunks, settles which drafts stay and draws where the target's own weights are drawn from: the chunks' sums say which chunk, which is then read once more.  The
+// third goes through the rows that draw from a difference; the last CTA of a sequence draws.  Bound: bytes, every row once and those of the third kernel twice.
 //
 // Weights are 32-bit powers of two of an exponent that is rounded twice, relative to itself; sums of a thread's tokens are 32-bit, all others 64-bit: a border between two tokens
 // lies within 2^-19.5 of the whole sum of where it belongs, and the same call always draws the same token.
@@ -74,20 +74,20 @@ struct VerifyWeight {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(l, scale.lo, fmaf(l, scale.hi, -base))));
     return l == -INFINITY ? 0.0f : y;  // (its two products may be infinite to either side)
   }
-  __device__ __forceinline__ double precise(float l) const {
-    if (l == -INFINITY || top == -INFINITY) return 0.0;
-    if (far) return l == top ? 1.0 : 0.0;
-    return exp2(fma(double(l), scale.exact(), -double(base)));
-  }
 };
 
-// how much of one sum's unit another's is: 2^(a's base - b's base)
-__device__ __forceinline__ double verify_rescale(const VerifyScale& s, float a, float b) {
-  if (a == -INFINITY) return 0.0;
-  if (a == b) return 1.0;
+__device__ __forceinline__ float verify_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// how much of b's unit a's is, for sums relative to the logits a <= b
+__device__ __forceinline__ float verify_rescale(const VerifyScale& s, float a, float b) {
+  if (a == b) return 1.0f;
+  if (a == -INFINITY) return 0.0f;
   const VerifyWeight x(s, a), y(s, b);
-  if (x.far || y.far) return exp2((double(a) - double(b)) * s.exact());
-  return exp2(double(x.base) - double(y.base));
+  return x.far || y.far ? 0.0f : verify_ex2(x.base - y.base);
 }
 
 template <class T, class F>
@@ -144,73 +144,132 @@ __device__ __forceinline__ void verify_load(const float* row, int begin, int voc
   for (int i = 0; i < E; ++i) l[i] = verify_logit(l[i]);
 }
 
-// The sequence of a row, in all threads: -1 for nobody's.
-__device__ __forceinline__ int verify_sequence(const VerifyParams& p, int row, int* shared) {
-  if (threadIdx.x == 0) *shared = -1;
-  __syncthreads();
-  for (int s = threadIdx.x; s < p.sequences; s += kVerifyThreads)
-    if (p.row0[s] <= row && row < p.row0[s + 1]) *shared = s;
-  __syncthreads();
-  return *shared;
-}
-
 __device__ __forceinline__ float verify_heat(const VerifyParams& p, int s) { return p.temperature != nullptr ? p.temperature[s] : 1.0f; }
 __device__ __forceinline__ float verify_draft_heat(const VerifyParams& p, int s) { return p.draft_temperature != nullptr ? p.draft_temperature[s] : verify_heat(p, s); }
 
-// a row's chunk: its largest logit and its sum
-template <int E>
-__device__ __forceinline__ void verify_chunk(const float (&l)[E], int begin, float heat, VerifySum* out, float* floats, double* doubles, int* ints) {
-  float top = l[0];
+constexpr int kVerifyStep = 512;  // tokens of a warp at a time: four times four per lane
+
+// A lane's 16 tokens from `begin` on, four neighbours of every 128; -infinity outside the row.
+__device__ __forceinline__ void verify_load16(const float* row, int begin, int vocab, float (&l)[16]) {
+  const int lane = threadIdx.x & 31;
+  const float* at = row + begin + lane * 4;
+  if ((reinterpret_cast<uintptr_t>(at) & 15) == 0 && begin >= 0 && begin + kVerifyStep <= vocab) {
 #pragma unroll
-  for (int i = 1; i < E; ++i) top = fmaxf(top, l[i]);
-  top = verify_block(top, VerifyMax(), floats);
-  VerifySum r;
-  r.top = top;
-  r.sum = 0.0;
-  r.best = 0x7fffffff;
-  if (top != -INFINITY) {
-    if (heat > 0.0f) {
-      const VerifyWeight weight(VerifyScale(heat), top);
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < E; ++i) sum[i & 3] += weight(l[i]);
-      r.sum = verify_block(double((sum[0] + sum[1]) + (sum[2] + sum[3])), VerifyAdd(), doubles);
-    } else {
-      int best = 0x7fffffff;
-#pragma unroll
-      for (int j = 0; j < E / 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (l[4 * j + i] == top) best = min(best, begin + (j * kVerifyThreads + int(threadIdx.x)) * 4 + i);
-      r.best = verify_block(best, VerifyMin(), ints);
+    for (int j = 0; j < 4; ++j) {
+      const float4 u = *reinterpret_cast<const float4*>(at + j * 128);
+      l[4 * j] = u.x, l[4 * j + 1] = u.y, l[4 * j + 2] = u.z, l[4 * j + 3] = u.w;
     }
+    return;
   }
-  if (threadIdx.x == 0) *out = r;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int t = begin + i / 4 * 128 + lane * 4 + i % 4;
+    l[i] = t >= 0 && t < vocab ? row[t] : -INFINITY;
+  }
 }
 
-// CTA = (row, chunk)
+// A row's chunk of `steps` times 512 tokens by a warp: its largest logit and its sum; every lane relative to its own largest so far
+__device__ __forceinline__ void verify_chunk(const float* row, int begin, int steps, int vocab, float heat, VerifySum* out) {
+  const int lane = threadIdx.x & 31;
+  const bool greedy = !(heat > 0.0f);
+  const VerifyScale scale(greedy ? 1.0f : heat);
+  VerifyWeight weight(scale, -INFINITY);
+  float sums[2] = {0.0f, 0.0f}, next[16];
+  int best = 0x7fffffff;
+  verify_load16(row, begin, vocab, next);
+#pragma unroll 1
+  for (int it = 0; it < steps; ++it) {
+    float l[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) l[i] = verify_logit(next[i]);
+    if (it + 1 < steps) verify_load16(row, begin + (it + 1) * kVerifyStep, vocab, next);
+    float top = l[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, l[i]);
+    if (top > weight.top) {
+      if (greedy) {
+        weight.top = top;
+#pragma unroll
+        for (int i = 15; i >= 0; --i)
+          if (l[i] == top) best = begin + it * kVerifyStep + i / 4 * 128 + lane * 4 + i % 4;
+      } else {
+        const VerifyWeight grown(scale, top);
+        const float by = weight.far || weight.top == -INFINITY ? 0.0f : verify_ex2(weight.base - grown.base);
+        sums[0] *= by;
+        sums[1] *= by;
+        weight = grown;
+      }
+    }
+    if (!greedy && !weight.far) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sums[i & 1] += weight(l[i]);
+    }
+  }
+  VerifySum r;
+  r.top = verify_warp(weight.top, VerifyMax());
+  r.sum = 0.0;
+  r.best = 0x7fffffff;
+  if (greedy) {
+    r.best = verify_warp(weight.top == r.top ? best : 0x7fffffff, VerifyMin());
+  } else if (r.top != -INFINITY) {
+    if (VerifyWeight(scale, r.top).far) {  // only the largest logits weigh anything: counted
+      int n = 0;
+      for (int it = 0; it < steps; ++it) {
+        verify_load16(row, begin + it * kVerifyStep, vocab, next);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) n += verify_logit(next[i]) == r.top;
+      }
+      r.sum = verify_warp(double(n), VerifyAdd());
+    } else {
+      r.sum = verify_warp(double(sums[0] + sums[1]) * double(verify_rescale(scale, weight.top, r.top)), VerifyAdd());
+    }
+  }
+  if (lane == 0) *out = r;
+}
+
+constexpr int kVerifyKnown = 1024;  // sequences whose rows a CTA keeps
+
+// A warp has every (grid's warps)-th chunk of either side of every row
 template <int E>
-__global__ void __launch_bounds__(kVerifyThreads) verify_sums_kernel(const VerifyParams p) {
-  __shared__ float floats[8];
-  __shared__ double doubles[8];
-  __shared__ int ints[8], sequence;
+__global__ void __launch_bounds__(kVerifyThreads, 4) verify_sums_kernel(const VerifyParams p) {
+  __shared__ int known[kVerifyKnown + 1];
   griddep_launch_dependents();
   griddep_wait();
-  const int row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (kVerifyThreads / 32);
   if (blockIdx.x == 0)
     for (int s = threadIdx.x; s < p.sequences; s += kVerifyThreads) p.done[s] = 0;
-  const float* target = p.target + row * p.ld_target;
-  float l[E], d[E];
-  verify_load<E>(target, verify_begin<E>(target, chunk), p.vocab, l);
-  const int s = verify_sequence(p, row, &sequence);
-  if (s < 0) return;
-  const float heat = verify_heat(p, s), draft_heat = verify_draft_heat(p, s);
-  const bool drafted = p.draft != nullptr && heat > 0.0f && draft_heat > 0.0f && row + 1 < p.row0[s + 1];
-  const float* draft = p.draft + row * p.ld_draft;
-  if (drafted) verify_load<E>(draft, verify_begin<E>(draft, chunk), p.vocab, d);
-  const long long at = (long long)row * p.chunks + chunk;
-  verify_chunk<E>(l, verify_begin<E>(target, chunk), heat, p.target_sum + at, floats, doubles, ints);
-  if (drafted) verify_chunk<E>(d, 0, draft_heat, p.draft_sum + at, floats, doubles, ints);
+  const int* row0 = p.row0;
+  if (p.sequences <= kVerifyKnown) {
+    for (int s = threadIdx.x; s <= p.sequences; s += kVerifyThreads) known[s] = p.row0[s];
+    row0 = known;
+    __syncthreads();
+  }
+  const int sides = p.draft != nullptr ? 2 : 1;
+  const long long items = (long long)p.rows * p.chunks * sides;
+  for (long long item = blockIdx.x * (kVerifyThreads / 32) + (threadIdx.x >> 5); item < items; item += warps) {
+    const int row = int(item / (p.chunks * sides)), in = int(item - (long long)row * (p.chunks * sides)), side = in >= p.chunks, chunk = in - side * p.chunks;
+    // the last sequence that begins at the row or in front of it: 32 probes at a time
+    int lo = 0, hi = p.sequences;
+    while (lo < hi) {
+      const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+      const int c = __popc(__ballot_sync(0xffffffffu, at < hi && row0[at] <= row));
+      if (c == 0) break;
+      hi = min(hi, lo + c * step);
+      lo = lo + (c - 1) * step + 1;
+    }
+    const int s = lo - 1;
+    if (s < 0 || row >= row0[s + 1]) continue;  // nobody's
+    const float heat = verify_heat(p, s);
+    if (side == 0) {
+      const float* target = p.target + row * p.ld_target;
+      verify_chunk(target, verify_begin<E>(target, chunk), E * kVerifyThreads / kVerifyStep, p.vocab, heat, p.target_sum + (long long)row * p.chunks + chunk);
+    } else {
+      const float draft_heat = verify_draft_heat(p, s);
+      if (!(heat > 0.0f) || !(draft_heat > 0.0f) || row + 1 >= row0[s + 1]) continue;
+      const float* draft = p.draft + row * p.ld_draft;
+      verify_chunk(draft, verify_begin<E>(draft, chunk), E * kVerifyThreads / kVerifyStep, p.vocab, draft_heat, p.draft_sum + (long long)row * p.chunks + chunk);
+    }
+  }
 }
 
 // a row's chunks joined, by a warp
@@ -229,7 +288,7 @@ __device__ __forceinline__ VerifySum verify_join(const VerifySum* part, int chun
   double sum = 0.0;
   if (top != -INFINITY && heat > 0.0f) {
     const VerifyScale scale(heat);
-    for (int c = lane; c < chunks; c += 32) sum += part[c].sum * verify_rescale(scale, part[c].top, top);
+    for (int c = lane; c < chunks; c += 32) sum += part[c].sum * double(verify_rescale(scale, part[c].top, top));
   }
   r.sum = verify_warp(sum, VerifyAdd());
   return r;
@@ -329,14 +388,14 @@ __device__ int verify_draw_target(const VerifyParams& p, int row, float heat, fl
     }
     rest = verify_block(double((sum[0] + sum[1]) + (sum[2] + sum[3])), VerifyAdd(), doubles);
   }
-  auto of = [&](int c) { return (c == chunk_of ? rest : part[c].sum) * verify_rescale(scale, part[c].top, all.top); };
+  auto of = [&](int c) { return (c == chunk_of ? rest : part[c].sum) * double(verify_rescale(scale, part[c].top, all.top)); };
   if (threadIdx.x < 32) {
     double total = 0.0;
     for (int c = threadIdx.x; c < p.chunks; c += 32) total += of(c);
     total = verify_warp(total, VerifyAdd());
     double want = double(pick) * total;
     int chunk = verify_find_chunk(of, p.chunks, want);
-    if (chunk >= 0) want /= verify_rescale(scale, part[chunk].top, all.top);
+    if (chunk >= 0) want /= double(verify_rescale(scale, part[chunk].top, all.top));
     if (threadIdx.x == 0) want_in = want, chunk_in = chunk;
   }
   __syncthreads();
@@ -374,11 +433,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_settle_kernel(const Ver
         if (greedy) {
           stays = a.top != -INFINITY && a.best == x;
         } else if (a.top != -INFINITY) {
-          const double here = VerifyWeight(VerifyScale(heat), a.top).precise(verify_logit(p.target[row * p.ld_target + x])) / a.sum;
+          const double here = double(VerifyWeight(VerifyScale(heat), a.top)(verify_logit(p.target[row * p.ld_target + x]))) / a.sum;
           double there = 1.0;
           if (!sure) {
             const VerifySum b = verify_join(p.draft_sum + (long long)row * p.chunks, p.chunks, draft_heat);
-            there = b.top == -INFINITY ? 0.0 : VerifyWeight(VerifyScale(draft_heat), b.top).precise(verify_logit(p.draft[row * p.ld_draft + x])) / b.sum;
+            there = b.top == -INFINITY ? 0.0 : double(VerifyWeight(VerifyScale(draft_heat), b.top)(verify_logit(p.draft[row * p.ld_draft + x]))) / b.sum;
           }
           stays = double(p.accept_u[row]) * there < here;
         }
@@ -432,33 +491,47 @@ struct VerifyDifference {
   __device__ __forceinline__ float operator()(float l, float d) const { return fmaxf(target(l) * by_target - draft(d) * by_draft, 0.0f); }
 };
 
-// CTA = (chunk, sequence), the last sequences first: their rows are what the first kernel has left in L2
+// CTA = (eight chunks, a warp each; sequence), the last sequences first: their rows are what the first kernel has left in L2
 template <int E>
-__global__ void __launch_bounds__(kVerifyThreads) verify_difference_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 4) verify_difference_kernel(const VerifyParams p) {
   __shared__ double doubles[8], want_in;
   __shared__ int ints[8], is_last, chunk_in;
   griddep_launch_dependents();
   griddep_wait();
-  const int s = p.sequences - 1 - int(blockIdx.y), chunk = blockIdx.x;
+  const int s = p.sequences - 1 - int(blockIdx.y), chunk = blockIdx.x * (kVerifyThreads / 32) + int(threadIdx.x >> 5);
   const VerifyTask task = p.task[s];
   if (task.row < 0) return;
   const float heat = verify_heat(p, s), draft_heat = verify_draft_heat(p, s);
   const float *target = p.target + task.row * p.ld_target, *draft = p.draft + task.row * p.ld_draft;
   const VerifyDifference weight(task, heat, draft_heat);
-  {
+  if (chunk < p.chunks) {
+    constexpr int kSteps = E * kVerifyThreads / kVerifyStep;
     const int begin = verify_begin<E>(target, chunk);
-    float l[E], d[E], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    verify_load<E>(target, begin, p.vocab, l);
-    verify_load<E>(draft, begin, p.vocab, d);
+    float l[16], d[16];
+    double sum = 0.0;
+    verify_load16(target, begin, p.vocab, l);
+    verify_load16(draft, begin, p.vocab, d);
+#pragma unroll 1
+    for (int it = 0; it < kSteps; ++it) {
+      float part[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < E; ++i) sum[i & 3] += weight(l[i], d[i]);
-    const double all = verify_block(double((sum[0] + sum[1]) + (sum[2] + sum[3])), VerifyAdd(), doubles);
-    if (threadIdx.x == 0) {
-      p.left[(long long)s * p.chunks + chunk] = all;
-      __threadfence();
-      is_last = atomicAdd(&p.done[s], 1) == p.chunks - 1;
+      for (int i = 0; i < 16; ++i) part[i & 1] += weight(verify_logit(l[i]), verify_logit(d[i]));
+      if (it + 1 < kSteps) {
+        verify_load16(target, begin + (it + 1) * kVerifyStep, p.vocab, l);
+        verify_load16(draft, begin + (it + 1) * kVerifyStep, p.vocab, d);
+      }
+      sum += double(part[0] + part[1]);
+    }
+    sum = verify_warp(sum, VerifyAdd());
+    if ((threadIdx.x & 31) == 0) {
+      p.left[(long long)s * p.chunks + chunk] = sum;
       __threadfence();
     }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    is_last = atomicAdd(&p.done[s], 1) == int(gridDim.x) - 1;
+    __threadfence();
   }
   __syncthreads();
   if (!is_last) return;
