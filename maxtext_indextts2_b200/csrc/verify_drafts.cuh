@@ -272,25 +272,40 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_sums_kernel(const Ve
   }
 }
 
-// a row's chunks joined, by a warp
+// a row's chunks joined, by a warp; 128 of them are read once
 __device__ __forceinline__ VerifySum verify_join(const VerifySum* part, int chunks, float heat) {
   const int lane = threadIdx.x & 31;
+  const VerifyScale scale(heat > 0.0f ? heat : 1.0f);
   VerifySum r;
   r.top = -INFINITY;
+  r.sum = 0.0;
   r.best = 0x7fffffff;
-  for (int c = lane; c < chunks; c += 32) {
-    const VerifySum x = part[c];
-    if (x.top > r.top) r.top = x.top, r.best = x.best;  // (of equal ones the first chunk's)
+  for (int c0 = 0; c0 < chunks; c0 += 128) {
+    VerifySum x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = c0 + i * 32 + lane;
+      x[i].top = -INFINITY;
+      x[i].sum = 0.0;
+      x[i].best = 0x7fffffff;
+      if (c < chunks) x[i] = part[c];
+    }
+    float top = r.top;
+    int best = r.best;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (x[i].top > top) top = x[i].top, best = x[i].best;  // (of equal ones the first chunk's)
+    const float all = verify_warp(top, VerifyMax());
+    r.best = verify_warp(top == all ? best : 0x7fffffff, VerifyMin());
+    double sum = 0.0;
+    if (all != -INFINITY && heat > 0.0f) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += x[i].sum * double(verify_rescale(scale, x[i].top, all));
+      sum = verify_warp(sum, VerifyAdd()) + r.sum * double(verify_rescale(scale, r.top, all));
+    }
+    r.sum = sum;
+    r.top = all;
   }
-  const float top = verify_warp(r.top, VerifyMax());
-  r.best = verify_warp(r.top == top ? r.best : 0x7fffffff, VerifyMin());
-  r.top = top;
-  double sum = 0.0;
-  if (top != -INFINITY && heat > 0.0f) {
-    const VerifyScale scale(heat);
-    for (int c = lane; c < chunks; c += 32) sum += part[c].sum * double(verify_rescale(scale, part[c].top, top));
-  }
-  r.sum = verify_warp(sum, VerifyAdd());
   return r;
 }
 
@@ -358,16 +373,15 @@ __device__ __forceinline__ int verify_find_token(Weight&& weight, int begin, dou
   return found != 0x7fffffff ? found : last;
 }
 
-// A token drawn from the target's own weights of a row; `without`: a token that is not drawn (-1: none).  By the CTA.  -1: nothing to draw.
+// A token drawn from the target's own weights of a row, whose sum is `all`; `without`: a token that is not drawn (-1: none).  By the CTA.  -1: nothing to draw.
 template <int E>
-__device__ int verify_draw_target(const VerifyParams& p, int row, float heat, float pick, int without, double* doubles, int* ints) {
+__device__ int verify_draw_target(const VerifyParams& p, int row, const VerifySum& all, float heat, float pick, int without, double* doubles, int* ints) {
   __shared__ double want_in;
   __shared__ int chunk_in;
   __syncthreads();
   const float* target = p.target + row * p.ld_target;
   const VerifySum* part = p.target_sum + (long long)row * p.chunks;
   const VerifyScale scale(heat);
-  const VerifySum all = verify_join(part, p.chunks, heat);  // (every warp)
   if (all.top == -INFINITY) return -1;
   // the chunk without its token: anew, for a difference would leave the rounding of what may be nearly all of it
   int chunk_of = -1;
@@ -410,6 +424,7 @@ template <int E>
 __global__ void __launch_bounds__(kVerifyThreads) verify_settle_kernel(const VerifyParams p) {
   __shared__ double doubles[8];
   __shared__ int ints[8], first_stop;
+  __shared__ VerifySum stop_sum;
   griddep_launch_dependents();
   const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) first_stop = 0x7fffffff;
@@ -423,27 +438,28 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_settle_kernel(const Ver
   const float heat = verify_heat(p, s), draft_heat = verify_draft_heat(p, s);
   const bool greedy = !(heat > 0.0f), sure = p.draft == nullptr || !(draft_heat > 0.0f);
   __syncthreads();
+  VerifySum a, b;  // of this warp's first row whose draft does not stay
+  int mine = -1;
+  a.top = b.top = -INFINITY;
+  a.sum = b.sum = 0.0;
+  a.best = b.best = 0x7fffffff;
   for (int row = first + warp; row < end; row += kVerifyThreads / 32) {
     const bool final = row == end - 1;
-    bool stays = false;
-    if (!final) {
-      const int x = p.token[row + 1];
-      if (x >= 0 && x < p.vocab) {
-        const VerifySum a = verify_join(p.target_sum + (long long)row * p.chunks, p.chunks, heat);
-        if (greedy) {
-          stays = a.top != -INFINITY && a.best == x;
-        } else if (a.top != -INFINITY) {
-          const double here = double(VerifyWeight(VerifyScale(heat), a.top)(verify_logit(p.target[row * p.ld_target + x]))) / a.sum;
-          double there = 1.0;
-          if (!sure) {
-            const VerifySum b = verify_join(p.draft_sum + (long long)row * p.chunks, p.chunks, draft_heat);
-            there = b.top == -INFINITY ? 0.0 : double(VerifyWeight(VerifyScale(draft_heat), b.top)(verify_logit(p.draft[row * p.ld_draft + x]))) / b.sum;
-          }
-          stays = double(p.accept_u[row]) * there < here;
-        }
-      }
+    const int x = final ? -1 : p.token[row + 1];
+    const bool known = x >= 0 && x < p.vocab;
+    const float logit = known ? verify_logit(p.target[row * p.ld_target + x]) : 0.0f, drafted = known && !greedy && !sure ? verify_logit(p.draft[row * p.ld_draft + x]) : 0.0f;
+    a = verify_join(p.target_sum + (long long)row * p.chunks, p.chunks, heat);
+    if (!final && !greedy && !sure) b = verify_join(p.draft_sum + (long long)row * p.chunks, p.chunks, draft_heat);
+    bool stays = known && a.top != -INFINITY;
+    if (stays && greedy) {
+      stays = a.best == x;
+    } else if (stays) {
+      const double here = double(VerifyWeight(VerifyScale(heat), a.top)(logit)) / a.sum;
+      const double there = sure ? 1.0 : b.top == -INFINITY ? 0.0 : double(VerifyWeight(VerifyScale(draft_heat), b.top)(drafted)) / b.sum;
+      stays = double(p.accept_u[row]) * there < here;
     }
     if (!stays) {
+      mine = row;
       if (lane == 0) atomicMin(&first_stop, row);
       break;
     }
@@ -454,28 +470,21 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_settle_kernel(const Ver
     if (row != stop) p.emitted[row] = row < stop ? p.token[row + 1] : -1;
   if (threadIdx.x == 0) p.accepted[s] = stop - first;
   const bool final = stop == end - 1;
-  if (greedy) {
-    if (warp == 0) {
-      const VerifySum a = verify_join(p.target_sum + (long long)stop * p.chunks, p.chunks, heat);
-      if (lane == 0) p.emitted[stop] = a.top == -INFINITY ? -1 : a.best;
-    }
-    return;
-  }
-  if (final || sure) {
+  if (!greedy && (final || sure)) {
+    if (mine == stop && lane == 0) stop_sum = a;
+    __syncthreads();
     const int x = final ? -1 : p.token[stop + 1];
-    int drawn = verify_draw_target<E>(p, stop, heat, p.pick_u[s], x >= 0 && x < p.vocab ? x : -1, doubles, ints);
-    if (drawn < 0 && !final) drawn = verify_draw_target<E>(p, stop, heat, p.pick_u[s], -1, doubles, ints);  // (the draft is all that the target may say)
+    int drawn = verify_draw_target<E>(p, stop, stop_sum, heat, p.pick_u[s], x >= 0 && x < p.vocab ? x : -1, doubles, ints);
+    if (drawn < 0 && !final) drawn = verify_draw_target<E>(p, stop, stop_sum, heat, p.pick_u[s], -1, doubles, ints);  // (the draft is all that the target may say)
     if (threadIdx.x == 0) p.emitted[stop] = drawn;
-    return;
-  }
-  if (warp == 0) {
-    VerifyTask t;
-    t.row = stop;
-    t.target = verify_join(p.target_sum + (long long)stop * p.chunks, p.chunks, heat);
-    t.draft = verify_join(p.draft_sum + (long long)stop * p.chunks, p.chunks, draft_heat);
-    if (lane == 0) {
-      p.emitted[stop] = -1;
-      if (t.target.top != -INFINITY) p.task[s] = t;
+  } else if (mine == stop && lane == 0) {
+    p.emitted[stop] = greedy && a.top != -INFINITY ? a.best : -1;
+    if (!greedy && a.top != -INFINITY) {
+      VerifyTask task;
+      task.row = stop;
+      task.target = a;
+      task.draft = b;
+      p.task[s] = task;
     }
   }
 }
@@ -550,7 +559,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_difference_kernel(co
     drawn = verify_find_token<E>([&](int t) { return t >= 0 && t < p.vocab ? weight(verify_logit(target[t]), verify_logit(draft[t])) : 0.0f; }, verify_begin<E>(target, chunk_in), want_in,
                                  doubles, ints);
   else  // (no difference that 32 bits show: the target's own)
-    drawn = verify_draw_target<E>(p, task.row, heat, p.pick_u[s], -1, doubles, ints);
+    drawn = verify_draw_target<E>(p, task.row, task.target, heat, p.pick_u[s], -1, doubles, ints);
   if (threadIdx.x == 0) p.emitted[task.row] = drawn;
 }
 
