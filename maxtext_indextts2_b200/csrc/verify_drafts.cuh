@@ -502,7 +502,7 @@ struct VerifyDifference {
 
 // CTA = (eight chunks, a warp each; sequence), the last sequences first: their rows are what the first kernel has left in L2
 template <int E>
-__global__ void __launch_bounds__(kVerifyThreads, 4) verify_difference_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 3) verify_difference_kernel(const VerifyParams p) {
   __shared__ double doubles[8], want_in;
   __shared__ int ints[8], is_last, chunk_in;
   griddep_launch_dependents();
@@ -523,12 +523,15 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_difference_kernel(co
 #pragma unroll 1
     for (int it = 0; it < kSteps; ++it) {
       float part[2] = {0.0f, 0.0f};
+      float x[16], y[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) part[i & 1] += weight(verify_logit(l[i]), verify_logit(d[i]));
+      for (int i = 0; i < 16; ++i) x[i] = l[i], y[i] = d[i];
       if (it + 1 < kSteps) {
         verify_load16(target, begin + (it + 1) * kVerifyStep, p.vocab, l);
         verify_load16(draft, begin + (it + 1) * kVerifyStep, p.vocab, d);
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part[i & 1] += weight(verify_logit(x[i]), verify_logit(y[i]));
       sum += double(part[0] + part[1]);
     }
     sum = verify_warp(sum, VerifyAdd());
