@@ -10,6 +10,8 @@
 //
 // Weights are 32-bit powers of two of an exponent that is rounded twice, relative to itself; sums of a thread's tokens are 32-bit, all others 64-bit: a border between two tokens
 // lies within 2^-19.5 of the whole sum of where it belongs, and the same call always draws the same token.
+//
+// The first two kernels let the next one start when they end: started as soon as it fits, it made 32 sequences of 4 rows over 32768 tokens 17.2 us, not 15.2.
 #pragma once
 
 #include "common.cuh"
@@ -233,7 +235,6 @@ constexpr int kVerifyKnown = 1024;  // sequences whose rows a CTA keeps
 template <int E>
 __global__ void __launch_bounds__(kVerifyThreads, 4) verify_sums_kernel(const VerifyParams p) {
   __shared__ int known[kVerifyKnown + 1];
-  griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31, warps = gridDim.x * (kVerifyThreads / 32);
   if (blockIdx.x == 0)
@@ -425,7 +426,6 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_settle_kernel(const Ver
   __shared__ double doubles[8];
   __shared__ int ints[8], first_stop;
   __shared__ VerifySum stop_sum;
-  griddep_launch_dependents();
   const int s = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) first_stop = 0x7fffffff;
   griddep_wait();
