@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 512 ? 15
   typedef typename Row::TH TH;
   __shared__ double part[32], inv_of_row;
   __shared__ float block_top[256], block_low[256], block_f[256], block_by[256];  // of a row; of the warps' rows four blocks each
-  griddep_launch_dependents();
+  // (what comes next starts when this ends: with an early start 333 rows of 2560 took 3.6 us, not 3.1)
   griddep_wait();
   const int lane = threadIdx.x & 31, threads = blockDim.x;  // of a row; rows of a warp each lie along threadIdx.y
   const int row = blockIdx.x * blockDim.y + threadIdx.y, block0 = threadIdx.y * 4;

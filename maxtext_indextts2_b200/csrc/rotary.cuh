@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 3) rotary_kernel(const RotaryP
   constexpr int S = VEC ? 8 : 1;  // pairs or channels of a unit
   extern __shared__ __align__(16) float2 turn[];  // [tokens][pairs]
   __shared__ long long place[kRotaryTokens];  // of a token in the pages of key head 0; -1: its keys and values have none; -2: it belongs to nobody
-  griddep_launch_dependents();
+  // (what comes next starts when this ends: with an early start 4001 tokens of 24 heads of 128 took 18.6 us, not 16.4)
   griddep_wait();
   const int row0 = blockIdx.x * tokens, rows = min(tokens, p.rows - row0), dim = p.dim, pairs = p.pairs;
   // units: all heads' turned pairs, then their channels that pass, then the values (so that the lanes of most warps do the same)
