@@ -700,6 +700,10 @@ struct PrefixTcShape {
   static constexpr int kQBytes = 128 * D * 2;
   static constexpr int kThreads = 32 * (1 + NQ + 4 * NQ);  // a warp that copies, one that issues MMAs for each half, four of the softmax for each
   static constexpr int kOCol = NQ * 2 * KT;
+  // Every second pair of weights by a polynomial, not the special-function units, whose weights are rounded to bf16 (2^-8) all the same.  With heads of 128 channels the units and the
+  // MMAs are both near their limits (575 rows of 16 heads over 16384 shared tokens: 122.7 us without, 116.2 so); with 64 the softmax's instructions bound (105.9 us without,
+  // 116.2 so), with 256 the MMAs (66.3 and 66.7)
+  static constexpr bool kByPolynomial = D == 128;
 };
 
 struct PrefixTcTail {
@@ -737,6 +741,25 @@ __device__ __forceinline__ float2 prefix_add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
+}
+
+// the largest; NaN where one is
+__device__ __forceinline__ float prefix_max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two numbers of at most 2^6 by 32-bit operations alone: n = x to the nearest integer is what x + 1.5 * 2^23 ends in, 2^(x - n) a polynomial that is 1 at 0 and off by at most 2^-13.2
+// on [-1/2, 1/2] (least squares, reweighted until the largest relative errors were alike).  What is less than 2^-126 (of -infinity too) becomes 2^-126, below a sum's last bit, and so does that of NaN.
+__device__ __forceinline__ float2 prefix_ex2_poly(float2 x) {
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 n = prefix_add2(x, make_float2(12582912.0f, 12582912.0f)), f = prefix_fma2(prefix_add2(n, make_float2(-12582912.0f, -12582912.0f)), make_float2(-1.0f, -1.0f), x);
+  float2 y = prefix_fma2(f, make_float2(0.05500895f, 0.05500895f), make_float2(0.24221101f, 0.24221101f));
+  y = prefix_fma2(y, f, make_float2(0.69328293f, 0.69328293f));
+  y = prefix_fma2(y, f, make_float2(1.0f, 1.0f));
+  return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
 }
 
 __device__ __forceinline__ void prefix_load_heads(void* dst, const CUtensorMap* tm, int c, int head, int row, uint64_t* bar) {
@@ -968,14 +991,16 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           for (int c = 0; c < KT; ++c)
             if (c >= beyond) x[c] = -INFINITY;
         }
+        auto max3 = [](float a, float b, float c) { return F::kByPolynomial ? prefix_max3(a, b, c) : fmaxf(fmaxf(a, b), c); };
         float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
         for (int c = 4; c + 8 <= KT; c += 8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(x[c + e], x[c + 4 + e]));
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[c + e], x[c + 4 + e]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[KT - 4 + e]);
-        const float now = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul);
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], mx[e], x[KT - 4 + e]);
+        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]), now = fmaxf(m, top * mul);
+        if (F::kByPolynomial && top != top) m = 0.0f, l = top;  // a score is none: so is the row (its weight by the polynomial is a number all the same)
         if (__any_sync(0xffffffffu, valid && now > m + 8.0f)) {  // (m = -inf: the first tile)
           const float fix = now == -INFINITY ? 1.0f : prefix_ex2(m - now);
           l *= fix;
@@ -1004,8 +1029,12 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float2 w = prefix_fma2(make_float2(x[c + 2 * e], x[c + 2 * e + 1]), mul2, base2);
-            w.x = prefix_ex2(w.x);
-            w.y = prefix_ex2(w.y);
+            if (F::kByPolynomial && e % 2 == 1) {
+              w = prefix_ex2_poly(w);
+            } else {
+              w.x = prefix_ex2(w.x);
+              w.y = prefix_ex2(w.y);
+            }
             sums[e & 1] = prefix_add2(sums[e & 1], w);
             pk[e] = pack_bf16x2(w.x, w.y);
           }
@@ -1124,7 +1153,7 @@ __global__ void __launch_bounds__(kPrefixJoinMost) prefix_join_kernel(const Pref
       for (int e = 0; e < 8; ++e) o[e] *= fix;
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        if (j0 + n * int(blockDim.y) >= all || st[n].x == -INFINITY) continue;  // (-infinity: a part of which the row sees nothing)
+        if (j0 + n * int(blockDim.y) >= all || st[n].y == 0.0f) continue;  // (0: a part of which the row sees nothing; of one whose scores are none the sum is none)
         const float f = exp2f(st[n].x - base);
         sum = fmaf(st[n].y, f, sum);
         o[0] = fmaf(v[n][0].x, f, o[0]), o[1] = fmaf(v[n][0].y, f, o[1]), o[2] = fmaf(v[n][0].z, f, o[2]), o[3] = fmaf(v[n][0].w, f, o[3]);
@@ -1147,7 +1176,7 @@ __global__ void __launch_bounds__(kPrefixJoinMost) prefix_join_kernel(const Pref
       for (int e = 0; e < 8; ++e) o[e] *= fix;
       for (int y = 1; y < int(blockDim.y); ++y) {
         const float* other = joint[y * blockDim.x + threadIdx.x];
-        if (other[8] == -INFINITY) continue;
+        if (other[9] == 0.0f) continue;
         const float f = exp2f(other[8] - base);
         sum = fmaf(other[9], f, sum);
 #pragma unroll

@@ -43,7 +43,7 @@ def rotated(x, pos, freq, amplitude, half):
 
 def attention(q, k_pages, v_pages, row0, lengths, page_map, heads, scale, softcap=0.0):
   """(out, bound) [rows, heads, dim] in 64 bits on the inputs' device; rows that see nothing are NaN.  The bound counts probabilities and results rounded to bfloat16
-  (half a step of each), scores and sums in 32 bits."""
+  (half a step of each), scores and sums in 32 bits, and weights off by 2^-13.2 each (2^-12.2 of a quotient of their sums, inside the 2^-12)."""
   kv, num_pages, page, dim = k_pages.shape
   out = torch.full((q.shape[0], heads, dim), math.nan, dtype=torch.float64, device=q.device)
   bound = torch.zeros_like(out)

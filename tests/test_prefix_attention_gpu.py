@@ -216,6 +216,36 @@ def test_numbers_that_a_prefix_has():
   assert torch.equal(got, clean)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_scores_that_are_none(dim):
+  """A NaN in a shared key reaches all rows of its key head, wherever in a tile the token is, and no other head.  Keys far below all others weigh nothing."""
+  rows = [4] * 32
+  c = Case(rows, [600 + n for n in rows], [(0, 32, 512)], heads=8, kv=2, dim=dim, page=16, seed=dim)
+  clean = c.check().clone()
+  for token in (4, 5, 6, 7, 511):
+    at = (1, int(c.maps[0, token // 16]), token % 16, 3)
+    was = c.k[at].clone()
+    c.k[at] = math.nan
+    got = c.run().double().view_as(clean)
+    c.k[at] = was
+    assert bool(got[:, 4:].isnan().all()) and torch.equal(got[:, :4], clean[:, :4])
+  c.q.abs_()
+  c.k[:, c.maps[0, 2].long(), 1::2] = -1e30
+  c.check()
+
+
+@pytest.mark.parametrize("sequences", [2, 40])
+def test_a_last_key_that_is_none(sequences):
+  """A NaN in the one token that a sequence has behind the prefix: a part of its own whose only score is none."""
+  c = Case([1] * sequences, [257] * sequences, [(0, sequences, 256)], heads=8, kv=2, dim=64, page=16)
+  clean = c.check().clone()
+  c.k[0, int(c.maps[1, 16]), 0, 9] = math.nan
+  got = c.run().double().view_as(clean)
+  assert bool(got[1, :4].isnan().all())
+  clean[1, :4] = got[1, :4] = 0
+  assert torch.equal(got, clean)
+
+
 def test_pages_outside_the_pool():
   """They are read as page 0, and a length ends with the page map."""
   c = Case([1, 2], [90, 80], dim=64, page=16, seed=3)
