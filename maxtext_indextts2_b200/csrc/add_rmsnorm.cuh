@@ -7,7 +7,8 @@
 // A row lives in the registers of its threads, eight neighbouring values of every 8 T (T threads), so that the sixteen lanes of half a warp hold a block of 128.  
 //
 // The mean (of sums of eight), the norm's factor and the scales' fractions are 64-bit, so that scales and 8-bit values are those of the definition; what 64 bits cost is spent
-// once per row and block, by one warp.  A value that 32 bits bring next to a border of two 8-bit values (one in 60,000) is formed again in 64.  Other results have two
+// once per row and block, by one warp.  Eight values are formed twice in 32 bits, by factors 2^-21 below and above theirs, which is more
+// than 32 bits' three roundings: where both are the same 8-bit values so is the definition's, otherwise (one in 8,000) they are formed again in 64.  Other results have two
 // roundings in 32 bits and their type's own.
 #pragma once
 
@@ -84,21 +85,14 @@ __device__ __forceinline__ float norm_odd(double v) {
   return double(t) == v || !(fabsf(t) < INFINITY) ? t : __uint_as_float(__float_as_uint(t) | 1u);
 }
 
-// Borders of 8-bit values: from 2^-6 on the numbers whose last 20 bits are 2^19, below (where 8-bit values are 2^-9 apart) some of those whose last 19 are 0.
-// At most 8: the number is a border or up to four last bits away from one.
-__device__ __forceinline__ uint32_t norm_off_border(float v) { return (__float_as_uint(v) + 0x80004u) & 0xfffffu; }
-__device__ __forceinline__ bool norm_next_to_border(float v) {
-  if (fabsf(v) >= 0x1p-6f) return norm_off_border(v) <= 8;
-  return ((__float_as_uint(v) + 4) & 0x7ffffu) <= 8 && fabsf(v) >= 0x1p-11f;  // (less is 0)
-}
-
 // CTA = a row, or eight rows of a warp each.  VEC: all rows lie on 16 bytes and end with whole eight values.
 template <class TX, class TR, bool E4M3, bool VEC, int J, int T>
 __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 512 ? 1536 / T : 1) add_rmsnorm_kernel(const AddNormParams p) {
   typedef AddNormRow<TX, TR> Row;
   typedef typename Row::TH TH;
   __shared__ double part[32], inv_of_row;
-  __shared__ float block_top[256], block_low[256], block_f[256], block_by[256];  // of a row; of the warps' rows four blocks each
+  __shared__ float2 block_f[256];
+  __shared__ float block_top[256], block_low[256], block_by[256];  // of a row; of the warps' rows four blocks each
   // (what comes next starts when this ends: with an early start 333 rows of 2560 took 3.6 us, not 3.1)
   griddep_wait();
   const int lane = threadIdx.x & 31, threads = blockDim.x;  // of a row; rows of a warp each lie along threadIdx.y
@@ -163,8 +157,7 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 512 ? 15
 #pragma unroll
       for (int i = 0; i < 8; ++i) mine = fmaxf(mine, fabsf(v[j][i]));
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (fabsf(v[j][i]) == mine) low = fmaf(fabsf(h[i]), fabsf(w[i]), -mine);
+      for (int i = 0; i < 8; ++i) low = fmaxf(low, fmaf(fabsf(h[i]), fabsf(w[i]), -mine));  // (of products that were rounded to less it is less)
       float top = mine;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -220,7 +213,8 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 512 ? 15
       const double rough = double(__frcp_rn(float(largest))), off = fma(-largest, rough, 1.0), recip = fma(rough, fma(off, off, off), rough);
       const float by = float(448.0 * recip);
       block_by[block0 + b] = by;
-      block_f[block0 + b] = float(inv * double(by));
+      const float f = float(inv * double(by));
+      block_f[block0 + b] = f < INFINITY ? make_float2(f * (1.0f - 0x1p-21f), f * (1.0f + 0x1p-21f)) : make_float2(0.0f, INFINITY);  // (no factor of 32 bits: no two values alike)
       p.scale[(long long)row * p.blocks + b] = float(largest * (1.0 / 448.0));
     }
     if (!single && lane == 0) inv_of_row = inv;
@@ -232,24 +226,14 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 512 ? 15
   for (int j = 0; j < J; ++j) {
     const int c = (threadIdx.x + j * threads) * 8, n = p.width - c;
     if (n <= 0) continue;
-    const float f = block_f[block0 + c / kScaleBlock];
-    uint32_t near = f < INFINITY ? 0xfffffu : 0u;
-    float least = INFINITY;
+    const float2 f = block_f[block0 + c / kScaleBlock];
+    uint32_t e[4], other = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[j][i] *= f;  // within four last bits
-      near = min(near, norm_off_border(v[j][i]));
-      least = fminf(least, fabsf(v[j][i]));
+    for (int i = 0; i < 4; ++i) {
+      e[i] = e4m3_pair(v[j][2 * i] * f.x, v[j][2 * i + 1] * f.x);
+      other |= e[i] ^ e4m3_pair(v[j][2 * i] * f.y, v[j][2 * i + 1] * f.y);
     }
-    if (near <= 8 || least < 0x1p-6f) {
-      bool border = !(f < INFINITY);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) border = border || norm_next_to_border(v[j][i]);
-      if (border) again |= 1 << j;
-    }
-    uint32_t e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = e4m3_pair(v[j][2 * i], v[j][2 * i + 1]);
+    if (other != 0) again |= 1 << j;
     uint8_t* to = static_cast<uint8_t*>(p.out) + row * p.ldo + c;
     if (VEC || n >= 8) {
       *reinterpret_cast<uint2*>(to) = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
@@ -259,7 +243,7 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 512 ? 15
         if (i < n) to[i] = uint8_t(e[i / 2] >> (i % 2 * 8));
     }
   }
-  // values next to a border once more, from memory (registers for this would be every row's)
+  // values next to a border once more, with their neighbours and from memory (registers for this would be every row's)
   __syncwarp();  // (a sum may have been stored by the next lane)
   if (again == 0) return;
   const double row_inv = single ? inv : inv_of_row;
@@ -275,8 +259,6 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 512 ? 15
       else h = norm_sum<TX, TR>(x0[row * p.ldx + c], Row::kAdd ? static_cast<float>(r0[row * p.ldr + c]) : 0.0f);
       const float w = p.weight == nullptr ? 1.0f : (p.weight_f32 ? static_cast<const float*>(p.weight)[c] : static_cast<float>(static_cast<const bf16*>(p.weight)[c])) + p.weight_offset;
       const int b = block0 + c / kScaleBlock;
-      const float first = h * w * block_f[b];
-      if (block_f[b] < INFINITY && !norm_next_to_border(first)) continue;
       static_cast<uint8_t*>(p.out)[row * p.ldo + c] = uint8_t(e4m3_pair(norm_odd(double(h) * double(w) * (row_inv * double(block_by[b]))), 0.0f));
     }
   }
