@@ -87,7 +87,7 @@ __device__ __forceinline__ float norm_odd(double v) {
 
 // CTA = a row, or eight rows of a warp each.  VEC: all rows lie on 16 bytes and end with whole eight values.
 template <class TX, class TR, bool E4M3, bool VEC, int J, int T>
-__global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 512 ? 1536 / T : 1) add_rmsnorm_kernel(const AddNormParams p) {
+__global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 768 ? 1536 / T : J == 3 ? 2 : 1) add_rmsnorm_kernel(const AddNormParams p) {
   typedef AddNormRow<TX, TR> Row;
   typedef typename Row::TH TH;
   __shared__ double part[32], inv_of_row;

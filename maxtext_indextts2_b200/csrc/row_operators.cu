@@ -13,7 +13,9 @@ constexpr int kMostWidth = 32768;  // four times eight values in each of 1024 th
 int value_bytes(int type) { return type == MTX_F32 ? 4 : type == MTX_BF16 ? 2 : 1; }
 
 // Threads of a row, each with J times eight of its values: a warp up to 512 values (no barrier, eight rows in a CTA), then as many warps as have eight values for each lane, from 4096
-// values on twice eight, from 16384 on four times.
+// values on twice eight, from 16384 on four times.  Where rows wait for SMs (more than 148) and a row's registers would leave room for one CTA, it has fewer, for two: to 8 bits 2000 rows of
+// 10000 took 59.9 us with one, 43.8 so, 1600 of 14336 with three times eight 51.4, not 64.0 (with x of 32 bits 82.0, not 70.9: not there).  100 rows of 10000 or 14336 took 5.8 and 8.2 us with
+// one, 6.3 and 9.2 so.
 template <class TX, class TR, bool E4M3, bool VEC>
 int launch_norm_rows(const AddNormParams& p, cudaStream_t st) {
   const int lanes = (p.width + 7) / 8;
@@ -21,10 +23,15 @@ int launch_norm_rows(const AddNormParams& p, cudaStream_t st) {
     const dim3 grid((p.rows + kNormWarpRows - 1) / kNormWarpRows), block(32, kNormWarpRows);
     return launch(lanes <= 32 ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 1, 256> : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 2, 256>, grid, block, 0, st, p);
   }
-  const int each = lanes <= 512 ? 1 : lanes <= 2048 ? 2 : 4, threads = ((lanes + each - 1) / each + 31) / 32 * 32;
+  const bool two = p.rows > 148;
+  const int each = lanes <= 512 ? 1 : lanes > 1536 && lanes <= 1920 && two && sizeof(TX) == 2 ? 3 : lanes <= 2048 ? 2 : 4, threads = ((lanes + each - 1) / each + 31) / 32 * 32;
   return launch(each == 1 ? (threads <= 256 ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 1, 256> : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 1, 512>)
-                : each == 2 ? (threads <= 512 ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 2, 512> : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 2, 1024>)
-                            : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 4, 1024>, dim3(p.rows), dim3(threads), 0, st, p);
+                : each == 2 ? (threads <= 512          ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 2, 512>
+                               : threads <= 768 && two ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 2, 768>
+                                                       : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 2, 1024>)
+                : each == 3 ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 3, 640>
+                            : (threads <= 768 ? add_rmsnorm_kernel<TX, TR, E4M3, VEC, 4, 768> : add_rmsnorm_kernel<TX, TR, E4M3, VEC, 4, 1024>),
+                dim3(p.rows), dim3(threads), 0, st, p);
 }
 
 template <class TX, class TR>

@@ -70,6 +70,44 @@ def test_shapes(rows, width, types):
   check(x, residual, weight, 0.5, 1e-5, total, out, scale)
 
 
+@pytest.mark.parametrize("width", [8200, 10001, 12289, 14336, 15353, 15361, 24577])
+@pytest.mark.parametrize("types", [(BF16, BF16, FP8), (F32, F32, FP8), (BF16, F32, F32)])
+def test_more_wide_rows_than_sms(width, types):
+  g = torch.Generator("cuda").manual_seed(width)
+  tx, tr, to = types
+  rows = 150
+  x = torch.randn(rows, width, generator=g, device="cuda").to(tx)
+  residual = (3 * torch.randn(rows, width, generator=g, device="cuda")).to(tr)
+  weight = 1 + 0.3 * torch.randn(width, generator=g, device="cuda")
+  total = torch.empty_like(residual)
+  out = torch.empty(rows, -(-width // 16) * 16, dtype=to, device="cuda")[:, :width]
+  scale = torch.empty(rows, -(-width // 128), device="cuda") if to == FP8 else None
+  call(x, residual, total, weight, 0.0, 1e-5, out, scale)
+  check(x, residual, weight, 0.0, 1e-5, total, out, scale)
+
+
+@pytest.mark.parametrize("first", [0, 1])
+def test_largest_products_that_round_alike(first):
+  """Of two neighbours whose products are the same number in 32 bits the larger one, by half a last bit, is a block's largest."""
+  g = torch.Generator().manual_seed(3)
+  x = torch.rand(512, 128, generator=g) - 0.5
+  weight = torch.ones(128)
+  x[:, 40 + first] = weight[40 + first] = 1 + 2.0**-12  # 1 + 2^-11 + 2^-24, an even number and half a last bit
+  x[:, 41 - first] = 1 + 2.0**-11
+  out = torch.empty(512, 128, dtype=FP8, device="cuda")
+  scale = torch.empty(512, 1, device="cuda")
+  call(x.cuda(), None, None, weight.cuda(), 0.0, 1e-5, out, scale)
+  check(x.cuda(), None, weight.cuda(), 0.0, 1e-5, None, out, scale)
+  # the mean is one of 32-bit sums of eight squares, of even and of odd places: 5 * 2^-24 off, more than what this looks for.  (A product and a sum in 64 bits, rounded once, are the fused step)
+  squares = x.double().view(512, 16, 8)
+  sums = torch.zeros(2, 512, 16)
+  for i in range(8):
+    sums[i % 2] = (squares[:, :, i] ** 2 + sums[i % 2].double()).float()
+  mean = (sums[0] + sums[1]).double().sum(1) / 128
+  want = (1 + 2.0**-12) ** 2 / (mean + float(torch.tensor(1e-5))).sqrt() / 448
+  assert torch.equal(scale.cpu()[:, 0], want.float())
+
+
 @pytest.mark.parametrize("shift", range(8))
 @pytest.mark.parametrize("width", [5, 136, 777, 1031, 8200])
 @pytest.mark.parametrize("types", [(BF16, BF16, BF16), (F32, F32, F32), (BF16, F32, BF16)])
