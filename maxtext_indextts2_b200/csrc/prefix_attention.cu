@@ -102,10 +102,12 @@ int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
   auto units = p.softcap > 0.0f ? prefix_units_kernel<D, true> : prefix_units_kernel<D, false>;
   MTX_TRY(allow_smem(units, prefix_smem_bytes<D>(), p.softcap > 0.0f ? cap_done : done));
   MTX_TRY(launch(units, dim3(w[1].workers), dim3(kPrefixThreads), prefix_smem_bytes<D>(), st, tk[1], tv[1], p, w[1]));
-  // the join: where rows and key heads are few, several threads share a place's parts
+  // the join: some 800 threads of an SM, several of them for each place where rows and key heads are few (64 of 860 CTAs: drafts of 48 sequences 54.0 us, twice as many 53.4, four times 56.0);
+  // where they are fewer than two per SM, six parts in flight and not four (64 rows of 4 key heads 33.6 us, not 35.0; the 860 CTAs 55.4, not 53.4)
   const int lanes = p.group * (D / 8) < 128 ? (p.group * (D / 8) + 31) / 32 * 32 : 128;
-  const int shares = (long long)p.rows * p.kv_heads < 2 * kPrefixSms ? kPrefixJoinMost / lanes : 1;
-  return launch(prefix_join_kernel<D>, dim3(p.rows, p.kv_heads), dim3(lanes, shares), 0, st, p, tc ? w[0] : w[1], w[1]);
+  const long long ctas = (long long)p.rows * p.kv_heads, room = 800ll * kPrefixSms / (ctas * lanes);
+  const int shares = room < 1 ? 1 : room < kPrefixJoinMost / lanes ? int(room) : kPrefixJoinMost / lanes;
+  return launch(ctas < 2 * kPrefixSms ? prefix_join_kernel<D, 6> : prefix_join_kernel<D, 4>, dim3(p.rows, p.kv_heads), dim3(lanes, shares), 0, st, p, tc ? w[0] : w[1], w[1]);
 }
 
 }  // namespace

@@ -1072,10 +1072,11 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 
 // ---- the join ----------------------------------------------------------------------------------------------------------------------
 
-// CTA = (row, key head); a thread has eight channels of a head, and every blockDim.y-th part of the row's: its prefix's (of `a`), then its tail's (of `b`), in the tokens' order.
+// CTA = (row, key head); a thread has eight channels of a head, and every blockDim.y-th part of the row's: its prefix's (of `a`), then its tail's (of `b`), in the tokens' order, N of them
+// in flight.
 constexpr int kPrefixJoinMost = 256;  // threads
 
-template <int D>
+template <int D, int N>
 __global__ void __launch_bounds__(kPrefixJoinMost) prefix_join_kernel(const PrefixAttnParams p, const PrefixWork a, const PrefixWork b) {
   __shared__ PrefixEntry found[4];  // the row's prefix and tail, the sums of both works
   __shared__ int is;
@@ -1127,7 +1128,6 @@ __global__ void __launch_bounds__(kPrefixJoinMost) prefix_join_kernel(const Pref
     }
     const bool written = tail.key0 == 0 && parts[1] == 1;  // already
     float top = -INFINITY, sum = 0.0f, o[8] = {};
-    constexpr int N = 4;  // parts in flight
     const int all = mine && !written ? parts[0] + parts[1] : 0;
     for (int j0 = threadIdx.y; j0 < all; j0 += N * blockDim.y) {
       float2 st[N];
