@@ -1,4 +1,6 @@
 // C entry points of the attention over shared prefixes (prefix_attention.cuh).
+#include <cmath>
+
 #include "host_util.cuh"
 #include "operator_args.cuh"
 #include "prefix_attention.cuh"
@@ -11,16 +13,26 @@ constexpr int kPrefixTcPairs = 256;             // most pairs of an item of pref
 
 int bits_of(int power_of_two) { return __builtin_ctz(unsigned(power_of_two)); }
 
-// Prefixes go to the tensor cores' kernel when their sequences bring at least 64 pairs on the average.
-bool prefix_on_tc(int rows, int prefixes, int group) { return prefixes > 0 && (long long)rows * group >= 64ll * prefixes; }
+// Prefixes may go to the tensor cores' kernel when their sequences bring at least 64 pairs on the average (its tiles have 128).
+bool prefix_may_tc(int rows, int prefixes, int group) { return prefixes > 0 && (long long)rows * group >= 64ll * prefixes; }
+
+// They do where that kernel, a fifth of the other's time for full tiles of 128 pairs, makes up for what it costs by itself (its launch, and some 20 MB of parts that the join reads): by pairs x
+// channels x tokens, as many as the page map has room for.  In us, tensor cores' kernel and tails' kernel, for pairs x tokens of 4 key heads and prefixes that fill the map:
+//   64 channels: 320 x 2048 25.1, 21.1;  640 x 2048 24.3, 23.5;  2560 x 512 27.5, 24.8;  320 x 8192 27.9, 33.6;  1280 x 2048 28.0, 32.3
+//   128: 512 x 2048 36.6, 32.1;  128 x 8192 35.3, 34.6;  2048 x 512 43.5, 38.1;  256 x 8192 43.1, 50.5;  1024 x 2048 40.5, 49.3;  2048 x 8192 64.7, 260.9
+//   256: 256 x 2048 48.0, 41.4;  1024 x 512 54.2, 49.3;  64 x 8192 43.5, 42.0;  128 x 8192 56.0, 65.9;  512 x 2048 49.9, 61.3
+bool prefix_on_tc(int rows, int prefixes, int group, int kv_heads, int dim, long long tokens) {
+  if (!prefix_may_tc(rows, prefixes, group)) return false;
+  const double pairs = double(rows) * group, tiles = ceil(pairs / prefixes / 128.0) * prefixes;
+  return (pairs - 128.0 / 5.0 * tiles) * kv_heads * dim * double(tokens) >= (dim == 64 ? 340e6 : 550e6);
+}
 
 // the scratch: the entries, a maximum, a sum and weighted values per place; where prefixes have a kernel of their own, the same for them
 struct PrefixLayout {
   size_t table[2], stat[2], part[2], bytes;
 
-  PrefixLayout(int rows, int sequences, int prefixes, int heads, int kv_heads, int dim) {
+  PrefixLayout(int rows, int sequences, int prefixes, int heads, int kv_heads, int dim, bool tc) {
     const size_t group = size_t(heads / kv_heads), all = size_t(rows) * group;
-    const bool tc = prefix_on_tc(rows, prefixes, int(group));
     bytes = 0;
     for (int k = 0; k < 2; ++k) {  // prefixes, tails
       // every pair has a place in one tail and at most one prefix, and another in every CTA that shares its item with the CTA before
@@ -64,8 +76,8 @@ int launch_prefix(PrefixAttnParams p, uint8_t* scratch, cudaStream_t st) {
   static std::atomic<uint64_t> done{0}, cap_done{0}, tc_done{0}, tc_cap_done{0};
   constexpr int KT = PrefixShape<D>::KT;
   typedef PrefixTcShape<D> Tc;
-  const bool tc = prefix_on_tc(p.rows, p.prefixes, p.group);
-  const PrefixLayout at(p.rows, p.sequences, p.prefixes, p.heads, p.kv_heads, D);
+  const bool tc = prefix_on_tc(p.rows, p.prefixes, p.group, p.kv_heads, D, (long long)p.max_pages * p.tokens_per_page);
+  const PrefixLayout at(p.rows, p.sequences, p.prefixes, p.heads, p.kv_heads, D, tc);
   p.box = p.tokens_per_page < KT ? p.tokens_per_page : KT;
   PrefixWork w[2];
   memset(w, 0, sizeof(w));
@@ -116,7 +128,9 @@ extern "C" {
 
 size_t mtx_prefix_attention_scratch_bytes(int rows, int sequences, int prefixes, int num_q_heads, int num_kv_heads, int head_dim) {
   if (rows < 1 || sequences < 1 || prefixes < 0 || num_kv_heads < 1 || num_q_heads < num_kv_heads || head_dim < 1) return 0;
-  return PrefixLayout(rows, sequences, prefixes, num_q_heads, num_kv_heads, head_dim).bytes;
+  const int group = num_q_heads / num_kv_heads;
+  // (with a kernel of their own for the prefixes there are more places, and as many entries)
+  return PrefixLayout(rows, sequences, prefixes, num_q_heads, num_kv_heads, head_dim, prefix_may_tc(rows, prefixes, group)).bytes;
 }
 
 int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, const void* v_pages, const mtx_prefix_batch* b, void* out, long long ldo, int num_q_heads,

@@ -21,6 +21,12 @@ def _no_stalls():
   assert count.value == 0
 
 
+@pytest.fixture(autouse=True, params=[False, True], ids=["short", "long"])
+def _page_map(request):
+  """Page maps with room for the tokens there are, or for so many that prefixes of 64 pairs and more have the tensor cores."""
+  Case.roomy = request.param
+
+
 class Case:
   """Sequences with `rows` rows each; `lengths` tokens; `prefixes`: (first sequence, sequences, tokens) whose whole pages are shared and whose rest is a copy."""
 
@@ -34,6 +40,9 @@ class Case:
     self.rows = self.row0[-1] + behind
     used = [-(-max(0, l) // page) for l in self.lengths]
     most = max(1, max(used, default=1)) + more_pages
+    pairs, each = sum(rows) * heads // kv, max(1, len(prefixes))
+    if self.roomy and prefixes and pairs >= 64 * each:
+      most = max(most, int(600e6 / ((pairs - 128 / 5 * each * -(-pairs // (each * 128))) * kv * dim)) // page + 1)
     self.num_pages = sum(used) + spare
     order = torch.randperm(self.num_pages, generator=g).tolist()
     maps, at = torch.zeros(max(1, self.sequences), most, dtype=torch.int32), 0
