@@ -474,8 +474,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_settle_kernel(const Ver
     if (mine == stop && lane == 0) stop_sum = a;
     __syncthreads();
     const int x = final ? -1 : p.token[stop + 1];
-    int drawn = verify_draw_target<E>(p, stop, stop_sum, heat, p.pick_u[s], x >= 0 && x < p.vocab ? x : -1, doubles, ints);
-    if (drawn < 0 && !final) drawn = verify_draw_target<E>(p, stop, stop_sum, heat, p.pick_u[s], -1, doubles, ints);  // (the draft is all that the target may say)
+    int drawn = -1;
+#pragma unroll 1
+    for (int without = x >= 0 && x < p.vocab ? x : -1;; without = -1) {
+      drawn = verify_draw_target<E>(p, stop, stop_sum, heat, p.pick_u[s], without, doubles, ints);
+      if (drawn >= 0 || without < 0) break;  // (otherwise the draft is all that the target may say)
+    }
     if (threadIdx.x == 0) p.emitted[stop] = drawn;
   } else if (mine == stop && lane == 0) {
     p.emitted[stop] = greedy && a.top != -INFINITY ? a.best : -1;

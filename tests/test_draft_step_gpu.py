@@ -18,7 +18,7 @@ BF16, FP8 = torch.bfloat16, torch.float8_e4m3fn
 class Server:
   """One layer: x -> norm -> q, k, v -> rotary, pages -> attention -> projection -> sum, norm -> vocabulary -> verification -> record."""
 
-  def __init__(self, sequences, drafts, prefix, width=256, heads=6, kv=2, dim=64, vocab=777, page=16, seed=0):
+  def __init__(self, sequences, drafts, prefix, width=256, heads=6, kv=2, dim=64, vocab=777, page=16, room=0, seed=0):
     g = torch.Generator().manual_seed(seed)
     self.lib, self.sequences, self.n, self.rows, self.prefix = _lib.load(), sequences, drafts + 1, sequences * (drafts + 1), prefix
     self.width, self.heads, self.kv, self.dim, self.vocab, self.page = width, heads, kv, dim, vocab, page
@@ -37,7 +37,7 @@ class Server:
     shared, own = prefix // page, 6
     self.num_pages = shared + own * sequences
     order = torch.randperm(self.num_pages, generator=g).int()
-    self.page_map = torch.cat([order[:shared].expand(sequences, -1), order[shared:].view(sequences, own)], 1).contiguous().cuda()
+    self.page_map = torch.cat([order[:shared].expand(sequences, -1), order[shared:].view(sequences, own), torch.zeros(sequences, room, dtype=torch.int32)], 1).contiguous().cuda()
     self.k = torch.randn(kv, self.num_pages, page, dim, generator=g).to(BF16).cuda()
     self.v = torch.randn(kv, self.num_pages, page, dim, generator=g).to(BF16).cuda()
     e = lambda *shape, t=BF16: torch.empty(*shape, dtype=t, device="cuda")
@@ -162,10 +162,10 @@ class Server:
     assert torch.equal(self.seen.cpu().int(), words)
 
 
-@pytest.mark.parametrize("sequences,drafts,prefix", [(1, 0, 0), (1, 3, 64), (9, 2, 160), (40, 3, 96)])
+@pytest.mark.parametrize("sequences,drafts,prefix,room", [(1, 0, 0, 0), (1, 3, 64, 0), (9, 2, 160, 0), (40, 3, 96, 0), (40, 3, 96, 600)])  # (with room for 9600 tokens more: on the tensor cores)
 @pytest.mark.parametrize("captured", [False, True])
-def test_steps(sequences, drafts, prefix, captured):
-  s = Server(sequences, drafts, prefix, seed=sequences)
+def test_steps(sequences, drafts, prefix, room, captured):
+  s = Server(sequences, drafts, prefix, room=room, seed=sequences)
   if captured:
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     for t in (s.x, s.drafted, s.accept, s.pick):
