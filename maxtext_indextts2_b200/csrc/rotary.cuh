@@ -2,7 +2,8 @@
 // Keys and values go to rows of their own or to the pages of their sequences.
 //
 // The angle is formed and brought into a turn in 64 bits (positions of some 100,000 lose the last digits of a 32-bit angle), cosine and sine are 32-bit.
-// CTA = one to four tokens: a thread computes the cosines and sines of a pair, then all turn the heads with them.  Bound: bytes; a token's projected heads are read once and written once.
+// CTA = one to sixteen tokens: a thread computes the cosines and sines of a pair, then all turn the heads with them.  Bound: bytes; a token's projected heads are read once and written once
+// (4001 tokens of 24 heads of 128 channels, 49 MB: 14.3 us, 3.4 TB/s).
 #pragma once
 
 #include <type_traits>
@@ -90,7 +91,7 @@ __device__ __forceinline__ void RotaryRaw<T, VEC>::pass(TO* p) const {
   }
 }
 
-constexpr int kRotaryTokens = 8;  // of a CTA, at most
+constexpr int kRotaryTokens = 16;  // of a CTA, at most
 
 // VEC: heads, rotated channels and everything's place are whole eight values, so that a thread turns eight pairs (or passes eight channels) at a time.
 // Every value is read and written by one thread alone: results may lie where the inputs are.  A thread has the same channels of all of its CTA's tokens (where they are is worked out
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 3) rotary_kernel(const RotaryP
   constexpr int S = VEC ? 8 : 1;  // pairs or channels of a unit
   extern __shared__ __align__(16) float2 turn[];  // [tokens][pairs]
   __shared__ long long place[kRotaryTokens];  // of a token in the pages of key head 0; -1: its keys and values have none; -2: it belongs to nobody
-  // (what comes next starts when this ends: with an early start 4001 tokens of 24 heads of 128 took 18.6 us, not 16.4)
+  // (what comes next starts when this ends: with an early start 4001 tokens of 24 heads of 128 channels took 18.6 us, not 16.4)
   griddep_wait();
   const int row0 = blockIdx.x * tokens, rows = min(tokens, p.rows - row0), dim = p.dim, pairs = p.pairs;
   // units: all heads' turned pairs, then their channels that pass, then the values (so that the lanes of most warps do the same)

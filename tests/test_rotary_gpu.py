@@ -69,6 +69,15 @@ def test_layouts(rows, heads, kv, dim, rot, half, types):
   assert close(c.q.cpu().view(rows, heads, dim), q, qs, 1.25) and close(c.k.cpu().view(rows, kv, dim), k, ks, 1.25)
 
 
+@pytest.mark.parametrize("rows,heads,kv,dim,rot,half", [(5000, 1, 1, 1024, 1024, True), (9000, 1, 1, 64, 64, True), (12001, 2, 1, 32, 20, False), (4500, 3, 2, 128, 64, True)])
+def test_many_tokens(rows, heads, kv, dim, rot, half):
+  """As many of a CTA as it takes, in one wave and in several, with the largest of cosines and sines."""
+  c = Case(rows, heads, kv, dim, rot, half, seed=rows)
+  run(c.batch())
+  q, k, _, qs, ks = c.want()
+  assert close(c.q.cpu().view(rows, heads, dim), q, qs, 1.0) and close(c.k.cpu().view(rows, kv, dim), k, ks, 1.0)
+
+
 @pytest.mark.parametrize("shift,extra", [(1, 0), (0, 3), (3, 5), (8, 8)])
 def test_places(shift, extra):
   for half in (False, True):
