@@ -769,7 +769,7 @@ int mtx_note_tokens(uint16_t* seen, long long ld_seen, uint32_t* touched, long l
  *   out = h * (weight_offset + weight) / sqrt(mean(h^2) + eps);  weight NULL: without that factor.
  * x, residual (and sum, of its type), weight [width]: MTX_BF16 or MTX_F32 each; out: MTX_BF16, MTX_F32, or MTX_E4M3 with out_scale
  * [rows, ceil(width / 128)], as mtx_quantize_fp8(block_rows = 1) gives them for out's fp32 values (8-bit values: base and pitch whole 16 bytes; the bytes behind a
- * row's last value stay).  Pitches in values; width <= 32768; other values at any multiple of their types' sizes, with any pitch.  sum may be residual or x, and out any
+ * row's last value stay).  Pitches in values; width <= 32768, rows <= 2^30; other values at any multiple of their types' sizes, with any pitch.  sum may be residual or x, and out any
  * input, where type and pitch are the same; nothing else may overlap.  A row with a NaN is NaN throughout, one with an infinity 0 but for NaN in its place. */
 int mtx_add_rmsnorm(const void* x, int x_type, long long ldx, const void* residual, int residual_type, long long ld_residual, void* sum, long long ld_sum, const void* weight,
                     int weight_type, float weight_offset, float eps, void* out, int out_type, long long ldo, float* out_scale, int rows, int width, mtx_stream stream);
@@ -787,7 +787,7 @@ int mtx_rotary_frequencies(int rot_dims, double base, int scaling, double factor
 /* Rotary positions for projected queries and keys, and the way of keys and values into the pages of mtx_paged_attention, for any number of rows of any sequences (beside
  * mtx_qkv_rope_append and mtx_paged_append). */
 typedef struct {
-  int32_t rows;
+  int32_t rows;             /* up to 2^30 */
   int32_t heads, kv_heads;  /* either may be 0 */
   int32_t dim;              /* channels of a head, up to 1024 */
   int32_t rot_dims;         /* the first of them are rotated: even, 0 .. dim; the others pass */
@@ -815,7 +815,7 @@ int mtx_rotary(const mtx_rotary_batch* b, mtx_stream stream);
 /* Attention of the last rows of each sequence over its pages, where neighbouring sequences share the first tokens of their contexts: mtx_paged_attention for several rows per
  * sequence, which reads the keys and values of a shared prefix once for all its sequences. */
 typedef struct {
-  int32_t rows, sequences;
+  int32_t rows, sequences;    /* up to 2^20, up to 2^16 */
   const int32_t* row0;        /* [sequences + 1] ascending: sequence s has the rows [row0[s], row0[s + 1]), its last tokens (none: it is left out) */
   const int32_t* lengths;     /* [sequences] tokens in the pages, the rows' own among them: row i of n sees the first lengths - n + i + 1 */
   const int32_t* page_map;    /* [sequences, max_pages_per_group] */
@@ -826,7 +826,10 @@ typedef struct {
 } mtx_prefix_batch;
 /* q, out [rows, num_q_heads * head_dim] bf16 at pitches ldq, ldo; k_pages, v_pages [num_kv_heads, num_pages, tokens_per_page, head_dim] bf16, tokens_per_page a power of two >= 8;
  * head_dim 64, 128 or 256; up to 16 query heads per key head.  out = softmax(cap(scale * <q, k>)) v, cap(x) = softcap * tanh(x / softcap) (0: off).  A row that sees no token, and rows
- * outside the sequences, are left as they were.  Page numbers outside the pool are read as page 0, lengths end with the page map.  All bases and pitches whole 16 bytes.
+ * outside the sequences, are left as they were; where row0 or prefix_seq0 descends all of them are.  Page numbers outside the pool are read as page 0, lengths end with the page map.  All
+ * bases and pitches whole 16 bytes.  The blocks of 64 (row, query head) pairs of a key head, one at least per sequence and prefix, times key heads and the page map's tiles of 4096 / head_dim
+ * tokens stay below 2^31.  max_pages_per_group * tokens_per_page, what a sequence can have, also says whether prefixes are work for the tensor cores: a page map not much longer than its
+ * sequences is the faster one for short prefixes.
  * scratch: written by every call, so one per stream (or graph) that runs at the same time; base on 256 bytes.  The same call gives the same bits every time. */
 size_t mtx_prefix_attention_scratch_bytes(int rows, int sequences, int prefixes, int num_q_heads, int num_kv_heads, int head_dim);
 int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, const void* v_pages, const mtx_prefix_batch* batch, void* out, long long ldo, int num_q_heads,
@@ -841,7 +844,7 @@ int mtx_prefix_attention_stalls(uint32_t* count);
  * accept_u * q(x) < p(x).  At the first that does not, the sequence goes on with a token drawn from max(p - q, 0) (over its sum); behind the last draft with one drawn from p.  Drawn is the
  * first token at which the sum of the weights in the tokens' order exceeds pick_u times their whole sum. */
 typedef struct {
-  int32_t rows, sequences, vocab;  /* vocab <= 2^28 */
+  int32_t rows, sequences, vocab;  /* up to 2^20, 65535 and 2^28; rows times parts of 1024 (for 592 and more parts of 4096: 4096) tokens stay below 2^31 */
   const int32_t* row0;             /* [sequences + 1] ascending, as in mtx_prefix_batch */
   const int32_t* token;            /* [rows]: the tokens of the step's rows; a drafted token outside the vocabulary does not stay */
   const float* target;             /* [rows, vocab] logits; NaN counts as -infinity, infinity as the largest number */

@@ -49,7 +49,7 @@ struct alignas(16) PrefixEntry {
   int prefix;        // a tail's prefix where it begins behind one, else -1
   int first, tiles;  // the first tile's first token: key0 rounded down to where a copy may begin; tiles of an item
   int pairs, units;  // of one key head in the entries before
-  int unused;
+  int bad;           // it ends before it begins; of the sums: one does, and nothing is done (places in the scratch are counted for entries side by side)
 };
 
 constexpr float kPrefixLog2e = 1.4426950408889634f;
@@ -82,12 +82,13 @@ __device__ __forceinline__ PrefixEntry prefix_entry(const PrefixAttnParams& p, i
   auto row_of = [&](int s) { return min(max(p.row0[s], 0), p.rows); };
   auto seq_of = [&](int i) { return min(max(bounds[i], 0), p.sequences); };
   PrefixEntry x;
-  x.pairs = x.units = x.unused = 0;
+  x.pairs = x.units = x.bad = 0;
   x.prefix = -1;
   if (e < p.prefixes) {
-    const int s0 = seq_of(e), s1 = max(seq_of(e + 1), s0);
+    const int s0 = seq_of(e), s1 = seq_of(e + 1);
     x.row = row_of(s0);
-    x.rows = s1 > s0 ? max(row_of(s1) - x.row, 0) : 0;
+    x.rows = row_of(s1) - x.row;
+    x.bad = s1 < s0 || x.rows < 0;
     x.key0 = 0;
     x.key1 = min(max(lens[e], 0), most);
     x.first_seen = x.key1;
@@ -96,7 +97,8 @@ __device__ __forceinline__ PrefixEntry prefix_entry(const PrefixAttnParams& p, i
     const int s = e - p.prefixes;
     const int r0 = row_of(s), r1 = row_of(s + 1), length = p.lengths[s];
     x.row = r0;
-    x.rows = max(r1 - r0, 0);
+    x.rows = r1 - r0;
+    x.bad = x.rows < 0;
     x.key1 = min(max(length, 0), most);
     x.first_seen = length < 0 ? -(1 << 30) : length - x.rows + 1;
     x.map = s;
@@ -138,13 +140,14 @@ __device__ __forceinline__ void prefix_build_table(const PrefixAttnParams& p, co
     lens = build->lens;
     __syncthreads();
   }
-  int units = 0, pairs = 0;
+  int units = 0, pairs = 0, bad = 0;
   for (int e0 = 0; e0 <= total; e0 += threads) {
     const int e = e0 + tid;
     PrefixEntry x;
     int u = 0, b = 0;
     if (e < total) {
       x = prefix_entry(p, k.kt, k.first + e, bounds, lens);
+      bad |= x.bad;
       b = x.tiles > 0 ? x.rows * p.group : 0;
       u = x.tiles * ((b + k.pairs - 1) / k.pairs);
     } else {
@@ -172,6 +175,7 @@ __device__ __forceinline__ void prefix_build_table(const PrefixAttnParams& p, co
       table[e] = x;
     }
   }
+  if (__syncthreads_or(bad) && tid == 0) table[total].units = 0, table[total].bad = 1;
   __syncthreads();
 }
 
@@ -1099,7 +1103,7 @@ __global__ void __launch_bounds__(kPrefixJoinMost) prefix_join_kernel(const Pref
     }
   }
   __syncthreads();
-  if (is == 0) return;
+  if (is == 0 || found[2].bad || found[3].bad) return;
   const PrefixEntry &front = found[0], &tail = found[1];
   if (min(tail.first_seen + row - tail.row, tail.key1) <= 0) return;
   const int lanes = D / 8, most = p.group * lanes;

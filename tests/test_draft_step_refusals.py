@@ -26,7 +26,7 @@ NORM = dict(x=A, x_type=_lib.BF16, ldx=256, residual=A, residual_type=_lib.BF16,
 
 @pytest.mark.parametrize("change,word", [
     (dict(x_type=_lib.E4M3), "x_type"), (dict(residual_type=2), "residual_type"), (dict(weight_type=7), "weight_type"), (dict(out_type=3), "out_type"), (dict(rows=-1), "bad rows"),
-    (dict(width=0), "bad rows"), (dict(width=32769, ldx=1 << 16, ld_residual=1 << 16, ld_sum=1 << 16, ldo=1 << 16), "bad rows"), (dict(ldx=255), "bad rows"), (dict(ld_residual=255), "bad rows"),
+    (dict(rows=(1 << 30) + 1), "bad rows"), (dict(width=0), "bad rows"), (dict(width=32769, ldx=1 << 16, ld_residual=1 << 16, ld_sum=1 << 16, ldo=1 << 16), "bad rows"), (dict(ldx=255), "bad rows"), (dict(ld_residual=255), "bad rows"),
     (dict(ld_sum=255), "bad rows"), (dict(ldo=255), "bad rows"), (dict(eps=-1.0), "eps"), (dict(eps=math.nan), "eps"), (dict(residual=None), "needs a residual"), (dict(x=None), "null"),
     (dict(out=None), "null"), (dict(out_scale=None), "null"), (dict(out=A + 8), "16-byte"), (dict(ldo=264), "16-byte"), (dict(x=A + 1), "multiples"),
     (dict(residual=A + 2, residual_type=_lib.F32), "multiples"), (dict(sum=A + 1), "multiples"), (dict(weight=A + 2), "multiples"), (dict(out=A + 2, out_type=_lib.F32), "multiples"),
@@ -51,7 +51,7 @@ PAGES = dict(k_pages=A, v_pages=A, groups=4, num_pages=8, tokens_per_page=16, ma
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(rows=-1), "bad rows"), (dict(heads=-1), "bad rows"), (dict(heads=0, kv_heads=0), "bad rows"), (dict(dim=0), "bad rows"), (dict(dim=1025), "bad rows"), (dict(rot_dims=66), "bad rows"),
+    (dict(rows=-1), "bad rows"), (dict(rows=(1 << 30) + 1), "bad rows"), (dict(heads=-1), "bad rows"), (dict(heads=0, kv_heads=0), "bad rows"), (dict(dim=0), "bad rows"), (dict(dim=1025), "bad rows"), (dict(rot_dims=66), "bad rows"),
     (dict(rot_dims=3), "bad rows"), (dict(rot_dims=-2), "bad rows"), (dict(type=2), "type"), (dict(out_type=2), "type"), (dict(ldq=255), "pitches"), (dict(ldk=127), "pitches"),
     (dict(ldq_out=255), "pitches"), (dict(ldk_out=127), "pitches"), (dict(pos=None), "null"), (dict(freq=None), "null"), (dict(q=None), "null"), (dict(q_out=None), "null"), (dict(k=None), "null"),
     (dict(k_out=None), "null"), (dict(q=A + 1), "multiples"), (dict(k_out=A + 1), "multiples"), (dict(pos=A + 2), "multiples"), (dict(freq=A + 4), "multiples"),

@@ -255,6 +255,18 @@ def test_a_last_key_that_is_none(sequences):
   assert torch.equal(got, clean)
 
 
+def test_sequences_that_descend():
+  """Rows of two sequences at once would have more parts than the scratch has places: nothing is written."""
+  c = Case([3] * 40, [200 + i for i in range(40)], [(0, 20, 64), (20, 20, 128)], heads=8, kv=2, dim=64, page=16)
+  for name, at, to in (("row0", 7, 120), ("row0", 20, 120), ("prefix_seq0", 0, 30)):
+    was = c.dev[name].clone()
+    c.dev[name][at] = to
+    c.out.fill_(7)
+    assert bool((c.run() == 7).all())
+    c.dev[name].copy_(was)
+  c.check()
+
+
 def test_pages_outside_the_pool():
   """They are read as page 0, and a length ends with the page map."""
   c = Case([1, 2], [90, 80], dim=64, page=16, seed=3)
