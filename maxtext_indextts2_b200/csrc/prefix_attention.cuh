@@ -299,7 +299,9 @@ __device__ __forceinline__ void prefix_load_tile(const PrefixRows& rows, int rou
 // Tails, and prefixes whose sequences bring few pairs.  Warp 4 copies K and V tiles of 8 KB each.  Warps 0 to 3 compute, each a tile of its own for 16 of the item's pairs, with S, P and O
 // in its registers: an item of up to 16 pairs has every fourth tile in a warp, one of up to 32 every second, one of up to 64 all.  Where several warps have parts of the
 // same pairs, they are joined in shared memory at the item's end.
-// Bound: the tails' bytes, each read once.
+// Bound: the tails' bytes, each read once.  64 sequences of 8 rows of 32 heads of 128 channels over up to 3000 tokens: 107 us, 255 MB at 2.4 TB/s.  A warp's tile of 32 tokens takes 2500 to 3000
+// cycles, most of them waits of its own chain (copy, 32 MMAs of scores, maximum, weights, 32 MMAs of values) with two or three warps on a scheduler, and an item some 5000 to begin, join
+// and store: short tails are bound by that.  (Queries in shared memory, and so three CTAs of an SM, were slower: 64 sequences of one row 39.2 us, not 35.5.)
 
 constexpr int kPrefixPairs = 64;    // pairs of an item: four MMA tiles
 constexpr int kPrefixWarps = 4;     // that compute; one more copies
@@ -357,6 +359,7 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   typedef PrefixShape<D> F;
   constexpr int KT = F::KT, CH = F::CH, NS = KT / 8, NO = D / 8, P = F::kPieces;
   extern __shared__ uint8_t smem_raw[];
+  static_assert(P % 2 == 0 && P <= 16 && P >= 2 * kPrefixWarps, "the warps' next tiles lie at most a ring further on");
   uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);  // piece: [CH][KT tokens][128 B], swizzled
   float* joint = reinterpret_cast<float*>(ring + P * kPrefixPieceBytes);         // [2][16 pairs][D + 4]
   PrefixTail* tail = reinterpret_cast<PrefixTail*>(joint + 2 * 16 * (D + 4));
@@ -695,7 +698,8 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 //   O += P V     tcgen05.mma with P as the TMEM operand and V as an MN-major one, fp32 in TMEM
 // Each half has two places for S: the next tile's is there before a softmax ends, so that neither waits for the other in turn (with one place of 128 tokens an item's tile of
 // 128 tokens took 3450 cycles: 2000 of softmax, 1000 of MMAs, the rest signals).  The accumulator is brought to a new maximum only when a pair's grew by more than 2^8.
-// Bound: MMAs, whose operands come from shared memory at 128 bytes a clock (of 256 pairs, 64 tokens and 128 channels 1280 cycles), and the special-function units (1024).
+// Bound: MMAs, whose operands come from shared memory at 128 bytes a clock (of 256 pairs, 64 tokens and 128 channels 1280 cycles), and the special-function units (1024).  A tile takes some
+// 1700 cycles: 575 rows of 16 heads over 16384 shared tokens, 77 GFLOP, in some 75 us.
 
 template <int D>
 struct PrefixTcShape {

@@ -107,7 +107,7 @@ int mtx_add_rmsnorm(const void* x, int x_type, long long ldx, const void* residu
   p.by_width = 1.0 / width;
   p.blocks = (width + kScaleBlock - 1) / kScaleBlock;
   const bool vec = width % 8 == 0 && rows_on_16(x, ldx, value_bytes(x_type)) && (!residual || rows_on_16(residual, ld_residual, value_bytes(residual_type))) &&
-                   (!sum || rows_on_16(sum, ld_sum, value_bytes(residual_type))) && rows_on_16(out, ldo, value_bytes(out_type));
+                   (!sum || rows_on_16(sum, ld_sum, value_bytes(residual_type))) && rows_on_16(out, ldo, value_bytes(out_type)) && lie_on(16, {weight});
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!residual) return x_type == MTX_F32 ? launch_add_rmsnorm<float, NoResidual>(p, vec, st) : launch_add_rmsnorm<bf16, NoResidual>(p, vec, st);
   if (residual_type == MTX_F32) return x_type == MTX_F32 ? launch_add_rmsnorm<float, float>(p, vec, st) : launch_add_rmsnorm<bf16, float>(p, vec, st);
