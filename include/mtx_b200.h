@@ -844,7 +844,7 @@ int mtx_prefix_attention_stalls(uint32_t* count);
  * accept_u * q(x) < p(x).  At the first that does not, the sequence goes on with a token drawn from max(p - q, 0) (over its sum); behind the last draft with one drawn from p.  Drawn is the
  * first token at which the sum of the weights in the tokens' order exceeds pick_u times their whole sum. */
 typedef struct {
-  int32_t rows, sequences, vocab;  /* up to 2^20, 65535 and 2^28; rows times parts of 1024 (for 592 and more parts of 4096: 4096) tokens stay below 2^31 */
+  int32_t rows, sequences, vocab;  /* up to 2^20, 65535 and 2^28; rows times their parts of 4096 tokens stay below 2^31 */
   const int32_t* row0;             /* [sequences + 1] ascending, as in mtx_prefix_batch */
   const int32_t* token;            /* [rows]: the tokens of the step's rows; a drafted token outside the vocabulary does not stay */
   const float* target;             /* [rows, vocab] logits; NaN counts as -infinity, infinity as the largest number */

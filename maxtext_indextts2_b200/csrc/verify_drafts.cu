@@ -8,8 +8,10 @@ namespace {
 constexpr int kMaxVocab = 1 << 28;
 constexpr int kMostSequences = 65535;  // (a grid's second dimension)
 
-// tokens per thread of a chunk: few where chunks of 4096 would leave SMs without one
-int verify_each(int rows, int vocab) { return (long long)rows * (vocab / 4096 + 1) < 4 * 148 ? 4 : 16; }
+// Tokens per thread of a chunk: 4 where there is little to read (chunks of 1024 are drawn from in less time, and they fill the SMs), 16 where there is much, and sooner in long rows (where a row's
+// sums are many).  With drafts, in us, 4 and 16:  1024 rows of 32768 71, 83;  2048 of 32768 123, 121;  500 of 65536 76.5, 79.2;  1250 of 50000 126, 118;  80 of 128000 38.2, 39.9;  160 of 128000
+// 54.5, 52.6;  20 of 264192 35.0, 38.1;  40 of 264192 43.9, 42.4;  320 of 264192 160, 132
+int verify_each(int rows, int vocab) { return double(rows) * vocab * (vocab > 65536 ? vocab / 65536.0 : 1.0) < 36e6 ? 4 : 16; }
 int verify_chunks(int each, int vocab) { return (vocab + 3 - 1) / (each * kVerifyThreads) + 1; }  // (rows begin up to three tokens behind a chunk's)
 
 // the scratch: sums of chunks of either side, of the differences, tasks, counters

@@ -96,6 +96,19 @@ def test_the_expanded_vocabulary():
   Case([2, 4], 264192, False, seed=2).check()
 
 
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("rows,vocab,pitch,shift", [([5] * 7 + [1], 264192, 0, 0), ([5] * 7 + [1], 262147, 1, 3), ([3, 2, 4], 786433, 3, 2), ([2, 3, 3], 1000003, 0, 1)])
+def test_much_to_read(rows, vocab, pitch, shift, draft):
+  """Chunks of 4096 tokens; greedy sequences beside others, masked logits and rows that leave one token."""
+  c = Case(rows, vocab, draft, seed=vocab, pitch=pitch, shift=shift, heat=[0.9, 0.0, 1.1] + [0.7] * (len(rows) - 3))
+  c.logits[c.row0[0], : vocab - 9000] = -math.inf
+  last = c.row0[-1] - 1
+  c.logits[last, :] = -math.inf
+  c.logits[last, vocab // 2] = 1.0
+  want = c.check()
+  assert want[-1][1][-1] in (vocab // 2, -1)
+
+
 @pytest.mark.parametrize("pitch,shift", [(0, 1), (1, 0), (3, 2), (5, 3), (4, 4)])
 def test_places(pitch, shift):
   Case([4, 2, 3], 9001, True, seed=pitch, pitch=pitch, shift=shift).check(near_most=0)
