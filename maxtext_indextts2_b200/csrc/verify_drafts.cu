@@ -14,15 +14,19 @@ constexpr int kMostSequences = 65535;  // (a grid's second dimension)
 int verify_each(int rows, int vocab) { return double(rows) * vocab * (vocab > 65536 ? vocab / 65536.0 : 1.0) < 36e6 ? 4 : 16; }
 int verify_chunks(int each, int vocab) { return (vocab + 3 - 1) / (each * kVerifyThreads) + 1; }  // (rows begin up to three tokens behind a chunk's)
 
+// Of the differences: chunks of 1024 tokens, or of 2048 beside those of 4096 (64 sequences of 264192 tokens 129.5 us with 4096, 127.0 with 2048, 128.0 with 1024)
+constexpr int verify_left_each(int each) { return each == 4 ? 4 : 8; }
+
 // the scratch: sums of chunks of either side, of the differences, tasks, counters
 struct VerifyLayout {
   size_t draft, left, task, done, bytes;
 
   VerifyLayout(int rows, int sequences, int vocab) {
-    const size_t chunks = size_t(verify_chunks(verify_each(rows, vocab), vocab));
+    const int each = verify_each(rows, vocab);
+    const size_t chunks = size_t(verify_chunks(each, vocab));
     draft = size_t(rows) * chunks * sizeof(VerifySum);
     left = 2 * draft;
-    task = left + size_t(sequences) * chunks * sizeof(double);
+    task = left + size_t(sequences) * verify_chunks(verify_left_each(each), vocab) * sizeof(double);
     done = task + size_t(sequences) * sizeof(VerifyTask);
     bytes = align_up(done + size_t(sequences) * sizeof(int), 256);
   }
@@ -34,7 +38,7 @@ int launch_verify(const VerifyParams& p, cudaStream_t st) {
   const long long ctas = ((long long)p.rows * p.chunks * (p.draft != nullptr ? 2 : 1) + kWarps - 1) / kWarps;
   if (p.rows > 0) MTX_TRY(launch(verify_sums_kernel<E>, dim3(unsigned(ctas < 4 * 148 ? ctas : 4 * 148)), dim3(kVerifyThreads), 0, st, p));
   MTX_TRY(launch(verify_settle_kernel<E>, dim3(p.sequences), dim3(kVerifyThreads), 0, st, p));
-  return p.task != nullptr ? launch(verify_difference_kernel<E>, dim3((p.chunks + kWarps - 1) / kWarps, p.sequences), dim3(kVerifyThreads), 0, st, p) : MTX_OK;
+  return p.task != nullptr ? launch(verify_difference_kernel<E, verify_left_each(E)>, dim3((p.left_chunks + kWarps - 1) / kWarps, p.sequences), dim3(kVerifyThreads), 0, st, p) : MTX_OK;
 }
 
 }  // namespace
@@ -76,6 +80,7 @@ int mtx_verify_drafts(const mtx_draft_batch* b, int32_t* accepted, int32_t* emit
   p.accepted = accepted;
   p.emitted = emitted;
   p.chunks = chunks;
+  p.left_chunks = verify_chunks(verify_left_each(each), b->vocab);
   if (b->rows > 0) {
     const VerifyLayout at(b->rows, b->sequences, b->vocab);
     uint8_t* base = static_cast<uint8_t*>(scratch);

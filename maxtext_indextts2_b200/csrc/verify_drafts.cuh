@@ -12,7 +12,7 @@
 // lies within 2^-19.5 of the whole sum of where it belongs, and the same call always draws the same token.
 //
 // The first two kernels let the next one start when they end: started as soon as it fits, it made 32 sequences of 4 rows over 32768 tokens (in chunks of 4096) 17.2 us, not 15.2.
-// 64 sequences of 5 rows over 264192 tokens take 130 us: 539 MB in 91 us, 5.9 TB/s, the decisions 12, 135 MB of the rows that differ, a third of them still in L2, 31.
+// 64 sequences of 5 rows over 264192 tokens take 127 us: 539 MB in 91 us, 5.9 TB/s, the decisions 12, the rows that differ, 76 MB of them, some 28.
 #pragma once
 
 #include "common.cuh"
@@ -36,6 +36,7 @@ struct VerifyTask {
 
 struct VerifyParams {
   int rows, sequences, vocab, chunks;
+  int left_chunks;  // of the differences
   const int *row0, *token;
   const float* target;
   long long ld_target;
@@ -44,7 +45,7 @@ struct VerifyParams {
   const float *temperature, *draft_temperature, *accept_u, *pick_u;
   int *accepted, *emitted;
   VerifySum *target_sum, *draft_sum;  // [rows, chunks]
-  double* left;                       // [sequences, chunks]: sums of max(p - q, 0)
+  double* left;                       // [sequences, left_chunks]: sums of max(p - q, 0)
   VerifyTask* task;                   // [sequences]
   int* done;                          // [sequences]: chunks that are through
 };
@@ -505,8 +506,8 @@ struct VerifyDifference {
   __device__ __forceinline__ float operator()(float l, float d) const { return fmaxf(target(l) * by_target - draft(d) * by_draft, 0.0f); }
 };
 
-// CTA = (eight chunks, a warp each; sequence), the last sequences first: their rows are what the first kernel has left in L2
-template <int E>
+// CTA = (eight chunks of D * 256 tokens, a warp each; sequence), the last sequences first: their rows are what the first kernel has left in L2
+template <int E, int D>
 __global__ void __launch_bounds__(kVerifyThreads, 3) verify_difference_kernel(const VerifyParams p) {
   __shared__ double doubles[8], want_in;
   __shared__ int ints[8], is_last, chunk_in;
@@ -518,9 +519,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_difference_kernel(co
   const float heat = verify_heat(p, s), draft_heat = verify_draft_heat(p, s);
   const float *target = p.target + task.row * p.ld_target, *draft = p.draft + task.row * p.ld_draft;
   const VerifyDifference weight(task, heat, draft_heat);
-  if (chunk < p.chunks) {
-    constexpr int kSteps = E * kVerifyThreads / kVerifyStep;
-    const int begin = verify_begin<E>(target, chunk);
+  if (chunk < p.left_chunks) {
+    constexpr int kSteps = D * kVerifyThreads / kVerifyStep;
+    const int begin = verify_begin<D>(target, chunk);
     float l[16], d[16];
     double sum = 0.0;
     verify_load16(target, begin, p.vocab, l);
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_difference_kernel(co
     }
     sum = verify_warp(sum, VerifyAdd());
     if ((threadIdx.x & 31) == 0) {
-      p.left[(long long)s * p.chunks + chunk] = sum;
+      p.left[(long long)s * p.left_chunks + chunk] = sum;
       __threadfence();
     }
   }
@@ -552,19 +553,19 @@ __global__ void __launch_bounds__(kVerifyThreads, 3) verify_difference_kernel(co
   }
   __syncthreads();
   if (!is_last) return;
-  const double* left = p.left + (long long)s * p.chunks;
+  const double* left = p.left + (long long)s * p.left_chunks;
   if (threadIdx.x < 32) {
     double total = 0.0;
-    for (int c = threadIdx.x; c < p.chunks; c += 32) total += __ldcg(left + c);
+    for (int c = threadIdx.x; c < p.left_chunks; c += 32) total += __ldcg(left + c);
     total = verify_warp(total, VerifyAdd());
     double want = double(p.pick_u[s]) * total;
-    const int found = verify_find_chunk([&](int c) { return __ldcg(left + c); }, p.chunks, want);
+    const int found = verify_find_chunk([&](int c) { return __ldcg(left + c); }, p.left_chunks, want);
     if (threadIdx.x == 0) want_in = want, chunk_in = found;
   }
   __syncthreads();
   int drawn;
   if (chunk_in >= 0)
-    drawn = verify_find_token<E>([&](int t) { return t >= 0 && t < p.vocab ? weight(verify_logit(target[t]), verify_logit(draft[t])) : 0.0f; }, verify_begin<E>(target, chunk_in), want_in,
+    drawn = verify_find_token<D>([&](int t) { return t >= 0 && t < p.vocab ? weight(verify_logit(target[t]), verify_logit(draft[t])) : 0.0f; }, verify_begin<D>(target, chunk_in), want_in,
                                  doubles, ints);
   else  // (no difference that 32 bits show: the target's own)
     drawn = verify_draw_target<E>(p, task.row, task.target, heat, p.pick_u[s], -1, doubles, ints);
