@@ -1008,7 +1008,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], mx[e], x[KT - 4 + e]);
         const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]), now = fmaxf(m, top * mul);
-        if (F::kByPolynomial && top != top) m = 0.0f, l = top;  // a score is none: so is the row (its weight by the polynomial is a number all the same)
+        if (F::kByPolynomial && !(top < INFINITY)) m = 0.0f, l = top - top;  // a score is none or infinite: the row is none (weights by the polynomial are numbers all the same)
         if (__any_sync(0xffffffffu, valid && now > m + 8.0f)) {  // (m = -inf: the first tile)
           const float fix = now == -INFINITY ? 1.0f : prefix_ex2(m - now);
           l *= fix;

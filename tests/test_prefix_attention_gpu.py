@@ -239,6 +239,14 @@ def test_scores_that_are_none(dim):
     c.k[at] = was
     assert bool(got[:, 4:].isnan().all()) and torch.equal(got[:, :4], clean[:, :4])
   c.q.abs_()
+  clean = c.check().clone()
+  for token in (4, 6, 63, 510):  # an infinite score: its weight is infinity over infinity
+    at = (0, int(c.maps[0, token // 16]), token % 16, 9)
+    was = c.k[at].clone()
+    c.k[at] = math.inf
+    got = c.run().double().view_as(clean)
+    c.k[at] = was
+    assert bool(got[:, :4].isnan().all()) and torch.equal(got[:, 4:], clean[:, 4:])
   c.k[:, c.maps[0, 2].long(), 1::2] = -1e30
   c.check()
 
