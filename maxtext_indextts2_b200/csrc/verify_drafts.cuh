@@ -66,12 +66,16 @@ struct VerifyScale {
   __device__ __forceinline__ float base(float top) const { return float(double(top) * exact()); }
 };
 
+// From an exponent of 2^30 on the largest logit alone weighs anything: the next smaller one is 2^-24 of it below, a weight of 2^-64 at most, and all of 2^28 tokens 2^-36.  There the rounding of `base`
+// (half of its last bit: up to 32 below 2^30, so that the largest weight lies within 2^-32 and 2^32) would reach the exponents that 32-bit numbers have.
+constexpr float kVerifyFar = 1073741824.0f;
+
 struct VerifyWeight {
   VerifyScale scale;
   float top, base;
-  bool far;  // logits next to the largest number: an exponent would overflow, and what is not the largest logit weighs nothing
+  bool far;  // only the largest logits weigh, 1 each
 
-  __device__ __forceinline__ VerifyWeight(const VerifyScale& s, float t) : scale(s), top(t), base(t == -INFINITY ? 0.0f : s.base(t)), far(!(fabsf(base) < 1e30f)) {}
+  __device__ __forceinline__ VerifyWeight(const VerifyScale& s, float t) : scale(s), top(t), base(t == -INFINITY ? 0.0f : s.base(t)), far(!(fabsf(base) < kVerifyFar)) {}
   __device__ __forceinline__ float operator()(float l) const {
     if (far) return l == top ? 1.0f : 0.0f;
     float y;

@@ -291,3 +291,28 @@ def _far(t, pitch):
   view = store.as_strided(t.shape, (pitch, 1))
   view.copy_(t)
   return view
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("heat,size", [(1.0, s) for s in (1e6, 1e7, 1e8, 3e8, 7e8, 1.5e9, 3e9, 1e10, 2e10, 1e15, 1e20, 1e30, 1e38)]
+                         + [(2.0**-20, s) for s in (20.0, 100.0, 700.0, 1000.0, 2900.0, 5000.0, 1e5)] + [(1e-6, 4000.0), (0.01, 1e8)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_large_logits_over_low_temperatures(heat, size, sign, draft):
+  """From where all tokens next to the largest count to where it alone does: exponents of 2^20 to infinity, either sign."""
+  c = Case([4, 3, 5, 2, 1, 6], 1500, draft, seed=23, heat=[heat] * 6)
+  g = torch.Generator().manual_seed(int(size) % 1000)
+  tops = 1200 + torch.randperm(200, generator=g)[:40]
+  own = torch.arange(1000, 1010)  # tokens of the draft's alone
+  for part, best_of in ((c.logits, tops),) + (((c.drafted, torch.cat([tops[:10], own, tops[10:25]])),) if draft else ()):
+    part.copy_(sign * size * (1 - 0.25 * sign * torch.rand(part.shape, generator=g)))
+    best = part.amax(1) + 0.05 * size
+    part[:, best_of] = best[:, None]
+    for i, t in enumerate(best_of[-15:].tolist() if part is c.drafted else best_of[10:].tolist()):  # up to five steps below the largest
+      for _ in range(i % 6):
+        part[:, t] = torch.nextafter(part[:, t], torch.tensor(-math.inf))
+  c.token = torch.cat([tops[:10], own])[torch.randint(0, 20, (c.rows,), generator=g)].int()
+  c.upload()
+  c.run()
+  want = c.compare(near_most=1)
+  assert all(t >= 0 for w in want for t in w[1][: w[0] + 1])
+  assert all(t in tops.tolist() for t in c.emitted.tolist() if t != -1)
