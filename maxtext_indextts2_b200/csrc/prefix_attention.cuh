@@ -49,7 +49,7 @@ struct alignas(16) PrefixEntry {
   int prefix;        // a tail's prefix where it begins behind one, else -1
   int first, tiles;  // the first tile's first token: key0 rounded down to where a copy may begin; tiles of an item
   int pairs, units;  // of one key head in the entries before
-  int bad;           // it ends before it begins; of the sums: one does, and nothing is done (places in the scratch are counted for entries side by side)
+  int bad;           // row0 or prefix_seq0 descends; of the sums: somewhere, and nothing is done (places in the scratch are counted for entries side by side)
 };
 
 constexpr float kPrefixLog2e = 1.4426950408889634f;
@@ -88,7 +88,7 @@ __device__ __forceinline__ PrefixEntry prefix_entry(const PrefixAttnParams& p, i
     const int s0 = seq_of(e), s1 = seq_of(e + 1);
     x.row = row_of(s0);
     x.rows = row_of(s1) - x.row;
-    x.bad = s1 < s0 || x.rows < 0;
+    x.bad = bounds[e + 1] < bounds[e] || x.rows < 0;
     x.key0 = 0;
     x.key1 = min(max(lens[e], 0), most);
     x.first_seen = x.key1;
@@ -98,7 +98,7 @@ __device__ __forceinline__ PrefixEntry prefix_entry(const PrefixAttnParams& p, i
     const int r0 = row_of(s), r1 = row_of(s + 1), length = p.lengths[s];
     x.row = r0;
     x.rows = r1 - r0;
-    x.bad = x.rows < 0;
+    x.bad = p.row0[s + 1] < p.row0[s];
     x.key1 = min(max(length, 0), most);
     x.first_seen = length < 0 ? -(1 << 30) : length - x.rows + 1;
     x.map = s;
@@ -141,6 +141,8 @@ __device__ __forceinline__ void prefix_build_table(const PrefixAttnParams& p, co
     __syncthreads();
   }
   int units = 0, pairs = 0, bad = 0;
+  if (k.first > 0)  // (the prefixes have a table of their own; tails that no other part joins are stored without a look at it)
+    for (int i = tid; i < p.prefixes; i += threads) bad |= bounds[i + 1] < bounds[i];
   for (int e0 = 0; e0 <= total; e0 += threads) {
     const int e = e0 + tid;
     PrefixEntry x;

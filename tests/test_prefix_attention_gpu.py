@@ -368,3 +368,15 @@ def test_long_prefixes(dim, heads, kv):
   first = c.check()
   for _ in range(5):
     assert torch.equal(c.run().double().view_as(first), first)
+
+
+@pytest.mark.parametrize("name,at,to", [("prefix_seq0", 0, 30), ("prefix_seq0", 1, 45), ("prefix_seq0", 2, 10), ("row0", 7, 120), ("row0", 39, 200), ("row0", 0, 500)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_short_sequences_that_descend(dim, name, at, to):
+  """Tails of one tile, that no other part joins, are not written either, with the prefixes in a kernel of their own or not; what lies behind the last row or sequence descends too."""
+  c = Case([3] * 40, [8 + i % 8 for i in range(40)], [(0, 20, 4), (20, 20, 3)], heads=8, kv=2, dim=dim, page=8, seed=dim)
+  was = c.dev[name].clone()
+  c.dev[name][at] = to
+  assert bool((c.run() == 7).all())
+  c.dev[name].copy_(was)
+  c.check()
