@@ -830,7 +830,8 @@ typedef struct {
  * bases and pitches whole 16 bytes.  The blocks of 64 (row, query head) pairs of a key head, one at least per sequence and prefix, times key heads and the page map's tiles of 4096 / head_dim
  * tokens stay below 2^31.  max_pages_per_group * tokens_per_page, what a sequence can have, also says whether prefixes are work for the tensor cores: a page map not much longer than its
  * sequences is the faster one for short prefixes.
- * scratch: written by every call, so one per stream (or graph) that runs at the same time; base on 256 bytes.  The same call gives the same bits every time. */
+ * scratch: written by every call, so one per stream (or graph) that runs at the same time; base on 256 bytes.  One for the largest step serves every call of no more rows, sequences and
+ * prefixes.  The same call gives the same bits every time. */
 size_t mtx_prefix_attention_scratch_bytes(int rows, int sequences, int prefixes, int num_q_heads, int num_kv_heads, int head_dim);
 int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, const void* v_pages, const mtx_prefix_batch* batch, void* out, long long ldo, int num_q_heads,
                          int num_kv_heads, int head_dim, int num_pages, int tokens_per_page, int max_pages_per_group, float scale, float softcap, void* scratch,
@@ -858,7 +859,8 @@ typedef struct {
 } mtx_draft_batch;
 /* accepted [sequences]: drafts that stay; emitted [rows]: a sequence's new tokens, those drafts and the drawn token, then -1 (as mtx_note_tokens skips it).  Rows outside the sequences
  * are left as they were.  A row that leaves nothing to draw (no logit above -infinity) gives -1 as mtx_sample_rows does.
- * scratch: written by every call, so one per stream (or graph) that runs at the same time; base on 16 bytes. */
+ * scratch: written by every call, so one per stream (or graph) that runs at the same time; base on 16 bytes.  One for the largest step serves every call of no more rows, sequences and
+ * tokens. */
 size_t mtx_verify_drafts_scratch_bytes(int rows, int sequences, int vocab);
 int mtx_verify_drafts(const mtx_draft_batch* b, int32_t* accepted, int32_t* emitted, void* scratch, size_t scratch_bytes, mtx_stream stream);
 

@@ -36,7 +36,7 @@ struct PrefixLayout {
     bytes = 0;
     for (int k = 0; k < 2; ++k) {  // prefixes, tails
       // every pair has a place in one tail and at most one prefix, and another in every CTA that shares its item with the CTA before
-      const size_t entries = k == 0 ? size_t(prefixes) : size_t(sequences) + (tc ? 0 : size_t(prefixes));
+      const size_t entries = k == 0 ? size_t(prefixes) : size_t(sequences) + size_t(prefixes);
       const size_t extra = k == 0 ? size_t(dim == 256 ? 128 : kPrefixTcPairs) * kPrefixSms : size_t(kPrefixPairs) * kPrefixWorkers;
       const size_t places = k == 0 && !tc ? 0 : all * size_t(kv_heads) * (k == 0 || tc ? 1 : 2) + extra;
       table[k] = bytes;
@@ -128,9 +128,8 @@ extern "C" {
 
 size_t mtx_prefix_attention_scratch_bytes(int rows, int sequences, int prefixes, int num_q_heads, int num_kv_heads, int head_dim) {
   if (rows < 1 || sequences < 1 || prefixes < 0 || num_kv_heads < 1 || num_q_heads < num_kv_heads || head_dim < 1) return 0;
-  const int group = num_q_heads / num_kv_heads;
-  // (with a kernel of their own for the prefixes there are more places, and as many entries)
-  return PrefixLayout(rows, sequences, prefixes, num_q_heads, num_kv_heads, head_dim, prefix_may_tc(rows, prefixes, group)).bytes;
+  // with a kernel of their own for the prefixes there are more places, and as many entries: enough for every smaller call, whichever kernel its prefixes have
+  return PrefixLayout(rows, sequences, prefixes, num_q_heads, num_kv_heads, head_dim, prefixes > 0).bytes;
 }
 
 int mtx_prefix_attention(const void* q, long long ldq, const void* k_pages, const void* v_pages, const mtx_prefix_batch* b, void* out, long long ldo, int num_q_heads,

@@ -11,7 +11,8 @@ constexpr int kMostSequences = 65535;  // (a grid's second dimension)
 // Tokens per thread of a chunk: 4 where there is little to read (chunks of 1024 are drawn from in less time, and they fill the SMs), 16 where there is much, and sooner in long rows (where a row's
 // sums are many).  With drafts, in us, 4 and 16:  1024 rows of 32768 71, 83;  2048 of 32768 123, 121;  500 of 65536 76.5, 79.2;  1250 of 50000 126, 118;  80 of 128000 38.2, 39.9;  160 of 128000
 // 54.5, 52.6;  20 of 264192 35.0, 38.1;  40 of 264192 43.9, 42.4;  320 of 264192 160, 132
-int verify_each(int rows, int vocab) { return double(rows) * vocab * (vocab > 65536 ? vocab / 65536.0 : 1.0) < 36e6 ? 4 : 16; }
+constexpr double kVerifyLittle = 36e6;
+int verify_each(int rows, int vocab) { return double(rows) * vocab * (vocab > 65536 ? vocab / 65536.0 : 1.0) < kVerifyLittle ? 4 : 16; }
 int verify_chunks(int each, int vocab) { return (vocab + 3 - 1) / (each * kVerifyThreads) + 1; }  // (rows begin up to three tokens behind a chunk's)
 
 // Of the differences: chunks of 1024 tokens, or of 2048 beside those of 4096 (64 sequences of 264192 tokens 129.5 us with 4096, 127.0 with 2048, 128.0 with 1024)
@@ -28,9 +29,16 @@ struct VerifyLayout {
     left = 2 * draft;
     task = left + size_t(sequences) * verify_chunks(verify_left_each(each), vocab) * sizeof(double);
     done = task + size_t(sequences) * sizeof(VerifyTask);
-    bytes = align_up(done + size_t(sequences) * sizeof(int), 256);
+    bytes = done + size_t(sequences) * sizeof(int);
   }
 };
+
+// What every call of at most so many rows, sequences and tokens finds room in: chunks of 1024 tokens of as many rows as may have them (kVerifyLittle / 1024 and a part of one for each row), or larger ones of all
+size_t verify_scratch(int rows, int sequences, int vocab) {
+  const size_t small = size_t(rows) * verify_chunks(4, vocab), large = size_t(rows) * verify_chunks(16, vocab), little = size_t(kVerifyLittle / 1024) + 1 + size_t(rows) + size_t(rows) / 512 + 1;
+  const size_t chunks = large > (small < little ? small : little) ? large : small < little ? small : little;
+  return align_up(2 * chunks * sizeof(VerifySum) + size_t(sequences) * (verify_chunks(4, vocab) * sizeof(double) + sizeof(VerifyTask) + sizeof(int)), 256);
+}
 
 template <int E>
 int launch_verify(const VerifyParams& p, cudaStream_t st) {
@@ -47,7 +55,7 @@ extern "C" {
 
 size_t mtx_verify_drafts_scratch_bytes(int rows, int sequences, int vocab) {
   if (rows < 1 || sequences < 1 || vocab < 1) return 0;
-  return VerifyLayout(rows, sequences, vocab).bytes;
+  return verify_scratch(rows, sequences, vocab);
 }
 
 int mtx_verify_drafts(const mtx_draft_batch* b, int32_t* accepted, int32_t* emitted, void* scratch, size_t scratch_bytes, mtx_stream stream) {

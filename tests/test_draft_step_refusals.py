@@ -175,3 +175,31 @@ def test_verification_without_a_batch(lib):
 def test_scratch_of_a_verification(lib):
   size = lib.mtx_verify_drafts_scratch_bytes
   assert size(0, 1, 64) == 0 and size(4, 0, 64) == 0 and size(4, 2, 0) == 0 and 0 < size(4, 2, 64) <= size(40, 8, 264192)
+
+
+def test_scratch_of_smaller_attentions(lib):
+  """What the largest step has is enough for every smaller one, on either side of where prefixes get a kernel of their own."""
+  size = lib.mtx_prefix_attention_scratch_bytes
+  steps = [1, 2, 5, 16, 20, 39, 40, 41, 64, 65, 128, 319, 320, 321, 1000, 65536]
+  for heads, kv, dim in ((16, 4, 128), (4, 4, 64), (16, 1, 256), (20, 4, 64)):
+    for rows in steps:
+      for sequences in steps[:9]:
+        prefixes = [size(rows, sequences, n, heads, kv, dim) for n in range(sequences + 1)]
+        assert prefixes == sorted(prefixes)
+    for sequences in (1, 64, 65536):
+      for prefixes in (0, 1, 40, 65536):
+        rows = [size(n, sequences, min(prefixes, sequences), heads, kv, dim) for n in steps]
+        assert rows == sorted(rows)
+        assert size(320, sequences, min(prefixes, sequences), heads, kv, dim) <= size(320, sequences + 1, min(prefixes, sequences), heads, kv, dim)
+
+
+def test_scratch_of_smaller_verifications(lib):
+  """Chunks get larger from some rows on, and a call needs less: what the largest step has is enough all the same."""
+  size = lib.mtx_verify_drafts_scratch_bytes
+  for vocab in (1, 1000, 32768, 50000, 65536, 65537, 128000, 264192, 1 << 20, 1 << 28):
+    rows = [size(n, 64, vocab) for n in list(range(1, 1300)) + [4000, 1 << 16, 1 << 20]]
+    assert rows == sorted(rows)
+    assert [size(100, n, vocab) for n in (1, 5, 64, 65535)] == sorted(size(100, n, vocab) for n in (1, 5, 64, 65535))
+  for n in (1, 33, 34, 320, 1095, 1100, 1 << 20):
+    tokens = [size(n, 64, v) for v in list(range(1, 300000, 997)) + [1 << 20, 1 << 24, 1 << 28]]
+    assert tokens == sorted(tokens)
