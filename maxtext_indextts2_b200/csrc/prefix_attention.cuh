@@ -818,12 +818,14 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     tail->failed = 0;
     fence_barrier_init();
   }
+  // Tensor memory behind the wait: a kernel in front that lets this one start before it has its own columns (the products do) would wait for these, and this CTA for that kernel.  What comes next
+  // starts when this CTA has its columns, for the same reason.
+  griddep_wait();
   if (warp == 1) {
     tmem_alloc(&tail->tmem_base, 512);
     tmem_relinquish();
+    griddep_launch_dependents();
   }
-  griddep_wait();
-  griddep_launch_dependents();
   const PrefixEntry* table = k.table;
   tcgen05_fence_before();
   if (!k.tabled) {

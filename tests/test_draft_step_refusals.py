@@ -2,6 +2,7 @@
 
 import ctypes
 import math
+import pathlib
 
 import pytest
 
@@ -203,3 +204,11 @@ def test_scratch_of_smaller_verifications(lib):
   for n in (1, 33, 34, 320, 1095, 1100, 1 << 20):
     tokens = [size(n, 64, v) for v in list(range(1, 300000, 997)) + [1 << 20, 1 << 24, 1 << 28]]
     assert tokens == sorted(tokens)
+
+
+def test_tensor_memory_is_taken_behind_the_wait():
+  """All columns taken before the kernels in front are through: one of those that starts its successor before it has its own columns would never get them, and neither kernel would end."""
+  source = (pathlib.Path(_lib.__file__).parent / "csrc" / "prefix_attention.cuh").read_text()
+  body = source[source.index("\nprefix_tc_kernel(") :]
+  body = body[: body.index("\n}\n")]
+  assert body.index("griddep_wait()") < body.index("tmem_alloc(") < body.index("griddep_launch_dependents()")

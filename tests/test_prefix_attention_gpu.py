@@ -380,3 +380,20 @@ def test_short_sequences_that_descend(dim, name, at, to):
   assert bool((c.run() == 7).all())
   c.dev[name].copy_(was)
   c.check()
+
+
+@pytest.mark.parametrize("dim,heads", [(64, 20), (128, 16), (256, 8)])
+def test_behind_short_products(dim, heads):
+  """Products of short sums in front, which start what comes next before they hold tensor memory of their own: every step ends, with the results that it has alone."""
+  lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+  c = Case([5] * 40, [300 + i for i in range(40)], [(0, 40, 256)], heads=heads, kv=4, dim=dim, page=16, seed=dim)
+  first = c.check()
+  x, w = torch.randn(32, 128, device="cuda").to(torch.bfloat16), torch.randn(19200, 128, device="cuda").to(torch.bfloat16)
+  ys = [torch.empty(32, 19200, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+  for _ in range(50):
+    for y in ys:
+      _lib.check(lib.mtx_linear(x.data_ptr(), w.data_ptr(), y.data_ptr(), 32, 19200, 128, 1, stream))
+    c.run()
+  assert torch.equal(c.out.double().view_as(first), first) and torch.equal(ys[0], ys[1])
+  want = x.double() @ w.double().T
+  assert bool(((ys[0].double() - want).abs() <= 2.0**-8 * want.abs() + 2.0**-13 * (x.double().abs() @ w.double().abs().T)).all())
