@@ -770,7 +770,8 @@ int mtx_note_tokens(uint16_t* seen, long long ld_seen, uint32_t* touched, long l
  * x, residual (and sum, of its type), weight [width]: MTX_BF16 or MTX_F32 each; out: MTX_BF16, MTX_F32, or MTX_E4M3 with out_scale
  * [rows, ceil(width / 128)], as mtx_quantize_fp8(block_rows = 1) gives them for out's fp32 values (8-bit values: base and pitch whole 16 bytes; the bytes behind a
  * row's last value stay).  Pitches in values; width <= 32768, rows <= 2^30; other values at any multiple of their types' sizes, with any pitch.  sum may be residual or x, and out any
- * input, where type and pitch are the same; nothing else may overlap.  A row with a NaN is NaN throughout, one with an infinity 0 but for NaN in its place. */
+ * input, where type and pitch are the same; nothing else may overlap.  Values of any size, as long as their products with the weights are 32-bit numbers.
+ * A row with a NaN is NaN throughout, one with an infinity 0 but for NaN in its place. */
 int mtx_add_rmsnorm(const void* x, int x_type, long long ldx, const void* residual, int residual_type, long long ld_residual, void* sum, long long ld_sum, const void* weight,
                     int weight_type, float weight_offset, float eps, void* out, int out_type, long long ldo, float* out_scale, int rows, int width, mtx_stream stream);
 

@@ -11,7 +11,7 @@
 // The mean, of 32-bit sums of eight squares (off by 5 * 2^-24 at most), the norm's factor and the scales' fractions are 64-bit, so that scales and 8-bit values are those of the definition with
 // that mean; what 64 bits cost is spent once per row and block, by one warp.  Eight values are formed twice in 32 bits, by factors 2^-21 below and above theirs, which is more than 32 bits' three
 // roundings: where both are the same 8-bit values so is the definition's, otherwise (of eight one in 10,000) they are formed again in 64.  Other results have two roundings in 32 bits and
-// their type's own.
+// their type's own.  A row whose squares 32 bits do not hold is formed in 64 bits throughout.
 #pragma once
 
 #include "fp8_linear.cuh"
@@ -100,9 +100,68 @@ __device__ __forceinline__ float norm_odd(double v) {
   return double(t) == v || !(fabsf(t) < INFINITY) ? t : __uint_as_float(__float_as_uint(t) | 1u);
 }
 
+// h as it was stored, from memory (behind a barrier of the threads that store the row's sum)
+template <class TX, class TR>
+__device__ __forceinline__ float norm_value(const AddNormParams& p, int row, int c) {
+  typedef AddNormRow<TX, TR> Row;
+  typedef typename Row::TH TH;
+  if (Row::kAdd && p.sum != nullptr) return static_cast<float>(static_cast<const TH*>(p.sum)[row * p.lds + c]);
+  return norm_sum<TX, TR>(static_cast<const TX*>(p.x)[row * p.ldx + c], Row::kAdd ? static_cast<float>(static_cast<const TH*>(p.residual)[row * p.ldr + c]) : 0.0f);
+}
+
+__device__ __forceinline__ float norm_weight(const AddNormParams& p, int c) {
+  return p.weight == nullptr ? 1.0f : (p.weight_f32 ? static_cast<const float*>(p.weight)[c] : static_cast<float>(static_cast<const bf16*>(p.weight)[c])) + p.weight_offset;
+}
+
+// NaN where one is
+__device__ __forceinline__ double norm_larger(double a, double b) { return a != a || b <= a ? a : b; }
+
+// A row whose squares 32 bits do not hold (values from some 2^60 on; mean and eps below 2^-100), or one with values that are no numbers: all of it in 64 bits and from memory, by the threads
+// that have the row, every warp its own sum.  Not inlined: the registers of such a row are no other row's.
+template <class TX, class TR, bool E4M3>
+__device__ __noinline__ void norm_row_in_64_bits(const AddNormParams& p, int row) {
+  const int lane = threadIdx.x & 31, threads = blockDim.x;
+  double sum = 0.0;
+  for (int c = lane; c < p.width; c += 32) {
+    const double h = norm_value<TX, TR>(p, row, c);
+    sum = fma(h, h, sum);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const double inv = rsqrt(sum * p.by_width + double(p.eps));
+  if (threads > 32) __syncthreads();  // (results in an input's place)
+  else __syncwarp();
+  if (!E4M3) {
+    for (int c = threadIdx.x; c < p.width; c += threads) {
+      const double y = double(norm_value<TX, TR>(p, row, c)) * double(norm_weight(p, c)) * inv;
+      if (p.out_type == MTX_F32) static_cast<float*>(p.out)[row * p.ldo + c] = float(y);
+      else static_cast<bf16*>(p.out)[row * p.ldo + c] = __float2bfloat16_rn(norm_odd(y));
+    }
+    return;
+  }
+  for (int b = threadIdx.x >> 5; b < p.blocks; b += threads >> 5) {
+    double y[4], largest = 0x1p-96;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = b * kScaleBlock + i * 32 + lane;
+      y[i] = c < p.width ? double(norm_value<TX, TR>(p, row, c)) * double(norm_weight(p, c)) * inv : 0.0;
+      largest = norm_larger(largest, fabs(y[i]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) largest = norm_larger(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    const double by = 448.0 / largest;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = b * kScaleBlock + i * 32 + lane;
+      if (c < p.width) static_cast<uint8_t*>(p.out)[row * p.ldo + c] = uint8_t(e4m3_pair(norm_odd(y[i] * double(float(by))), 0.0f));
+    }
+    if (lane == 0) p.scale[(long long)row * p.blocks + b] = float(largest * (1.0 / 448.0));
+  }
+}
+
 // CTA = a row, or eight rows of a warp each.  VEC: all rows and the weights lie on 16 bytes and end with whole eight values.
 template <class TX, class TR, bool E4M3, bool VEC, int J, int T>
-__global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 768 ? 1536 / T : J == 3 ? 2 : 1) add_rmsnorm_kernel(const AddNormParams p) {
+__global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 768 ? 1536 / T : J == 3 ? 2 : 1) add_rmsnorm_kernel(const __grid_constant__ AddNormParams p) {
   typedef AddNormRow<TX, TR> Row;
   typedef typename Row::TH TH;
   __shared__ double part[32], inv_of_row;
@@ -199,8 +258,14 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 768 ? 15
   } else {
     __syncwarp();
   }
+  auto held = [](double mean) { return mean >= 0x1p-100 && mean < double(INFINITY); };  // by 32-bit squares
   if (!E4M3) {
-    const float f = __frsqrt_rn(float(whole()));
+    const double mean = whole();
+    if (!held(mean)) {
+      norm_row_in_64_bits<TX, TR, false>(p, row);
+      return;
+    }
+    const float f = __frsqrt_rn(float(mean));
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int c = (threadIdx.x + j * threads) * 8;
@@ -220,7 +285,8 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 768 ? 15
   }
   // one warp has the row's factor and the blocks' fractions, a lane a block
   if (threadIdx.x < 32) {
-    inv = rsqrt(whole());
+    const double mean = whole();
+    inv = held(mean) ? rsqrt(mean) : -1.0;
     for (int b = lane; b < p.blocks; b += 32) {
       const float top = block_top[block0 + b], low = block_low[block0 + b];
       double largest = (double(top) + double(fabsf(low) < INFINITY ? low : 0.0f)) * inv;
@@ -260,8 +326,12 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 768 ? 15
   }
   // values next to a border once more, with their neighbours and from memory (registers for this would be every row's)
   __syncwarp();  // (a sum may have been stored by the next lane)
-  if (again == 0) return;
   const double row_inv = single ? inv : inv_of_row;
+  if (row_inv < 0.0) {  // (here nothing of the row is in registers; what is stored so far is stored again)
+    norm_row_in_64_bits<TX, TR, true>(p, row);
+    return;
+  }
+  if (again == 0) return;
 #pragma unroll 1
   for (int j = 0; j < J; ++j) {
     if (!(again >> j & 1)) continue;
@@ -269,10 +339,7 @@ __global__ void __launch_bounds__(T, J == 1 ? 1536 / T : J == 2 && T <= 768 ? 15
     for (int i = 0; i < 8; ++i) {
       const int c = (threadIdx.x + j * threads) * 8 + i;
       if (c >= p.width) break;
-      float h;
-      if (Row::kAdd && p.sum != nullptr) h = static_cast<float>(static_cast<const TH*>(p.sum)[row * p.lds + c]);
-      else h = norm_sum<TX, TR>(x0[row * p.ldx + c], Row::kAdd ? static_cast<float>(r0[row * p.ldr + c]) : 0.0f);
-      const float w = p.weight == nullptr ? 1.0f : (p.weight_f32 ? static_cast<const float*>(p.weight)[c] : static_cast<float>(static_cast<const bf16*>(p.weight)[c])) + p.weight_offset;
+      const float h = norm_value<TX, TR>(p, row, c), w = norm_weight(p, c);
       const int b = block0 + c / kScaleBlock;
       static_cast<uint8_t*>(p.out)[row * p.ldo + c] = uint8_t(e4m3_pair(norm_odd(double(h) * double(w) * (row_inv * double(block_by[b]))), 0.0f));
     }

@@ -245,3 +245,30 @@ def test_the_next_product_reads_it():
   want = (out.double() * spread(scale, 1, rows)) @ (wq.view(FP8).double() * spread(ws, 128, n)).T
   size = (out.double().abs() * spread(scale, 1, rows)) @ (wq.view(FP8).double().abs() * spread(ws, 128, n)).T
   assert bool(((y.double() - want).abs() <= size * (132 * 2.0**-23 + 12 * 2.0**-24)).all())
+
+
+@pytest.mark.parametrize("width", [100, 512, 1000, 1280, 5376, 8203, 20000])
+@pytest.mark.parametrize("types", [(F32, None, BF16), (F32, F32, F32), (F32, F32, FP8), (BF16, BF16, BF16), (BF16, None, FP8), (BF16, BF16, FP8)])
+@pytest.mark.parametrize("size", [62, 66, 90, 126, -49, -55, -70, -100])
+def test_squares_beyond_32_bits(width, types, size):
+  """Rows of values around 2^size, whose squares 32 bits do not hold, beside rows of ordinary ones and rows of both."""
+  g = torch.Generator().manual_seed(width + size)
+  tx, tr, to = types
+  x = torch.randn(6, width, generator=g).clamp(-3.5, 3.5)
+  residual = None if tr is None else torch.randn(6, width, generator=g).clamp(-3.5, 3.5)
+  for r in (0, 2, 5):
+    x[r] *= 2.0 ** (size - 2)
+    if tr is not None:
+      residual[r] *= 2.0 ** (size - 2)
+  x[3, width // 2] = 2.0**size
+  x, residual = x.to(tx), None if tr is None else residual.to(tr)
+  weight = 1 + 0.3 * torch.randn(width, generator=g)
+  eps = 0.0 if size < 0 else 1e-5
+  pitch = -(-width // 16) * 16
+  for where in ("apart", "in place") if to == BF16 else ("apart",):
+    a, r = x.cuda(), None if residual is None else residual.cuda()
+    total = None if r is None else r if where == "in place" else torch.empty_like(r)
+    out = a if where == "in place" and tx == BF16 else torch.empty(6, pitch, dtype=to, device="cuda")[:, :width]
+    scale = torch.empty(6, -(-width // 128), device="cuda") if to == FP8 else None
+    call(a, r, total, weight.cuda(), 0.0, eps, out, scale)
+    check(x, residual, weight, 0.0, eps, total, out, scale)
