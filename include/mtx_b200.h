@@ -844,7 +844,8 @@ int mtx_prefix_attention_stalls(uint32_t* count);
 /* Verification of drafted tokens, beside mtx_sample_rows: the step's rows of a sequence are its last token and the drafted ones, so that row r's logits decide on token[r + 1], and the
  * last row's on a token behind all drafts.  With p, q the softmax of the target's and the draft's logits over their temperatures and x the drafted token: x stays when
  * accept_u * q(x) < p(x).  At the first that does not, the sequence goes on with a token drawn from max(p - q, 0) (over its sum); behind the last draft with one drawn from p.  Drawn is the
- * first token at which the sum of the weights in the tokens' order exceeds pick_u times their whole sum. */
+ * first token at which the sum of the weights in the tokens' order exceeds pick_u times their whole sum (32-bit weights and 64-bit sums: borders are those of the formula within 2^-19.5 of p's sum,
+ * of max(p - q, 0) within 2^-18.5). */
 typedef struct {
   int32_t rows, sequences, vocab;  /* up to 2^20, 65535 and 2^28; rows times their parts of 4096 tokens stay below 2^31 */
   const int32_t* row0;             /* [sequences + 1] ascending, as in mtx_prefix_batch */

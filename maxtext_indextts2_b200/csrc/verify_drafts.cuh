@@ -8,8 +8,10 @@
 // sequence, joins the chunks, settles which drafts stay and draws where the target's own weights are drawn from: the chunks' sums say which chunk, which is then read once more.  The
 // third goes through the rows that draw from a difference; the last CTA of a sequence draws.  Bound: bytes, every row once and those of the third kernel twice.
 //
-// Weights are 32-bit powers of two of an exponent that is rounded twice, relative to itself; sums of a thread's tokens are 32-bit, all others 64-bit: a border between two tokens
-// lies within 2^-19.5 of the whole sum of where it belongs, and the same call always draws the same token.
+// Weights are 32-bit powers of two (the results are tokens and comparisons: 64-bit weights would cost the first kernel's pace) of an exponent that is rounded twice, relative to itself; sums of a
+// thread's tokens are 32-bit, all others 64-bit.  A border between two tokens lies within 2^-19.5 of the whole sum of where it belongs where p is drawn from.  Where max(p - q, 0) is, it lies within
+// 2^-18.5 of p's whole sum, however little of that the difference leaves: both sums' errors come to q's part beside its weights' own.  (A draft is turned down as seldom as
+// that difference is small.)  The same call always draws the same token.
 //
 // The first two kernels let the next one start when they end: started as soon as it fits, it made 32 sequences of 4 rows over 32768 tokens (in chunks of 4096) 17.2 us, not 15.2.
 // 64 sequences of 5 rows over 264192 tokens take 127 us: 539 MB in 91 us, 5.9 TB/s, the decisions 12, the rows that differ, 76 MB of them, some 28.
@@ -45,7 +47,7 @@ struct VerifyParams {
   const float *temperature, *draft_temperature, *accept_u, *pick_u;
   int *accepted, *emitted;
   VerifySum *target_sum, *draft_sum;  // [rows, chunks]
-  double* left;                       // [sequences, left_chunks]: sums of max(p - q, 0)
+  double* left;                       // [sequences, left_chunks]: sums of max(p - q, 0), in p's weights
   VerifyTask* task;                   // [sequences]
   int* done;                          // [sequences]: chunks that are through
 };
@@ -499,15 +501,21 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_settle_kernel(const Ver
   }
 }
 
-// max(p - q, 0) of a row's tokens
+// max(p - q, 0) of a row's tokens, in p's weights: t - d (sum of p's weights / sum of q's), that factor in two parts, so that what both weigh alike cancels to the last bit (as products with 1 / sum
+// of either side, each rounded, a difference of 10^-4 of p drew its tokens by up to 2^-15 of it beside)
 struct VerifyDifference {
   VerifyWeight target, draft;
-  float by_target, by_draft;
+  float hi, lo;
 
-  __device__ __forceinline__ VerifyDifference(const VerifyTask& t, float heat, float draft_heat)
-      : target(VerifyScale(heat), t.target.top), draft(VerifyScale(draft_heat), t.draft.top), by_target(float(1.0 / t.target.sum)),
-        by_draft(t.draft.top == -INFINITY ? 0.0f : float(1.0 / t.draft.sum)) {}
-  __device__ __forceinline__ float operator()(float l, float d) const { return fmaxf(target(l) * by_target - draft(d) * by_draft, 0.0f); }
+  __device__ __forceinline__ VerifyDifference(const VerifyTask& t, float heat, float draft_heat) : target(VerifyScale(heat), t.target.top), draft(VerifyScale(draft_heat), t.draft.top) {
+    const double by = t.draft.top == -INFINITY ? 0.0 : t.target.sum / t.draft.sum;
+    hi = float(by);
+    lo = float(by - double(hi));
+  }
+  __device__ __forceinline__ float operator()(float l, float d) const {
+    const float w = draft(d);
+    return fmaxf(fmaf(-w, lo, fmaf(-w, hi, target(l))), 0.0f);
+  }
 };
 
 // CTA = (eight chunks of D * 256 tokens, a warp each; sequence), the last sequences first: their rows are what the first kernel has left in L2

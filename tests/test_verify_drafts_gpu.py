@@ -316,3 +316,42 @@ def test_large_logits_over_low_temperatures(heat, size, sign, draft):
   want = c.compare(near_most=1)
   assert all(t >= 0 for w in want for t in w[1][: w[0] + 1])
   assert all(t in tops.tolist() for t in c.emitted.tolist() if t != -1)
+
+
+@pytest.mark.parametrize("left", [1e-2, 1e-4, 1e-6, 1e-7])
+def test_what_a_draft_leaves_of_its_target(left):
+  """A draft that has one token more, whose share is `left`: of all others the same part is left, so that they are drawn by their own weights, within 2^-19 of their sum (weights off by 2^-20.5, a
+  thread's sums of up to 16 of them by 2^-20)."""
+  c = Case([2] * 300, 3000, True, seed=24, heat=[1.0] * 300, spread=2.0)
+  c.logits[:, 2000], c.logits[:, 700] = 8.0, -math.inf
+  c.drafted.copy_(c.logits)
+  c.drafted[:, 700] = math.log(left) + torch.logsumexp(c.logits, 1)
+  c.token[:] = 700
+  c.upload()
+  c.run()
+  assert c.accepted.tolist() == [0] * 300
+  for s, drawn in enumerate(c.emitted[::2].tolist()):
+    up = c.logits[2 * s].double().exp().cumsum(0)
+    want = float(c.pick[s]) * float(up[-1])
+    low, high = (float(up[drawn - 1]) if drawn > 0 else 0.0) - 2.0**-19 * float(up[-1]), float(up[drawn]) + 2.0**-19 * float(up[-1])
+    assert low <= want <= high and drawn != 700, (s, drawn, want / float(up[-1]), low / float(up[-1]), high / float(up[-1]))
+
+
+@pytest.mark.parametrize("apart", [1e-1, 1e-2, 1e-3, 1e-4, 1e-5])
+def test_drafts_next_to_their_target(apart):
+  """Drawn from a difference that is small beside the target: a border lies within 2^-18.5 of the target's whole sum.  (Weights are off by 2^-20.5 of themselves, and so are both whole sums: of the
+  target's part of a sum once that, of the draft's part three times.)"""
+  c = Case([2] * 40, 32768, True, seed=25, heat=[1.0] * 40, apart=apart)
+  c.accept[:] = 1 - 2.0**-24
+  p, q = (torch.softmax(x.double(), 1) for x in (c.logits, c.drafted))
+  token = torch.where(p > 1e-6, q / p, 0.0).argmax(1)  # the one that the draft says most too often
+  c.token[1::2] = token[::2].int()
+  c.upload()
+  c.run()
+  assert c.accepted.tolist() == [0] * 40
+  for s, drawn in enumerate(c.emitted[::2].tolist()):
+    weight = (p[2 * s] - q[2 * s]).clamp(min=0)
+    up = weight.cumsum(0)
+    want = float(c.pick[s]) * float(up[-1])
+    assert (float(up[drawn - 1]) if drawn > 0 else 0.0) - 2.0**-18.5 <= want <= float(up[drawn]) + 2.0**-18.5
+    assert abs(float(weight[drawn])) > 0 or float(q[2 * s, drawn] - p[2 * s, drawn]) < 2.0**-18.5 * float(p[2 * s, drawn])
