@@ -397,3 +397,17 @@ def test_behind_short_products(dim, heads):
   assert torch.equal(c.out.double().view_as(first), first) and torch.equal(ys[0], ys[1])
   want = x.double() @ w.double().T
   assert bool(((ys[0].double() - want).abs() <= 2.0**-8 * want.abs() + 2.0**-13 * (x.double().abs() @ w.double().abs().T)).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("count", [129, 200, 300])
+def test_many_sequences_of_few_prefixes(count, dim):
+  """More sequences than a CTA keeps entries of, with the prefixes in a kernel of their own where the page map has room."""
+  g = torch.Generator().manual_seed(count)
+  rows = torch.randint(1, 4, (count,), generator=g).tolist()
+  lengths = [150 + n + int(t) for n, t in zip(rows, torch.randint(0, 100, (count,), generator=g))]
+  first = Case(rows, lengths, [(0, count, 150)], heads=8, kv=2, dim=dim, page=16, seed=count)
+  got = first.check()
+  for _ in range(3):
+    assert torch.equal(first.run().double().view_as(got), got)
+  Case(rows, lengths, [(0, 70, 100), (70, count - 70, 140)], heads=8, kv=2, dim=dim, page=16, seed=count + 1).check()
