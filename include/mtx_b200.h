@@ -769,8 +769,8 @@ int mtx_note_tokens(uint16_t* seen, long long ld_seen, uint32_t* touched, long l
  *   out = h * (weight_offset + weight) / sqrt(mean(h^2) + eps);  weight NULL: without that factor.
  * x, residual (and sum, of its type), weight [width]: MTX_BF16 or MTX_F32 each; out: MTX_BF16, MTX_F32, or MTX_E4M3 with out_scale
  * [rows, ceil(width / 128)], as mtx_quantize_fp8(block_rows = 1) gives them for out's fp32 values (8-bit values: base and pitch whole 16 bytes; the bytes behind a
- * row's last value stay).  Pitches in values; width <= 32768, rows <= 2^30; other values at any multiple of their types' sizes, with any pitch.  sum may be residual or x, and out any
- * input, where type and pitch are the same; nothing else may overlap.  Values of any size, as long as their products with the weights are 32-bit numbers.
+ * row's last value stay).  Pitches in values; width <= 32768, rows <= 2^30; other values at any multiple of their types' sizes, with any pitch.  sum may be residual or x, and out
+ * either of them, where type and pitch are the same; nothing else may overlap.  Values of any size, as long as their products with the weights are 32-bit numbers.
  * A row with a NaN is NaN throughout, one with an infinity 0 but for NaN in its place. */
 int mtx_add_rmsnorm(const void* x, int x_type, long long ldx, const void* residual, int residual_type, long long ld_residual, void* sum, long long ld_sum, const void* weight,
                     int weight_type, float weight_offset, float eps, void* out, int out_type, long long ldo, float* out_scale, int rows, int width, mtx_stream stream);
@@ -827,7 +827,8 @@ typedef struct {
 } mtx_prefix_batch;
 /* q, out [rows, num_q_heads * head_dim] bf16 at pitches ldq, ldo; k_pages, v_pages [num_kv_heads, num_pages, tokens_per_page, head_dim] bf16, tokens_per_page a power of two >= 8;
  * head_dim 64, 128 or 256; up to 16 query heads per key head.  out = softmax(cap(scale * <q, k>)) v, cap(x) = softcap * tanh(x / softcap) (0: off).  A row that sees no token, and rows
- * outside the sequences, are left as they were; where row0 or prefix_seq0 descends all of them are.  Page numbers outside the pool are read as page 0, lengths end with the page map.  All
+ * outside the sequences, are left as they were; where row0 or prefix_seq0 descends all of them are.  Page numbers outside the pool are read as page 0; of the tokens
+ * that a row sees, those behind the page map's end are left out.  All
  * bases and pitches whole 16 bytes.  The blocks of 64 (row, query head) pairs of a key head, one at least per sequence and prefix, times key heads and the page map's tiles of 4096 / head_dim
  * tokens stay below 2^31.  max_pages_per_group * tokens_per_page, what a sequence can have, also says whether prefixes are work for the tensor cores: a page map not much longer than its
  * sequences is the faster one for short prefixes.

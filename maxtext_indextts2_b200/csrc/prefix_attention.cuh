@@ -539,7 +539,7 @@ prefix_units_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           for (int n = 0; n < NO; ++n) o[n][2 * h] *= fix, o[n][2 * h + 1] *= fix;
         }
       }
-      uint32_t a[KT / 16][4];
+      uint32_t a[KT / 16][4];  // weights as bf16, half a step of 2^-8 each: the MMAs take both factors in the values' type
 #pragma unroll
       for (int n = 0; n < NS; ++n)
 #pragma unroll
@@ -1047,6 +1047,8 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
               w.x = prefix_ex2(w.x);
               w.y = prefix_ex2(w.y);
             }
+            // the sum is of the weights before they are rounded to the values' type for the MMA: unpacking them again is two instructions more for each pair, in the half of the kernel that bounds heads
+            // of 64 channels.  Where one key has nearly all of a row it is off by that rounding, half a step of 2^-8, as its result is anyway
             sums[e & 1] = prefix_add2(sums[e & 1], w);
             pk[e] = pack_bf16x2(w.x, w.y);
           }
